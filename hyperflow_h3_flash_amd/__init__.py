@@ -3,6 +3,7 @@
 Importing the package does not touch the GPU or load the HIP library; the first device forward does.
 """
 
+from .block import AdapterPlan, AttentionPlan, RotaryAxes, adapter_add, packed_attention, qk_norm_rope
 from .int8 import (
     ACTIVATIONS,
     ARITHMETIC_OPTIONS,
@@ -24,6 +25,8 @@ __version__ = "0.1.0"
 __all__ = [
     "ACTIVATIONS",
     "ARITHMETIC_OPTIONS",
+    "AdapterPlan",
+    "AttentionPlan",
     "INT8_GEMMS",
     "KERNEL_OPTIONS",
     "ROTATE_ARITHMETICS",
@@ -31,8 +34,12 @@ __all__ = [
     "Int8RotLinear",
     "LowRankLinear",
     "RANK_MULTIPLE",
+    "RotaryAxes",
+    "adapter_add",
     "fuse_qkv",
     "hadamard_factors",
+    "packed_attention",
+    "qk_norm_rope",
     "regular_hadamard",
     "resolve_int8_gemm",
     "set_arithmetic_options",

@@ -1,7 +1,8 @@
-"""ctypes binding of ``libhf_convrot.so`` (the C ABI of include/hf_convrot.h) and the build recipe that makes it.
+"""ctypes binding of ``libhf_convrot.so`` and ``libhf_block.so`` (the C ABIs of include/hf_convrot.h and
+include/hf_block.h) and the build recipe that makes them.
 
-The library is built in-tree by ``build_library()`` (hipcc, gfx950) and loaded from next to this file. There is no
-fallback: when the library is missing or does not load, ``library()`` raises.
+Each library is built in-tree by ``build_library()`` (hipcc, gfx950) and loaded from next to this file. There is no
+fallback: when one is missing or does not load, ``library()`` or ``block_library()`` raises.
 """
 
 from __future__ import annotations
@@ -9,12 +10,16 @@ from __future__ import annotations
 import ctypes
 import os
 import subprocess
+from concurrent.futures import ThreadPoolExecutor
 from functools import lru_cache
 
 PACKAGE_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PACKAGE_DIR)
 LIB_PATH = os.path.join(PACKAGE_DIR, "libhf_convrot.so")
 SOURCE = os.path.join(PACKAGE_DIR, "csrc", "convrot_abi.hip")
+#: The operators around the INT8 linears of an attention block (include/hf_block.h), a library of their own.
+BLOCK_LIB_PATH = os.path.join(PACKAGE_DIR, "libhf_block.so")
+BLOCK_SOURCE = os.path.join(PACKAGE_DIR, "csrc", "block_abi.hip")
 #: The benchmark's calibration kernels (matrix-core ceiling), a library of their own outside the C ABI.
 CEILINGS_LIB_PATH = os.path.join(PACKAGE_DIR, "libhf_ceilings.so")
 CEILINGS_SOURCE = os.path.join(PACKAGE_DIR, "csrc", "ceilings.hip")
@@ -72,6 +77,21 @@ SIGNATURES = {
                                    _I32, _P, _P, _I64, _I64, _I64, _I64, _P], ctypes.c_int),
 }
 
+#: Every function include/hf_block.h declares.
+_F = ctypes.c_float
+BLOCK_SIGNATURES = {
+    "hf_qk_norm_rope": ([_P, _I64, _I64, _I32, _P, _I64, _I64, _I32, _P, _I64, _I64, _P, _I64, _I64, _P, _I32, _I64,
+                         _I32, _P, _P, _I32, _I32, _I32, _P, _P, _I32, _F, _I64, _I32, _I32, _P], ctypes.c_int),
+    "hf_attention_plan": ([_P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _I64], ctypes.c_int64),
+    "hf_attention_ws_bytes": ([_P, _I64], ctypes.c_int64),
+    "hf_attention": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _F, _P, _P, _I64, _P, _I64,
+                      _I32, _P], ctypes.c_int),
+    "hf_adapter_plan": ([_P, _P, _I64, _I32, _P, _I64], ctypes.c_int64),
+    "hf_adapter_ws_bytes": ([_P, _I64, _I64, _I64, _I32], ctypes.c_int64),
+    "hf_adapter_add": ([_P, _I64, _P, _I64, _P, _P, _I32, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _I32, _P],
+                       ctypes.c_int),
+}
+
 #: Queries of hf_route.
 ROUTE_UP_ROWS, ROUTE_ROTATE_LOWRANK, ROUTE_STREAM_WEIGHT = 0, 1, 2
 
@@ -93,32 +113,46 @@ def _compile(source: str, target: str, verbose: bool) -> None:
 
 
 def build_library(verbose: bool = False) -> str:
-    """Compile csrc/ into libhf_convrot.so, and the benchmark's libhf_ceilings.so, for gfx950 (always recompiles).
-    Returns the convrot library's path."""
-    _compile(SOURCE, LIB_PATH, verbose)
-    _compile(CEILINGS_SOURCE, CEILINGS_LIB_PATH, verbose)
+    """Compile csrc/ into libhf_convrot.so, libhf_block.so and the benchmark's libhf_ceilings.so, for gfx950 (always
+    recompiles), side by side. Returns the convrot library's path."""
+    with ThreadPoolExecutor(3) as pool:
+        jobs = [pool.submit(_compile, source, target, verbose) for source, target in
+                ((SOURCE, LIB_PATH), (BLOCK_SOURCE, BLOCK_LIB_PATH), (CEILINGS_SOURCE, CEILINGS_LIB_PATH))]
+    for job in jobs:
+        job.result()
     library.cache_clear()
+    block_library.cache_clear()
     ceilings_library.cache_clear()
     return LIB_PATH
+
+
+def _load(path: str, signatures: dict) -> ctypes.CDLL:
+    if not os.path.exists(path):
+        raise RuntimeError(
+            f"{path} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
+            "(hipcc --offload-arch=gfx950)"
+        )
+    try:
+        lib = ctypes.CDLL(path)
+    except OSError as exc:
+        raise RuntimeError(f"cannot load {path}: {exc}") from exc
+    for name, (argtypes, restype) in signatures.items():
+        fn = getattr(lib, name)
+        fn.argtypes = argtypes
+        fn.restype = restype
+    return lib
 
 
 @lru_cache(maxsize=None)
 def library() -> ctypes.CDLL:
     """The loaded library with argument types set. Raises RuntimeError when it is missing or does not load."""
-    if not os.path.exists(LIB_PATH):
-        raise RuntimeError(
-            f"{LIB_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'` "
-            "(hipcc --offload-arch=gfx950)"
-        )
-    try:
-        lib = ctypes.CDLL(LIB_PATH)
-    except OSError as exc:
-        raise RuntimeError(f"cannot load {LIB_PATH}: {exc}") from exc
-    for name, (argtypes, restype) in SIGNATURES.items():
-        fn = getattr(lib, name)
-        fn.argtypes = argtypes
-        fn.restype = restype
-    return lib
+    return _load(LIB_PATH, SIGNATURES)
+
+
+@lru_cache(maxsize=None)
+def block_library() -> ctypes.CDLL:
+    """The attention block's operators, as `library`."""
+    return _load(BLOCK_LIB_PATH, BLOCK_SIGNATURES)
 
 
 @lru_cache(maxsize=None)

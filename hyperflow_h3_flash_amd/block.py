@@ -1,0 +1,459 @@
+"""The operators that an attention block runs around its INT8 linears, on the gfx950 kernels of ``libhf_block.so``:
+
+* `qk_norm_rope` with `RotaryAxes`: the RMS norm of each query and key head and the rotation of its channels by the
+  token's position on one or several axes (time, height, width), in one pass;
+* `packed_attention` with `AttentionPlan`: attention over the sequences of several requests packed one behind the
+  other, full or causal, with grouped heads, from single tokens against a cache to whole clips;
+* `adapter_add` with `AdapterPlan` and `AdapterBank`: low-rank adapters of many requests beside a shared projection;
+* `AttentionBlock`: all of them between an `Int8RotLinear` q/k/v projection and an output projection.
+
+The reference holds these layers in its model library (the blocks its transformer keeps,
+src/hyperflow_h3_flash/transformer.py:339-380, call them between ``to_q``/``to_k``/``to_v`` and ``to_out``); they have
+no counterpart in its own files.
+
+As the linears, they compute host tensors on the CPU (``host_block.py``, the same definitions) and device tensors on the
+kernels, and raise when the library is missing. They are forward only: this framework's layers are frozen, and a call
+that would have to be differentiated is refused. A plan holds what depends on lengths and requests alone (no data), is
+built once on the host and serves every layer and step of that batch, on any stream.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+from collections.abc import Sequence
+
+import torch
+from torch import Tensor, nn
+
+from . import _native, host_block
+from .int8 import _check, _on, _raw_stream, _same_device, _workspace
+
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1}
+_POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+
+
+def _forward_only(what: str, *tensors: Tensor | None) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} is forward only: call it under torch.no_grad(), or on tensors that do not "
+                                   "require a gradient")
+
+
+def _lib(device: torch.device) -> ctypes.CDLL:
+    try:
+        return _native.block_library()
+    except RuntimeError as exc:
+        raise RuntimeError(f"tensors on {device} need the gfx950 HIP library: {exc}") from exc
+
+
+def _dtype_code(what: str, t: Tensor) -> int:
+    code = _DTYPES.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what} takes bfloat16 or float16, got {t.dtype}")
+    return code
+
+
+def _heads(t: Tensor) -> tuple[Tensor, int, int]:
+    """``t`` [tokens, heads, D] with its token and head strides as the kernels take them: channels side by side, 16-byte
+    vectors (a copy where it lies otherwise). The stride of a dimension of one is never used."""
+    rows, heads, d = t.shape
+    token, head, channel = t.stride()
+    if rows <= 1:
+        token = heads * d
+    if heads == 1:
+        head = d
+    if (channel != 1 and d > 1) or token % 8 or head % 8 or t.data_ptr() % 16:
+        t = torch.empty((rows, heads, d), dtype=t.dtype, device=t.device).copy_(t)
+        token, head = heads * d, d
+    return t, token, head
+
+
+def _check_out(out: Tensor, like: Tensor, what: str) -> None:
+    if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
+        raise ValueError(f"{what}: out is {tuple(out.shape)} {out.dtype} on {out.device}, expected "
+                         f"{tuple(like.shape)} {like.dtype} on {like.device}")
+
+
+class _Resident:
+    """A host buffer and its copy on a device, uploaded once. The copy is complete before the constructor returns, so any
+    stream may read it; `on` keeps its memory from being given out again while another stream than its own reads it."""
+
+    def __init__(self, host: Tensor, device: torch.device) -> None:
+        self.host = host
+        self.device_copy = host.to(device)
+        self._stream = _raw_stream(self.device_copy.get_device())
+
+    def on(self, stream: int) -> int:
+        if stream != self._stream:
+            self.device_copy.record_stream(torch.cuda.current_stream(self.device_copy.device))
+        return self.device_copy.data_ptr()
+
+
+# ------------------------------------------------------------------------------------------------- norms and rotation
+
+class RotaryAxes:
+    """The rotation of channel pairs by positions on one or several axes.
+
+    ``dims`` gives each axis its channels (each even, their sum a multiple of 16): axis a with n channels turns n / 2
+    pairs by ``position[a] * theta ** (-2 i / n)``, i = 0 .. n / 2 - 1, the axes' pairs one behind the other.
+    ``interleaved`` pairs channels (2p, 2p + 1), otherwise (p, p + sum(dims) / 2). Channels after ``sum(dims)`` are not
+    turned. ``device`` uploads the tables at once (otherwise the first call on a device does)."""
+
+    def __init__(self, dims: Sequence[int], *, theta: float = 10000.0, interleaved: bool = True,
+                 device: torch.device | str | None = None) -> None:
+        dims = tuple(int(n) for n in dims)
+        if not dims or any(n <= 0 or n % 2 for n in dims) or sum(dims) % 16 or len(dims) > 16:
+            raise ValueError(f"dims must be up to 16 positive even widths whose sum is a multiple of 16, got {dims}")
+        if not (theta > 0 and math.isfinite(theta)):
+            raise ValueError(f"theta must be positive and finite, got {theta}")
+        self.dims, self.theta, self.interleaved = dims, float(theta), bool(interleaved)
+        self.pairs = sum(dims) // 2
+        rates, axis = [], []
+        for a, n in enumerate(dims):
+            rates += [self.theta ** (-2.0 * i / n) for i in range(n // 2)]
+            axis += [a] * (n // 2)
+        #: Angle per position step, and each pair's axis (float64 and int32, on the host).
+        self.rates = torch.tensor(rates, dtype=torch.float64)
+        self.axis = torch.tensor(axis, dtype=torch.int32)
+        self._tables: dict[int, tuple[_Resident, _Resident]] = {}
+        if device is not None and torch.device(device).type == "cuda":
+            self.tables(torch.empty(0, device=device).device)
+
+    def tables(self, device: torch.device) -> tuple[_Resident, _Resident]:
+        """(revolutions per position step, axis of each pair) on ``device``."""
+        found = self._tables.get(device.index)
+        if found is None:
+            with _on(device):
+                found = (_Resident(self.rates / (2 * math.pi), device), _Resident(self.axis, device))
+            self._tables[device.index] = found
+        return found
+
+
+def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: RotaryAxes | None, *,
+                 q_weight: Tensor | None = None, k_weight: Tensor | None = None, norm: bool = True, eps: float = 1e-6,
+                 out: tuple[Tensor, Tensor | None] | None = None) -> tuple[Tensor, Tensor | None]:
+    """Norm each head of ``q`` [T, Hq, D] and ``k`` [T, Hk, D] (or None) and rotate its channels by the token's position.
+
+    ``x / sqrt(mean(x ** 2) + eps) * weight`` over the head's channels (``norm=False``: as it is; a weight of None is
+    one; weights [D] in the inputs' type or float32), then the rotation of ``rotary`` (None: none) at ``positions``
+    [T, axes] (or [T] for one axis; int32, int64 or float32). Computed in float32, rounded once to the inputs' type
+    (bfloat16 or float16). q and k may be views with any token and head strides, such as slices of a fused projection.
+    ``out`` may name the results' tensors, the inputs themselves among them. D is a multiple of 16, up to 256."""
+    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
+        raise ValueError("qk_norm_rope expects q [T, Hq, D] and k [T, Hk, D]")
+    T, hq, D = q.shape
+    hk = 0 if k is None else k.shape[1]
+    if k is not None and k.dtype != q.dtype:
+        raise ValueError(f"q and k differ in type: {q.dtype}, {k.dtype}")
+    if D % 16 or D == 0 or D > 256:
+        raise ValueError(f"the head's width must be a multiple of 16 up to 256, got {D}")
+    if rotary is not None:
+        if 2 * rotary.pairs > D:
+            raise ValueError(f"{2 * rotary.pairs} rotated channels exceed the head's {D}")
+        axes = len(rotary.dims)
+        if positions is None or positions.dtype not in _POSITIONS:
+            raise ValueError("positions must be an int32, int64 or float32 tensor")
+        if positions.dim() == 1 and axes == 1:
+            positions = positions[:, None]
+        if positions.shape != (T, axes):
+            raise ValueError(f"positions must be [{T}, {axes}], got {tuple(positions.shape)}")
+    else:
+        positions = None
+    for w in (q_weight, k_weight):
+        if w is not None and (not norm or w.shape != (D,)):
+            raise ValueError(f"a weight must be [{D}] and needs norm=True")
+    if not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps}")
+    if out is not None:
+        _check_out(out[0], q, "qk_norm_rope")
+        if k is not None:
+            _check_out(out[1], k, "qk_norm_rope")
+    _same_device(q.device, k, positions, q_weight, k_weight)
+    _forward_only("qk_norm_rope", q, k, q_weight, k_weight)
+    code = _dtype_code("qk_norm_rope", q)
+    if not q.is_cuda:
+        result = host_block.qk_norm_rope(q, k, positions, rotary, q_weight, k_weight, norm, eps)
+        if out is None:
+            return result
+        out[0].copy_(result[0])
+        if k is not None:
+            out[1].copy_(result[1])
+        return out
+
+    lib = _lib(q.device)
+    if norm:
+        weights = [w for w in (q_weight, k_weight) if w is not None]
+        if any(w.dtype != q.dtype for w in weights):  # float32 is read as it is, and serves any mixture
+            q_weight, k_weight = (None if w is None else w.to(torch.float32) for w in (q_weight, k_weight))
+        q_weight, k_weight = (None if w is None else w if w.is_contiguous() and w.data_ptr() % 16 == 0
+                              else w.clone(memory_format=torch.contiguous_format) for w in (q_weight, k_weight))
+    wide = any(w is not None and w.dtype == torch.float32 for w in (q_weight, k_weight))
+    q, qt, qh = _heads(q)
+    if out is None:
+        qo, qot, qoh = torch.empty((T, hq, D), dtype=q.dtype, device=q.device), hq * D, D
+    else:
+        qo, qot, qoh = _heads(out[0])
+    ko, kt, kh, kot, koh = None, 0, 0, 0, 0
+    if k is not None:
+        k, kt, kh = _heads(k)
+        if out is None:
+            ko, kot, koh = torch.empty((T, hk, D), dtype=q.dtype, device=q.device), hk * D, D
+        else:
+            ko, kot, koh = _heads(out[1])
+    device = q.device
+    stream = _raw_stream(device.index)
+    pos_ptr = turns = axis = None
+    pos_type = ld = axes = pairs = 0
+    if rotary is not None:
+        axes, pairs = len(rotary.dims), rotary.pairs
+        if positions.stride(1) != 1 and axes > 1 or positions.stride(0) < axes:
+            positions = positions.contiguous()
+        pos_ptr, pos_type = positions.data_ptr(), _POSITIONS[positions.dtype]
+        ld = positions.stride(0) if T > 1 else axes
+        t, x = rotary.tables(device)
+        turns, axis = t.on(stream), x.on(stream)
+    with _on(device):
+        status = lib.hf_qk_norm_rope(
+            q.data_ptr(), qt, qh, hq, None if k is None else k.data_ptr(), kt, kh, hk, qo.data_ptr(), qot, qoh,
+            None if ko is None else ko.data_ptr(), kot, koh, pos_ptr, pos_type, ld, axes, turns, axis, pairs,
+            rotary is not None and rotary.interleaved, norm, None if q_weight is None else q_weight.data_ptr(),
+            None if k_weight is None else k_weight.data_ptr(), wide, eps, T, D, code, stream)
+    _check(status, "hf_qk_norm_rope")
+    if out is None:
+        return qo, ko
+    if qo is not out[0]:
+        out[0].copy_(qo)
+    if ko is not None and ko is not out[1]:
+        out[1].copy_(ko)
+    return out
+
+
+# ---------------------------------------------------------------------------------------------------------- attention
+
+class _Plan:
+    """A planner's result on the host, with its copy on the device when that is not the host."""
+
+    def _fill(self, name: str, lib: ctypes.CDLL, device: torch.device, *args) -> None:
+        plan = getattr(lib, name)
+        size = plan(*args, None, 0)
+        _check(min(size, 0), name)
+        host = torch.zeros(size, dtype=torch.uint8)
+        size = plan(*args, host.data_ptr(), size)
+        _check(min(size, 0), name)
+        with _on(device):
+            self.data = _Resident(host, device)
+        self.bytes = size
+        self._host = host.data_ptr()
+
+
+def _plan_device(device: torch.device | str) -> torch.device:
+    device = torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    return device
+
+
+def _lengths(values: Sequence[int], what: str) -> list[int]:
+    lengths = [int(v) for v in values]
+    if any(v < 0 for v in lengths):
+        raise ValueError(f"{what} must not be negative")
+    return lengths
+
+
+def _array(ctype, values: Sequence[int]):
+    return (ctype * max(len(values), 1))(*values)
+
+
+class AttentionPlan(_Plan):
+    """The work of attention over sequences packed one behind the other, for `packed_attention`.
+
+    Sequence b has ``q_lengths[b]`` queries and ``kv_lengths[b]`` keys (the same when None); ``heads`` query heads share
+    ``kv_heads`` key heads in equal groups. ``causal``: query i sees the keys up to i + kv_length - q_length (the last
+    query sees all: a prompt, a prompt's last part, or one new token). Built from lengths on the host, once for all
+    layers and steps of a batch."""
+
+    def __init__(self, q_lengths: Sequence[int], kv_lengths: Sequence[int] | None = None, *, heads: int,
+                 kv_heads: int | None = None, head_dim: int, causal: bool = False,
+                 device: torch.device | str = "cuda") -> None:
+        self.q_lengths = _lengths(q_lengths, "q_lengths")
+        self.kv_lengths = self.q_lengths if kv_lengths is None else _lengths(kv_lengths, "kv_lengths")
+        if len(self.q_lengths) != len(self.kv_lengths):
+            raise ValueError(f"{len(self.q_lengths)} query lengths and {len(self.kv_lengths)} key lengths")
+        self.heads, self.kv_heads = int(heads), int(heads if kv_heads is None else kv_heads)
+        if self.heads < 1 or self.kv_heads < 1 or self.heads % self.kv_heads:
+            raise ValueError(f"{self.heads} heads cannot share {self.kv_heads} key heads equally")
+        self.head_dim, self.causal = int(head_dim), bool(causal)
+        if self.head_dim < 16 or self.head_dim % 16 or self.head_dim > 128:
+            raise ValueError(f"head_dim must be a multiple of 16 up to 128, got {head_dim}")
+        self.q_rows, self.kv_rows = sum(self.q_lengths), sum(self.kv_lengths)
+        self.device = _plan_device(device)
+        if self.device.type != "cuda":
+            return
+        lib = _lib(self.device)
+        q, kv = _array(ctypes.c_int64, self.q_lengths), _array(ctypes.c_int64, self.kv_lengths)
+        cus = torch.cuda.get_device_properties(self.device).multi_processor_count
+        self._fill("hf_attention_plan", lib, self.device, ctypes.addressof(q), ctypes.addressof(kv),
+                   len(self.q_lengths), self.heads, self.kv_heads, self.head_dim, self.causal, cus)
+        self.ws_bytes = lib.hf_attention_ws_bytes(self._host, self.bytes)
+
+
+def _keys(t: Tensor) -> tuple[Tensor, int, int]:
+    """`_heads` for keys and values, whose rows may not overlap nor lie 2^23 elements apart or more."""
+    t, token, head = _heads(t)
+    if t.shape[0] > 1 and not t.shape[2] <= token < 1 << 23:
+        t = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+        token, head = t.shape[1] * t.shape[2], t.shape[2]
+    return t, token, head
+
+
+def packed_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, *, scale: float | None = None,
+                     out: Tensor | None = None) -> Tensor:
+    """Attention of packed sequences: ``softmax(scale q k^T) v`` within each sequence of ``plan``.
+
+    ``q`` [sum q_lengths, heads, head_dim], ``k`` and ``v`` [sum kv_lengths, kv_heads, head_dim], bfloat16 or float16,
+    any token and head strides (slices of a fused projection or a cache); the result is like q. ``scale`` (default
+    ``head_dim ** -0.5``) is positive. A query that sees no key gets zeros; what k and v hold at keys that a query does
+    not see never reaches it. Scores, weights' sums and outputs are summed in float32; the weights enter the second
+    product in the inputs' type."""
+    d = plan.head_dim
+    if q.shape != (plan.q_rows, plan.heads, d) or k.shape != (plan.kv_rows, plan.kv_heads, d) or k.shape != v.shape:
+        raise ValueError(f"the plan is for q ({plan.q_rows}, {plan.heads}, {d}) and k, v ({plan.kv_rows}, "
+                         f"{plan.kv_heads}, {d}); got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise ValueError(f"q, k and v differ in type: {q.dtype}, {k.dtype}, {v.dtype}")
+    code = _dtype_code("packed_attention", q)
+    scale = d ** -0.5 if scale is None else float(scale)
+    if not (scale > 0 and math.isfinite(scale)):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if out is not None:
+        _check_out(out, q, "packed_attention")
+    _same_device(q.device, k, v)
+    if q.device != plan.device:
+        raise ValueError(f"tensors on {q.device}, the plan is for {plan.device}")
+    _forward_only("packed_attention", q, k, v)
+    if not q.is_cuda:
+        result = host_block.packed_attention(q, k, v, plan, scale)
+        return result if out is None else out.copy_(result)
+    lib = _lib(q.device)
+    q, qt, qh = _heads(q)
+    k, kt, kh = _keys(k)
+    v, vt, vh = _keys(v)
+    if out is None:
+        o, ot, oh = torch.empty(q.shape, dtype=q.dtype, device=q.device), plan.heads * d, d
+    else:
+        o, ot, oh = _heads(out)
+    stream = _raw_stream(q.get_device())
+    with _on(q.device):
+        ws, nbytes = _workspace(q.device, plan.ws_bytes)
+        status = lib.hf_attention(q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, o.data_ptr(), ot,
+                                  oh, scale, plan._host, plan.data.on(stream), plan.bytes,
+                                  None if ws is None else ws.data_ptr(), nbytes, code, stream)
+    _check(status, "hf_attention")
+    return o if out is None or o is out else out.copy_(o)
+
+
+# ----------------------------------------------------------------------------------------------------------- adapters
+
+class AdapterPlan(_Plan):
+    """Which adapter each row of a packed batch takes, for `adapter_add`: ``ids[i]`` (-1: none) for the ``lengths[i]``
+    rows of request i (None: one row each), the requests one behind the other, out of ``adapters``. Built on the host,
+    once for all projections of the batch."""
+
+    def __init__(self, ids: Sequence[int], lengths: Sequence[int] | None = None, *, adapters: int,
+                 device: torch.device | str = "cuda") -> None:
+        self.ids = [int(i) for i in ids]
+        self.lengths = [1] * len(self.ids) if lengths is None else _lengths(lengths, "lengths")
+        if len(self.ids) != len(self.lengths):
+            raise ValueError(f"{len(self.ids)} requests and {len(self.lengths)} lengths")
+        self.adapters = int(adapters)
+        if any(not -1 <= i < self.adapters for i in self.ids):
+            raise ValueError(f"adapters must be -1 .. {self.adapters - 1}, got {sorted(set(self.ids))}")
+        self.rows = sum(self.lengths)
+        self.device = _plan_device(device)
+        self._ws: dict[tuple[int, int, int], int] = {}
+        if self.device.type != "cuda":
+            return
+        ids_c, lens_c = _array(ctypes.c_int32, self.ids), _array(ctypes.c_int64, self.lengths)
+        self._fill("hf_adapter_plan", _lib(self.device), self.device, ctypes.addressof(ids_c),
+                   ctypes.addressof(lens_c), len(self.ids), self.adapters)
+
+    def _ws_bytes(self, lib: ctypes.CDLL, K: int, N: int, r: int) -> int:
+        key = (K, N, r)
+        found = self._ws.get(key)
+        if found is None:
+            found = lib.hf_adapter_ws_bytes(self._host, self.bytes, K, N, r)
+            _check(min(found, 0), "hf_adapter_ws_bytes")
+            self._ws[key] = found
+        return found
+
+
+def _rows16(t: Tensor) -> Tensor:
+    """``t`` [rows, columns] with columns side by side, row strides in whole 16-byte vectors and such a start."""
+    if (t.stride(1) == 1 or t.shape[1] == 1) and t.data_ptr() % 16 == 0 and (
+            t.shape[0] <= 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1])):
+        return t
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+
+
+def _rows2(t: Tensor) -> Tensor:
+    if (t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
+        return t
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+
+
+def _ld(t: Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else -(-t.shape[1] // 8) * 8
+
+
+def adapter_add(y: Tensor, x: Tensor, down: Tensor, up: Tensor, plan: AdapterPlan, *, scale: Tensor | None = None,
+                out: Tensor | None = None) -> Tensor:
+    """``y[m] + scale[a] * (x[m] @ down[a]^T) @ up[a]^T`` for the adapter a of each row (``plan``), ``y[m]`` where it has
+    none: the low-rank adapters of many requests beside the projection that gave ``y``.
+
+    ``x`` [M, K], ``y`` [M, N], ``down`` [adapters, r, K], ``up`` [adapters, N, r] in one type (bfloat16 or float16),
+    ``scale`` float32 [adapters] (None: ones). Summed in float32, rounded once. ``out`` may be ``y``, which is then
+    updated in place. K is a multiple of 8, r of 8 up to 512."""
+    if x.dim() != 2 or y.dim() != 2 or x.shape[0] != plan.rows or y.shape[0] != plan.rows:
+        raise ValueError(f"the plan has {plan.rows} rows; got x {tuple(x.shape)}, y {tuple(y.shape)}")
+    K, N = x.shape[1], y.shape[1]
+    if down.dim() != 3 or down.shape[0] != plan.adapters or down.shape[2] != K:
+        raise ValueError(f"down must be [{plan.adapters}, r, {K}], got {tuple(down.shape)}")
+    r = down.shape[1]
+    if up.shape != (plan.adapters, N, r):
+        raise ValueError(f"up must be [{plan.adapters}, {N}, {r}], got {tuple(up.shape)}")
+    if K % 8 or K == 0 or r % 8 or not 0 < r <= 512:
+        raise ValueError(f"K must be a multiple of 8 and r one up to 512, got K={K}, r={r}")
+    if any(t.dtype != y.dtype for t in (x, down, up)):
+        raise ValueError(f"y, x, down and up differ in type: {y.dtype}, {x.dtype}, {down.dtype}, {up.dtype}")
+    if scale is not None and (scale.shape != (plan.adapters,) or scale.dtype != torch.float32):
+        raise ValueError(f"scale must be float32 [{plan.adapters}]")
+    if out is not None:
+        _check_out(out, y, "adapter_add")
+    code = _dtype_code("adapter_add", y)
+    _same_device(y.device, x, down, up, scale)
+    if y.device != plan.device:
+        raise ValueError(f"tensors on {y.device}, the plan is for {plan.device}")
+    _forward_only("adapter_add", y, x, down, up, scale)
+    if not y.is_cuda:
+        result = host_block.adapter_add(y, x, down, up, plan, scale)
+        return result if out is None else out.copy_(result)
+    lib = _lib(y.device)
+    nbytes = plan._ws_bytes(lib, K, N, r) if N else 0
+    in_place = out is y
+    x, y = _rows16(x), _rows2(y)
+    down, up = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+                for t in (down, up))
+    if scale is not None and not scale.is_contiguous():
+        scale = scale.contiguous()
+    o = y if in_place else torch.empty(y.shape, dtype=y.dtype, device=y.device) if out is None else _rows2(out)
+    stream = _raw_stream(y.get_device())
+    with _on(y.device):
+        ws, nbytes = _workspace(y.device, nbytes)
+        status = lib.hf_adapter_add(x.data_ptr(), _ld(x), y.data_ptr(), _ld(y), down.data_ptr(), up.data_ptr(), r,
+                                    None if scale is None else scale.data_ptr(), o.data_ptr(), _ld(o), N, K,
+                                    plan._host, plan.data.on(stream), plan.bytes,
+                                    None if ws is None else ws.data_ptr(), nbytes, code, stream)
+    _check(status, "hf_adapter_add")
+    return o if out is None or o is out else out.copy_(o)
