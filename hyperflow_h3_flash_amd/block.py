@@ -376,8 +376,9 @@ class AdapterPlan(_Plan):
         if self.device.type != "cuda":
             return
         ids_c, lens_c = _array(ctypes.c_int32, self.ids), _array(ctypes.c_int64, self.lengths)
+        cus = torch.cuda.get_device_properties(self.device).multi_processor_count
         self._fill("hf_adapter_plan", _lib(self.device), self.device, ctypes.addressof(ids_c),
-                   ctypes.addressof(lens_c), len(self.ids), self.adapters)
+                   ctypes.addressof(lens_c), len(self.ids), self.adapters, cus)
 
     def _ws_bytes(self, lib: ctypes.CDLL, K: int, N: int, r: int) -> int:
         key = (K, N, r)
@@ -440,7 +441,6 @@ def adapter_add(y: Tensor, x: Tensor, down: Tensor, up: Tensor, plan: AdapterPla
         result = host_block.adapter_add(y, x, down, up, plan, scale)
         return result if out is None else out.copy_(result)
     lib = _lib(y.device)
-    nbytes = plan._ws_bytes(lib, K, N, r) if N else 0
     in_place = out is y
     x, y = _rows16(x), _rows2(y)
     down, up = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
@@ -450,7 +450,7 @@ def adapter_add(y: Tensor, x: Tensor, down: Tensor, up: Tensor, plan: AdapterPla
     o = y if in_place else torch.empty(y.shape, dtype=y.dtype, device=y.device) if out is None else _rows2(out)
     stream = _raw_stream(y.get_device())
     with _on(y.device):
-        ws, nbytes = _workspace(y.device, nbytes)
+        ws, nbytes = _workspace(y.device, plan._ws_bytes(lib, K, N, r) if N else 0)
         status = lib.hf_adapter_add(x.data_ptr(), _ld(x), y.data_ptr(), _ld(y), down.data_ptr(), up.data_ptr(), r,
                                     None if scale is None else scale.data_ptr(), o.data_ptr(), _ld(o), N, K,
                                     plan._host, plan.data.on(stream), plan.bytes,

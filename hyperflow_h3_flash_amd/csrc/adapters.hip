@@ -3,22 +3,23 @@
 //
 // HBM-bound with many rows (x once, y once, out once; the adapters' weights stay in the L2s), latency-bound with few.
 //
-// The plan holds the rows sorted by adapter and cut into tiles of at most 64 rows of one adapter, so requests in any
-// order and rows of one adapter that lie apart share a tile; rows are read and written where they lie.
-//   adapter_down_kernel  u = x A^T, fp32: a workgroup a tile and a share of K, its four waves on every fourth 64 k.
-//   adapter_up_kernel    out = y + scale (u B^T): a workgroup a tile and a range of columns.
-// u goes through a fp32 workspace, one plane per share of K (joined in a fixed order, no atomics). For the second
-// product each u is split into a leading and a trailing 16-bit value (x A^T is not rounded to 16 bits: the doubled
-// rank costs nothing where memory is the bound), after a power-of-two scale of its row that keeps fp16 in range.
+// The plan holds the rows sorted by adapter and cut into tiles of 32 or 64 rows of one adapter, so requests in any order
+// and rows of one adapter that lie apart share a tile; rows are read and written where they lie.
+//   adapter_down_kernel  u = x A^T in fp32: a workgroup a tile, its waves on every NW-th step of 64 k.
+//   adapter_join_kernel  only where few tiles over a deep K are cut along K, or the rank is over 128: adds the shares.
+//   adapter_up_kernel    out = y + scale (u B^T): a workgroup 32 rows of a tile and a range of columns.
+// No atomics: every sum has a fixed order.
+//
+// u is handed on as two 16-bit values, a leading and a trailing one, in the operand order of the second product (x A^T is
+// not rounded to 16 bits: the doubled rank costs nothing where memory is the bound), after a power-of-two scale of its
+// row that keeps fp16 in range.
 #pragma once
 
 #include "block_types.h"
 
 namespace hf {
 
-constexpr int kAdThreads = 256;
-constexpr int kAdRows = 64;  // rows of a tile
-constexpr int kAdChunk = 64;  // K of one step
+constexpr int kAdChunk = 64;  // k of one step
 
 struct AdapterTile {
   int32_t adapter, start, count, pad;
@@ -28,244 +29,358 @@ struct AdapterArgs {
   const uint16_t *x, *y, *down, *up;
   const float* scale;
   uint16_t* out;
-  float* u;  // [splits][rows][r32]
+  v4u* frags;       // [tiles][r32 / 16][row blocks][leading, trailing][64]
+  float* factors;   // [tiles][tile rows]
+  float* planes;    // [splits][tiles][tile rows][r32], where the sums are joined
   const AdapterTile* tiles;
   const int32_t* rows;
-  int64_t ldx, ldy, ldo, K, N, n_rows;
-  int r, r32, splits, chunks_per_split, blocks_per_wg, in_place;
+  int64_t ldx, ldy, ldo, K, N;
+  int live_tiles, tile_rows, r, r32, splits, blocks_per_wg, col_groups, in_place, stream_y;
 };
 
-// RB rank blocks of 32 from blockIdx.z * 32 RB on, rows blockIdx.x's tile, K share blockIdx.y.
-template <class T, int RB>
-__global__ __launch_bounds__(kAdThreads) void adapter_down_kernel(AdapterArgs a) {
-  __shared__ v4f part[4][4][64];  // one 32 x 32 block of each wave
-  const AdapterTile tile = a.tiles[blockIdx.x];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, sub = lane & 31, half = lane >> 5;
-  const int rank0 = blockIdx.z * 32 * RB;
-  const bool two = tile.count > 32;
-  const uint16_t* xr[2];
+// Row `row` of a tile's u, fp32 in LDS at p, into operand order with its factor: four neighbouring lanes a row, `part`
+// of 0 to 3.
+template <class T>
+__device__ __forceinline__ void adapter_operands(const AdapterArgs& a, const AdapterTile& tile, int tile_index,
+                                                 const float* p, int row, int part, int blocks) {
+  float most = 0.0f;
+  for (int j = part; j < a.r32 / 8; j += 4)
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    const int i = min(n * 32 + sub, tile.count - 1);  // a row past the tile repeats its last one: not stored
-    xr[n] = a.x + (int64_t)a.rows[tile.start + i] * a.ldx + 32 * half;
-  }
-  const uint16_t* dr[RB];
+    for (int e = 0; e < 8; ++e)
+      if (8 * j + e < a.r) most = fmaxf(most, fabsf(p[8 * j + e]));
+  most = fmaxf(most, __shfl_xor(most, 1, 64));
+  most = fmaxf(most, __shfl_xor(most, 2, 64));
+  // 2^(6 - exponent): the row's largest lands in [2^6, 2^7), where fp16 holds it and its trailing part is normal. Rows
+  // of infinities and of values near the ends of fp32 stay as they are.
+  const bool fine = most >= 0x1p-100f && most <= 0x1p100f;
+  const float grow = fine ? __uint_as_float((260u - (__float_as_uint(most) >> 23)) << 23) : 1.0f;
+  const float scale = a.scale ? a.scale[tile.adapter] : 1.0f;
+  if (part == 0) a.factors[(int64_t)tile_index * a.tile_rows + row] = scale / grow;  // exact: a power of two
+  v4u* frags = a.frags + (int64_t)tile_index * (a.r32 / 16) * blocks * 128;
+  for (int j = part; j < a.r32 / 8; j += 4) {
+    v4u lead, trail;
 #pragma unroll
-  for (int b = 0; b < RB; ++b) {
-    const int j = min(rank0 + 32 * b + sub, a.r - 1);  // likewise
-    dr[b] = a.down + ((int64_t)tile.adapter * a.r + j) * a.K + 32 * half;
-  }
-  v16f acc[RB][2];
-#pragma unroll
-  for (int b = 0; b < RB; ++b) acc[b][0] = acc[b][1] = (v16f){0};
-  const int64_t chunks = (a.K + kAdChunk - 1) / kAdChunk;
-  const int64_t c_lo = (int64_t)blockIdx.y * a.chunks_per_split;
-  const int64_t c_hi = min(c_lo + a.chunks_per_split, chunks);
-  const v4u zero = {0, 0, 0, 0};
-  // Lane half h holds k 32h .. 32h + 31 of the chunk in both operands: 64 contiguous bytes a lane, a whole line a row.
-  for (int64_t c = c_lo + wave; c < c_hi; c += 4) {
-    const int64_t k0 = c * kAdChunk;
-    v4u xv[2][4], dv[RB][4];
-    if (k0 + kAdChunk <= a.K) {
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        xv[0][s] = *(const v4u*)(xr[0] + k0 + 8 * s);
-        xv[1][s] = two ? *(const v4u*)(xr[1] + k0 + 8 * s) : zero;
-      }
-#pragma unroll
-      for (int b = 0; b < RB; ++b)
-#pragma unroll
-        for (int s = 0; s < 4; ++s) dv[b][s] = *(const v4u*)(dr[b] + k0 + 8 * s);
-    } else {
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const bool in = k0 + 32 * half + 8 * s < a.K;
-        xv[0][s] = in ? *(const v4u*)(xr[0] + k0 + 8 * s) : zero;
-        xv[1][s] = in && two ? *(const v4u*)(xr[1] + k0 + 8 * s) : zero;
-#pragma unroll
-        for (int b = 0; b < RB; ++b) dv[b][s] = in ? *(const v4u*)(dr[b] + k0 + 8 * s) : zero;
-      }
+    for (int e = 0; e < 4; ++e) {
+      const int rank = 8 * j + 2 * e;
+      const float v = rank < a.r ? p[rank] * grow : 0.0f, w = rank + 1 < a.r ? p[rank + 1] * grow : 0.0f;
+      lead[e] = T::pack(v, w);
+      const float v1 = T::lo(lead[e]), w1 = T::hi(lead[e]);
+      // An infinity or NaN has no trailing part.
+      trail[e] = T::pack(fabsf(v1) < __builtin_inff() ? v - v1 : 0.0f, fabsf(w1) < __builtin_inff() ? w - w1 : 0.0f);
     }
+    v4u* to = frags + ((j >> 1) * blocks + (row >> 5)) * 128 + (j & 1) * 32 + (row & 31);
+    to[0] = lead;
+    to[64] = trail;
+  }
+}
+
+// Stages of a wave's ring and bytes of one: RB rank blocks and NB row blocks of 32 rows x 64 k.
+__host__ __device__ constexpr int ad_stage_bytes(int rb, int nb) { return 4096 * (rb + nb); }
+__host__ __device__ constexpr int ad_stages(int rb, int nb, int nw) {
+  return 147456 / (ad_stage_bytes(rb, nb) * nw) < 4 ? 147456 / (ad_stage_bytes(rb, nb) * nw) : 4;
+}
+__host__ __device__ constexpr int ad_down_lds(int rb, int nb, int nw) {
+  return ad_stages(rb, nb, nw) * ad_stage_bytes(rb, nb) * nw;
+}
+
+// Tile blockIdx.x, K share blockIdx.y, ranks from 32 RB blockIdx.z on.
+//
+// Each wave streams its own steps of 64 k through a ring of its own in LDS (16 bytes a lane, whole 128-byte lines, past
+// the registers), so the loop has no barrier; the waves' sums are added at the end. Rows lie 128 bytes apart in LDS,
+// swizzled so that fragment reads are conflict-free.
+template <class T, int RB, int NB, int NW>
+__global__ __launch_bounds__(64 * NW, 1) void adapter_down_kernel(AdapterArgs a) {
+  constexpr int S = ad_stages(RB, NB, NW), kStage = ad_stage_bytes(RB, NB), kLoads = 4 * (RB + NB);
+  static_assert(S >= 2, "the next step is loaded while one is computed");
+  extern __shared__ __attribute__((aligned(1024))) unsigned char ad_lds[];
+  const AdapterTile tile = a.tiles[blockIdx.x];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int sub = lane & 31, half = lane >> 5;
+  const int rank0 = blockIdx.z * 32 * RB;
+  unsigned char HF_LDS* ring = (unsigned char HF_LDS*)ad_lds + wave * S * kStage;
+
+  // Load i of a step fills rows 8i .. 8i + 7 of the step's NB x 32 rows of x and RB x 32 of A; lane l row l / 8, from
+  // chunk swizzle128(row, l % 8). Rows past the tile or the rank repeat the last one; what comes of them is not used.
+  const uint16_t* from[kLoads];
 #pragma unroll
-    for (int s = 0; s < 4; ++s)
+  for (int i = 0; i < kLoads; ++i) {
+    const int r = 8 * i + (lane >> 3), c = swizzle128(r & 31, lane & 7);
+    from[i] = i < 4 * NB ? a.x + (int64_t)a.rows[tile.start + min(r, tile.count - 1)] * a.ldx + 8 * c
+                         : a.down + ((int64_t)tile.adapter * a.r + min(rank0 + r - 32 * NB, a.r - 1)) * a.K + 8 * c;
+  }
+  const int64_t full = a.K / kAdChunk;  // whole steps; what is left of K comes after the loop
+  const int64_t share = (full + a.splits - 1) / a.splits;
+  const int64_t c_lo = min(share * blockIdx.y, full), c_hi = min(c_lo + share, full);
+  const int steps = c_hi - c_lo > wave ? (int)((c_hi - c_lo - wave + NW - 1) / NW) : 0;
+  auto load = [&](int step, int slot) {
+    const int64_t k0 = (c_lo + wave + (int64_t)step * NW) * kAdChunk;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      __builtin_amdgcn_global_load_lds((const void __attribute__((address_space(1)))*)(from[i] + k0),
+                                       (void HF_LDS*)(ring + slot * kStage + i * 1024), 16, 0, 0);
+  };
+
+  v16f acc[RB][NB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b)
+#pragma unroll
+    for (int n = 0; n < NB; ++n) acc[b][n] = (v16f){0};
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+    if (s < steps) load(s, s);
+  int slot = 0;
+#pragma unroll 1
+  for (int step = 0; step < steps; ++step) {
+    // The step's loads have landed; those of the S - 1 steps after it may be on their way.
+    constexpr int kAhead = (S - 1) * kLoads;
+    static_assert(kAhead == 8 || kAhead == 12 || kAhead == 16 || kAhead == 20 || kAhead == 24, "a wait for this ring");
+    if (step + S > steps) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    else if constexpr (kAhead == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+    else if constexpr (kAhead == 12) asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
+    else if constexpr (kAhead == 16) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+    else if constexpr (kAhead == 20) asm volatile("s_waitcnt vmcnt(20)" ::: "memory");
+    else asm volatile("s_waitcnt vmcnt(24)" ::: "memory");
+    const unsigned char HF_LDS* at = ring + slot * kStage;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const int chunk = swizzle128(sub, 2 * s + half) * 16 + sub * 128;
+      v4u xf[NB];
+#pragma unroll
+      for (int n = 0; n < NB; ++n) xf[n] = *(const v4u HF_LDS*)(at + n * 4096 + chunk);
 #pragma unroll
       for (int b = 0; b < RB; ++b) {
-        acc[b][0] = T::mfma(dv[b][s], xv[0][s], acc[b][0]);
-        if (two) acc[b][1] = T::mfma(dv[b][s], xv[1][s], acc[b][1]);
+        const v4u df = *(const v4u HF_LDS*)(at + (NB + b) * 4096 + chunk);
+#pragma unroll
+        for (int n = 0; n < NB; ++n) acc[b][n] = T::mfma(df, xf[n], acc[b][n]);
       }
+    }
+    // Every read of the slot has returned: it takes the step S further on. Filled after the products rather than before
+    // them, the whole ring is on its way whenever the wave waits, and latency is what the loop would wait for.
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (step + S < steps) load(step + S, slot);
+    slot = slot + 1 == S ? 0 : slot + 1;
   }
-  // Lane (row sub, half h) of a block holds ranks 8g + 4h + i. The waves' blocks are added in wave order; thread
-  // (g = wave, lane) adds and stores value group g.
-  float* u = a.u + (int64_t)blockIdx.y * a.n_rows * a.r32;
+  if (a.K % kAdChunk && wave == 0 && blockIdx.y + 1 == gridDim.y) {
+    const v4u zero = {0, 0, 0, 0};
+    for (int64_t k0 = full * kAdChunk; k0 < a.K; k0 += 16) {
+      const int64_t k = k0 + 8 * half;
+      v4u xf[NB];
 #pragma unroll
-  for (int b = 0; b < RB; ++b) {
+      for (int n = 0; n < NB; ++n)
+        xf[n] = k < a.K ? *(const v4u*)(a.x + (int64_t)a.rows[tile.start + min(32 * n + sub, tile.count - 1)] * a.ldx + k)
+                        : zero;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      if (n && !two) break;
-      __syncthreads();
+      for (int b = 0; b < RB; ++b) {
+        const v4u df = k < a.K ? *(const v4u*)(a.down + ((int64_t)tile.adapter * a.r +
+                                                         min(rank0 + 32 * b + sub, a.r - 1)) * a.K + k)
+                               : zero;
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        part[wave][g][lane] = (v4f){acc[b][n][4 * g], acc[b][n][4 * g + 1], acc[b][n][4 * g + 2], acc[b][n][4 * g + 3]};
-      __syncthreads();
-      const v4f sum = ((part[0][wave][lane] + part[1][wave][lane]) + part[2][wave][lane]) + part[3][wave][lane];
-      const int i = n * 32 + sub, rank = rank0 + 32 * b + 8 * wave + 4 * half;
-      if (i < tile.count && rank < a.r32) *(v4f*)(u + (int64_t)(tile.start + i) * a.r32 + rank) = sum;
+        for (int n = 0; n < NB; ++n) acc[b][n] = T::mfma(df, xf[n], acc[b][n]);
+      }
     }
   }
-}
 
-// Sum over the K shares of 8 ranks of u.
-__device__ __forceinline__ void adapter_u8(const AdapterArgs& a, int64_t row, int rank, float out[8]) {
-  const float* p = a.u + row * a.r32 + rank;
-  v4f s0 = *(const v4f*)p, s1 = *(const v4f*)(p + 4);
-  for (int i = 1; i < a.splits; ++i) {
-    p += a.n_rows * a.r32;
-    s0 += *(const v4f*)p;
-    s1 += *(const v4f*)(p + 4);
+  // The waves' sums, added in wave order. A lane (row sub, half h) holds ranks 8g + 4h + i of a block.
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  v4f* part = (v4f*)ad_lds;  // [wave][block][g][lane]
+#pragma unroll
+  for (int b = 0; b < RB; ++b)
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+        part[((wave * RB * NB + b * NB + n) * 4 + g) * 64 + lane] =
+            (v4f){acc[b][n][4 * g], acc[b][n][4 * g + 1], acc[b][n][4 * g + 2], acc[b][n][4 * g + 3]};
+  __syncthreads();
+  constexpr int kSums = RB * NB * 256, kPer = (kSums + 64 * NW - 1) / (64 * NW);
+  v4f sums[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int at = tid + i * 64 * NW;
+    if (at < kSums) {
+      sums[i] = part[at];
+#pragma unroll
+      for (int w = 1; w < NW; ++w) sums[i] += part[w * kSums + at];
+    }
+  }
+  const bool join = a.splits > 1 || gridDim.z > 1;
+  float* u = (float*)ad_lds;
+  int pitch = a.r32 + 4;
+  if (join) {
+    u = a.planes + ((int64_t)blockIdx.y * a.live_tiles + blockIdx.x) * a.tile_rows * a.r32;
+    pitch = a.r32;
+  } else {
+    __syncthreads();
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    out[e] = rank + e < a.r ? s0[e] : 0.0f;
-    out[4 + e] = rank + 4 + e < a.r ? s1[e] : 0.0f;
+  for (int i = 0; i < kPer; ++i) {
+    const int at = tid + i * 64 * NW;
+    const int l = at & 63, g = (at >> 6) & 3, n = (at >> 8) % NB, b = (at >> 8) / NB;
+    const int rank = rank0 + 32 * b + 8 * g + 4 * (l >> 5);
+    if (at < kSums && rank < a.r32) *(v4f*)(u + (32 * n + (l & 31)) * pitch + rank) = sums[i];
   }
+  if (join) return;
+  __syncthreads();
+  for (int row = tid >> 2; row < 32 * NB; row += 16 * NW)
+    adapter_operands<T>(a, tile, blockIdx.x, u + row * pitch, row, tid & 3, NB);
 }
 
-// VEC: y and out take 16-byte accesses.
-template <class T, bool VEC>
-__global__ __launch_bounds__(kAdThreads) void adapter_up_kernel(AdapterArgs a) {
-  extern __shared__ v4u ad_lds[];  // u in operand order: [k step][row block][leading, trailing][lane]
-  __shared__ float row_scale[kAdRows];
+// The K shares of a tile's u added in order, then into operand order. 256 threads.
+template <class T>
+__global__ __launch_bounds__(256) void adapter_join_kernel(AdapterArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char ad_lds[];
+  float* u = (float*)ad_lds;
   const AdapterTile tile = a.tiles[blockIdx.x];
+  const int per_row = a.r32 / 4;
+  const int64_t plane = (int64_t)a.live_tiles * a.tile_rows * a.r32;
+  const float* from = a.planes + (int64_t)blockIdx.x * a.tile_rows * a.r32;
+  for (int i = threadIdx.x; i < a.tile_rows * per_row; i += 256) {
+    v4f sum = *(const v4f*)(from + 4 * i);
+    for (int s = 1; s < a.splits; ++s) sum += *(const v4f*)(from + s * plane + 4 * i);
+    *(v4f*)(u + i / per_row * (a.r32 + 4) + i % per_row * 4) = sum;
+  }
+  __syncthreads();
+  for (int row = threadIdx.x >> 2; row < a.tile_rows; row += 64)
+    adapter_operands<T>(a, tile, blockIdx.x, u + row * (a.r32 + 4), row, threadIdx.x & 3, a.tile_rows / 32);
+}
+
+constexpr int kAdUpThreads = 256;
+constexpr int kAdUpPitch = 68;  // floats of a row of 64 columns in LDS: 16-byte accesses of 16 rows meet every bank once
+constexpr int kAdUpStage = 16 * kAdUpPitch * 4;
+
+// Row block blockIdx.x / col_groups (of a tile) and a group of its columns, neighbours in memory side by side in the
+// launch; VEC: y and out take 16-byte accesses.
+//
+// A wave computes 32 rows x 64 columns transposed (the weight is the first operand), turns them in LDS, in fp32, and adds
+// them to y in whole 128-byte lines of a row. y of the next 64 columns is on its way meanwhile. STEPS steps of 16 ranks have
+// their weights in registers at once.
+template <class T, bool VEC, int STEPS>
+__global__ __launch_bounds__(kAdUpThreads, 3) void adapter_up_kernel(AdapterArgs a) {
+  extern __shared__ __attribute__((aligned(1024))) unsigned char ad_lds[];
+  const int blocks = a.tile_rows / 32;
+  const int row_block = blockIdx.x / a.col_groups, group = blockIdx.x - row_block * a.col_groups;
+  const int tile_index = row_block / blocks, block = row_block - tile_index * blocks;
+  const AdapterTile tile = a.tiles[tile_index];
+  const int count = min(tile.count - 32 * block, 32);
+  if (count <= 0 || (tile.adapter < 0 && a.in_place)) return;
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, sub = lane & 31, half = lane >> 5;
   const int64_t n_blocks = (a.N + 63) / 64;
-  const int64_t b_lo = (int64_t)blockIdx.y * a.blocks_per_wg;
+  const int64_t b_lo = (int64_t)group * a.blocks_per_wg;
   const int64_t b_hi = min(b_lo + a.blocks_per_wg, n_blocks);
-  if (tile.adapter < 0) {
-    if (a.in_place) return;
-    const int64_t n0 = b_lo * 64, n1 = min(b_hi * 64, a.N);
-    constexpr int E = VEC ? 8 : 1;
-    const int64_t per_row = (n1 - n0) / E;
-    for (int64_t i = tid; i < per_row * tile.count; i += kAdThreads) {
-      const int64_t row = a.rows[tile.start + i / per_row], n = n0 + i % per_row * E;
+
+  // This lane's rows of y and out: 8i + lane / 8, columns 8 (lane % 8) .. of 64.
+  int64_t at[4];
+  bool live[4];
+  float factor[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = 8 * i + (lane >> 3);
+    live[i] = r < count;
+    at[i] = a.rows[tile.start + 32 * block + min(r, count - 1)];
+    factor[i] = tile.adapter < 0 ? 0.0f : a.factors[(int64_t)tile_index * a.tile_rows + 32 * block + r];
+  }
+  const int col8 = 8 * (lane & 7);
+  auto load_y = [&](int64_t blk, v4u* v) {
+    const int64_t col = blk * 64 + col8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = (v4u){0, 0, 0, 0};
       if (VEC) {
-        *(v4u*)(a.out + row * a.ldo + n) = *(const v4u*)(a.y + row * a.ldy + n);
-      } else {
-        a.out[row * a.ldo + n] = a.y[row * a.ldy + n];
+        if (live[i] && blk < b_hi && col < a.N) {
+          const v4u* from = (const v4u*)(a.y + at[i] * a.ldy + col);
+          v[i] = a.stream_y ? __builtin_nontemporal_load(from) : *from;
+        }
+      } else if (live[i] && blk < b_hi) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (col + e < a.N) v[i][e >> 1] |= (uint32_t)a.y[at[i] * a.ldy + col + e] << (16 * (e & 1));
       }
+    }
+  };
+  auto store = [&](int64_t blk, int i, v4u v) {
+    const int64_t col = blk * 64 + col8;
+    if (VEC) {
+      if (live[i] && col < a.N) store_stream((v4i*)(a.out + at[i] * a.ldo + col), __builtin_bit_cast(v4i, v));
+    } else if (live[i]) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (col + e < a.N) a.out[at[i] * a.ldo + col + e] = (uint16_t)(v[e >> 1] >> (16 * (e & 1)));
+    }
+  };
+  if (tile.adapter < 0) {
+    for (int64_t blk = b_lo + wave; blk < b_hi; blk += 4) {
+      v4u v[4];
+      load_y(blk, v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) store(blk, i, v[i]);
     }
     return;
   }
-  const float scale = a.scale ? a.scale[tile.adapter] : 1.0f;
+  v4u yv[4], yn[4];
+  load_y(b_lo + wave, yn);
   const int steps = a.r32 / 16;
+  v4u* operands = (v4u*)ad_lds;  // [step][leading, trailing][lane]
   {
-    // Thread (row tid / 4, part tid % 4): the row's largest |u|, then its ranks 8 at a time into operand order.
-    const int row = tid >> 2, part = tid & 3;
-    const bool live = row < tile.count;
-    float most = 0.0f;
-    for (int j = part; j < a.r32 / 8; j += 4) {
-      float v[8];
-      if (live) {
-        adapter_u8(a, tile.start + row, 8 * j, v);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(v[e]));
-      }
-    }
-    most = fmaxf(most, __shfl_xor(most, 1, 64));
-    most = fmaxf(most, __shfl_xor(most, 2, 64));
-    // 2^(6 - exponent): the row's largest lands in [2^6, 2^7), where fp16 holds it and its trailing part is normal.
-    const bool fine = most >= 0x1p-100f && most <= 0x1p100f;
-    const float grow = fine ? __uint_as_float((uint32_t)(127 + 6 + 127 - (int)(__float_as_uint(most) >> 23)) << 23) : 1.0f;
-    if (part == 0) row_scale[row] = scale / grow;  // exact up to scale's own rounding: a power of two
-    for (int j = part; j < a.r32 / 8; j += 4) {
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.0f;
-      if (live) adapter_u8(a, tile.start + row, 8 * j, v);
-      v4u lead, trail;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float p = v[2 * e] * grow, q = v[2 * e + 1] * grow;
-        lead[e] = T::pack(p, q);
-        const float p1 = T::lo(lead[e]), q1 = T::hi(lead[e]);
-        // An infinity or NaN has no trailing part.
-        trail[e] = T::pack(fabsf(p1) < __builtin_inff() ? p - p1 : 0.0f, fabsf(q1) < __builtin_inff() ? q - q1 : 0.0f);
-      }
-      v4u* to = ad_lds + ((j >> 1) * 2 + (row >> 5)) * 128 + (j & 1) * 32 + (row & 31);
-      to[0] = lead;
-      to[64] = trail;
-    }
+    const v4u* from = a.frags + (int64_t)tile_index * steps * blocks * 128 + block * 128;
+    for (int i = tid; i < steps * 128; i += kAdUpThreads) operands[i] = from[(int64_t)(i >> 7) * blocks * 128 + (i & 127)];
   }
   __syncthreads();
-  const bool two = tile.count > 32;
-  // Output column of operand row m = 8g + 4h + i of column block b: 64 * block + 32h + 16b + 4g + i, so that a lane
-  // (row sub, half h) ends with 32 neighbouring columns: 64 bytes, and a row's two lanes a whole line.
-  const int col_of_sub = ((sub >> 2) & 1) * 32 + (sub >> 3) * 4 + (sub & 3);
-  int64_t at[2];
-  bool live[2];
-#pragma unroll
-  for (int n = 0; n < 2; ++n) {
-    live[n] = n * 32 + sub < tile.count;
-    at[n] = a.rows[tile.start + min(n * 32 + sub, tile.count - 1)];
-  }
-  const float f[2] = {row_scale[sub], row_scale[32 + sub]};
+  float* turn = (float*)(ad_lds + steps * 2048 + wave * kAdUpStage);
   const uint16_t* up = a.up + (int64_t)tile.adapter * a.N * a.r;
+#pragma unroll 1
   for (int64_t blk = b_lo + wave; blk < b_hi; blk += 4) {
-    const int64_t n0 = blk * 64;
-    const int64_t col = n0 + 32 * half;  // this lane's first output column
-    v4u yv[2][4];
-    if (VEC) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+    for (int i = 0; i < 4; ++i) yv[i] = yn[i];
+    load_y(blk + 4, yn);
+    v16f acc[2];
+    acc[0] = acc[1] = (v16f){0};
+#pragma unroll 1
+    for (int s0 = 0; s0 < steps; s0 += STEPS) {
+      v4u w[STEPS][2];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          yv[n][c] = live[n] && col + 8 * c < a.N ? *(const v4u*)(a.y + at[n] * a.ldy + col + 8 * c) : (v4u){0, 0, 0, 0};
-    }
-    v16f acc[2][2];
+      for (int b = 0; b < 2; ++b) {
+        const uint16_t* row = up + min(blk * 64 + 32 * b + sub, a.N - 1) * a.r + 8 * half + 16 * s0;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) acc[b][0] = acc[b][1] = (v16f){0};
-    const uint16_t* ur[2];
+        for (int s = 0; s < STEPS; ++s)  // r is a multiple of 8: ranks past it are not read
+          w[s][b] = 16 * (s0 + s) + 8 * half < a.r ? *(const v4u*)(row + 16 * s) : (v4u){0, 0, 0, 0};
+      }
 #pragma unroll
-    for (int b = 0; b < 2; ++b) ur[b] = up + min(n0 + 16 * b + col_of_sub, a.N - 1) * a.r + 8 * half;
-    for (int s = 0; s < steps; ++s) {
-      v4u w[2];
-      const bool in = 16 * s + 8 * half < a.r;  // r is a multiple of 8: ranks past it are not read
-#pragma unroll
-      for (int b = 0; b < 2; ++b) w[b] = in ? *(const v4u*)(ur[b] + 16 * s) : (v4u){0, 0, 0, 0};
-#pragma unroll
-      for (int n = 0; n < 2; ++n) {
-        if (n && !two) break;
-        const v4u lead = ad_lds[(s * 2 + n) * 128 + lane], trail = ad_lds[(s * 2 + n) * 128 + 64 + lane];
+      for (int s = 0; s < STEPS; ++s) {
+        if (STEPS > 2 && s0 + s >= steps) break;  // steps is even
+        const v4u lead = operands[(s0 + s) * 128 + lane], trail = operands[(s0 + s) * 128 + 64 + lane];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          acc[b][n] = T::mfma(w[b], lead, acc[b][n]);
-          acc[b][n] = T::mfma(w[b], trail, acc[b][n]);
+          acc[b] = T::mfma(w[s][b], lead, acc[b]);
+          acc[b] = T::mfma(w[s][b], trail, acc[b]);
         }
       }
     }
+    // Lane (row sub, half h) holds columns 32b + 8g + 4h + i; 16 rows at a time go through LDS.
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-      if (!live[n]) continue;
-      if (VEC) {
+    for (int p = 0; p < 2; ++p) {
+      if ((sub >> 4) == p) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          v4u o;
+        for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int v = 8 * (c & 1) + 2 * e;
-            o[e] = T::pack(fmaf(acc[c >> 1][n][v], f[n], T::lo(yv[n][c][e])),
-                           fmaf(acc[c >> 1][n][v + 1], f[n], T::hi(yv[n][c][e])));
-          }
-          if (col + 8 * c < a.N) *(v4u*)(a.out + at[n] * a.ldo + col + 8 * c) = o;
-        }
-      } else {
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const int64_t j = col + c;
-          if (j < a.N)
-            a.out[at[n] * a.ldo + j] =
-                (uint16_t)T::pack(fmaf(acc[c >> 4][n][c & 15], f[n], T::lo(a.y[at[n] * a.ldy + j])), 0.0f);
-        }
+          for (int g = 0; g < 4; ++g)
+            *(v4f*)(turn + (sub & 15) * kAdUpPitch + 32 * b + 8 * g + 4 * half) =
+                (v4f){acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]};
       }
+      wave_lds_sync();
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int i = 2 * p + x;
+        const v4f lo = *(const v4f*)(turn + (8 * x + (lane >> 3)) * kAdUpPitch + col8);
+        const v4f hi = *(const v4f*)(turn + (8 * x + (lane >> 3)) * kAdUpPitch + col8 + 4);
+        v4u o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float d0 = e < 2 ? lo[2 * e] : hi[2 * e - 4], d1 = e < 2 ? lo[2 * e + 1] : hi[2 * e - 3];
+          o[e] = T::pack(fmaf(d0, factor[i], T::lo(yv[i][e])), fmaf(d1, factor[i], T::hi(yv[i][e])));
+        }
+        store(blk, i, o);
+      }
+      wave_lds_sync();
     }
   }
 }

@@ -188,7 +188,8 @@ constexpr int32_t kAdapterMagic = 0x48464144;
 struct AdapterHeader {
   int32_t magic, adapters, tiles, live_tiles;  // the first live_tiles tiles have an adapter
   int64_t bytes, rows, live_rows;
-  int32_t pad[22];
+  int32_t tile_rows;
+  int32_t pad[21];
 };
 static_assert(sizeof(AdapterHeader) == 128, "tiles start on a 128-byte line");
 
@@ -198,56 +199,97 @@ bool adapter_header(const void* plan, int64_t bytes, AdapterHeader* h) {
   return h->magic == kAdapterMagic && h->bytes == bytes;
 }
 
-// K shares of the first product: a few workgroups per compute unit when there are few tiles, at most 8 (each is read
-// again by every workgroup of the second product) and at least 4 steps of 64 a share.
-int adapter_splits(int64_t tiles, int64_t K, int cus) {
-  const int64_t chunks = (K + hf::kAdChunk - 1) / hf::kAdChunk;
-  int64_t s = tiles > 0 ? (2 * cus + tiles - 1) / tiles : 1;
-  s = std::min(s, std::min((int64_t)8, (chunks + 3) / 4));
-  return (int)std::max(s, (int64_t)1);
+// Rank blocks of 32 that a workgroup of the first product takes, and how many such parts the rank has.
+inline int adapter_rank_blocks(int r32) { return r32 <= 32 ? 1 : r32 <= 64 ? 2 : 4; }
+inline int adapter_rank_parts(int r32) { return (r32 / 32 + adapter_rank_blocks(r32) - 1) / adapter_rank_blocks(r32); }
+inline int adapter_waves(int rb, int nb) { return rb == 4 ? 3 : nb == 1 && rb == 1 ? 8 : nb == 1 ? 6 : 4; }
+
+// K shares of the first product. One while its waves have few steps of 64 k each; beyond that, as many as fill the
+// device, and the sums are joined by a launch of their own.
+int adapter_splits(const AdapterHeader& h, int64_t K, int r32, int cus) {
+  const int rb = adapter_rank_blocks(r32), nb = h.tile_rows / 32;
+  const int64_t steps = K / hf::kAdChunk / adapter_waves(rb, nb);
+  const int64_t wgs = (int64_t)h.live_tiles * adapter_rank_parts(r32);
+  if (wgs == 0 || steps < 12 || 2 * wgs > cus) return 1;
+  return (int)std::min(std::min((int64_t)cus / wgs, steps / 6), (int64_t)16);
+}
+
+// The workspace: rows' factors, u in operand order, and the shares where they are joined.
+struct AdapterSpace {
+  int64_t frags, planes, bytes;
+};
+AdapterSpace adapter_space(const AdapterHeader& h, int r32, int splits) {
+  const int64_t rows = (int64_t)h.live_tiles * h.tile_rows;
+  AdapterSpace s;
+  s.frags = up_to(rows * 4, 256);
+  s.planes = s.frags + rows * r32 * 4;
+  s.bytes = s.planes + (splits > 1 || adapter_rank_parts(r32) > 1 ? splits * rows * r32 * 4 : 0);
+  return s;
+}
+
+// Dynamic LDS past 64 KiB has to be asked for, once per device and kernel.
+void allow_lds(const void* kernel, std::once_flag* once, int bytes) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0) dev = 0;
+  std::once_flag spare;
+  std::call_once(dev < 64 ? once[dev] : spare,
+                 [&] { (void)hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes); });
+}
+
+template <class T, int RB, int NB, int NW>
+void launch_adapter_down(const hf::AdapterArgs& a, hipStream_t stream) {
+  static std::once_flag once[64];
+  constexpr int lds = hf::ad_down_lds(RB, NB, NW);
+  static_assert(lds >= 4096 * RB * NB * NW && lds >= NB * 32 * (RB * 32 + 4) * 4, "the sums fit the rings");
+  allow_lds(reinterpret_cast<const void*>(&hf::adapter_down_kernel<T, RB, NB, NW>), once, lds);
+  const dim3 grid(a.live_tiles, a.splits, adapter_rank_parts(a.r32));
+  hipLaunchKernelGGL((hf::adapter_down_kernel<T, RB, NB, NW>), grid, dim3(64 * NW), lds, stream, a);
+}
+
+template <class T, bool VEC, int STEPS>
+void launch_adapter_up(const hf::AdapterArgs& a, dim3 grid, hipStream_t stream) {
+  static std::once_flag once[64];
+  allow_lds(reinterpret_cast<const void*>(&hf::adapter_up_kernel<T, VEC, STEPS>), once, 512 / 16 * 2048 + 4 * hf::kAdUpStage);
+  hipLaunchKernelGGL((hf::adapter_up_kernel<T, VEC, STEPS>), grid, dim3(hf::kAdUpThreads),
+                     a.r32 / 16 * 2048 + 4 * hf::kAdUpStage, stream, a);
 }
 
 template <class T>
 int launch_adapters(hf::AdapterArgs& a, const AdapterHeader& h, bool vec, hipStream_t stream) {
   const int cus = compute_units();
   if (h.live_tiles > 0) {
-    const int rb = a.r32 / 32 >= 4 ? 4 : a.r32 / 32 >= 2 ? 2 : 1;
-    const dim3 grid(h.live_tiles, a.splits, (a.r32 / 32 + rb - 1) / rb);
-    if (rb == 1) hipLaunchKernelGGL((hf::adapter_down_kernel<T, 1>), grid, dim3(hf::kAdThreads), 0, stream, a);
-    else if (rb == 2) hipLaunchKernelGGL((hf::adapter_down_kernel<T, 2>), grid, dim3(hf::kAdThreads), 0, stream, a);
-    else hipLaunchKernelGGL((hf::adapter_down_kernel<T, 4>), grid, dim3(hf::kAdThreads), 0, stream, a);
+    switch (adapter_rank_blocks(a.r32) * 4 + a.tile_rows / 32) {
+      case 1 * 4 + 1: launch_adapter_down<T, 1, 1, 8>(a, stream); break;
+      case 1 * 4 + 2: launch_adapter_down<T, 1, 2, 4>(a, stream); break;
+      case 2 * 4 + 1: launch_adapter_down<T, 2, 1, 6>(a, stream); break;
+      case 2 * 4 + 2: launch_adapter_down<T, 2, 2, 4>(a, stream); break;
+      case 4 * 4 + 1: launch_adapter_down<T, 4, 1, 3>(a, stream); break;
+      default: launch_adapter_down<T, 4, 2, 3>(a, stream); break;
+    }
     if (int st = launch_status()) return st;
+    if (a.splits > 1 || adapter_rank_parts(a.r32) > 1) {
+      static std::once_flag once[64];
+      allow_lds(reinterpret_cast<const void*>(&hf::adapter_join_kernel<T>), once, 64 * 516 * 4);
+      hipLaunchKernelGGL(hf::adapter_join_kernel<T>, dim3(h.live_tiles), dim3(256),
+                         (size_t)a.tile_rows * (a.r32 + 4) * 4, stream, a);
+      if (int st = launch_status()) return st;
+    }
   }
-  const int tiles = a.in_place ? h.live_tiles : h.tiles;
-  if (tiles == 0) return HF_OK;
-  // Column blocks of a workgroup: at least one a wave; with many tiles up to 8 a wave, for one reading of u.
+  const int64_t row_blocks = (int64_t)(a.in_place ? h.live_tiles : h.tiles) * (a.tile_rows / 32);
+  if (row_blocks == 0) return HF_OK;
+  // Column blocks of a workgroup: one a wave with few rows; with many rows up to 4 a wave, for one reading of u.
   const int64_t blocks = (a.N + 63) / 64;
-  const int64_t want = std::max((int64_t)1, (int64_t)8 * cus / tiles);  // workgroups a tile
-  a.blocks_per_wg = (int)std::min(std::max(up_to((blocks + want - 1) / want, 4), (int64_t)4), (int64_t)32);
-  const dim3 grid(tiles, (unsigned)((blocks + a.blocks_per_wg - 1) / a.blocks_per_wg));
-  const size_t lds = (size_t)hf::kAdRows * a.r32 * 4;
-  if (vec) hipLaunchKernelGGL((hf::adapter_up_kernel<T, true>), grid, dim3(hf::kAdThreads), lds, stream, a);
-  else hipLaunchKernelGGL((hf::adapter_up_kernel<T, false>), grid, dim3(hf::kAdThreads), lds, stream, a);
+  const int64_t want = std::max((int64_t)1, (int64_t)8 * cus / row_blocks);  // workgroups a row block
+  a.blocks_per_wg = (int)std::min(std::max(up_to((blocks + want - 1) / want, 4), (int64_t)4), (int64_t)16);
+  // A y that the Infinity Cache (256 MiB) does not hold beside what was written with it is read past the caches.
+  a.stream_y = h.rows * a.N * 2 > (int64_t)128 << 20;
+  a.col_groups = (int)((blocks + a.blocks_per_wg - 1) / a.blocks_per_wg);
+  if (row_blocks * a.col_groups > 0x7fffffff) return HF_ERR_SIZE;
+  const dim3 grid((unsigned)(row_blocks * a.col_groups));
+  if (vec && a.r32 == 32) launch_adapter_up<T, true, 2>(a, grid, stream);
+  else if (vec) launch_adapter_up<T, true, 4>(a, grid, stream);
+  else launch_adapter_up<T, false, 4>(a, grid, stream);
   return launch_status();
-}
-
-// The second product's u tile takes up to 128 KiB of LDS (rank 512).
-void allow_adapter_lds() {
-  static std::once_flag once[64];
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0) dev = 0;
-  std::once_flag spare;
-  std::call_once(dev < 64 ? once[dev] : spare, [] {
-    const int most = hf::kAdRows * 512 * 4;
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&hf::adapter_up_kernel<hf::Bf16, true>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, most);
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&hf::adapter_up_kernel<hf::Bf16, false>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, most);
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&hf::adapter_up_kernel<hf::Fp16, true>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, most);
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&hf::adapter_up_kernel<hf::Fp16, false>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, most);
-  });
 }
 
 }  // namespace
@@ -369,9 +411,9 @@ int hf_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, 
                           : launch_attention_of<hf::Fp16>(a, h, (hipStream_t)stream);
 }
 
-int64_t hf_adapter_plan(const int32_t* ids, const int64_t* lens, int64_t count, int32_t adapters, void* plan,
-                        int64_t bytes) {
-  if (count < 0 || (count > 0 && !ids) || adapters < 0) return HF_ERR_ARGUMENT;
+int64_t hf_adapter_plan(const int32_t* ids, const int64_t* lens, int64_t count, int32_t adapters, int32_t cus,
+                        void* plan, int64_t bytes) {
+  if (count < 0 || (count > 0 && !ids) || adapters < 0 || cus < 0) return HF_ERR_ARGUMENT;
   int64_t rows = 0;
   for (int64_t i = 0; i < count; ++i) {
     if (ids[i] < -1 || ids[i] >= adapters || (lens && lens[i] < 0)) return HF_ERR_ARGUMENT;
@@ -385,18 +427,22 @@ int64_t hf_adapter_plan(const int32_t* ids, const int64_t* lens, int64_t count, 
     std::vector<int64_t> at(keys + 1, 0);
     for (int64_t i = 0; i < count; ++i) at[(ids[i] < 0 ? adapters : ids[i]) + 1] += lens ? lens[i] : 1;
     for (size_t i = 0; i < keys; ++i) at[i + 1] += at[i];
+    // Tiles of 64 rows read the weights half as often; tiles of 32 where those would not fill the device twice.
+    int64_t wide = 0;
+    for (size_t key = 0; key + 1 < keys; ++key) wide += (at[key + 1] - at[key] + 63) / 64;
+    const int tile_rows = wide >= 2 * (cus ? cus : compute_units()) ? 64 : 32;
     std::vector<hf::AdapterTile> tiles;
     int32_t live_tiles = 0;
     for (size_t key = 0; key < keys; ++key) {
-      for (int64_t r = at[key]; r < at[key + 1]; r += hf::kAdRows)
+      for (int64_t r = at[key]; r < at[key + 1]; r += tile_rows)
         tiles.push_back({key == (size_t)adapters ? -1 : (int32_t)key, (int32_t)r,
-                         (int32_t)std::min((int64_t)hf::kAdRows, at[key + 1] - r), 0});
+                         (int32_t)std::min((int64_t)tile_rows, at[key + 1] - r), 0});
       if (key + 1 < keys) live_tiles = (int32_t)tiles.size();
     }
     AdapterHeader h;
     memset(&h, 0, sizeof(h));
     h.magic = kAdapterMagic, h.adapters = adapters, h.tiles = (int32_t)tiles.size(), h.live_tiles = live_tiles;
-    h.rows = rows, h.live_rows = at[keys - 1];
+    h.rows = rows, h.live_rows = at[keys - 1], h.tile_rows = tile_rows;
     h.bytes = (int64_t)sizeof(h) + (int64_t)(tiles.size() * sizeof(hf::AdapterTile)) + 4 * rows;
     if (plan) {
       if (bytes < h.bytes) return HF_ERR_SIZE;
@@ -420,7 +466,8 @@ int64_t hf_adapter_plan(const int32_t* ids, const int64_t* lens, int64_t count, 
 int64_t hf_adapter_ws_bytes(const void* plan, int64_t bytes, int64_t K, int64_t N, int32_t r) {
   AdapterHeader h;
   if (!adapter_header(plan, bytes, &h) || K <= 0 || N <= 0 || r <= 0 || r > 512) return HF_ERR_ARGUMENT;
-  return adapter_splits(h.live_tiles, K, compute_units()) * h.live_rows * up_to(r, 32) * 4;
+  const int r32 = (int)up_to(r, 32);
+  return adapter_space(h, r32, adapter_splits(h, K, r32, compute_units())).bytes;
 }
 
 int hf_adapter_add(const void* x, int64_t ldx, const void* y, int64_t ldy, const void* down, const void* up, int32_t r,
@@ -442,18 +489,18 @@ int hf_adapter_add(const void* x, int64_t ldx, const void* y, int64_t ldy, const
 
   hf::AdapterArgs a = {};
   a.x = (const uint16_t*)x, a.y = (const uint16_t*)y, a.down = (const uint16_t*)down, a.up = (const uint16_t*)up;
-  a.scale = scale, a.out = (uint16_t*)out, a.u = (float*)ws;
+  a.scale = scale, a.out = (uint16_t*)out;
   const unsigned char* dev = (const unsigned char*)plan_dev + sizeof(h);
   a.tiles = (const hf::AdapterTile*)dev;
   a.rows = (const int32_t*)(dev + (int64_t)h.tiles * (int64_t)sizeof(hf::AdapterTile));
-  a.ldx = ldx, a.ldy = ldy, a.ldo = ldo, a.K = K, a.N = N, a.n_rows = h.live_rows, a.r = r;
-  a.r32 = (int)up_to(r, 32);
-  a.splits = adapter_splits(h.live_tiles, K, compute_units());
-  const int64_t chunks = (K + hf::kAdChunk - 1) / hf::kAdChunk;
-  a.chunks_per_split = (int)((chunks + a.splits - 1) / a.splits);
-  a.in_place = in_place;
-  if (h.live_rows > 0 && (!ws || ws_bytes < (int64_t)a.splits * h.live_rows * a.r32 * 4)) return HF_ERR_ARGUMENT;
-  allow_adapter_lds();
+  a.ldx = ldx, a.ldy = ldy, a.ldo = ldo, a.K = K, a.N = N, a.live_tiles = h.live_tiles, a.tile_rows = h.tile_rows;
+  a.r = r, a.r32 = (int)up_to(r, 32), a.in_place = in_place;
+  a.splits = adapter_splits(h, K, a.r32, compute_units());
+  const AdapterSpace space = adapter_space(h, a.r32, a.splits);
+  if (h.live_rows > 0 && (!ws || ws_bytes < space.bytes)) return HF_ERR_ARGUMENT;
+  a.factors = (float*)ws;
+  a.frags = (hf::v4u*)((unsigned char*)ws + space.frags);
+  a.planes = (float*)((unsigned char*)ws + space.planes);
   const bool vec = aligned(y, 16) && aligned(out, 16) && ldy % 8 == 0 && ldo % 8 == 0 && N % 8 == 0;
   return dtype == HF_BF16 ? launch_adapters<hf::Bf16>(a, h, vec, (hipStream_t)stream)
                           : launch_adapters<hf::Fp16>(a, h, vec, (hipStream_t)stream);

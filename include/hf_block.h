@@ -55,7 +55,7 @@ int hf_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, int32_t head
  * does not see never reach it, whatever k and v hold there.
  *
  * hf_attention_plan (host) lays out the work of a batch once for all layers and steps of these lengths: with
- * plan == NULL it returns the plan's bytes, otherwise it fills `plan` (host memory of that many bytes; `bytes` is
+ * plan == NULL it returns the plan's bytes (`cus`: the device's compute units, 0 for the current one's), otherwise it fills `plan` (host memory of that many bytes; `bytes` is
  * checked) and returns the bytes, or a negative HF_ERR_*. hf_attention_ws_bytes gives the workspace that a filled plan
  * needs (0: none), or HF_ERR_ARGUMENT for bytes that hold no plan. The caller copies the plan to the device and passes
  * both copies to hf_attention: `plan` (host) for the launch, `plan_dev` for the kernels.
@@ -83,8 +83,8 @@ int hf_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, 
  * Requires: K, r, ldx multiples of 8, r <= 512; x, down, up 16-byte aligned; y, out 2-byte aligned (16-byte aligned with
  * strides and N multiples of 8 for whole-vector access); ws 16-byte aligned; M, N, K < 2^31.
  */
-int64_t hf_adapter_plan(const int32_t* ids, const int64_t* lens, int64_t count, int32_t adapters, void* plan,
-                        int64_t bytes);
+int64_t hf_adapter_plan(const int32_t* ids, const int64_t* lens, int64_t count, int32_t adapters, int32_t cus,
+                        void* plan, int64_t bytes);
 int64_t hf_adapter_ws_bytes(const void* plan, int64_t bytes, int64_t K, int64_t N, int32_t r);
 int hf_adapter_add(const void* x, int64_t ldx, const void* y, int64_t ldy, const void* down, const void* up, int32_t r,
                    const float* scale, void* out, int64_t ldo, int64_t N, int64_t K, const void* plan,

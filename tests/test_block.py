@@ -227,15 +227,15 @@ def test_argument_checks_reject_before_launching(lib):
     assert attention_plan(lib, [1 << 31], [5]) == attention_plan(lib, [1 << 30, 1 << 30], [5, 5]) == -5
 
     ids, lens = (ctypes.c_int32 * 2)(0, -1), (ctypes.c_int64 * 2)(40, 3)
-    size = lib.hf_adapter_plan(ids, lens, 2, 1, None, 0)
+    size = lib.hf_adapter_plan(ids, lens, 2, 1, 256, None, 0)
     buf = ctypes.create_string_buffer(size)
-    assert lib.hf_adapter_plan(ids, lens, 2, 1, buf, size - 1) == -5
-    assert lib.hf_adapter_plan(ids, lens, 2, 1, buf, size) == size
-    assert lib.hf_adapter_plan(ids, lens, 2, 0, None, 0) == -1  # adapter 0 of none
-    assert lib.hf_adapter_plan((ctypes.c_int32 * 1)(-2), None, 1, 3, None, 0) == -1
-    assert lib.hf_adapter_plan(ids, (ctypes.c_int64 * 2)(1 << 31, 1), 2, 1, None, 0) == -5
+    assert lib.hf_adapter_plan(ids, lens, 2, 1, 256, buf, size - 1) == -5
+    assert lib.hf_adapter_plan(ids, lens, 2, 1, 256, buf, size) == size
+    assert lib.hf_adapter_plan(ids, lens, 2, 0, 256, None, 0) == -1  # adapter 0 of none
+    assert lib.hf_adapter_plan((ctypes.c_int32 * 1)(-2), None, 1, 3, 256, None, 0) == -1
+    assert lib.hf_adapter_plan(ids, (ctypes.c_int64 * 2)(1 << 31, 1), 2, 1, 256, None, 0) == -5
     need = lib.hf_adapter_ws_bytes(buf, size, 512, 64, 24)
-    assert need >= 40 * 32 * 4 and need % (40 * 32 * 4) == 0
+    assert need >= 40 * 32 * 4
     assert lib.hf_adapter_ws_bytes(buf, size - 1, 512, 64, 24) == lib.hf_adapter_ws_bytes(buf, size, 512, 64, 520) == -1
 
     def adapt(x=fake, ldx=512, y=fake, ldy=64, down=fake, r=24, out=fake, ldo=64, N=64, K=512, plan=buf, dev=fake,
@@ -292,17 +292,19 @@ def test_attention_plan_covers_every_row_and_key_once(lib, q, kv, heads, kv_head
     assert want == set(tiles) and not shares and sorted(used) == list(range(slots))
 
 
+@pytest.mark.parametrize("cus", [1, 256])
 @pytest.mark.parametrize("ids,lens", [([0, 2, -1, 0], [70, 1, 5, 3]), ([-1], [9]), ([], []), ([1] * 200, None),
                                       ([2, 1, 0, 1, 2, -1], [0, 64, 65, 1, 200, 64])])
-def test_adapter_plan_covers_every_row_once(lib, ids, lens):
+def test_adapter_plan_covers_every_row_once(lib, ids, lens, cus):
     n = [1] * len(ids) if lens is None else lens
     ids_c = (ctypes.c_int32 * max(len(ids), 1))(*ids)
     lens_c = None if lens is None else (ctypes.c_int64 * max(len(ids), 1))(*lens)
-    size = lib.hf_adapter_plan(ids_c, lens_c, len(ids), 3, None, 0)
+    size = lib.hf_adapter_plan(ids_c, lens_c, len(ids), 3, cus, None, 0)
     buf = ctypes.create_string_buffer(size)
-    assert lib.hf_adapter_plan(ids_c, lens_c, len(ids), 3, buf, size) == size
+    assert lib.hf_adapter_plan(ids_c, lens_c, len(ids), 3, cus, buf, size) == size
     _, adapters, tiles, live = struct.unpack_from("4i", buf.raw)
-    _, rows, live_rows = struct.unpack_from("3q", buf.raw, 16)
+    _, rows, live_rows, tile_rows = struct.unpack_from("3qi", buf.raw, 16)
+    assert tile_rows in (32, 64) and (tile_rows == 32 or cus == 1)
     of = [a for a, c in zip(ids, n) for _ in range(c)]
     assert (adapters, rows, live_rows) == (3, len(of), sum(a >= 0 for a in of))
     tile = np.frombuffer(buf.raw, np.int32, tiles * 4, 128).reshape(tiles, 4)
@@ -310,7 +312,7 @@ def test_adapter_plan_covers_every_row_once(lib, ids, lens):
     assert sorted(order.tolist()) == list(range(rows))
     at = 0
     for i, (a, start, count, _) in enumerate(tile.tolist()):
-        assert start == at and 1 <= count <= 64 and (a >= 0) == (i < live)
+        assert start == at and 1 <= count <= tile_rows and (a >= 0) == (i < live)
         assert all(of[r] == a for r in order[start:start + count])
         assert (np.diff(order[start:start + count]) > 0).all()
         at += count

@@ -281,6 +281,16 @@ def test_widths(K, N):
     adapt(K + N, [0, 2, -1], [70, 3, 9], 3, 32, K, N, BF)
 
 
+@pytest.mark.parametrize("r", [16, 64, 128, 200])
+def test_few_rows_over_a_deep_k(r):
+    adapt(r, [0, 1], [9, 40], 2, r, 14344, 72, BF)
+
+
+@pytest.mark.parametrize("r", [8, 64, 96, 160])
+def test_many_rows(r):
+    adapt(r, [1, 0, -1, 1], [17000, 15990, 33, 40], 2, r, 200, 136, BF)
+
+
 def test_many_requests_in_any_order():
     ids = [(i * 7) % 12 - 1 for i in range(150)]
     adapt(5, ids, [1 + i % 3 for i in range(150)], 11, 16, 512, 256, BF, scaled=False)
