@@ -25,6 +25,10 @@
 namespace hf {
 
 constexpr int kAtKeys = 64;
+// What a lane's weights of one tile may sum to before their maximum is taken anew: fp16 holds them, and the sums have as
+// much room for large values as that many keys of equal weight take.
+constexpr float kAtMost = 512.0f;
+constexpr int kAtShort = 16;  // tiles from which on a workgroup's keys are taken the pipelined way
 
 // A work item: rows row0 .. of sequence (q0, nq, k0, nk) and key head `head`, over keys [key_lo, key_hi). slot < 0: the
 // result goes to out; else the unnormalised sums go to workspace tile `slot`.
@@ -55,6 +59,34 @@ __device__ __forceinline__ int at_swizzle(int r) {
 // Floats of a workspace tile of `rows` rows: O [rows][32 DB], then m and l per row.
 __host__ __device__ constexpr int at_slot_floats(int rows, int db) { return rows * (32 * db + 2); }
 
+// 16 bytes a lane from the buffer's byte `off` to LDS, lane l to dst + 16 l. The builtin for it makes the compiler wait
+// for every such load before any transposing read of LDS, those of the other buffer's next tile among them (3 % of the
+// time of long sequences); as an asm it stays out of that count, and the loop's own waits order it. It has no output
+// register, and its address registers are read when it issues.
+// The s_nop covers the distance that the load needs from scalar registers and m0 written just before it.
+__device__ __forceinline__ void at_load_lds(v4i rsrc, unsigned char HF_LDS* dst, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :: "s"((uint32_t)(uintptr_t)dst), "v"(off), "s"(rsrc) : "memory");
+}
+// The raw descriptor (stride 0) of `bytes` bytes from `base` on: bytes at and after its end read as zero.
+__device__ __forceinline__ v4i at_rsrc(const void* base, uint32_t bytes) {
+  const uint64_t p = (uint64_t)base;
+  return (v4i){(int)(uint32_t)p, (int)((uint32_t)(p >> 32) & 0xffffu), (int)bytes, 0x00020000};
+}
+
+// Every load has landed, the queries' among them: told to the compiler here, it need not wait for them inside a loop, where
+// it would wait for the next tile too.
+__device__ __forceinline__ void at_landed() { __builtin_amdgcn_s_waitcnt(0x0f70); }
+// The workgroup's barrier, after this wave's reads of LDS have returned and its loads to LDS have landed.
+__device__ __forceinline__ void at_barrier() {
+  __builtin_amdgcn_sched_barrier(0);
+  __builtin_amdgcn_s_waitcnt(0x0070);
+  asm volatile("s_barrier" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+// Keeps what is computed from v inside the loop (registers are scarcer there than vector operations).
+__device__ __forceinline__ void at_opaque(uint32_t& v) { asm volatile("" : "+v"(v)); }
+
 // Lane l exchanges with lane l ^ 32: max of both.
 __device__ __forceinline__ float half_max(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -67,7 +99,7 @@ __device__ __forceinline__ float half_sum(float v) {
 
 // NW waves of 32 rows; D up to 32 * DB channels.
 template <class T, int DB, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void attention_kernel(AttentionArgs a) {
+__global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_kernel(AttentionArgs a) {
   constexpr int PITCH = DB > 2 ? 256 : 128, KS = 2 * DB;
   constexpr int kTile = kAtKeys * PITCH;       // bytes of one K or V tile
   constexpr int kLoads = kTile / 1024 / NW;    // 1 KiB loads of a wave a tile
@@ -86,10 +118,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attention_kernel(AttentionArgs a) 
   const int head = it.head * a.group + (live ? (int)(row - (int64_t)token * a.group) : 0);
   // Last key the row sees; -1 for none.
   const int last = live ? (a.causal ? min(token + it.nk - it.nq, it.nk - 1) : it.nk - 1) : -1;
-  int wave_first = live ? last : 0x7fffffff;  // the least of the wave's rows: tiles up to it need no mask
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) wave_first = min(wave_first, __shfl_xor(wave_first, off, 64));
-  wave_first = __builtin_amdgcn_readfirstlane(wave_first);
+  // The least of the wave's live rows, its first one's (later rows see no less): tiles up to it need no mask.
+  const int wave_first = __builtin_amdgcn_readfirstlane(live ? last : 0x7fffffff);
 
   v4u qf[KS];
   {
@@ -99,198 +129,331 @@ __global__ __launch_bounds__(64 * NW, 2) void attention_kernel(AttentionArgs a) 
       qf[s] = live && 16 * s + 8 * half < a.D ? *(const v4u*)(q + 16 * s) : (v4u){0, 0, 0, 0};
   }
 
-  // A wave's loads of a tile: load i fills rows (kLoads wave + i) kRowsPerLoad ..; lane l row l / kChunks, chunk
-  // l % kChunks of LDS from chunk (l % kChunks) ^ f(row) of the key. Rows past the sequence and chunks past D read as
-  // zero: their offset lies past the descriptor, which starts at the tile, so that offsets stay small however long the
-  // sequence is.
-  const uint16_t* kbase = a.k + (int64_t)it.k0 * a.k_token + it.head * a.k_head;
-  const uint16_t* vbase = a.v + (int64_t)it.k0 * a.v_token + it.head * a.v_head;
-  uint32_t kpart[kLoads], vpart[kLoads];
+  // A wave's loads of a tile: load i fills rows kRowsPerLoad (NW i + wave) ..; lane l row l / kChunks, chunk l % kChunks of
+  // LDS from chunk (l % kChunks) ^ f(row) of the key. With four waves f does not depend on i. Rows past the sequence and
+  // chunks past D read as zero: their offset lies past the descriptor, which starts at the tile, so that offsets stay
+  // small however long the sequence is.
+  const uint16_t* kbase = a.k + ((int64_t)it.k0 + it.key_lo) * a.k_token + it.head * a.k_head;
+  const uint16_t* vbase = a.v + ((int64_t)it.k0 + it.key_lo) * a.v_token + it.head * a.v_head;
+  const int kstride = (int)a.k_token, vstride = (int)a.v_token;
+  constexpr int kParts = NW >= 4 ? 1 : kLoads < 4 ? kLoads : 4;
+  uint32_t kpart[kParts], vpart[kParts];
 #pragma unroll
-  for (int i = 0; i < kLoads; ++i) {
-    const int r = (kLoads * wave + i) * kRowsPerLoad + lane / kChunks;
+  for (int i = 0; i < kParts; ++i) {
+    const int r = (NW * i + wave) * kRowsPerLoad + lane / kChunks;
     const int c = (lane % kChunks) ^ at_swizzle<PITCH>(r);
-    kpart[i] = c * 8 < a.D ? (uint32_t)(lane / kChunks * (int)a.k_token * 2 + c * 16) : 0x80000000u;
-    vpart[i] = c * 8 < a.D ? (uint32_t)(lane / kChunks * (int)a.v_token * 2 + c * 16) : 0x80000000u;
+    kpart[i] = c * 8 < a.D ? (uint32_t)(lane / kChunks * kstride * 2 + c * 16) : 0x80000000u;
+    vpart[i] = c * 8 < a.D ? (uint32_t)(lane / kChunks * vstride * 2 + c * 16) : 0x80000000u;
   }
-  auto load_tile = [&](const uint16_t* base, int64_t stride, const uint32_t* part, int key0, unsigned char HF_LDS* dst) {
-    const int rows = min(kAtKeys, it.nk - key0);
-    const __amdgpu_buffer_rsrc_t rsrc =
-        make_rsrc(base + (int64_t)key0 * stride, (uint32_t)((rows - 1) * (int)stride * 2 + a.D * 2));
+  auto load_tile = [&](const uint16_t* base, int stride, uint32_t (&part)[kParts], int t, unsigned char HF_LDS* dst,
+                       bool zeros = false) __attribute__((always_inline)) {
+    const int rows = min(kAtKeys, it.nk - it.key_lo - t * kAtKeys);
+    const v4i rsrc =
+        at_rsrc(base + (int64_t)t * kAtKeys * stride, zeros ? 0u : (uint32_t)((rows - 1) * stride * 2 + a.D * 2));
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int blk = kLoads * wave + i;
-      const uint32_t off = part[i] + (uint32_t)(blk * kRowsPerLoad * (int)stride * 2);
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (void HF_LDS*)(dst + blk * 1024), 16, off, 0, 0, 0);
+      const int blk = NW * i + wave;
+      at_load_lds(rsrc, dst + blk * 1024, part[i % kParts] + (uint32_t)(blk * kRowsPerLoad * stride * 2));
     }
   };
 
-  // Fragment addresses within a tile. K: lane (key sub, half) chunk 2s + half. V: lane reads 4 channels of key
-  // 4 half + (lane % 16) / 4 (+ 8 for the second part), channels 16 ((lane / 16) % 2) + 4 (lane % 4).
-  int kaddr[KS];
-#pragma unroll
-  for (int s = 0; s < KS; ++s) kaddr[s] = sub * PITCH + (((2 * s + half) ^ at_swizzle<PITCH>(sub)) * 16);
-  int vaddr[DB][2];
-#pragma unroll
-  for (int d = 0; d < DB; ++d)
-#pragma unroll
-    for (int p = 0; p < 2; ++p) {
-      const int r = 8 * p + 4 * half + ((lane & 15) >> 2);
-      const int c = 4 * d + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-      vaddr[d][p] = r * PITCH + ((c ^ at_swizzle<PITCH>(r)) * 16) + (lane & 1) * 8;
-    }
+  // Fragment addresses within a tile. K: lane (key sub, half) reads chunk 2s + half of step s; V: 4 channels of key
+  // 4 half + (lane % 16) / 4 (+ 8 for the second part p), channels 32 d + 16 ((lane / 16) % 2) + 4 (lane % 4). Steps,
+  // parts and channel blocks change bits of the chunk that the swizzle changes too, so they are exclusive ors of one
+  // address each (taken anew in every tile: sixteen registers less).
+  uint32_t kaddr = (uint32_t)(sub * PITCH + ((half ^ at_swizzle<PITCH>(sub)) * 16));
+  uint32_t vaddr;
+  {
+    const int r = 4 * half + ((lane & 15) >> 2), ch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+    vaddr = (uint32_t)(r * PITCH + ((ch ^ at_swizzle<PITCH>(r)) * 16) + (lane & 1) * 8);
+  }
+  auto kfrag = [&](const unsigned char HF_LDS* kt, int ks, int b) __attribute__((always_inline)) {
+    return *(const v4u HF_LDS*)(kt + (kaddr ^ (uint32_t)(32 * ks)) + b * 32 * PITCH);
+  };
+  auto vfrag = [&](const unsigned char HF_LDS* vt, int ks, int d) __attribute__((always_inline)) {
+    typedef short v8s __attribute__((ext_vector_type(8)));
+    const unsigned char HF_LDS* at = vt + ks * 16 * PITCH;
+    const v4s f0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s HF_LDS*)(at + (vaddr ^ (uint32_t)(64 * d))));
+    const v4s f1 =
+        __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s HF_LDS*)(at + 8 * PITCH + (vaddr ^ (uint32_t)(64 * d + 32))));
+    return __builtin_bit_cast(v4u, (v8s)__builtin_shufflevector(f0, f1, 0, 1, 2, 3, 4, 5, 6, 7));
+  };
 
   v16f o[DB];
   float m, l;
   const float c = a.scale_log2;
 
-  // SAFE: values that are not finite are taken out of the products and added where they are seen.
-  auto run = [&](auto safe_t) {
-    constexpr bool SAFE = decltype(safe_t)::value;
+  // Scores of 64 keys against the wave's 32 rows: value 4g + i of block b is key 32b + 8g + 4h + i.
+  auto scores = [&](const unsigned char HF_LDS* kt, v16f (&s)[2]) __attribute__((always_inline)) {
+    s[0] = s[1] = (v16f){0};
 #pragma unroll
-    for (int d = 0; d < DB; ++d) o[d] = (v16f){0};
-    m = -__builtin_inff();
-    l = 0.0f;
-    int buf = 0;
-    if (it.key_lo < it.key_hi) {
-      load_tile(kbase, a.k_token, kpart, it.key_lo, lds);
-      load_tile(vbase, a.v_token, vpart, it.key_lo, lds + kTile);
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+        s[b] = T::mfma(kfrag(kt, ks, b), qf[ks], s[b]);
+  };
+
+  // Keys that a row does not see out of its scores; tiles that every row of the wave sees in full need none of it.
+  auto mask = [&](int key0, v16f (&s)[2]) __attribute__((always_inline)) {
+    if (key0 + kAtKeys - 1 > wave_first) {
+      const int left = last - key0 - 4 * half;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) {
+          if (32 * b + 8 * (v >> 2) + (v & 3) > left) s[b][v] = -__builtin_inff();
+          if (v & 1) __builtin_amdgcn_sched_barrier(0);  // two comparisons at a time: scalar registers are scarce
+        }
     }
-    for (int key0 = it.key_lo; key0 < it.key_hi; key0 += kAtKeys) {
-      // This wave's loads of the tile have landed, and after the barrier everyone's; all have left the other buffer.
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      unsigned char HF_LDS* kt = lds + buf * 2 * kTile;
-      unsigned char HF_LDS* vt = kt + kTile;
-      buf ^= 1;
-      if (key0 + kAtKeys < it.key_hi) {
-        load_tile(kbase, a.k_token, kpart, key0 + kAtKeys, lds + buf * 2 * kTile);
-        load_tile(vbase, a.v_token, vpart, key0 + kAtKeys, lds + buf * 2 * kTile + kTile);
-      }
-      v16f s[2];
-      s[0] = s[1] = (v16f){0};
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-          s[b] = T::mfma(*(const v4u HF_LDS*)(kt + kaddr[ks] + b * 32 * PITCH), qf[ks], s[b]);
-      if (key0 + kAtKeys - 1 > wave_first) {
-        const int left = last - key0 - 4 * half;  // value 4g + i of block b is key 32b + 8g + 4h + i
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int v = 0; v < 16; ++v)
-            if (32 * b + 8 * (v >> 2) + (v & 3) > left) s[b][v] = -__builtin_inff();
-      }
+  };
+
+  // Scores to weights, in the operand order of the second product: p = 2^(c (s - m)). m need not be the running maximum,
+  // only near enough that the weights keep their precision and their sums stay in range: it is taken in the first tile
+  // that a row sees, and anew when a tile's weights sum to more than kAtMost (or to NaN). Looking for the maximum in every
+  // tile would be a seventh of the vector unit's work. Each row goes by its own scores alone, so that its bits do not
+  // depend on the rows that share its wave. The sums over the keys are rescaled when m moves (`rescale`).
+  auto exponentials = [&](const v16f (&s)[2], v4u (&pf)[4], int p, float mc, float (&part)[2])
+                          __attribute__((always_inline)) {  // two of them, p of 16
+    const int b = p >> 3, v = 2 * (p & 7);
+    const float p0 = __builtin_amdgcn_exp2f(fmaf(s[b][v], c, -mc));
+    const float p1 = __builtin_amdgcn_exp2f(fmaf(s[b][v + 1], c, -mc));
+    part[0] += p0;
+    part[1] += p1;
+    asm volatile("" : "+v"(part[0]), "+v"(part[1]));  // here, not after the last slot
+    pf[p >> 2][p & 3] = T::pack(p0, p1);
+  };
+  auto centre = [&]() __attribute__((always_inline)) { return m == -__builtin_inff() ? 0.0f : m * c; };
+  // After all 16: their sum, or, where m has to move, new weights first.
+  auto settle = [&](const v16f (&s)[2], v4u (&pf)[4], float (&part)[2]) __attribute__((always_inline)) {
+    float sum = part[0] + part[1];
+    if (__any(!(sum <= kAtMost) || m == -__builtin_inff())) {
       float top = m;
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) top = fmaxf(top, s[b][v]);
+      for (int v = 0; v < 16; ++v) top = fmaxf(fmaxf(top, s[0][v]), s[1][v]);
       top = half_max(top);
-      // The maximum that the weights are taken against follows the running one only when it falls 2^8 behind: the
-      // weights then stay below 2^8, which costs no precision, and the sums are rescaled a few times a row at most.
-      // Each row goes by its own scores alone, so that its bits do not depend on the rows that share its wave.
-      const bool behind = (top - m) * c > 8.0f;  // also from -inf; NaN (still nothing seen) compares false
-      if (__any(behind)) {
-        const float alpha = behind ? __builtin_amdgcn_exp2f((m - top) * c) : 1.0f;
-        m = behind ? top : m;
-        l *= alpha;
+      const bool move = half_max(sum <= kAtMost ? 0.0f : 1.0f) > 0.0f || m == -__builtin_inff();
+      m = move ? top : m;
+      const float mc = centre();
+      part[0] = part[1] = 0.0f;
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+      for (int p = 0; p < 16; ++p) exponentials(s, pf, p, mc, part);
+      sum = part[0] + part[1];
+    }
+    return sum;
+  };
+  auto rescale = [&](float used) __attribute__((always_inline)) {
+    if (__any(used != m)) {
+      const float alpha = used != m ? __builtin_amdgcn_exp2f((used - m) * c) : 1.0f;
+      l *= alpha;
 #pragma unroll
-          for (int v = 0; v < 16; ++v) o[d][v] *= alpha;
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) o[d][v] *= alpha;
+    }
+  };
+
+  // Weights times the 64 keys' values, added to the sums.
+  auto values = [&](const unsigned char HF_LDS* vt, const v4u (&pf)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+        o[d] = T::mfma(vfrag(vt, ks, d), pf[ks], o[d]);
+  };
+  // The same with values that are not finite taken out of the product and added where they are seen.
+  auto safe_values = [&](int key0, const unsigned char HF_LDS* vt, const v4u (&pf)[4]) __attribute__((always_inline)) {
+    const int left = last - key0 - 4 * half;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      v16f high = (v16f){0}, low = (v16f){0};  // how many +inf (or NaN) and -inf (or NaN) values a row sees
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) {
+        const v4u f = vfrag(vt, ks, d);
+        v4u fine, up, down, sees;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int j = 2 * e + x;
+            const uint32_t bits = (f[e] >> (16 * x)) & 0xffffu;
+            const bool finite = (bits & T::kExponent) != T::kExponent;
+            const bool nan = !finite && (bits & 0x7fffu) != T::kExponent;
+            w[0] |= (finite ? bits : 0u) << (16 * x);
+            w[1] |= (!finite && (nan || !(bits & 0x8000u)) ? T::kOne : 0u) << (16 * x);
+            w[2] |= (!finite && (nan || (bits & 0x8000u)) ? T::kOne : 0u) << (16 * x);
+            // The key of operand element j in step ks: 16 ks + 8 (j / 4) + 4 h + j % 4.
+            w[3] |= (16 * ks + 8 * (j >> 2) + (j & 3) <= left ? T::kOne : 0u) << (16 * x);
+          }
+          fine[e] = w[0], up[e] = w[1], down[e] = w[2], sees[e] = w[3];
+        }
+        o[d] = T::mfma(fine, pf[ks], o[d]);
+        high = T::mfma(up, sees, high);
+        low = T::mfma(down, sees, low);
       }
-      const float mc = m == -__builtin_inff() ? 0.0f : m * c;
-      v4u pf[4];
-      float sum = 0.0f;
 #pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int v = 0; v < 16; v += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(fmaf(s[b][v], c, -mc));
-          const float p1 = __builtin_amdgcn_exp2f(fmaf(s[b][v + 1], c, -mc));
-          sum += p0 + p1;
-          pf[2 * b + (v >> 3)][(v & 7) >> 1] = T::pack(p0, p1);
-        }
-      l += sum;
-      if constexpr (!SAFE) {
-#pragma unroll
-        for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-          for (int d = 0; d < DB; ++d) {
-            const v4s f0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s HF_LDS*)(vt + vaddr[d][0] + ks * 16 * PITCH));
-            const v4s f1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s HF_LDS*)(vt + vaddr[d][1] + ks * 16 * PITCH));
-            typedef short v8s __attribute__((ext_vector_type(8)));
-            const v8s f = __builtin_shufflevector(f0, f1, 0, 1, 2, 3, 4, 5, 6, 7);
-            o[d] = T::mfma(__builtin_bit_cast(v4u, f), pf[ks], o[d]);
-          }
-      } else {
-        const int left = last - key0 - 4 * half;
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          v16f high = (v16f){0}, low = (v16f){0};  // how many +inf (or NaN) and -inf (or NaN) values a row sees
-#pragma unroll
-          for (int ks = 0; ks < 4; ++ks) {
-            const v4s f0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s HF_LDS*)(vt + vaddr[d][0] + ks * 16 * PITCH));
-            const v4s f1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s HF_LDS*)(vt + vaddr[d][1] + ks * 16 * PITCH));
-            v4u fine, up, down, sees;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-              for (int x = 0; x < 2; ++x) {
-                const int j = 2 * e + x;
-                const uint32_t bits = (uint16_t)(j < 4 ? f0[j & 3] : f1[j & 3]);
-                const bool finite = (bits & T::kExponent) != T::kExponent;
-                const bool nan = !finite && (bits & 0x7fffu) != T::kExponent;
-                w[0] |= (finite ? bits : 0u) << (16 * x);
-                w[1] |= (!finite && (nan || !(bits & 0x8000u)) ? T::kOne : 0u) << (16 * x);
-                w[2] |= (!finite && (nan || (bits & 0x8000u)) ? T::kOne : 0u) << (16 * x);
-                // The key of operand element j in step ks: 16 ks + 8 (j / 4) + 4 h + j % 4.
-                w[3] |= (16 * ks + 8 * (j >> 2) + (j & 3) <= left ? T::kOne : 0u) << (16 * x);
-              }
-              fine[e] = w[0], up[e] = w[1], down[e] = w[2], sees[e] = w[3];
-            }
-            o[d] = T::mfma(fine, pf[ks], o[d]);
-            high = T::mfma(up, sees, high);
-            low = T::mfma(down, sees, low);
-          }
-#pragma unroll
-          for (int v = 0; v < 16; ++v) {
-            if (high[v] > 0.0f) o[d][v] += __builtin_inff();
-            if (low[v] > 0.0f) o[d][v] -= __builtin_inff();
-          }
-        }
+      for (int v = 0; v < 16; ++v) {
+        if (high[v] > 0.0f) o[d][v] += __builtin_inff();
+        if (low[v] > 0.0f) o[d][v] -= __builtin_inff();
       }
     }
   };
-  run(std::false_type{});
+
+  const int tiles = (it.key_hi - it.key_lo + kAtKeys - 1) / kAtKeys;
+  auto load_k = [&](int t) __attribute__((always_inline)) {
+    if (t < tiles) load_tile(kbase, kstride, kpart, t, lds + (t & 1) * 2 * kTile);
+  };
+  auto load_v = [&](int t) __attribute__((always_inline)) {
+    if (t < tiles) load_tile(vbase, vstride, vpart, t, lds + (t & 1) * 2 * kTile + kTile);
+  };
+  auto tile_at = [&](int t) __attribute__((always_inline)) -> const unsigned char HF_LDS* { return lds + (t & 1) * 2 * kTile; };
+
+  auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = (v16f){0};
+    m = last >= it.key_lo ? -__builtin_inff() : 0.0f;  // rows that see none of the keys need no maximum
+    l = 0.0f;
+  };
+  // One tile after the other: few rows, where memory is what it waits for, and the safe way.
+  auto plainly = [&](auto safe_t) __attribute__((always_inline)) {
+    clear();
+    if (tiles <= 0) return;
+    load_k(0);
+    load_v(0);
+    at_landed();
+#pragma unroll 1
+    for (int t = 0; t < tiles; ++t) {
+      // This wave's loads of the tile have landed, and after the barrier everyone's; all have left the other buffer.
+      at_barrier();
+      load_k(t + 1);
+      load_v(t + 1);
+      const int key0 = it.key_lo + t * kAtKeys;
+      v16f s[2];
+      v4u pf[4];
+      float part[2] = {0.0f, 0.0f};
+      scores(tile_at(t), s);
+      mask(key0, s);
+      const float used = m, mc = centre();
+#pragma unroll
+      for (int p = 0; p < 16; ++p) exponentials(s, pf, p, mc, part);
+      const float sum = settle(s, pf, part);
+      rescale(used);
+      l += sum;
+      if constexpr (decltype(safe_t)::value) safe_values(key0, tile_at(t) + kTile, pf);
+      else values(tile_at(t) + kTile, pf);
+    }
+  };
+
+  // Many rows, where the matrix and the vector unit are both near their bound: while the scores of tile t become weights,
+  // the matrix unit multiplies the scores of tile t + 1 and the weights and values of tile t - 1, all in one stretch of
+  // independent instructions. Keys t + 2 and values t are loaded meanwhile, into the buffers that keys t and values t - 2
+  // have left. The first tile multiplies zeros, the last one scores that nobody reads: steps of their own for them cost
+  // the loop the registers that it needs (the compiler then spills the queries, and the loop takes a third longer).
+  auto pipelined = [&]() __attribute__((always_inline)) {
+    clear();
+    if (tiles <= 0) return;
+    v16f s0[2], s1[2];
+    v4u p0[4], p1[4];
+    float used = m, sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p1[i] = (v4u){0, 0, 0, 0};
+    load_k(0);
+    load_k(1);
+    load_tile(vbase, 0, vpart, 0, lds + 3 * kTile, true);
+    at_landed();
+    at_barrier();
+    scores(tile_at(0), s0);
+    auto step = [&](int t, v16f (&s)[2], v16f (&next)[2], v4u (&pf)[4], const v4u (&before)[4])
+                    __attribute__((always_inline)) {
+      at_barrier();
+      at_opaque(kpart[0]);
+      at_opaque(vpart[0]);
+      at_opaque(kaddr);
+      at_opaque(vaddr);
+      load_k(t + 2);
+      load_v(t);
+      mask(it.key_lo + t * kAtKeys, s);
+      // What the weights of tile t - 1 left to do before they are multiplied.
+      rescale(used);
+      l += sum;
+      used = m;
+      // Slot i holds product i, the reading of product i + kAhead's operand, and a share of the exponentials. The order is held slot by slot: two waves that run this share
+      // a SIMD, and each finds the matrix unit or the vector unit free.
+      constexpr int kScores = 4 * DB, kSlots = 8 * DB, kAhead = 4;
+      const unsigned char HF_LDS* kt = tile_at(t + 1);
+      const unsigned char HF_LDS* vt = tile_at(t - 1) + kTile;
+      auto operand = [&](int i) __attribute__((always_inline)) {
+        return i < kScores ? kfrag(kt, i >> 1, i & 1) : vfrag(vt, (i - kScores) / DB, (i - kScores) % DB);
+      };
+      v4u ring[kAhead];
+#pragma unroll
+      for (int i = 0; i < kAhead; ++i) ring[i] = operand(i);
+      float part[2] = {0.0f, 0.0f};
+      const float mc = centre();
+      next[0] = next[1] = (v16f){0};
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < kSlots; ++i) {
+        if (i < kScores) next[i & 1] = T::mfma(ring[i % kAhead], qf[i >> 1], next[i & 1]);
+        else o[(i - kScores) % DB] = T::mfma(ring[i % kAhead], before[(i - kScores) / DB], o[(i - kScores) % DB]);
+        if (i + kAhead < kSlots) ring[i % kAhead] = operand(i + kAhead);
+#pragma unroll
+        for (int p = (16 * i + kSlots - 1) / kSlots; p * kSlots < 16 * (i + 1); ++p) exponentials(s, pf, p, mc, part);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      // The weights are wanted in this stretch, not after a branch.
+      asm volatile("" : "+v"(pf[0]), "+v"(pf[1]), "+v"(pf[2]), "+v"(pf[3]));
+      sum = settle(s, pf, part);
+    };
+    auto finish = [&](const v4u (&pf)[4]) __attribute__((always_inline)) {
+      rescale(used);
+      l += sum;
+      at_barrier();
+      values(tile_at(tiles - 1) + kTile, pf);
+    };
+    int t = 0;
+#pragma unroll 1
+    for (; t + 1 < tiles; t += 2) {
+      step(t, s0, s1, p0, p1);
+      step(t + 1, s1, s0, p1, p0);
+    }
+    if (t < tiles) {
+      step(t, s0, s1, p0, p1);
+      finish(p0);
+    } else {
+      finish(p1);
+    }
+  };
+  // Below kAtShort tiles the steps that the pipelined way adds at its ends cost more than it gains.
+  if (NW > 1 && tiles >= kAtShort) pipelined();
+  else plainly(std::false_type{});
   // A key whose values are not finite poisons rows that do not see it (0 * inf); that shows as a NaN in the sums, and
-  // then the item runs again the safe way. The vote goes through the buffers' first bytes.
+  // then the item runs again the safe way.
   {
-    bool nan = false;
+    float all = 0.0f;  // NaN if one of the sums is, or infinities of both signs are
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
-      for (int v = 0; v < 16; ++v) nan |= o[d][v] != o[d][v];
-    bool again = __any(live && nan);
-    if constexpr (NW > 1) {
+      for (int v = 0; v < 16; ++v) all += o[d][v];
+    bool again = __any(live && all != all);
+    if constexpr (NW > 1) {  // the workgroup decides together; nobody reads the keys' buffers any more
       int HF_LDS* votes = (int HF_LDS*)lds;
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
       if (lane == 0) votes[wave] = again;
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      at_barrier();
 #pragma unroll
       for (int w = 0; w < NW; ++w) again |= votes[w] != 0;
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (again) at_barrier();
     }
-    if (again) run(std::true_type{});
+    if (again) plainly(std::true_type{});
   }
   l = half_sum(l);
+  if (last < it.key_lo) m = -__builtin_inff();
 
   if (it.slot >= 0) {
     // Shares go out as they are: row-major, and the row's maximum and sum behind them.
     float* part = a.ws + (int64_t)it.slot * at_slot_floats(32 * NW, DB);
     const int r = wave * 32 + sub;
+    if (!live) return;  // the end of a tile's rows: nobody joins them
 #pragma unroll
     for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -328,32 +491,36 @@ __global__ __launch_bounds__(64 * NW, 2) void attention_kernel(AttentionArgs a) 
     }
 }
 
-// The shares of a tile joined: out = sum_s 2^((m_s - M) c) O_s / sum_s 2^((m_s - M) c) l_s. Eight channels a thread;
-// blockIdx.y takes kJoinRows rows of the tile.
-constexpr int kJoinThreads = 256;
+// The shares of a tile joined: out = sum_s 2^((m_s - M) c) O_s / sum_s 2^((m_s - M) c) l_s. A wave a row: lane group
+// lane / 16 takes every fourth share, eight channels a lane. blockIdx.y takes kJoinRows rows of the tile.
+constexpr int kJoinRows = 4;
 template <class T, int DB>
-__global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(AttentionArgs a, int tile_rows) {
-  constexpr int kLanes = 4 * DB, kRows = kJoinThreads / 16;
+__global__ __launch_bounds__(64 * kJoinRows) void attention_join_kernel(AttentionArgs a, int tile_rows) {
   const AttentionJoin j = a.joins[blockIdx.x];
-  const int r = blockIdx.y * kRows + threadIdx.x / 16, d = threadIdx.x % 16 * 8;
+  const int lane = threadIdx.x & 63, group = lane >> 4;
+  const int r = blockIdx.y * kJoinRows + (threadIdx.x >> 6), d = 8 * (lane & 15);
   const int64_t row = (int64_t)j.row0 + r;
-  if (threadIdx.x % 16 >= kLanes || d >= a.D || r >= tile_rows || row >= (int64_t)j.nq * a.group) return;
+  if (r >= tile_rows || row >= (int64_t)j.nq * a.group) return;
   const int token = (int)((uint32_t)row / (uint32_t)a.group);
   const int head = j.head * a.group + (int)(row - (int64_t)token * a.group);
   const int64_t step = at_slot_floats(tile_rows, DB);
   const float* part = a.ws + (int64_t)j.slot0 * step;
   const float* stat = part + tile_rows * 32 * DB + 2 * r;
   float top = -__builtin_inff();
-  for (int s = 0; s < j.slots; ++s) top = fmaxf(top, stat[s * step]);
+  for (int s = lane; s < j.slots; s += 64) top = fmaxf(top, stat[s * step]);
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
   float l = 0.0f, o[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] = 0.0f;
-  for (int s = 0; s < j.slots; ++s) {
+  const bool inside = d < 32 * DB;
+#pragma unroll 2
+  for (int s = group; s < j.slots; s += 4) {
     const v2f ml = *(const v2f*)(stat + s * step);
+    const float* p = part + s * step + r * 32 * DB + (inside ? d : 0);
+    const v4f x = *(const v4f*)p, y = *(const v4f*)(p + 4);
     // A share whose keys the row does not see has m = -inf and adds nothing.
     const float f = ml[0] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((ml[0] - top) * a.scale_log2);
-    const float* p = part + s * step + r * 32 * DB + d;
-    const v4f x = *(const v4f*)p, y = *(const v4f*)(p + 4);
     l = fmaf(ml[1], f, l);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -361,6 +528,13 @@ __global__ __launch_bounds__(kJoinThreads) void attention_join_kernel(AttentionA
       o[4 + e] = fmaf(y[e], f, o[4 + e]);
     }
   }
+#pragma unroll
+  for (int off = 16; off <= 32; off <<= 1) {
+    l += __shfl_xor(l, off, 64);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] += __shfl_xor(o[e], off, 64);
+  }
+  if (group != 0 || d >= a.D) return;
   const int last = a.causal ? min(token + j.nk - j.nq, j.nk - 1) : j.nk - 1;
   const float inv = 1.0f / l;
   v4u out;

@@ -57,7 +57,7 @@ void launch_rope_lanes(const hf::RopeArgs& a, int lanes, bool interleaved, bool 
 
 constexpr int32_t kAttentionMagic = 0x48464154;
 struct AttentionHeader {
-  int32_t magic, waves, heads, kv_heads, D, causal, items, joins;
+  int32_t magic, rows, heads, kv_heads, D, causal, items, joins;
   int64_t bytes, slots, q_rows, kv_rows;
   int32_t pad[16];
 };
@@ -89,8 +89,7 @@ bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t cou
     if (q_rows > limit || kv_rows > limit || q_lens[b] * group > limit - 4096) return false;
     widest = std::max(widest, q_lens[b] * group);
   }
-  const int waves = widest <= 32 ? 1 : 4;
-  const int rows = 32 * waves;
+  const int rows = widest <= 32 ? 32 : 128;
   struct Piece {
     hf::AttentionItem item;
     int64_t cost;
@@ -117,11 +116,36 @@ bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t cou
     k0 += nk;
   }
   std::stable_sort(tiles.begin(), tiles.end(), [](const Piece& x, const Piece& y) { return x.cost > y.cost; });
-  // Tiles longer than an equal share of the device are cut along the keys.
-  const int64_t share = std::max((total + 2 * cus - 1) / (2 * cus), (int64_t)4);
+  // The device takes `places` workgroups at a time, the longest tiles first. Tiles that would end well after an equal share
+  // of all work (few rows over many keys, or the last round of equal tiles) are cut along the keys into parts that fill
+  // what the whole ones leave; a part costs about two tiles of keys more (its start, its sums' way through memory).
+  const int64_t places = 2 * (int64_t)cus, share = (total + places - 1) / places;
+  std::vector<int64_t> load((size_t)places, 0);  // a heap, the least loaded place first
+  const auto less = [](int64_t x, int64_t y) { return x > y; };
+  size_t whole = 0;
+  int64_t left = total;
+  for (; whole < tiles.size(); ++whole) {
+    const int64_t end = load.front() + tiles[whole].cost;
+    if (end > share + share / 16 + 4) break;
+    std::pop_heap(load.begin(), load.end(), less);
+    load.back() = end;
+    std::push_heap(load.begin(), load.end(), less);
+    left -= tiles[whole].cost;
+  }
+  // No more parts than places, so that none waits for another; parts of six tiles and more.
+  int64_t part = std::max((left + places - 1) / places, (int64_t)6);
+  for (;; part += part / 32 + 1) {
+    int64_t parts = 0, longest = 0;
+    for (size_t t = whole; t < tiles.size(); ++t) {
+      parts += std::max((tiles[t].cost + part - 1) / part, (int64_t)1);
+      longest = std::max(longest, tiles[t].cost);
+    }
+    if (parts <= places || part >= longest) break;
+  }
   int64_t slots = 0;
-  for (const Piece& p : tiles) {
-    const int64_t parts = std::max((p.cost + share - 1) / share, (int64_t)1);
+  for (size_t t = 0; t < tiles.size(); ++t) {
+    const Piece& p = tiles[t];
+    const int64_t parts = t < whole ? 1 : std::max((p.cost + part - 1) / part, (int64_t)1);
     if (parts == 1) {
       w->items.push_back(p.item);
       continue;
@@ -139,7 +163,7 @@ bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t cou
   }
   memset(&w->head, 0, sizeof(w->head));
   w->head.magic = kAttentionMagic;
-  w->head.waves = waves;
+  w->head.rows = rows;
   w->head.heads = heads, w->head.kv_heads = kv_heads, w->head.D = D, w->head.causal = causal != 0;
   w->head.items = (int32_t)w->items.size(), w->head.joins = (int32_t)w->joins.size();
   w->head.slots = slots, w->head.q_rows = q_rows, w->head.kv_rows = kv_rows;
@@ -149,7 +173,7 @@ bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t cou
 }
 
 int64_t attention_slot_bytes(const AttentionHeader& h) {
-  return (int64_t)hf::at_slot_floats(32 * h.waves, attention_db(h.D)) * 4;
+  return (int64_t)hf::at_slot_floats(h.rows, attention_db(h.D)) * 4;
 }
 
 constexpr int attention_lds(int db) { return 4 * hf::kAtKeys * (db > 2 ? 256 : 128); }
@@ -162,7 +186,8 @@ int launch_attention(const hf::AttentionArgs& a, const AttentionHeader& h, hipSt
   if (int st = launch_status()) return st;
   if (h.joins > 0) {
     constexpr int rows = 32 * NW;
-    hipLaunchKernelGGL((hf::attention_join_kernel<T, DB>), dim3(h.joins, rows / 16), dim3(hf::kJoinThreads), 0, stream,
+    hipLaunchKernelGGL((hf::attention_join_kernel<T, DB>), dim3(h.joins, rows / hf::kJoinRows),
+                       dim3(64 * hf::kJoinRows), 0, stream,
                        a, rows);
     return launch_status();
   }
@@ -171,13 +196,14 @@ int launch_attention(const hf::AttentionArgs& a, const AttentionHeader& h, hipSt
 
 template <class T>
 int launch_attention_of(const hf::AttentionArgs& a, const AttentionHeader& h, hipStream_t stream) {
-  switch (attention_db(h.D) * 8 + h.waves) {
-    case 2 * 8 + 1: return launch_attention<T, 2, 1>(a, h, stream);
-    case 2 * 8 + 4: return launch_attention<T, 2, 4>(a, h, stream);
-    case 3 * 8 + 1: return launch_attention<T, 3, 1>(a, h, stream);
-    case 3 * 8 + 4: return launch_attention<T, 3, 4>(a, h, stream);
-    case 4 * 8 + 1: return launch_attention<T, 4, 1>(a, h, stream);
-    case 4 * 8 + 4: return launch_attention<T, 4, 4>(a, h, stream);
+  switch (attention_db(h.D) * 16 + h.rows / 32) {
+#define HF_ATTENTION(DB)                                                                                     \
+  case DB * 16 + 1: return launch_attention<T, DB, 1>(a, h, stream);                                         \
+  case DB * 16 + 4: return launch_attention<T, DB, 4>(a, h, stream);
+    HF_ATTENTION(2)
+    HF_ATTENTION(3)
+    HF_ATTENTION(4)
+#undef HF_ATTENTION
     default: return HF_ERR_ARGUMENT;
   }
 }

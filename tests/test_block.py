@@ -260,12 +260,12 @@ def test_argument_checks_reject_before_launching(lib):
 ])
 def test_attention_plan_covers_every_row_and_key_once(lib, q, kv, heads, kv_heads, causal):
     raw = attention_plan(lib, q, kv, heads, kv_heads, 64, causal).raw
-    _, waves, *_, items, joins = struct.unpack_from("8i", raw)
+    _, rows, *_, items, joins = struct.unpack_from("8i", raw)
     size, slots, q_rows, kv_rows = struct.unpack_from("4q", raw, 32)
     assert size == len(raw) and (q_rows, kv_rows) == (sum(q), sum(kv))
     item = np.frombuffer(raw, np.int32, items * 12, 128).reshape(items, 12)
     join = np.frombuffer(raw, np.int32, joins * 8, 128 + items * 48).reshape(joins, 8)
-    rows, group = 32 * waves, heads // kv_heads
+    group = heads // kv_heads
     tiles = {}
     for q0, nq, k0, nk, row0, lo, hi, head, slot, *_ in item.tolist():
         assert 0 <= lo <= hi <= nk and lo % 64 == 0 and row0 % rows == 0
