@@ -1,8 +1,10 @@
-"""MI355X-native INT8 "convrot" linear for HyperFlow H3 Flash: a drop-in for ``hyperflow_h3_flash.int8``.
+"""MI355X-native INT8 "convrot" linear for HyperFlow H3 Flash: a drop-in for ``hyperflow_h3_flash.int8``, and the
+operators of an attention block around it (norms and rotation, packed attention, adapters of many requests).
 
 Importing the package does not touch the GPU or load the HIP library; the first device forward does.
 """
 
+from .attention_block import AdapterBank, AttentionBlock
 from .block import AdapterPlan, AttentionPlan, RotaryAxes, adapter_add, packed_attention, qk_norm_rope
 from .int8 import (
     ACTIVATIONS,
@@ -25,7 +27,9 @@ __version__ = "0.1.0"
 __all__ = [
     "ACTIVATIONS",
     "ARITHMETIC_OPTIONS",
+    "AdapterBank",
     "AdapterPlan",
+    "AttentionBlock",
     "AttentionPlan",
     "INT8_GEMMS",
     "KERNEL_OPTIONS",

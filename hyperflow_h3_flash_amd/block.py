@@ -19,6 +19,7 @@ built once on the host and serves every layer and step of that batch, on any str
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 from collections.abc import Sequence
@@ -27,18 +28,23 @@ import torch
 from torch import Tensor, nn
 
 from . import _native, host_block
-from .int8 import _check, _on, _raw_stream, _same_device, _workspace
+from .int8 import _check, _on, _raw_stream, _same_device
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_HERE = contextlib.nullcontext()
+#: The current device's index.
+_device_index = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
+
+# With few rows the host time of a call is as long as its kernels (a kernel of 5 us in a call of 10): the functions below
+# read each property once, and leave their straight path only where something is unusual.
 
 def _forward_only(what: str, *tensors: Tensor | None) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError(f"{what} is forward only: call it under torch.no_grad(), or on tensors that do not "
-                                   "require a gradient")
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            raise RuntimeError(f"{what} is forward only: call it under torch.no_grad(), or on tensors that do not "
+                               "require a gradient")
 
 
 def _lib(device: torch.device) -> ctypes.CDLL:
@@ -48,17 +54,24 @@ def _lib(device: torch.device) -> ctypes.CDLL:
         raise RuntimeError(f"tensors on {device} need the gfx950 HIP library: {exc}") from exc
 
 
-def _dtype_code(what: str, t: Tensor) -> int:
-    code = _DTYPES.get(t.dtype)
+def _dtype_code(what: str, dtype: torch.dtype) -> int:
+    code = _DTYPES.get(dtype)
     if code is None:
-        raise ValueError(f"{what} takes bfloat16 or float16, got {t.dtype}")
+        raise ValueError(f"{what} takes bfloat16 or float16, got {dtype}")
     return code
+
+
+def _current(index: int, device: torch.device):
+    """A context in which the device of that index is current: nothing to do when it is already."""
+    return _HERE if _device_index() == index else torch.cuda.device(device)
 
 
 def _heads(t: Tensor) -> tuple[Tensor, int, int]:
     """``t`` [tokens, heads, D] with its token and head strides as the kernels take them: channels side by side, 16-byte
     vectors (a copy where it lies otherwise). The stride of a dimension of one is never used."""
     rows, heads, d = t.shape
+    if t.is_contiguous() and t.data_ptr() % 16 == 0 and d % 8 == 0:
+        return t, heads * d, d
     token, head, channel = t.stride()
     if rows <= 1:
         token = heads * d
@@ -68,6 +81,11 @@ def _heads(t: Tensor) -> tuple[Tensor, int, int]:
         t = torch.empty((rows, heads, d), dtype=t.dtype, device=t.device).copy_(t)
         token, head = heads * d, d
     return t, token, head
+
+
+def _vector(t: Tensor) -> Tensor:
+    """``t`` [n] with its values side by side from a 16-byte boundary."""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _check_out(out: Tensor, like: Tensor, what: str) -> None:
@@ -83,12 +101,13 @@ class _Resident:
     def __init__(self, host: Tensor, device: torch.device) -> None:
         self.host = host
         self.device_copy = host.to(device)
+        self._ptr = self.device_copy.data_ptr()
         self._stream = _raw_stream(self.device_copy.get_device())
 
     def on(self, stream: int) -> int:
         if stream != self._stream:
             self.device_copy.record_stream(torch.cuda.current_stream(self.device_copy.device))
-        return self.device_copy.data_ptr()
+        return self._ptr
 
 
 # ------------------------------------------------------------------------------------------------- norms and rotation
@@ -141,21 +160,23 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: 
     [T, axes] (or [T] for one axis; int32, int64 or float32). Computed in float32, rounded once to the inputs' type
     (bfloat16 or float16). q and k may be views with any token and head strides, such as slices of a fused projection.
     ``out`` may name the results' tensors, the inputs themselves among them. D is a multiple of 16, up to 256."""
-    if q.dim() != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2])):
+    dtype, shape = q.dtype, q.shape
+    if len(shape) != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != shape[0] or k.shape[2] != shape[2])):
         raise ValueError("qk_norm_rope expects q [T, Hq, D] and k [T, Hk, D]")
-    T, hq, D = q.shape
+    T, hq, D = shape
     hk = 0 if k is None else k.shape[1]
-    if k is not None and k.dtype != q.dtype:
-        raise ValueError(f"q and k differ in type: {q.dtype}, {k.dtype}")
+    if k is not None and k.dtype is not dtype:
+        raise ValueError(f"q and k differ in type: {dtype}, {k.dtype}")
     if D % 16 or D == 0 or D > 256:
         raise ValueError(f"the head's width must be a multiple of 16 up to 256, got {D}")
+    axes = pairs = 0
     if rotary is not None:
-        if 2 * rotary.pairs > D:
-            raise ValueError(f"{2 * rotary.pairs} rotated channels exceed the head's {D}")
-        axes = len(rotary.dims)
+        axes, pairs = len(rotary.dims), rotary.pairs
+        if 2 * pairs > D:
+            raise ValueError(f"{2 * pairs} rotated channels exceed the head's {D}")
         if positions is None or positions.dtype not in _POSITIONS:
             raise ValueError("positions must be an int32, int64 or float32 tensor")
-        if positions.dim() == 1 and axes == 1:
+        if axes == 1 and positions.dim() == 1:
             positions = positions[:, None]
         if positions.shape != (T, axes):
             raise ValueError(f"positions must be [{T}, {axes}], got {tuple(positions.shape)}")
@@ -170,9 +191,13 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: 
         _check_out(out[0], q, "qk_norm_rope")
         if k is not None:
             _check_out(out[1], k, "qk_norm_rope")
-    _same_device(q.device, k, positions, q_weight, k_weight)
-    _forward_only("qk_norm_rope", q, k, q_weight, k_weight)
-    code = _dtype_code("qk_norm_rope", q)
+    index = q.get_device()
+    for t in (k, positions, q_weight, k_weight):
+        if t is not None and t.get_device() != index:
+            _same_device(q.device, t)
+    if torch.is_grad_enabled():
+        _forward_only("qk_norm_rope", q, k, q_weight, k_weight)
+    code = _dtype_code("qk_norm_rope", dtype)
     if not q.is_cuda:
         result = host_block.qk_norm_rope(q, k, positions, rotary, q_weight, k_weight, norm, eps)
         if out is None:
@@ -182,44 +207,50 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: 
             out[1].copy_(result[1])
         return out
 
-    lib = _lib(q.device)
+    device = q.device
+    lib = _lib(device)
+    qw = kw = None
+    wide = False
     if norm:
-        weights = [w for w in (q_weight, k_weight) if w is not None]
-        if any(w.dtype != q.dtype for w in weights):  # float32 is read as it is, and serves any mixture
+        wide = ((q_weight is not None and q_weight.dtype is not dtype)
+                or (k_weight is not None and k_weight.dtype is not dtype))
+        if wide:  # float32 is read as it is, and serves any mixture
             q_weight, k_weight = (None if w is None else w.to(torch.float32) for w in (q_weight, k_weight))
-        q_weight, k_weight = (None if w is None else w if w.is_contiguous() and w.data_ptr() % 16 == 0
-                              else w.clone(memory_format=torch.contiguous_format) for w in (q_weight, k_weight))
-    wide = any(w is not None and w.dtype == torch.float32 for w in (q_weight, k_weight))
+        if q_weight is not None:
+            q_weight = _vector(q_weight)
+            qw = q_weight.data_ptr()
+        if k_weight is not None:
+            k_weight = _vector(k_weight)
+            kw = k_weight.data_ptr()
     q, qt, qh = _heads(q)
     if out is None:
-        qo, qot, qoh = torch.empty((T, hq, D), dtype=q.dtype, device=q.device), hq * D, D
+        qo, qot, qoh = q.new_empty((T, hq, D)), hq * D, D
     else:
         qo, qot, qoh = _heads(out[0])
-    ko, kt, kh, kot, koh = None, 0, 0, 0, 0
+    ko = k_ptr = ko_ptr = None
+    kt = kh = kot = koh = 0
     if k is not None:
         k, kt, kh = _heads(k)
         if out is None:
-            ko, kot, koh = torch.empty((T, hk, D), dtype=q.dtype, device=q.device), hk * D, D
+            ko, kot, koh = k.new_empty((T, hk, D)), hk * D, D
         else:
             ko, kot, koh = _heads(out[1])
-    device = q.device
-    stream = _raw_stream(device.index)
+        k_ptr, ko_ptr = k.data_ptr(), ko.data_ptr()
+    stream = _raw_stream(index)
     pos_ptr = turns = axis = None
-    pos_type = ld = axes = pairs = 0
+    pos_type = ld = 0
     if rotary is not None:
-        axes, pairs = len(rotary.dims), rotary.pairs
-        if positions.stride(1) != 1 and axes > 1 or positions.stride(0) < axes:
+        if not positions.is_contiguous() and (positions.stride(0) < axes or (axes > 1 and positions.stride(1) != 1)):
             positions = positions.contiguous()
         pos_ptr, pos_type = positions.data_ptr(), _POSITIONS[positions.dtype]
         ld = positions.stride(0) if T > 1 else axes
-        t, x = rotary.tables(device)
-        turns, axis = t.on(stream), x.on(stream)
-    with _on(device):
+        tables = rotary._tables.get(index) or rotary.tables(device)
+        turns, axis = tables[0].on(stream), tables[1].on(stream)
+    with _current(index, device):
         status = lib.hf_qk_norm_rope(
-            q.data_ptr(), qt, qh, hq, None if k is None else k.data_ptr(), kt, kh, hk, qo.data_ptr(), qot, qoh,
-            None if ko is None else ko.data_ptr(), kot, koh, pos_ptr, pos_type, ld, axes, turns, axis, pairs,
-            rotary is not None and rotary.interleaved, norm, None if q_weight is None else q_weight.data_ptr(),
-            None if k_weight is None else k_weight.data_ptr(), wide, eps, T, D, code, stream)
+            q.data_ptr(), qt, qh, hq, k_ptr, kt, kh, hk, qo.data_ptr(), qot, qoh, ko_ptr, kot, koh, pos_ptr, pos_type,
+            ld, axes, turns, axis, pairs, rotary is not None and rotary.interleaved, norm, qw, kw, wide, eps, T, D,
+            code, stream)
     _check(status, "hf_qk_norm_rope")
     if out is None:
         return qo, ko
@@ -288,7 +319,10 @@ class AttentionPlan(_Plan):
         if self.head_dim < 16 or self.head_dim % 16 or self.head_dim > 128:
             raise ValueError(f"head_dim must be a multiple of 16 up to 128, got {head_dim}")
         self.q_rows, self.kv_rows = sum(self.q_lengths), sum(self.kv_lengths)
+        self._q_shape = (self.q_rows, self.heads, self.head_dim)
+        self._kv_shape = (self.kv_rows, self.kv_heads, self.head_dim)
         self.device = _plan_device(device)
+        self._index = -1 if self.device.index is None else self.device.index
         if self.device.type != "cuda":
             return
         lib = _lib(self.device)
@@ -302,7 +336,7 @@ class AttentionPlan(_Plan):
 def _keys(t: Tensor) -> tuple[Tensor, int, int]:
     """`_heads` for keys and values, whose rows may not overlap nor lie 2^23 elements apart or more."""
     t, token, head = _heads(t)
-    if t.shape[0] > 1 and not t.shape[2] <= token < 1 << 23:
+    if not t.shape[2] <= token < 1 << 23 and t.shape[0] > 1:
         t = torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
         token, head = t.shape[1] * t.shape[2], t.shape[2]
     return t, token, head
@@ -317,39 +351,42 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, *, sc
     ``head_dim ** -0.5``) is positive. A query that sees no key gets zeros; what k and v hold at keys that a query does
     not see never reaches it. Scores, weights' sums and outputs are summed in float32; the weights enter the second
     product in the inputs' type."""
-    d = plan.head_dim
-    if q.shape != (plan.q_rows, plan.heads, d) or k.shape != (plan.kv_rows, plan.kv_heads, d) or k.shape != v.shape:
-        raise ValueError(f"the plan is for q ({plan.q_rows}, {plan.heads}, {d}) and k, v ({plan.kv_rows}, "
-                         f"{plan.kv_heads}, {d}); got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise ValueError(f"q, k and v differ in type: {q.dtype}, {k.dtype}, {v.dtype}")
-    code = _dtype_code("packed_attention", q)
-    scale = d ** -0.5 if scale is None else float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
+    if q.shape != plan._q_shape or k.shape != plan._kv_shape or v.shape != plan._kv_shape:
+        raise ValueError(f"the plan is for q {plan._q_shape} and k, v {plan._kv_shape}; got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    dtype = q.dtype
+    if k.dtype is not dtype or v.dtype is not dtype:
+        raise ValueError(f"q, k and v differ in type: {dtype}, {k.dtype}, {v.dtype}")
+    code = _dtype_code("packed_attention", dtype)
+    scale = plan.head_dim ** -0.5 if scale is None else float(scale)
+    if not 0 < scale < math.inf:
         raise ValueError(f"scale must be positive and finite, got {scale}")
     if out is not None:
         _check_out(out, q, "packed_attention")
-    _same_device(q.device, k, v)
-    if q.device != plan.device:
+    index = q.get_device()
+    if k.get_device() != index or v.get_device() != index or index != plan._index:
+        _same_device(q.device, k, v)
         raise ValueError(f"tensors on {q.device}, the plan is for {plan.device}")
-    _forward_only("packed_attention", q, k, v)
+    if torch.is_grad_enabled():
+        _forward_only("packed_attention", q, k, v)
     if not q.is_cuda:
         result = host_block.packed_attention(q, k, v, plan, scale)
         return result if out is None else out.copy_(result)
-    lib = _lib(q.device)
+    device = plan.device
+    lib = _lib(device)
     q, qt, qh = _heads(q)
     k, kt, kh = _keys(k)
     v, vt, vh = _keys(v)
     if out is None:
-        o, ot, oh = torch.empty(q.shape, dtype=q.dtype, device=q.device), plan.heads * d, d
+        o, ot, oh = q.new_empty(plan._q_shape), plan.heads * plan.head_dim, plan.head_dim
     else:
         o, ot, oh = _heads(out)
-    stream = _raw_stream(q.get_device())
-    with _on(q.device):
-        ws, nbytes = _workspace(q.device, plan.ws_bytes)
+    stream = _raw_stream(index)
+    nbytes = plan.ws_bytes
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device).data_ptr() if nbytes else None
+    with _current(index, device):
         status = lib.hf_attention(q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, o.data_ptr(), ot,
-                                  oh, scale, plan._host, plan.data.on(stream), plan.bytes,
-                                  None if ws is None else ws.data_ptr(), nbytes, code, stream)
+                                  oh, scale, plan._host, plan.data.on(stream), plan.bytes, ws, nbytes, code, stream)
     _check(status, "hf_attention")
     return o if out is None or o is out else out.copy_(o)
 
@@ -371,7 +408,9 @@ class AdapterPlan(_Plan):
         if any(not -1 <= i < self.adapters for i in self.ids):
             raise ValueError(f"adapters must be -1 .. {self.adapters - 1}, got {sorted(set(self.ids))}")
         self.rows = sum(self.lengths)
+        self.live_rows = sum(n for i, n in zip(self.ids, self.lengths) if i >= 0)
         self.device = _plan_device(device)
+        self._index = -1 if self.device.index is None else self.device.index
         self._ws: dict[tuple[int, int, int], int] = {}
         if self.device.type != "cuda":
             return
@@ -381,25 +420,22 @@ class AdapterPlan(_Plan):
                    ctypes.addressof(lens_c), len(self.ids), self.adapters, cus)
 
     def _ws_bytes(self, lib: ctypes.CDLL, K: int, N: int, r: int) -> int:
-        key = (K, N, r)
-        found = self._ws.get(key)
-        if found is None:
-            found = lib.hf_adapter_ws_bytes(self._host, self.bytes, K, N, r)
-            _check(min(found, 0), "hf_adapter_ws_bytes")
-            self._ws[key] = found
+        found = lib.hf_adapter_ws_bytes(self._host, self.bytes, K, N, r) if N else 0
+        _check(min(found, 0), "hf_adapter_ws_bytes")
+        self._ws[K, N, r] = found
         return found
 
 
 def _rows16(t: Tensor) -> Tensor:
     """``t`` [rows, columns] with columns side by side, row strides in whole 16-byte vectors and such a start."""
-    if (t.stride(1) == 1 or t.shape[1] == 1) and t.data_ptr() % 16 == 0 and (
-            t.shape[0] <= 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1])):
+    if t.data_ptr() % 16 == 0 and (t.is_contiguous() or (
+            (t.stride(1) == 1 or t.shape[1] == 1) and t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1])):
         return t
     return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
 
 
 def _rows2(t: Tensor) -> Tensor:
-    if (t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1]):
+    if t.is_contiguous() or ((t.stride(1) == 1 or t.shape[1] == 1) and (t.shape[0] <= 1 or t.stride(0) >= t.shape[1])):
         return t
     return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
 
@@ -416,8 +452,9 @@ def adapter_add(y: Tensor, x: Tensor, down: Tensor, up: Tensor, plan: AdapterPla
     ``x`` [M, K], ``y`` [M, N], ``down`` [adapters, r, K], ``up`` [adapters, N, r] in one type (bfloat16 or float16),
     ``scale`` float32 [adapters] (None: ones). Summed in float32, rounded once. ``out`` may be ``y``, which is then
     updated in place. K is a multiple of 8, r of 8 up to 512."""
-    if x.dim() != 2 or y.dim() != 2 or x.shape[0] != plan.rows or y.shape[0] != plan.rows:
-        raise ValueError(f"the plan has {plan.rows} rows; got x {tuple(x.shape)}, y {tuple(y.shape)}")
+    rows = plan.rows
+    if x.dim() != 2 or y.dim() != 2 or x.shape[0] != rows or y.shape[0] != rows:
+        raise ValueError(f"the plan has {rows} rows; got x {tuple(x.shape)}, y {tuple(y.shape)}")
     K, N = x.shape[1], y.shape[1]
     if down.dim() != 3 or down.shape[0] != plan.adapters or down.shape[2] != K:
         raise ValueError(f"down must be [{plan.adapters}, r, {K}], got {tuple(down.shape)}")
@@ -426,34 +463,45 @@ def adapter_add(y: Tensor, x: Tensor, down: Tensor, up: Tensor, plan: AdapterPla
         raise ValueError(f"up must be [{plan.adapters}, {N}, {r}], got {tuple(up.shape)}")
     if K % 8 or K == 0 or r % 8 or not 0 < r <= 512:
         raise ValueError(f"K must be a multiple of 8 and r one up to 512, got K={K}, r={r}")
-    if any(t.dtype != y.dtype for t in (x, down, up)):
-        raise ValueError(f"y, x, down and up differ in type: {y.dtype}, {x.dtype}, {down.dtype}, {up.dtype}")
-    if scale is not None and (scale.shape != (plan.adapters,) or scale.dtype != torch.float32):
+    dtype = y.dtype
+    if x.dtype is not dtype or down.dtype is not dtype or up.dtype is not dtype:
+        raise ValueError(f"y, x, down and up differ in type: {dtype}, {x.dtype}, {down.dtype}, {up.dtype}")
+    if scale is not None and (scale.shape != (plan.adapters,) or scale.dtype is not torch.float32):
         raise ValueError(f"scale must be float32 [{plan.adapters}]")
     if out is not None:
         _check_out(out, y, "adapter_add")
-    code = _dtype_code("adapter_add", y)
-    _same_device(y.device, x, down, up, scale)
-    if y.device != plan.device:
+    code = _dtype_code("adapter_add", dtype)
+    index = y.get_device()
+    if (x.get_device() != index or down.get_device() != index or up.get_device() != index or index != plan._index
+            or (scale is not None and scale.get_device() != index)):
+        _same_device(y.device, x, down, up, scale)
         raise ValueError(f"tensors on {y.device}, the plan is for {plan.device}")
-    _forward_only("adapter_add", y, x, down, up, scale)
+    if torch.is_grad_enabled():
+        _forward_only("adapter_add", y, x, down, up, scale)
+    if plan.live_rows == 0:  # no row has an adapter: y itself
+        return y.clone() if out is None else out if out is y else out.copy_(y)
     if not y.is_cuda:
         result = host_block.adapter_add(y, x, down, up, plan, scale)
         return result if out is None else out.copy_(result)
-    lib = _lib(y.device)
+    device = plan.device
+    lib = _lib(device)
     in_place = out is y
     x, y = _rows16(x), _rows2(y)
-    down, up = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
-                for t in (down, up))
+    if not down.is_contiguous() or down.data_ptr() % 16:
+        down = down.clone(memory_format=torch.contiguous_format)
+    if not up.is_contiguous() or up.data_ptr() % 16:
+        up = up.clone(memory_format=torch.contiguous_format)
     if scale is not None and not scale.is_contiguous():
         scale = scale.contiguous()
-    o = y if in_place else torch.empty(y.shape, dtype=y.dtype, device=y.device) if out is None else _rows2(out)
-    stream = _raw_stream(y.get_device())
-    with _on(y.device):
-        ws, nbytes = _workspace(y.device, plan._ws_bytes(lib, K, N, r) if N else 0)
+    o = y if in_place else y.new_empty((rows, N)) if out is None else _rows2(out)
+    stream = _raw_stream(index)
+    with _current(index, device):
+        nbytes = plan._ws.get((K, N, r))
+        if nbytes is None:
+            nbytes = plan._ws_bytes(lib, K, N, r)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device).data_ptr() if nbytes else None
         status = lib.hf_adapter_add(x.data_ptr(), _ld(x), y.data_ptr(), _ld(y), down.data_ptr(), up.data_ptr(), r,
                                     None if scale is None else scale.data_ptr(), o.data_ptr(), _ld(o), N, K,
-                                    plan._host, plan.data.on(stream), plan.bytes,
-                                    None if ws is None else ws.data_ptr(), nbytes, code, stream)
+                                    plan._host, plan.data.on(stream), plan.bytes, ws, nbytes, code, stream)
     _check(status, "hf_adapter_add")
     return o if out is None or o is out else out.copy_(o)

@@ -83,6 +83,18 @@ __host__ __device__ constexpr int ad_down_lds(int rb, int nb, int nw) {
   return ad_stages(rb, nb, nw) * ad_stage_bytes(rb, nb) * nw;
 }
 
+// Waits until at most n of the wave's loads are on their way (n from 2 to 24, any other: none).
+__device__ __forceinline__ void ad_wait(int n) {
+  switch (n) {
+#define HF_WAIT(N) case N: asm volatile("s_waitcnt vmcnt(" #N ")" ::: "memory"); break;
+    HF_WAIT(2) HF_WAIT(3) HF_WAIT(4) HF_WAIT(5) HF_WAIT(6) HF_WAIT(7) HF_WAIT(8) HF_WAIT(9) HF_WAIT(10) HF_WAIT(11)
+    HF_WAIT(12) HF_WAIT(13) HF_WAIT(14) HF_WAIT(15) HF_WAIT(16) HF_WAIT(17) HF_WAIT(18) HF_WAIT(19) HF_WAIT(20)
+    HF_WAIT(21) HF_WAIT(22) HF_WAIT(23) HF_WAIT(24)
+#undef HF_WAIT
+    default: asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); break;
+  }
+}
+
 // Tile blockIdx.x, K share blockIdx.y, ranks from 32 RB blockIdx.z on.
 //
 // Each wave streams its own steps of 64 k through a ring of its own in LDS (16 bytes a lane, whole 128-byte lines, past
@@ -100,7 +112,8 @@ __global__ __launch_bounds__(64 * NW, 1) void adapter_down_kernel(AdapterArgs a)
   unsigned char HF_LDS* ring = (unsigned char HF_LDS*)ad_lds + wave * S * kStage;
 
   // Load i of a step fills rows 8i .. 8i + 7 of the step's NB x 32 rows of x and RB x 32 of A; lane l row l / 8, from
-  // chunk swizzle128(row, l % 8). Rows past the tile or the rank repeat the last one; what comes of them is not used.
+  // chunk swizzle128(row, l % 8). Groups of 8 rows past the tile or the rank are not loaded, and rows past them within a
+  // group repeat the last one: what comes of them is not used.
   const uint16_t* from[kLoads];
 #pragma unroll
   for (int i = 0; i < kLoads; ++i) {
@@ -112,12 +125,16 @@ __global__ __launch_bounds__(64 * NW, 1) void adapter_down_kernel(AdapterArgs a)
   const int64_t share = (full + a.splits - 1) / a.splits;
   const int64_t c_lo = min(share * blockIdx.y, full), c_hi = min(c_lo + share, full);
   const int steps = c_hi - c_lo > wave ? (int)((c_hi - c_lo - wave + NW - 1) / NW) : 0;
-  auto load = [&](int step, int slot) {
+  const int x_loads = min(4 * NB, (tile.count + 7) / 8);
+  const int loads = x_loads + min(4 * RB, (a.r - rank0) / 8);
+  auto load = [&](int step, int slot) __attribute__((always_inline)) {
     const int64_t k0 = (c_lo + wave + (int64_t)step * NW) * kAdChunk;
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i)
+    for (int i = 0; i < kLoads; ++i) {
+      if (i < 4 * NB ? i >= x_loads : i - 4 * NB >= loads - x_loads) continue;
       __builtin_amdgcn_global_load_lds((const void __attribute__((address_space(1)))*)(from[i] + k0),
                                        (void HF_LDS*)(ring + slot * kStage + i * 1024), 16, 0, 0);
+    }
   };
 
   v16f acc[RB][NB];
@@ -132,14 +149,8 @@ __global__ __launch_bounds__(64 * NW, 1) void adapter_down_kernel(AdapterArgs a)
 #pragma unroll 1
   for (int step = 0; step < steps; ++step) {
     // The step's loads have landed; those of the S - 1 steps after it may be on their way.
-    constexpr int kAhead = (S - 1) * kLoads;
-    static_assert(kAhead == 8 || kAhead == 12 || kAhead == 16 || kAhead == 20 || kAhead == 24, "a wait for this ring");
-    if (step + S > steps) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    else if constexpr (kAhead == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-    else if constexpr (kAhead == 12) asm volatile("s_waitcnt vmcnt(12)" ::: "memory");
-    else if constexpr (kAhead == 16) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
-    else if constexpr (kAhead == 20) asm volatile("s_waitcnt vmcnt(20)" ::: "memory");
-    else asm volatile("s_waitcnt vmcnt(24)" ::: "memory");
+    static_assert((S - 1) * kLoads <= 24, "a wait for this ring");
+    ad_wait(step + S > steps ? 0 : (S - 1) * loads);
     const unsigned char HF_LDS* at = ring + slot * kStage;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {

@@ -59,21 +59,6 @@ __device__ __forceinline__ int at_swizzle(int r) {
 // Floats of a workspace tile of `rows` rows: O [rows][32 DB], then m and l per row.
 __host__ __device__ constexpr int at_slot_floats(int rows, int db) { return rows * (32 * db + 2); }
 
-// 16 bytes a lane from the buffer's byte `off` to LDS, lane l to dst + 16 l. The builtin for it makes the compiler wait
-// for every such load before any transposing read of LDS, those of the other buffer's next tile among them (3 % of the
-// time of long sequences); as an asm it stays out of that count, and the loop's own waits order it. It has no output
-// register, and its address registers are read when it issues.
-// The s_nop covers the distance that the load needs from scalar registers and m0 written just before it.
-__device__ __forceinline__ void at_load_lds(v4i rsrc, unsigned char HF_LDS* dst, uint32_t off) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
-               :: "s"((uint32_t)(uintptr_t)dst), "v"(off), "s"(rsrc) : "memory");
-}
-// The raw descriptor (stride 0) of `bytes` bytes from `base` on: bytes at and after its end read as zero.
-__device__ __forceinline__ v4i at_rsrc(const void* base, uint32_t bytes) {
-  const uint64_t p = (uint64_t)base;
-  return (v4i){(int)(uint32_t)p, (int)((uint32_t)(p >> 32) & 0xffffu), (int)bytes, 0x00020000};
-}
-
 // Every load has landed, the queries' among them: told to the compiler here, it need not wait for them inside a loop, where
 // it would wait for the next tile too.
 __device__ __forceinline__ void at_landed() { __builtin_amdgcn_s_waitcnt(0x0f70); }
@@ -148,12 +133,13 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_kernel(Att
   auto load_tile = [&](const uint16_t* base, int stride, uint32_t (&part)[kParts], int t, unsigned char HF_LDS* dst,
                        bool zeros = false) __attribute__((always_inline)) {
     const int rows = min(kAtKeys, it.nk - it.key_lo - t * kAtKeys);
-    const v4i rsrc =
-        at_rsrc(base + (int64_t)t * kAtKeys * stride, zeros ? 0u : (uint32_t)((rows - 1) * stride * 2 + a.D * 2));
+    const __amdgpu_buffer_rsrc_t rsrc =
+        make_rsrc(base + (int64_t)t * kAtKeys * stride, zeros ? 0u : (uint32_t)((rows - 1) * stride * 2 + a.D * 2));
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int blk = NW * i + wave;
-      at_load_lds(rsrc, dst + blk * 1024, part[i % kParts] + (uint32_t)(blk * kRowsPerLoad * stride * 2));
+      const uint32_t off = part[i % kParts] + (uint32_t)(blk * kRowsPerLoad * stride * 2);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (void HF_LDS*)(dst + blk * 1024), 16, off, 0, 0, 0);
     }
   };
 

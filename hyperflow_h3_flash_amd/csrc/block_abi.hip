@@ -350,17 +350,17 @@ int hf_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, int32_t head
   a.side[1] = {(const uint16_t*)k, (uint16_t*)k_out, kw, k_token, k_head, ko_token, ko_head, heads_k};
   a.pos = pos, a.ld_pos = ld_pos, a.turns = turns, a.axis = axis, a.T = T, a.pos_type = pos_type, a.pairs = pairs;
   a.D = D, a.weight_f32 = weight_f32, a.eps = eps;
-  // A workgroup takes 4 tokens of all heads when that still gives every compute unit several; with fewer tokens one
+  // A workgroup takes 4 tokens of a side's heads when that still gives every compute unit several; with fewer tokens one
   // token, and then a share of its heads, down to one round of rows.
   const int lanes = D <= 64 ? 4 : D <= 128 ? 8 : 16, round = hf::kRopeThreads / lanes;
   const int64_t cus = compute_units();
-  const int64_t heads = heads_q + heads_k;
+  const int64_t heads = std::max(heads_q, heads_k);
   a.tokens = T >= 16 * cus ? 4 : 1;
   const int64_t groups = (T + a.tokens - 1) / a.tokens;
   int64_t parts = std::min(std::max((int64_t)1, 4 * cus / groups), (heads + round - 1) / round);
   a.heads_per_wg = (int)((heads + parts - 1) / parts);
   parts = (heads + a.heads_per_wg - 1) / a.heads_per_wg;
-  const dim3 grid((unsigned)groups, (unsigned)parts);
+  const dim3 grid((unsigned)groups, (unsigned)parts, heads_k > 0 ? 2 : 1);
   const size_t lds = (size_t)a.tokens * pairs * sizeof(float) * 2;
   if (dtype == HF_BF16) launch_rope_lanes<hf::Bf16>(a, lanes, interleaved, norm, grid, lds, (hipStream_t)stream);
   else launch_rope_lanes<hf::Fp16>(a, lanes, interleaved, norm, grid, lds, (hipStream_t)stream);

@@ -9,8 +9,8 @@
 // chunk with chunk, interleaved pairs lie inside a chunk. Channels after the rotary width are taken two neighbouring
 // chunks a lane. The sum of squares goes over LPR lanes by lane exchanges.
 //
-// A workgroup takes all heads (or a share of them, when there are few tokens) of a few tokens: their sines and cosines
-// are computed once into LDS and serve every head. The angle is reduced in fp64 to less than half a turn before the
+// A workgroup takes all query heads or all key heads (or a share of them, when there are few tokens) of a few tokens: their
+// sines and cosines are computed once into LDS and serve every head. The angle is reduced in fp64 to less than half a turn before the
 // sine, so positions of any size keep the sine's own accuracy: one fp64 product a token and pair, for 64 to 112 heads.
 #pragma once
 
@@ -46,21 +46,30 @@ __device__ __forceinline__ double rope_position(const RopeArgs& a, int64_t at) {
   return (double)((const float*)a.pos)[at];
 }
 
+// 8 weights from d on, in fp32.
+template <class T>
+__device__ __forceinline__ void rope_weights(const void* w, int d, bool f32, float* out) {
+  if (f32) {
+    const v4f a = *(const v4f*)((const float*)w + d), b = *(const v4f*)((const float*)w + d + 4);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = a[e], out[4 + e] = b[e];
+  } else {
+    const v4u a = *(const v4u*)((const uint16_t*)w + d);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[2 * e] = T::lo(a[e]), out[2 * e + 1] = T::hi(a[e]);
+  }
+}
+
+// Tokens blockIdx.x * tokens .., heads blockIdx.y * heads_per_wg .. of side blockIdx.z.
 template <class T, int LPR, bool INTERLEAVED, bool NORM>
 __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(RopeArgs a) {
   extern __shared__ v2f rope_table[];  // [tokens][pairs] of (cos, sin)
+  const RopeSide s = a.side[blockIdx.z];
+  const int h_lo = blockIdx.y * a.heads_per_wg, nh = min(h_lo + a.heads_per_wg, s.heads) - h_lo;
+  if (nh <= 0) return;
   const int tid = threadIdx.x;
   const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
   const int nt = (int)min((int64_t)a.tokens, a.T - t0);
-  for (int i = tid; i < nt * a.pairs; i += kRopeThreads) {
-    const int t = i / a.pairs, p = i - t * a.pairs;
-    const double turn = rope_position(a, (t0 + t) * a.ld_pos + a.axis[p]) * a.turns[p];
-    const float part = (float)(turn - rint(turn));
-    float s, c;
-    sincospif(2.0f * part, &s, &c);
-    rope_table[i] = (v2f){c, s};
-  }
-  __syncthreads();
 
   constexpr int kRows = kRopeThreads / LPR;
   const int lane = tid % LPR, row = tid / LPR;
@@ -69,90 +78,88 @@ __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(RopeArgs a) 
   // First channels of the lane's two chunks.
   const int c0 = rotary ? 8 * lane : 2 * a.pairs + 16 * (lane - rotary_lanes);
   const int c1 = rotary ? a.pairs + 8 * lane : c0 + 8;
-  const int h_lo = blockIdx.y * a.heads_per_wg;
-  const int h_hi = min(h_lo + a.heads_per_wg, a.side[0].heads + a.side[1].heads);
 
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    const RopeSide s = a.side[which];
-    const int first = which ? a.side[0].heads : 0;
-    const int lo = max(h_lo, first) - first, nh = min(h_hi, first + s.heads) - first - lo;
-    if (nh <= 0) continue;
-    float w[16];
-    if (NORM) {
+  // Rows (t, h) of this side in order, kRows of them at a time; U of those rounds are on their way before the first is
+  // used, the first ones before the table is made.
+  constexpr int U = 4;
+  const int rows = nt * nh;
+  v4u in[U][2];
+  int tt[U], hh[U];
+  auto load = [&](int r0) __attribute__((always_inline)) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int d = (e < 8 ? c0 : c1 - 8) + e;
-        w[e] = 1.0f;
-        if (active && s.w) {
-          if (a.weight_f32) {
-            w[e] = ((const float*)s.w)[d];
-          } else {
-            w[e] = T::lo(((const uint16_t*)s.w)[d]);
-          }
-        }
+    for (int u = 0; u < U; ++u) {
+      const int r = r0 + u * kRows;
+      tt[u] = r / nh;
+      hh[u] = h_lo + (r - tt[u] * nh);
+      in[u][0] = in[u][1] = (v4u){0, 0, 0, 0};
+      if (r < rows && active) {
+        const uint16_t* x = s.x + (t0 + tt[u]) * s.x_token + hh[u] * s.x_head;
+        in[u][0] = *(const v4u*)(x + c0);
+        in[u][1] = *(const v4u*)(x + c1);
       }
     }
-    // Rows (t, h) of this side in order, kRows of them at a time; U of those rounds are loaded before the first is
-    // used.
-    constexpr int U = 4;
-    const int rows = nt * nh;
-    for (int r0 = row; r0 < rows; r0 += kRows * U) {
-      v4u in[U][2];
-      int tt[U], hh[U];
+  };
+  load(row);
+  float w[16];
+  if (NORM) {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int r = r0 + u * kRows;
-        tt[u] = r / nh;
-        hh[u] = lo + (r - tt[u] * nh);
-        if (r < rows && active) {
-          const uint16_t* x = s.x + (t0 + tt[u]) * s.x_token + hh[u] * s.x_head;
-          in[u][0] = *(const v4u*)(x + c0);
-          in[u][1] = *(const v4u*)(x + c1);
-        } else {
-          in[u][0] = in[u][1] = (v4u){0, 0, 0, 0};
-        }
+    for (int e = 0; e < 16; ++e) w[e] = 1.0f;
+    if (active && s.w) {
+      rope_weights<T>(s.w, c0, a.weight_f32, w);
+      rope_weights<T>(s.w, c1, a.weight_f32, w + 8);
+    }
+  }
+  for (int i = tid; i < nt * a.pairs; i += kRopeThreads) {
+    const int t = i / a.pairs, p = i - t * a.pairs;
+    const double turn = rope_position(a, (t0 + t) * a.ld_pos + a.axis[p]) * a.turns[p];
+    const float part = (float)(turn - rint(turn));
+    float sin, cos;
+    sincospif(2.0f * part, &sin, &cos);
+    rope_table[i] = (v2f){cos, sin};
+  }
+  __syncthreads();
+
+  for (int r0 = row; r0 < rows; r0 += kRows * U) {
+    if (r0 != row) load(r0);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float x[16];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[2 * e] = T::lo(in[u][e / 4][e % 4]);
+        x[2 * e + 1] = T::hi(in[u][e / 4][e % 4]);
       }
+      if (NORM) {
+        float sum = 0.0f;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float x[16];
+        for (int e = 0; e < 16; ++e) sum = fmaf(x[e], x[e], sum);
+#pragma unroll
+        for (int off = LPR / 2; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        const float r = 1.0f / sqrtf(sum / (float)a.D + a.eps);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[e] = (x[e] * r) * w[e];
+      }
+      if (r0 + u * kRows >= rows || !active) continue;
+      if (rotary) {
+        const v2f* table = rope_table + tt[u] * a.pairs;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          x[2 * e] = T::lo(in[u][e / 4][e % 4]);
-          x[2 * e + 1] = T::hi(in[u][e / 4][e % 4]);
+          // Interleaved: pair e % 4 of chunk e / 4; halves: channel e of both chunks.
+          const int p = INTERLEAVED ? (e < 4 ? c0 / 2 : c1 / 2 - 4) + e : c0 + e;
+          const int i = INTERLEAVED ? 2 * e : e, j = INTERLEAVED ? 2 * e + 1 : e + 8;
+          const v2f cs = table[p];
+          const float x0 = x[i], x1 = x[j];
+          x[i] = fmaf(x0, cs[0], -(x1 * cs[1]));
+          x[j] = fmaf(x0, cs[1], x1 * cs[0]);
         }
-        if (NORM) {
-          float sum = 0.0f;
+      }
+      uint16_t* o = s.out + (t0 + tt[u]) * s.o_token + hh[u] * s.o_head;
 #pragma unroll
-          for (int e = 0; e < 16; ++e) sum = fmaf(x[e], x[e], sum);
+      for (int c = 0; c < 2; ++c) {
+        v4u v;
 #pragma unroll
-          for (int off = LPR / 2; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
-          const float r = 1.0f / sqrtf(sum / (float)a.D + a.eps);
-#pragma unroll
-          for (int e = 0; e < 16; ++e) x[e] = (x[e] * r) * w[e];
-        }
-        if (r0 + u * kRows >= rows || !active) continue;
-        if (rotary) {
-          const v2f* table = rope_table + tt[u] * a.pairs;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            // Interleaved: pair e % 4 of chunk e / 4; halves: channel e of both chunks.
-            const int p = INTERLEAVED ? (e < 4 ? c0 / 2 : c1 / 2 - 4) + e : c0 + e;
-            const int i = INTERLEAVED ? 2 * e : e, j = INTERLEAVED ? 2 * e + 1 : e + 8;
-            const v2f cs = table[p];
-            const float x0 = x[i], x1 = x[j];
-            x[i] = fmaf(x0, cs[0], -(x1 * cs[1]));
-            x[j] = fmaf(x0, cs[1], x1 * cs[0]);
-          }
-        }
-        uint16_t* o = s.out + (t0 + tt[u]) * s.o_token + hh[u] * s.o_head;
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          v4u v;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = T::pack(x[8 * c + 2 * e], x[8 * c + 2 * e + 1]);
-          *(v4u*)(o + (c ? c1 : c0)) = v;
-        }
+        for (int e = 0; e < 4; ++e) v[e] = T::pack(x[8 * c + 2 * e], x[8 * c + 2 * e + 1]);
+        *(v4u*)(o + (c ? c1 : c0)) = v;
       }
     }
   }

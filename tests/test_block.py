@@ -94,6 +94,101 @@ def test_host_adapters():
     U.check(y, *ref)
 
 
+# -------------------------------------------------------------------------------------------------------------- module
+
+def make_block(dim=64, heads=4, kv_heads=2, head_dim=16, group=16, adapters=2, device="cpu"):
+    from hyperflow_h3_flash_amd import AttentionBlock
+
+    block = AttentionBlock(dim, heads, head_dim, group, kv_heads=kv_heads, adapters=adapters, adapter_rank=5)
+    gen = torch.Generator().manual_seed(2)
+    for layer in (block.qkv, block.out):
+        layer.qweight.copy_(torch.randint(-127, 128, layer.qweight.shape, generator=gen, dtype=torch.int8))
+        layer.wscale.copy_(0.02 * torch.rand(layer.wscale.shape, generator=gen) / layer.in_features ** 0.5)
+    block.norm_q.copy_(1 + 0.1 * torch.randn(head_dim, generator=gen))
+    block.norm_k.copy_(1 + 0.1 * torch.randn(head_dim, generator=gen))
+    for bank in (block.qkv_adapters, block.out_adapters) if adapters else ():
+        for i in range(adapters):
+            bank.load(i, torch.randn(5, bank.in_features, generator=gen), torch.randn(bank.out_features, 5, generator=gen),
+                      scale=0.1 + i)
+    return block.to(device)
+
+
+def test_block_is_its_parts_and_requests_stay_alone():
+    from hyperflow_h3_flash_amd import AttentionBlock, Int8RotLinear
+
+    block = make_block()
+    lengths, ids = [5, 9, 1], [1, -1, 0]
+    x = rnd(1, 15, 64).to(BF)
+    positions = torch.randint(0, 50, (15, 2), generator=torch.Generator().manual_seed(3))
+    rotary = RotaryAxes((8, 8))
+
+    def run(rows, lengths, ids, module=block):
+        plan = AttentionPlan(lengths, heads=4, kv_heads=2, head_dim=16, causal=True, device="cpu")
+        adapters = AdapterPlan(ids, lengths, adapters=2, device="cpu") if module.qkv_adapters is not None else None
+        return module(x[rows], plan, positions=positions[rows], rotary=rotary, adapters=adapters)
+
+    whole = run(slice(0, 15), lengths, ids)
+    assert whole.shape == (15, 64) and whole.dtype is BF
+    at = 0
+    for n, i in zip(lengths, ids):
+        assert torch.equal(run(slice(at, at + n), [n], [i]), whole[at:at + n])
+        at += n
+    # the parts by hand
+    qkv = block.qkv(x)
+    plan = AdapterPlan(ids, lengths, adapters=2, device="cpu")
+    qkv = block.qkv_adapters(qkv, x, plan).view(15, 8, 16)
+    q, k = qk_norm_rope(qkv[:, :4], qkv[:, 4:6], positions, rotary, q_weight=block.norm_q, k_weight=block.norm_k)
+    o = packed_attention(q, k, qkv[:, 6:], AttentionPlan(lengths, heads=4, kv_heads=2, head_dim=16, causal=True,
+                                                         device="cpu")).reshape(15, 64)
+    assert torch.equal(block.out_adapters(block.out(o), o, plan), whole)
+    # from a model's own projections
+    layers = [Int8RotLinear(64, n, 16) for n in (64, 32, 32)]
+    for layer, rows in zip(layers, (slice(0, 64), slice(64, 96), slice(96, 128))):
+        layer.qweight.copy_(block.qkv.qweight[rows])
+        layer.wscale.copy_(block.qkv.wscale[rows])
+    again = AttentionBlock.from_projections(*layers, block.out, 16)
+    assert again.kv_heads == 2 and not any(p.requires_grad or p.is_meta for p in again.parameters())
+    plain = make_block(adapters=0)
+    plain.norm_q.fill_(1)
+    plain.norm_k.fill_(1)
+    assert torch.equal(run(slice(0, 15), lengths, ids, again), run(slice(0, 15), lengths, ids, plain))
+    banked = AttentionBlock.from_projections(*layers, block.out, 16, adapters=2, adapter_rank=8)
+    assert torch.equal(run(slice(0, 15), lengths, ids, banked), run(slice(0, 15), lengths, ids, plain))
+
+
+def test_refusals_of_the_block():
+    from hyperflow_h3_flash_amd import AdapterBank, AttentionBlock, Int8RotLinear
+
+    bank = AdapterBank(32, 16, 2, 5)
+    assert bank.rank == 8
+    for bad in (
+        lambda: AdapterBank(32, 16, 0, 8), lambda: AdapterBank(32, 16, 2, 0),
+        lambda: bank.load(2, torch.zeros(4, 32), torch.zeros(16, 4)),
+        lambda: bank.load(0, torch.zeros(9, 32), torch.zeros(16, 9)),
+        lambda: bank.load(0, torch.zeros(4, 32), torch.zeros(16, 5)),
+        lambda: make_block(adapters=0)(rnd(1, 3, 64).to(BF), AttentionPlan([3], heads=4, kv_heads=2, head_dim=16,
+                                                                          device="cpu"),
+                                       adapters=AdapterPlan([0], [3], adapters=1, device="cpu")),
+        lambda: AttentionBlock.from_projections(*(Int8RotLinear(64, n, 16) for n in (64, 32, 64)),
+                                                Int8RotLinear(64, 64, 16), 16),
+        lambda: AttentionBlock.from_projections(*(Int8RotLinear(64, 64, 16) for _ in range(3)),
+                                                Int8RotLinear(32, 64, 16), 16),
+    ):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_example_runs_on_the_host():
+    import importlib.util
+
+    spec = importlib.util.spec_from_file_location("example", os.path.join(_native.REPO_DIR, "examples",
+                                                                          "packed_attention_block.py"))
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    y = example.main(requests=((2, 2, 3), (1, 2, 2), (1, 1, 1)), dim=256, heads=2, device="cpu")
+    assert y.shape == (17, 256) and y.isfinite().all()
+
+
 # ----------------------------------------------------------------------------------------------------------- refusals
 
 def test_refusals_of_the_norm_and_rotation():

@@ -333,6 +333,28 @@ def test_adapter_strides():
         assert (out[:, :3] == 0).all()
 
 
+# -------------------------------------------------------------------------------------------------------------- module
+
+def test_block_equals_its_parts():
+    from test_block import make_block
+
+    block = make_block(dim=512, heads=8, kv_heads=2, head_dim=64, group=256, device="cuda")
+    lengths, ids = [5, 300, 1, 64], [1, -1, 0, 1]
+    T = sum(lengths)
+    x = rnd(1, T, 512).to(BF)
+    positions = torch.randint(0, 50, (T, 2), generator=torch.Generator().manual_seed(3)).cuda()
+    rotary = RotaryAxes((32, 32))
+    plan = AttentionPlan(lengths, heads=8, kv_heads=2, head_dim=64)
+    adapters = AdapterPlan(ids, lengths, adapters=2)
+    got = block(x, plan, positions=positions, rotary=rotary, adapters=adapters)
+    qkv = block.qkv_adapters(block.qkv(x), x, adapters).view(T, 12, 64)
+    q, k = qk_norm_rope(qkv[:, :8], qkv[:, 8:10], positions, rotary, q_weight=block.norm_q, k_weight=block.norm_k)
+    o = packed_attention(q, k, qkv[:, 10:], plan)
+    U.check(o, *U.attention(q, k, qkv[:, 10:], lengths, lengths, False, 64 ** -0.5))
+    o = o.view(T, 512)
+    assert torch.equal(block.out_adapters(block.out(o), o, adapters), got)
+
+
 # ------------------------------------------------------------------------------------------------------------ streams
 
 def test_plans_on_another_stream_and_in_a_graph():
