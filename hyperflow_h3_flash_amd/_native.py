@@ -87,7 +87,7 @@ BLOCK_SIGNATURES = {
     "hf_attention": ([_P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _P, _I64, _I64, _F, _P, _P, _I64, _P, _I64,
                       _I32, _P], ctypes.c_int),
     "hf_adapter_plan": ([_P, _P, _I64, _I32, _I32, _P, _I64], ctypes.c_int64),
-    "hf_adapter_ws_bytes": ([_P, _I64, _I64, _I64, _I32], ctypes.c_int64),
+    "hf_adapter_ws_bytes": ([_P, _I64, _I64, _I32, _I32], ctypes.c_int64),
     "hf_adapter_add": ([_P, _I64, _P, _I64, _P, _P, _I32, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _I32, _P],
                        ctypes.c_int),
 }

@@ -419,10 +419,10 @@ class AdapterPlan(_Plan):
         self._fill("hf_adapter_plan", _lib(self.device), self.device, ctypes.addressof(ids_c),
                    ctypes.addressof(lens_c), len(self.ids), self.adapters, cus)
 
-    def _ws_bytes(self, lib: ctypes.CDLL, K: int, N: int, r: int) -> int:
-        found = lib.hf_adapter_ws_bytes(self._host, self.bytes, K, N, r) if N else 0
+    def _ws_bytes(self, lib: ctypes.CDLL, K: int, r: int, code: int) -> int:
+        found = lib.hf_adapter_ws_bytes(self._host, self.bytes, K, r, code)
         _check(min(found, 0), "hf_adapter_ws_bytes")
-        self._ws[K, N, r] = found
+        self._ws[K, r, code] = found
         return found
 
 
@@ -496,9 +496,9 @@ def adapter_add(y: Tensor, x: Tensor, down: Tensor, up: Tensor, plan: AdapterPla
     o = y if in_place else y.new_empty((rows, N)) if out is None else _rows2(out)
     stream = _raw_stream(index)
     with _current(index, device):
-        nbytes = plan._ws.get((K, N, r))
+        nbytes = plan._ws.get((K, r, code))
         if nbytes is None:
-            nbytes = plan._ws_bytes(lib, K, N, r)
+            nbytes = plan._ws_bytes(lib, K, r, code)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device).data_ptr() if nbytes else None
         status = lib.hf_adapter_add(x.data_ptr(), _ld(x), y.data_ptr(), _ld(y), down.data_ptr(), up.data_ptr(), r,
                                     None if scale is None else scale.data_ptr(), o.data_ptr(), _ld(o), N, K,

@@ -6,13 +6,14 @@
 // The plan holds the rows sorted by adapter and cut into tiles of 32 or 64 rows of one adapter, so requests in any order
 // and rows of one adapter that lie apart share a tile; rows are read and written where they lie.
 //   adapter_down_kernel  u = x A^T in fp32: a workgroup a tile, its waves on every NW-th step of 64 k.
-//   adapter_join_kernel  only where few tiles over a deep K are cut along K, or the rank is over 128: adds the shares.
+//   adapter_join_kernel  only where few tiles over a deep K are cut along K, or an fp16 rank is over 128: adds the shares.
 //   adapter_up_kernel    out = y + scale (u B^T): a workgroup 32 rows of a tile and a range of columns.
 // No atomics: every sum has a fixed order.
 //
 // u is handed on as two 16-bit values, a leading and a trailing one, in the operand order of the second product (x A^T is
-// not rounded to 16 bits: the doubled rank costs nothing where memory is the bound), after a power-of-two scale of its
-// row that keeps fp16 in range.
+// not rounded to 16 bits: the doubled rank costs nothing where memory is the bound). For fp16 each row of u first gets a
+// power-of-two scale that keeps it in range, so a workgroup needs all of its ranks; bfloat16 has float32's range, and its
+// ranks may be shared out among workgroups.
 #pragma once
 
 #include "block_types.h"
@@ -38,26 +39,30 @@ struct AdapterArgs {
   int live_tiles, tile_rows, r, r32, splits, blocks_per_wg, col_groups, in_place, stream_y;
 };
 
-// Row `row` of a tile's u, fp32 in LDS at p, into operand order with its factor: four neighbouring lanes a row, `part`
-// of 0 to 3.
+// Row `row` of a tile's u, fp32 in LDS at p, ranks lo to hi, into operand order, and the row's factor: four neighbouring
+// lanes a row, `part` of 0 to 3. For fp16 lo is 0 and hi the whole rank.
 template <class T>
 __device__ __forceinline__ void adapter_operands(const AdapterArgs& a, const AdapterTile& tile, int tile_index,
-                                                 const float* p, int row, int part, int blocks) {
-  float most = 0.0f;
-  for (int j = part; j < a.r32 / 8; j += 4)
+                                                 const float* p, int row, int part, int blocks, int lo, int hi) {
+  p -= lo;
+  float grow = 1.0f;
+  if constexpr (T::kNarrow) {
+    float most = 0.0f;
+    for (int j = part; j < hi / 8; j += 4)
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (8 * j + e < a.r) most = fmaxf(most, fabsf(p[8 * j + e]));
-  most = fmaxf(most, __shfl_xor(most, 1, 64));
-  most = fmaxf(most, __shfl_xor(most, 2, 64));
-  // 2^(6 - exponent): the row's largest lands in [2^6, 2^7), where fp16 holds it and its trailing part is normal. Rows
-  // of infinities and of values near the ends of fp32 stay as they are.
-  const bool fine = most >= 0x1p-100f && most <= 0x1p100f;
-  const float grow = fine ? __uint_as_float((260u - (__float_as_uint(most) >> 23)) << 23) : 1.0f;
+      for (int e = 0; e < 8; ++e)
+        if (8 * j + e < a.r) most = fmaxf(most, fabsf(p[8 * j + e]));
+    most = fmaxf(most, __shfl_xor(most, 1, 64));
+    most = fmaxf(most, __shfl_xor(most, 2, 64));
+    // 2^(6 - exponent): the row's largest lands in [2^6, 2^7), where fp16 holds it and its trailing part is normal. Rows
+    // of infinities and of values near the ends of fp32 stay as they are.
+    const bool fine = most >= 0x1p-100f && most <= 0x1p100f;
+    grow = fine ? __uint_as_float((260u - (__float_as_uint(most) >> 23)) << 23) : 1.0f;
+  }
   const float scale = a.scale ? a.scale[tile.adapter] : 1.0f;
-  if (part == 0) a.factors[(int64_t)tile_index * a.tile_rows + row] = scale / grow;  // exact: a power of two
+  if (part == 0 && lo == 0) a.factors[(int64_t)tile_index * a.tile_rows + row] = scale / grow;  // exact: a power of two
   v4u* frags = a.frags + (int64_t)tile_index * (a.r32 / 16) * blocks * 128;
-  for (int j = part; j < a.r32 / 8; j += 4) {
+  for (int j = lo / 8 + part; j < hi / 8; j += 4) {
     v4u lead, trail;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -214,26 +219,24 @@ __global__ __launch_bounds__(64 * NW, 1) void adapter_down_kernel(AdapterArgs a)
       for (int w = 1; w < NW; ++w) sums[i] += part[w * kSums + at];
     }
   }
-  const bool join = a.splits > 1 || gridDim.z > 1;
+  const bool join = a.splits > 1 || (T::kNarrow && gridDim.z > 1);
+  constexpr int kPitch = 32 * RB + 4;
   float* u = (float*)ad_lds;
-  int pitch = a.r32 + 4;
-  if (join) {
-    u = a.planes + ((int64_t)blockIdx.y * a.live_tiles + blockIdx.x) * a.tile_rows * a.r32;
-    pitch = a.r32;
-  } else {
-    __syncthreads();
-  }
+  float* plane = a.planes + ((int64_t)blockIdx.y * a.live_tiles + blockIdx.x) * a.tile_rows * a.r32;
+  if (!join) __syncthreads();
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int at = tid + i * 64 * NW;
     const int l = at & 63, g = (at >> 6) & 3, n = (at >> 8) % NB, b = (at >> 8) / NB;
-    const int rank = rank0 + 32 * b + 8 * g + 4 * (l >> 5);
-    if (at < kSums && rank < a.r32) *(v4f*)(u + (32 * n + (l & 31)) * pitch + rank) = sums[i];
+    const int row = 32 * n + (l & 31), rank = 32 * b + 8 * g + 4 * (l >> 5);
+    if (at >= kSums || rank0 + rank >= a.r32) continue;
+    if (join) *(v4f*)(plane + row * a.r32 + rank0 + rank) = sums[i];
+    else *(v4f*)(u + row * kPitch + rank) = sums[i];
   }
   if (join) return;
   __syncthreads();
   for (int row = tid >> 2; row < 32 * NB; row += 16 * NW)
-    adapter_operands<T>(a, tile, blockIdx.x, u + row * pitch, row, tid & 3, NB);
+    adapter_operands<T>(a, tile, blockIdx.x, u + row * kPitch, row, tid & 3, NB, rank0, min(rank0 + 32 * RB, a.r32));
 }
 
 // The K shares of a tile's u added in order, then into operand order. 256 threads.
@@ -252,7 +255,8 @@ __global__ __launch_bounds__(256) void adapter_join_kernel(AdapterArgs a) {
   }
   __syncthreads();
   for (int row = threadIdx.x >> 2; row < a.tile_rows; row += 64)
-    adapter_operands<T>(a, tile, blockIdx.x, u + row * (a.r32 + 4), row, threadIdx.x & 3, a.tile_rows / 32);
+    adapter_operands<T>(a, tile, blockIdx.x, u + row * (a.r32 + 4), row, threadIdx.x & 3, a.tile_rows / 32, 0,
+                        a.r32);
 }
 
 constexpr int kAdUpThreads = 256;

@@ -225,31 +225,39 @@ bool adapter_header(const void* plan, int64_t bytes, AdapterHeader* h) {
   return h->magic == kAdapterMagic && h->bytes == bytes;
 }
 
-// Rank blocks of 32 that a workgroup of the first product takes, and how many such parts the rank has.
-inline int adapter_rank_blocks(int r32) { return r32 <= 32 ? 1 : r32 <= 64 ? 2 : 4; }
-inline int adapter_rank_parts(int r32) { return (r32 / 32 + adapter_rank_blocks(r32) - 1) / adapter_rank_blocks(r32); }
+// How the first product of a call is cut: rank blocks of 32 that a workgroup takes, rank parts, K shares, and whether a
+// launch of its own joins them.
+struct AdapterCut {
+  int rank_blocks, parts, splits;
+  bool join;
+};
 inline int adapter_waves(int rb, int nb) { return rb == 4 ? 3 : nb == 1 && rb == 1 ? 8 : nb == 1 ? 6 : 4; }
-
-// K shares of the first product. One while its waves have few steps of 64 k each; beyond that, as many as fill the
-// device, and the sums are joined by a launch of their own.
-int adapter_splits(const AdapterHeader& h, int64_t K, int r32, int cus) {
-  const int rb = adapter_rank_blocks(r32), nb = h.tile_rows / 32;
-  const int64_t steps = K / hf::kAdChunk / adapter_waves(rb, nb);
-  const int64_t wgs = (int64_t)h.live_tiles * adapter_rank_parts(r32);
-  if (wgs == 0 || steps < 12 || 2 * wgs > cus) return 1;
-  return (int)std::min(std::min((int64_t)cus / wgs, steps / 6), (int64_t)16);
+AdapterCut adapter_cut(const AdapterHeader& h, int64_t K, int r32, int32_t dtype, int cus) {
+  AdapterCut c;
+  c.rank_blocks = r32 <= 32 ? 1 : r32 <= 64 ? 2 : 4;
+  c.parts = (r32 / 32 + c.rank_blocks - 1) / c.rank_blocks;
+  // One K share while the waves have few steps of 64 k each; beyond that, as many as fill the device (4042 rows x 5376 ->
+  // 7168, rank 64, 14 steps: both products 59 us whole, 55 us in two shares with their join; 64 single rows, 10 steps:
+  // the join's launch would cost more than it gains).
+  const int64_t steps = K / hf::kAdChunk / adapter_waves(c.rank_blocks, h.tile_rows / 32);
+  const int64_t wgs = (int64_t)h.live_tiles * c.parts;
+  c.splits = 1;
+  if (wgs > 0 && steps >= 12 && 2 * wgs <= cus)
+    c.splits = (int)std::min(std::min((int64_t)cus / wgs, steps / 6), (int64_t)16);
+  c.join = c.splits > 1 || (dtype == HF_FP16 && c.parts > 1);
+  return c;
 }
 
 // The workspace: rows' factors, u in operand order, and the shares where they are joined.
 struct AdapterSpace {
   int64_t frags, planes, bytes;
 };
-AdapterSpace adapter_space(const AdapterHeader& h, int r32, int splits) {
+AdapterSpace adapter_space(const AdapterHeader& h, int r32, const AdapterCut& c) {
   const int64_t rows = (int64_t)h.live_tiles * h.tile_rows;
   AdapterSpace s;
   s.frags = up_to(rows * 4, 256);
   s.planes = s.frags + rows * r32 * 4;
-  s.bytes = s.planes + (splits > 1 || adapter_rank_parts(r32) > 1 ? splits * rows * r32 * 4 : 0);
+  s.bytes = s.planes + (c.join ? c.splits * rows * r32 * 4 : 0);
   return s;
 }
 
@@ -263,12 +271,12 @@ void allow_lds(const void* kernel, std::once_flag* once, int bytes) {
 }
 
 template <class T, int RB, int NB, int NW>
-void launch_adapter_down(const hf::AdapterArgs& a, hipStream_t stream) {
+void launch_adapter_down(const hf::AdapterArgs& a, int parts, hipStream_t stream) {
   static std::once_flag once[64];
   constexpr int lds = hf::ad_down_lds(RB, NB, NW);
   static_assert(lds >= 4096 * RB * NB * NW && lds >= NB * 32 * (RB * 32 + 4) * 4, "the sums fit the rings");
   allow_lds(reinterpret_cast<const void*>(&hf::adapter_down_kernel<T, RB, NB, NW>), once, lds);
-  const dim3 grid(a.live_tiles, a.splits, adapter_rank_parts(a.r32));
+  const dim3 grid(a.live_tiles, a.splits, parts);
   hipLaunchKernelGGL((hf::adapter_down_kernel<T, RB, NB, NW>), grid, dim3(64 * NW), lds, stream, a);
 }
 
@@ -281,19 +289,19 @@ void launch_adapter_up(const hf::AdapterArgs& a, dim3 grid, hipStream_t stream) 
 }
 
 template <class T>
-int launch_adapters(hf::AdapterArgs& a, const AdapterHeader& h, bool vec, hipStream_t stream) {
+int launch_adapters(hf::AdapterArgs& a, const AdapterHeader& h, const AdapterCut& c, bool vec, hipStream_t stream) {
   const int cus = compute_units();
   if (h.live_tiles > 0) {
-    switch (adapter_rank_blocks(a.r32) * 4 + a.tile_rows / 32) {
-      case 1 * 4 + 1: launch_adapter_down<T, 1, 1, 8>(a, stream); break;
-      case 1 * 4 + 2: launch_adapter_down<T, 1, 2, 4>(a, stream); break;
-      case 2 * 4 + 1: launch_adapter_down<T, 2, 1, 6>(a, stream); break;
-      case 2 * 4 + 2: launch_adapter_down<T, 2, 2, 4>(a, stream); break;
-      case 4 * 4 + 1: launch_adapter_down<T, 4, 1, 3>(a, stream); break;
-      default: launch_adapter_down<T, 4, 2, 3>(a, stream); break;
+    switch (c.rank_blocks * 4 + a.tile_rows / 32) {
+      case 1 * 4 + 1: launch_adapter_down<T, 1, 1, 8>(a, c.parts, stream); break;
+      case 1 * 4 + 2: launch_adapter_down<T, 1, 2, 4>(a, c.parts, stream); break;
+      case 2 * 4 + 1: launch_adapter_down<T, 2, 1, 6>(a, c.parts, stream); break;
+      case 2 * 4 + 2: launch_adapter_down<T, 2, 2, 4>(a, c.parts, stream); break;
+      case 4 * 4 + 1: launch_adapter_down<T, 4, 1, 3>(a, c.parts, stream); break;
+      default: launch_adapter_down<T, 4, 2, 3>(a, c.parts, stream); break;
     }
     if (int st = launch_status()) return st;
-    if (a.splits > 1 || adapter_rank_parts(a.r32) > 1) {
+    if (c.join) {
       static std::once_flag once[64];
       allow_lds(reinterpret_cast<const void*>(&hf::adapter_join_kernel<T>), once, 64 * 516 * 4);
       hipLaunchKernelGGL(hf::adapter_join_kernel<T>, dim3(h.live_tiles), dim3(256),
@@ -303,7 +311,8 @@ int launch_adapters(hf::AdapterArgs& a, const AdapterHeader& h, bool vec, hipStr
   }
   const int64_t row_blocks = (int64_t)(a.in_place ? h.live_tiles : h.tiles) * (a.tile_rows / 32);
   if (row_blocks == 0) return HF_OK;
-  // Column blocks of a workgroup: one a wave with few rows; with many rows up to 4 a wave, for one reading of u.
+  // Column blocks of a workgroup: one a wave with few rows; with many rows up to 4 a wave, for one reading of u (up to 8:
+  // 475 -> 508 us at 32768 rows x 15360 columns).
   const int64_t blocks = (a.N + 63) / 64;
   const int64_t want = std::max((int64_t)1, (int64_t)8 * cus / row_blocks);  // workgroups a row block
   a.blocks_per_wg = (int)std::min(std::max(up_to((blocks + want - 1) / want, 4), (int64_t)4), (int64_t)16);
@@ -350,18 +359,29 @@ int hf_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, int32_t head
   a.side[1] = {(const uint16_t*)k, (uint16_t*)k_out, kw, k_token, k_head, ko_token, ko_head, heads_k};
   a.pos = pos, a.ld_pos = ld_pos, a.turns = turns, a.axis = axis, a.T = T, a.pos_type = pos_type, a.pairs = pairs;
   a.D = D, a.weight_f32 = weight_f32, a.eps = eps;
-  // A workgroup takes 4 tokens of a side's heads when that still gives every compute unit several; with fewer tokens one
-  // token, and then a share of its heads, down to one round of rows.
+  // A workgroup takes as many tokens of a side as give it four rounds of rows, while every compute unit gets two of them;
+  // a share of one token's heads, down to one round, when there are few tokens.
   const int lanes = D <= 64 ? 4 : D <= 128 ? 8 : 16, round = hf::kRopeThreads / lanes;
   const int64_t cus = compute_units();
-  const int64_t heads = std::max(heads_q, heads_k);
-  a.tokens = T >= 16 * cus ? 4 : 1;
-  const int64_t groups = (T + a.tokens - 1) / a.tokens;
-  int64_t parts = std::min(std::max((int64_t)1, 4 * cus / groups), (heads + round - 1) / round);
-  a.heads_per_wg = (int)((heads + parts - 1) / parts);
-  parts = (heads + a.heads_per_wg - 1) / a.heads_per_wg;
-  const dim3 grid((unsigned)groups, (unsigned)parts, heads_k > 0 ? 2 : 1);
-  const size_t lds = (size_t)a.tokens * pairs * sizeof(float) * 2;
+  int64_t blocks = 0;
+  int most = 1;
+  for (int i = 0; i < 2; ++i) {
+    hf::RopeSide& s = a.side[i];
+    s.tokens = 1, s.heads_per_wg = s.heads, s.parts = 1;
+    if (s.heads == 0) continue;
+    while (s.tokens < 16 && s.tokens * s.heads < 4 * round && T / (2 * s.tokens) >= 2 * cus) s.tokens *= 2;
+    if (s.tokens == 1) {
+      const int64_t want = std::min(std::max((int64_t)1, 4 * cus / T), (int64_t)(s.heads + round - 1) / round);
+      s.heads_per_wg = (int)((s.heads + want - 1) / want);
+      s.parts = (s.heads + s.heads_per_wg - 1) / s.heads_per_wg;
+    }
+    blocks += (T + s.tokens - 1) / s.tokens * s.parts;
+    if (i == 0) a.q_blocks = (int)blocks;
+    most = std::max(most, s.tokens);
+  }
+  if (blocks > 0x7fffffff) return HF_ERR_SIZE;
+  const dim3 grid((unsigned)blocks);
+  const size_t lds = (size_t)most * pairs * sizeof(float) * 2;
   if (dtype == HF_BF16) launch_rope_lanes<hf::Bf16>(a, lanes, interleaved, norm, grid, lds, (hipStream_t)stream);
   else launch_rope_lanes<hf::Fp16>(a, lanes, interleaved, norm, grid, lds, (hipStream_t)stream);
   return launch_status();
@@ -489,11 +509,12 @@ int64_t hf_adapter_plan(const int32_t* ids, const int64_t* lens, int64_t count, 
   }
 }
 
-int64_t hf_adapter_ws_bytes(const void* plan, int64_t bytes, int64_t K, int64_t N, int32_t r) {
+int64_t hf_adapter_ws_bytes(const void* plan, int64_t bytes, int64_t K, int32_t r, int32_t dtype) {
   AdapterHeader h;
-  if (!adapter_header(plan, bytes, &h) || K <= 0 || N <= 0 || r <= 0 || r > 512) return HF_ERR_ARGUMENT;
+  if (!adapter_header(plan, bytes, &h) || K <= 0 || r <= 0 || r > 512 || (dtype != HF_BF16 && dtype != HF_FP16))
+    return HF_ERR_ARGUMENT;
   const int r32 = (int)up_to(r, 32);
-  return adapter_space(h, r32, adapter_splits(h, K, r32, compute_units())).bytes;
+  return adapter_space(h, r32, adapter_cut(h, K, r32, dtype, compute_units())).bytes;
 }
 
 int hf_adapter_add(const void* x, int64_t ldx, const void* y, int64_t ldy, const void* down, const void* up, int32_t r,
@@ -521,15 +542,16 @@ int hf_adapter_add(const void* x, int64_t ldx, const void* y, int64_t ldy, const
   a.rows = (const int32_t*)(dev + (int64_t)h.tiles * (int64_t)sizeof(hf::AdapterTile));
   a.ldx = ldx, a.ldy = ldy, a.ldo = ldo, a.K = K, a.N = N, a.live_tiles = h.live_tiles, a.tile_rows = h.tile_rows;
   a.r = r, a.r32 = (int)up_to(r, 32), a.in_place = in_place;
-  a.splits = adapter_splits(h, K, a.r32, compute_units());
-  const AdapterSpace space = adapter_space(h, a.r32, a.splits);
+  const AdapterCut cut = adapter_cut(h, K, a.r32, dtype, compute_units());
+  a.splits = cut.splits;
+  const AdapterSpace space = adapter_space(h, a.r32, cut);
   if (h.live_rows > 0 && (!ws || ws_bytes < space.bytes)) return HF_ERR_ARGUMENT;
   a.factors = (float*)ws;
   a.frags = (hf::v4u*)((unsigned char*)ws + space.frags);
   a.planes = (float*)((unsigned char*)ws + space.planes);
   const bool vec = aligned(y, 16) && aligned(out, 16) && ldy % 8 == 0 && ldo % 8 == 0 && N % 8 == 0;
-  return dtype == HF_BF16 ? launch_adapters<hf::Bf16>(a, h, vec, (hipStream_t)stream)
-                          : launch_adapters<hf::Fp16>(a, h, vec, (hipStream_t)stream);
+  return dtype == HF_BF16 ? launch_adapters<hf::Bf16>(a, h, cut, vec, (hipStream_t)stream)
+                          : launch_adapters<hf::Fp16>(a, h, cut, vec, (hipStream_t)stream);
 }
 
 }  // extern "C"

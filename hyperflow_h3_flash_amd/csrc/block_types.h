@@ -12,6 +12,7 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 
 struct Bf16 {
   static constexpr uint32_t kExponent = 0x7f80u, kOne = 0x3f80u;
+  static constexpr bool kNarrow = false;  // float32's exponents
   static __device__ __forceinline__ float lo(uint32_t pair) { return bf16_lo(pair); }
   static __device__ __forceinline__ float hi(uint32_t pair) { return bf16_hi(pair); }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
@@ -26,6 +27,7 @@ struct Bf16 {
 
 struct Fp16 {
   static constexpr uint32_t kExponent = 0x7c00u, kOne = 0x3c00u;
+  static constexpr bool kNarrow = true;
   static __device__ __forceinline__ float lo(uint32_t pair) {
     return (float)__builtin_bit_cast(_Float16, (uint16_t)(pair & 0xffffu));
   }

@@ -26,7 +26,7 @@ struct RopeSide {
   uint16_t* out;
   const void* w;
   int64_t x_token, x_head, o_token, o_head;
-  int heads;
+  int heads, tokens, heads_per_wg, parts;  // tokens and heads of a workgroup, workgroups of a token
 };
 
 struct RopeArgs {
@@ -36,7 +36,7 @@ struct RopeArgs {
   const double* turns;
   const int32_t* axis;
   int64_t T;
-  int pos_type, pairs, D, tokens, heads_per_wg, weight_f32;
+  int pos_type, pairs, D, q_blocks, weight_f32;
   float eps;
 };
 
@@ -60,16 +60,17 @@ __device__ __forceinline__ void rope_weights(const void* w, int d, bool f32, flo
   }
 }
 
-// Tokens blockIdx.x * tokens .., heads blockIdx.y * heads_per_wg .. of side blockIdx.z.
+// The first q_blocks workgroups take the queries, the others the keys.
 template <class T, int LPR, bool INTERLEAVED, bool NORM>
 __global__ __launch_bounds__(kRopeThreads) void qk_norm_rope_kernel(RopeArgs a) {
   extern __shared__ v2f rope_table[];  // [tokens][pairs] of (cos, sin)
-  const RopeSide s = a.side[blockIdx.z];
-  const int h_lo = blockIdx.y * a.heads_per_wg, nh = min(h_lo + a.heads_per_wg, s.heads) - h_lo;
-  if (nh <= 0) return;
+  const bool key = (int)blockIdx.x >= a.q_blocks;
+  const RopeSide s = a.side[key];
+  const int block = (int)blockIdx.x - (key ? a.q_blocks : 0), group = block / s.parts;
+  const int h_lo = (block - group * s.parts) * s.heads_per_wg, nh = min(h_lo + s.heads_per_wg, s.heads) - h_lo;
   const int tid = threadIdx.x;
-  const int64_t t0 = (int64_t)blockIdx.x * a.tokens;
-  const int nt = (int)min((int64_t)a.tokens, a.T - t0);
+  const int64_t t0 = (int64_t)group * s.tokens;
+  const int nt = (int)min((int64_t)s.tokens, a.T - t0);
 
   constexpr int kRows = kRopeThreads / LPR;
   const int lane = tid % LPR, row = tid / LPR;

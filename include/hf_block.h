@@ -85,7 +85,7 @@ int hf_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, 
  */
 int64_t hf_adapter_plan(const int32_t* ids, const int64_t* lens, int64_t count, int32_t adapters, int32_t cus,
                         void* plan, int64_t bytes);
-int64_t hf_adapter_ws_bytes(const void* plan, int64_t bytes, int64_t K, int64_t N, int32_t r);
+int64_t hf_adapter_ws_bytes(const void* plan, int64_t bytes, int64_t K, int32_t r, int32_t dtype);
 int hf_adapter_add(const void* x, int64_t ldx, const void* y, int64_t ldy, const void* down, const void* up, int32_t r,
                    const float* scale, void* out, int64_t ldo, int64_t N, int64_t K, const void* plan,
                    const void* plan_dev, int64_t plan_bytes, void* ws, int64_t ws_bytes, int32_t dtype,

@@ -329,9 +329,10 @@ def test_argument_checks_reject_before_launching(lib):
     assert lib.hf_adapter_plan(ids, lens, 2, 0, 256, None, 0) == -1  # adapter 0 of none
     assert lib.hf_adapter_plan((ctypes.c_int32 * 1)(-2), None, 1, 3, 256, None, 0) == -1
     assert lib.hf_adapter_plan(ids, (ctypes.c_int64 * 2)(1 << 31, 1), 2, 1, 256, None, 0) == -5
-    need = lib.hf_adapter_ws_bytes(buf, size, 512, 64, 24)
+    need = lib.hf_adapter_ws_bytes(buf, size, 512, 24, 1)
     assert need >= 40 * 32 * 4
-    assert lib.hf_adapter_ws_bytes(buf, size - 1, 512, 64, 24) == lib.hf_adapter_ws_bytes(buf, size, 512, 64, 520) == -1
+    assert lib.hf_adapter_ws_bytes(buf, size - 1, 512, 24, 1) == lib.hf_adapter_ws_bytes(buf, size, 512, 520, 1) == -1
+    assert lib.hf_adapter_ws_bytes(buf, size, 512, 24, 2) == -1
 
     def adapt(x=fake, ldx=512, y=fake, ldy=64, down=fake, r=24, out=fake, ldo=64, N=64, K=512, plan=buf, dev=fake,
               ws=fake, ws_bytes=need, dtype=1):
