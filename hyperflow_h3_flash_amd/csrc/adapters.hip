@@ -261,15 +261,16 @@ __global__ __launch_bounds__(256) void adapter_join_kernel(AdapterArgs a) {
 
 constexpr int kAdUpThreads = 256;
 constexpr int kAdUpPitch = 68;  // floats of a row of 64 columns in LDS: 16-byte accesses of 16 rows meet every bank once
+constexpr int kAdSteps = 4;
 constexpr int kAdUpStage = 16 * kAdUpPitch * 4;
 
 // Row block blockIdx.x / col_groups (of a tile) and a group of its columns, neighbours in memory side by side in the
 // launch; VEC: y and out take 16-byte accesses.
 //
 // A wave computes 32 rows x 64 columns transposed (the weight is the first operand), turns them in LDS, in fp32, and adds
-// them to y in whole 128-byte lines of a row. y of the next 64 columns is on its way meanwhile. STEPS steps of 16 ranks have
-// their weights in registers at once.
-template <class T, bool VEC, int STEPS>
+// them to y in whole 128-byte lines of a row. y of the next 64 columns is on its way meanwhile. kAdSteps
+// steps of 16 ranks have their weights in registers at once.
+template <class T, bool VEC>
 __global__ __launch_bounds__(kAdUpThreads, 3) void adapter_up_kernel(AdapterArgs a) {
   extern __shared__ __attribute__((aligned(1024))) unsigned char ad_lds[];
   const int blocks = a.tile_rows / 32;
@@ -350,18 +351,18 @@ __global__ __launch_bounds__(kAdUpThreads, 3) void adapter_up_kernel(AdapterArgs
     v16f acc[2];
     acc[0] = acc[1] = (v16f){0};
 #pragma unroll 1
-    for (int s0 = 0; s0 < steps; s0 += STEPS) {
-      v4u w[STEPS][2];
+    for (int s0 = 0; s0 < steps; s0 += kAdSteps) {
+      v4u w[kAdSteps][2];
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         const uint16_t* row = up + min(blk * 64 + 32 * b + sub, a.N - 1) * a.r + 8 * half + 16 * s0;
 #pragma unroll
-        for (int s = 0; s < STEPS; ++s)  // r is a multiple of 8: ranks past it are not read
+        for (int s = 0; s < kAdSteps; ++s)  // r is a multiple of 8: ranks past it are not read
           w[s][b] = 16 * (s0 + s) + 8 * half < a.r ? *(const v4u*)(row + 16 * s) : (v4u){0, 0, 0, 0};
       }
 #pragma unroll
-      for (int s = 0; s < STEPS; ++s) {
-        if (STEPS > 2 && s0 + s >= steps) break;  // steps is even
+      for (int s = 0; s < kAdSteps; ++s) {
+        if (s0 + s >= steps) break;
         const v4u lead = operands[(s0 + s) * 128 + lane], trail = operands[(s0 + s) * 128 + 64 + lane];
 #pragma unroll
         for (int b = 0; b < 2; ++b) {

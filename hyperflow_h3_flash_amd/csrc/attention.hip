@@ -25,6 +25,7 @@
 namespace hf {
 
 constexpr int kAtKeys = 64;
+constexpr int kAtWaves = 4, kAtRows = 32 * kAtWaves;  // of a workgroup
 // What a lane's weights of one tile may sum to before their maximum is taken anew: fp16 holds them, and the sums have as
 // much room for large values as that many keys of equal weight take.
 constexpr float kAtMost = 512.0f;
@@ -56,8 +57,8 @@ __device__ __forceinline__ int at_swizzle(int r) {
   return PITCH == 256 ? ((r & 3) << 2) | ((r >> 2) & 3) : (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
 }
 
-// Floats of a workspace tile of `rows` rows: O [rows][32 DB], then m and l per row.
-__host__ __device__ constexpr int at_slot_floats(int rows, int db) { return rows * (32 * db + 2); }
+// Floats of a workspace tile: O [kAtRows][32 DB], then m and l per row.
+__host__ __device__ constexpr int at_slot_floats(int db) { return kAtRows * (32 * db + 2); }
 
 // Every load has landed, the queries' among them: told to the compiler here, it need not wait for them inside a loop, where
 // it would wait for the next tile too.
@@ -82,12 +83,12 @@ __device__ __forceinline__ float half_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// NW waves of 32 rows; D up to 32 * DB channels.
-template <class T, int DB, int NW>
-__global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_kernel(AttentionArgs a) {
+// D up to 32 * DB channels.
+template <class T, int DB>
+__global__ __launch_bounds__(64 * kAtWaves, 2) void attention_kernel(AttentionArgs a) {
   constexpr int PITCH = DB > 2 ? 256 : 128, KS = 2 * DB;
   constexpr int kTile = kAtKeys * PITCH;       // bytes of one K or V tile
-  constexpr int kLoads = kTile / 1024 / NW;    // 1 KiB loads of a wave a tile
+  constexpr int kLoads = kTile / 1024 / kAtWaves;    // 1 KiB loads of a wave a tile
   constexpr int kRowsPerLoad = 1024 / PITCH, kChunks = PITCH / 16;
   extern __shared__ __attribute__((aligned(1024))) unsigned char at_lds[];
   unsigned char HF_LDS* lds = (unsigned char HF_LDS*)at_lds;
@@ -114,31 +115,28 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_kernel(Att
       qf[s] = live && 16 * s + 8 * half < a.D ? *(const v4u*)(q + 16 * s) : (v4u){0, 0, 0, 0};
   }
 
-  // A wave's loads of a tile: load i fills rows kRowsPerLoad (NW i + wave) ..; lane l row l / kChunks, chunk l % kChunks of
-  // LDS from chunk (l % kChunks) ^ f(row) of the key. With four waves f does not depend on i. Rows past the sequence and
+  // A wave's loads of a tile: load i fills rows kRowsPerLoad (4 i + wave) ..; lane l row l / kChunks, chunk l % kChunks of
+  // LDS from chunk (l % kChunks) ^ f(row) of the key; f does not depend on i. Rows past the sequence and
   // chunks past D read as zero: their offset lies past the descriptor, which starts at the tile, so that offsets stay
   // small however long the sequence is.
   const uint16_t* kbase = a.k + ((int64_t)it.k0 + it.key_lo) * a.k_token + it.head * a.k_head;
   const uint16_t* vbase = a.v + ((int64_t)it.k0 + it.key_lo) * a.v_token + it.head * a.v_head;
   const int kstride = (int)a.k_token, vstride = (int)a.v_token;
-  constexpr int kParts = NW >= 4 ? 1 : kLoads < 4 ? kLoads : 4;
-  uint32_t kpart[kParts], vpart[kParts];
-#pragma unroll
-  for (int i = 0; i < kParts; ++i) {
-    const int r = (NW * i + wave) * kRowsPerLoad + lane / kChunks;
-    const int c = (lane % kChunks) ^ at_swizzle<PITCH>(r);
-    kpart[i] = c * 8 < a.D ? (uint32_t)(lane / kChunks * kstride * 2 + c * 16) : 0x80000000u;
-    vpart[i] = c * 8 < a.D ? (uint32_t)(lane / kChunks * vstride * 2 + c * 16) : 0x80000000u;
+  uint32_t kpart, vpart;
+  {
+    const int r = wave * kRowsPerLoad + lane / kChunks, c = (lane % kChunks) ^ at_swizzle<PITCH>(r);
+    kpart = c * 8 < a.D ? (uint32_t)(lane / kChunks * kstride * 2 + c * 16) : 0x80000000u;
+    vpart = c * 8 < a.D ? (uint32_t)(lane / kChunks * vstride * 2 + c * 16) : 0x80000000u;
   }
-  auto load_tile = [&](const uint16_t* base, int stride, uint32_t (&part)[kParts], int t, unsigned char HF_LDS* dst,
+  auto load_tile = [&](const uint16_t* base, int stride, uint32_t part, int t, unsigned char HF_LDS* dst,
                        bool zeros = false) __attribute__((always_inline)) {
     const int rows = min(kAtKeys, it.nk - it.key_lo - t * kAtKeys);
     const __amdgpu_buffer_rsrc_t rsrc =
         make_rsrc(base + (int64_t)t * kAtKeys * stride, zeros ? 0u : (uint32_t)((rows - 1) * stride * 2 + a.D * 2));
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      const int blk = NW * i + wave;
-      const uint32_t off = part[i % kParts] + (uint32_t)(blk * kRowsPerLoad * stride * 2);
+      const int blk = kAtWaves * i + wave;
+      const uint32_t off = part + (uint32_t)(blk * kRowsPerLoad * stride * 2);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (void HF_LDS*)(dst + blk * 1024), 16, off, 0, 0, 0);
     }
   };
@@ -352,8 +350,8 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_kernel(Att
     auto step = [&](int t, v16f (&s)[2], v16f (&next)[2], v4u (&pf)[4], const v4u (&before)[4])
                     __attribute__((always_inline)) {
       at_barrier();
-      at_opaque(kpart[0]);
-      at_opaque(vpart[0]);
+      at_opaque(kpart);
+      at_opaque(vpart);
       at_opaque(kaddr);
       at_opaque(vaddr);
       load_k(t + 2);
@@ -411,7 +409,7 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_kernel(Att
     }
   };
   // Below kAtShort tiles the steps that the pipelined way adds at its ends cost more than it gains.
-  if (NW > 1 && tiles >= kAtShort) pipelined();
+  if (tiles >= kAtShort) pipelined();
   else plainly(std::false_type{});
   // A key whose values are not finite poisons rows that do not see it (0 * inf); that shows as a NaN in the sums, and
   // then the item runs again the safe way.
@@ -422,14 +420,14 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_kernel(Att
 #pragma unroll
       for (int v = 0; v < 16; ++v) all += o[d][v];
     bool again = __any(live && all != all);
-    if constexpr (NW > 1) {  // the workgroup decides together; nobody reads the keys' buffers any more
-      int HF_LDS* votes = (int HF_LDS*)lds;
-      if (lane == 0) votes[wave] = again;
-      at_barrier();
+    // The workgroup decides together. After the pipelined way nobody reads the keys' buffers any more; after the plain one
+    // the last tile's, which its number tells, may still be read.
+    int HF_LDS* votes = (int HF_LDS*)(lds + (tiles & 1) * 2 * kTile);
+    if (lane == 0) votes[wave] = again;
+    at_barrier();
 #pragma unroll
-      for (int w = 0; w < NW; ++w) again |= votes[w] != 0;
-      if (again) at_barrier();
-    }
+    for (int w = 0; w < kAtWaves; ++w) again |= votes[w] != 0;
+    if (again) at_barrier();
     if (again) plainly(std::true_type{});
   }
   l = half_sum(l);
@@ -437,7 +435,7 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_kernel(Att
 
   if (it.slot >= 0) {
     // Shares go out as they are: row-major, and the row's maximum and sum behind them.
-    float* part = a.ws + (int64_t)it.slot * at_slot_floats(32 * NW, DB);
+    float* part = a.ws + (int64_t)it.slot * at_slot_floats(DB);
     const int r = wave * 32 + sub;
     if (!live) return;  // the end of a tile's rows: nobody joins them
 #pragma unroll
@@ -446,7 +444,7 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_kernel(Att
       for (int g = 0; g < 4; ++g)
         *(v4f*)(part + r * 32 * DB + 32 * d + 8 * g + 4 * half) =
             (v4f){o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
-    if (half == 0) *(v2f*)(part + 32 * NW * 32 * DB + 2 * r) = (v2f){m, l};
+    if (half == 0) *(v2f*)(part + kAtRows * 32 * DB + 2 * r) = (v2f){m, l};
     return;
   }
   // A row that sees no key is zero; 1 / l otherwise (a row of weights that are all NaN stays NaN).
@@ -481,17 +479,17 @@ __global__ __launch_bounds__(64 * NW, NW == 1 ? 1 : 2) void attention_kernel(Att
 // lane / 16 takes every fourth share, eight channels a lane. blockIdx.y takes kJoinRows rows of the tile.
 constexpr int kJoinRows = 4;
 template <class T, int DB>
-__global__ __launch_bounds__(64 * kJoinRows) void attention_join_kernel(AttentionArgs a, int tile_rows) {
+__global__ __launch_bounds__(64 * kJoinRows) void attention_join_kernel(AttentionArgs a) {
   const AttentionJoin j = a.joins[blockIdx.x];
   const int lane = threadIdx.x & 63, group = lane >> 4;
   const int r = blockIdx.y * kJoinRows + (threadIdx.x >> 6), d = 8 * (lane & 15);
   const int64_t row = (int64_t)j.row0 + r;
-  if (r >= tile_rows || row >= (int64_t)j.nq * a.group) return;
+  if (row >= (int64_t)j.nq * a.group) return;
   const int token = (int)((uint32_t)row / (uint32_t)a.group);
   const int head = j.head * a.group + (int)(row - (int64_t)token * a.group);
-  const int64_t step = at_slot_floats(tile_rows, DB);
+  const int64_t step = at_slot_floats(DB);
   const float* part = a.ws + (int64_t)j.slot0 * step;
-  const float* stat = part + tile_rows * 32 * DB + 2 * r;
+  const float* stat = part + kAtRows * 32 * DB + 2 * r;
   float top = -__builtin_inff();
   for (int s = lane; s < j.slots; s += 64) top = fmaxf(top, stat[s * step]);
 #pragma unroll

@@ -57,7 +57,7 @@ void launch_rope_lanes(const hf::RopeArgs& a, int lanes, bool interleaved, bool 
 
 constexpr int32_t kAttentionMagic = 0x48464154;
 struct AttentionHeader {
-  int32_t magic, rows, heads, kv_heads, D, causal, items, joins;
+  int32_t magic, heads, kv_heads, D, causal, items, joins, pad0;
   int64_t bytes, slots, q_rows, kv_rows;
   int32_t pad[16];
 };
@@ -81,15 +81,13 @@ struct AttentionWork {
 bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t count, int heads, int kv_heads, int D,
                       int causal, int cus, AttentionWork* w) {
   const int64_t group = heads / kv_heads, limit = 0x7fffffff;
-  int64_t q_rows = 0, kv_rows = 0, widest = 0;
+  int64_t q_rows = 0, kv_rows = 0;
   for (int64_t b = 0; b < count; ++b) {
     if (q_lens[b] < 0 || kv_lens[b] < 0 || q_lens[b] > limit || kv_lens[b] > limit) return false;
     q_rows += q_lens[b];
     kv_rows += kv_lens[b];
     if (q_rows > limit || kv_rows > limit || q_lens[b] * group > limit - 4096) return false;
-    widest = std::max(widest, q_lens[b] * group);
   }
-  const int rows = widest <= 32 ? 32 : 128;
   struct Piece {
     hf::AttentionItem item;
     int64_t cost;
@@ -100,8 +98,8 @@ bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t cou
   for (int64_t b = 0; b < count; ++b) {
     const int64_t nq = q_lens[b], nk = kv_lens[b];
     for (int h = 0; h < kv_heads; ++h)
-      for (int64_t r = 0; r < nq * group; r += rows) {
-        const int64_t last = std::min(r + rows, nq * group) - 1;
+      for (int64_t r = 0; r < nq * group; r += hf::kAtRows) {
+        const int64_t last = std::min(r + hf::kAtRows, nq * group) - 1;
         const int64_t hi = causal ? std::min(std::max(last / group + nk - nq + 1, (int64_t)0), nk) : nk;
         Piece p;
         memset(&p, 0, sizeof(p));
@@ -163,7 +161,6 @@ bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t cou
   }
   memset(&w->head, 0, sizeof(w->head));
   w->head.magic = kAttentionMagic;
-  w->head.rows = rows;
   w->head.heads = heads, w->head.kv_heads = kv_heads, w->head.D = D, w->head.causal = causal != 0;
   w->head.items = (int32_t)w->items.size(), w->head.joins = (int32_t)w->joins.size();
   w->head.slots = slots, w->head.q_rows = q_rows, w->head.kv_rows = kv_rows;
@@ -173,22 +170,21 @@ bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t cou
 }
 
 int64_t attention_slot_bytes(const AttentionHeader& h) {
-  return (int64_t)hf::at_slot_floats(h.rows, attention_db(h.D)) * 4;
+  return (int64_t)hf::at_slot_floats(attention_db(h.D)) * 4;
 }
 
 constexpr int attention_lds(int db) { return 4 * hf::kAtKeys * (db > 2 ? 256 : 128); }
 
-template <class T, int DB, int NW>
+template <class T, int DB>
 int launch_attention(const hf::AttentionArgs& a, const AttentionHeader& h, hipStream_t stream) {
   constexpr int lds = attention_lds(DB);
   static_assert(lds <= 64 * 1024, "dynamic LDS that needs no attribute");
-  hipLaunchKernelGGL((hf::attention_kernel<T, DB, NW>), dim3(h.items), dim3(64 * NW), lds, stream, a);
+  hipLaunchKernelGGL((hf::attention_kernel<T, DB>), dim3(h.items), dim3(64 * hf::kAtWaves), lds, stream, a);
   if (int st = launch_status()) return st;
   if (h.joins > 0) {
-    constexpr int rows = 32 * NW;
-    hipLaunchKernelGGL((hf::attention_join_kernel<T, DB>), dim3(h.joins, rows / hf::kJoinRows),
+    hipLaunchKernelGGL((hf::attention_join_kernel<T, DB>), dim3(h.joins, hf::kAtRows / hf::kJoinRows),
                        dim3(64 * hf::kJoinRows), 0, stream,
-                       a, rows);
+                       a);
     return launch_status();
   }
   return HF_OK;
@@ -196,15 +192,10 @@ int launch_attention(const hf::AttentionArgs& a, const AttentionHeader& h, hipSt
 
 template <class T>
 int launch_attention_of(const hf::AttentionArgs& a, const AttentionHeader& h, hipStream_t stream) {
-  switch (attention_db(h.D) * 16 + h.rows / 32) {
-#define HF_ATTENTION(DB)                                                                                     \
-  case DB * 16 + 1: return launch_attention<T, DB, 1>(a, h, stream);                                         \
-  case DB * 16 + 4: return launch_attention<T, DB, 4>(a, h, stream);
-    HF_ATTENTION(2)
-    HF_ATTENTION(3)
-    HF_ATTENTION(4)
-#undef HF_ATTENTION
-    default: return HF_ERR_ARGUMENT;
+  switch (attention_db(h.D)) {
+    case 2: return launch_attention<T, 2>(a, h, stream);
+    case 3: return launch_attention<T, 3>(a, h, stream);
+    default: return launch_attention<T, 4>(a, h, stream);
   }
 }
 
@@ -280,11 +271,11 @@ void launch_adapter_down(const hf::AdapterArgs& a, int parts, hipStream_t stream
   hipLaunchKernelGGL((hf::adapter_down_kernel<T, RB, NB, NW>), grid, dim3(64 * NW), lds, stream, a);
 }
 
-template <class T, bool VEC, int STEPS>
+template <class T, bool VEC>
 void launch_adapter_up(const hf::AdapterArgs& a, dim3 grid, hipStream_t stream) {
   static std::once_flag once[64];
-  allow_lds(reinterpret_cast<const void*>(&hf::adapter_up_kernel<T, VEC, STEPS>), once, 512 / 16 * 2048 + 4 * hf::kAdUpStage);
-  hipLaunchKernelGGL((hf::adapter_up_kernel<T, VEC, STEPS>), grid, dim3(hf::kAdUpThreads),
+  allow_lds(reinterpret_cast<const void*>(&hf::adapter_up_kernel<T, VEC>), once, 512 / 16 * 2048 + 4 * hf::kAdUpStage);
+  hipLaunchKernelGGL((hf::adapter_up_kernel<T, VEC>), grid, dim3(hf::kAdUpThreads),
                      a.r32 / 16 * 2048 + 4 * hf::kAdUpStage, stream, a);
 }
 
@@ -321,9 +312,8 @@ int launch_adapters(hf::AdapterArgs& a, const AdapterHeader& h, const AdapterCut
   a.col_groups = (int)((blocks + a.blocks_per_wg - 1) / a.blocks_per_wg);
   if (row_blocks * a.col_groups > 0x7fffffff) return HF_ERR_SIZE;
   const dim3 grid((unsigned)(row_blocks * a.col_groups));
-  if (vec && a.r32 == 32) launch_adapter_up<T, true, 2>(a, grid, stream);
-  else if (vec) launch_adapter_up<T, true, 4>(a, grid, stream);
-  else launch_adapter_up<T, false, 4>(a, grid, stream);
+  if (vec) launch_adapter_up<T, true>(a, grid, stream);
+  else launch_adapter_up<T, false>(a, grid, stream);
   return launch_status();
 }
 
@@ -359,8 +349,10 @@ int hf_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, int32_t head
   a.side[1] = {(const uint16_t*)k, (uint16_t*)k_out, kw, k_token, k_head, ko_token, ko_head, heads_k};
   a.pos = pos, a.ld_pos = ld_pos, a.turns = turns, a.axis = axis, a.T = T, a.pos_type = pos_type, a.pairs = pairs;
   a.D = D, a.weight_f32 = weight_f32, a.eps = eps;
-  // A workgroup takes as many tokens of a side as give it four rounds of rows, while every compute unit gets two of them;
-  // a share of one token's heads, down to one round, when there are few tokens.
+  // A workgroup takes as many tokens of a side as give it three rounds of rows, while every compute unit gets two of them
+  // (heads of 128, one round -> three: 37710 tokens x 7 heads each 60 -> 57 us, 16384 x 32 each 130 -> 105, 4099 x 32 and
+  // 8 24 -> 20; four rounds and more: 37710 x 56 each 393 -> 411); a share of one token's heads, down to one round, when
+  // there are few tokens.
   const int lanes = D <= 64 ? 4 : D <= 128 ? 8 : 16, round = hf::kRopeThreads / lanes;
   const int64_t cus = compute_units();
   int64_t blocks = 0;
@@ -369,7 +361,7 @@ int hf_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, int32_t head
     hf::RopeSide& s = a.side[i];
     s.tokens = 1, s.heads_per_wg = s.heads, s.parts = 1;
     if (s.heads == 0) continue;
-    while (s.tokens < 16 && s.tokens * s.heads < 4 * round && T / (2 * s.tokens) >= 2 * cus) s.tokens *= 2;
+    while (s.tokens < 16 && s.tokens * s.heads < 3 * round && T / (2 * s.tokens) >= 2 * cus) s.tokens *= 2;
     if (s.tokens == 1) {
       const int64_t want = std::min(std::max((int64_t)1, 4 * cus / T), (int64_t)(s.heads + round - 1) / round);
       s.heads_per_wg = (int)((s.heads + want - 1) / want);
@@ -473,10 +465,12 @@ int64_t hf_adapter_plan(const int32_t* ids, const int64_t* lens, int64_t count, 
     std::vector<int64_t> at(keys + 1, 0);
     for (int64_t i = 0; i < count; ++i) at[(ids[i] < 0 ? adapters : ids[i]) + 1] += lens ? lens[i] : 1;
     for (size_t i = 0; i < keys; ++i) at[i + 1] += at[i];
-    // Tiles of 64 rows read the weights half as often; tiles of 32 where those would not fill the device twice.
+    // Tiles of 64 rows read the weights half as often, tiles of 32 are twice as many: 64 once those fill the device
+    // (rows, rank, tiles of 32 -> 64: 8192, 64: 75 -> 77 us; 16384, 32: 114 -> 108; 32768, 64: 330 -> 306; 32768, 128:
+    // 475 -> 428; 300, 64: 20 -> 23).
     int64_t wide = 0;
     for (size_t key = 0; key + 1 < keys; ++key) wide += (at[key + 1] - at[key] + 63) / 64;
-    const int tile_rows = wide >= 2 * (cus ? cus : compute_units()) ? 64 : 32;
+    const int tile_rows = wide >= (cus ? cus : compute_units()) ? 64 : 32;
     std::vector<hf::AdapterTile> tiles;
     int32_t live_tiles = 0;
     for (size_t key = 0; key < keys; ++key) {

