@@ -16,6 +16,12 @@
 // LDS. Tiles of 64 keys, K and V, double-buffered, loaded past the registers (16 bytes a lane) while the tile before is
 // computed. Rows are 256 (D > 64) or 128 bytes; chunk c of row r lies at c ^ f(r) so that both the 16-row fragment reads
 // of K and the 4-row transposing reads of V touch every bank once.
+//
+// Bound: the card's power with long sequences, the keys' bytes with single tokens. 37710 tokens x 7 heads of 128: 4.62 ms,
+// 1103 TFLOP/s (71 % of what a large library product of the same type reaches, 1555); the matrix unit is busy 64 % of
+// the cycles, at 1.6 GHz; the same launch on zeros takes 3.3 ms (1530 TFLOP/s) at full clock. So energy counts, not slots:
+// leaving out the search for the maximum saved 1 %, adding the weights up two at a time with dot products nothing.
+// 16 single tokens of 32 / 8 heads against 77411 keys: 59 us and 4 for the join, 5.0 TB/s (a copy: 5.2).
 #pragma once
 
 #include <type_traits>
@@ -29,7 +35,10 @@ constexpr int kAtWaves = 4, kAtRows = 32 * kAtWaves;  // of a workgroup
 // What a lane's weights of one tile may sum to before their maximum is taken anew: fp16 holds them, and the sums have as
 // much room for large values as that many keys of equal weight take.
 constexpr float kAtMost = 512.0f;
-constexpr int kAtShort = 16;  // tiles from which on a workgroup's keys are taken the pipelined way
+// Tiles from which on a workgroup's keys are taken the pipelined way. Its two ends cost it a tile more: 8 tiles a row
+// (cross attention with 511 keys) 126 us plainly, 130 pipelined; prompts of 1 to 65 tiles 204 and 205; 590 tiles 4769 and
+// 4668.
+constexpr int kAtShort = 16;
 
 // A work item: rows row0 .. of sequence (q0, nq, k0, nk) and key head `head`, over keys [key_lo, key_hi). slot < 0: the
 // result goes to out; else the unnormalised sums go to workspace tile `slot`.
@@ -48,7 +57,7 @@ struct AttentionArgs {
   const AttentionItem* items;
   const AttentionJoin* joins;
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;
-  int group, D, causal, items_count;
+  int group, D, causal;
   float scale_log2;
 };
 
@@ -87,8 +96,8 @@ __device__ __forceinline__ float half_sum(float v) {
 template <class T, int DB>
 __global__ __launch_bounds__(64 * kAtWaves, 2) void attention_kernel(AttentionArgs a) {
   constexpr int PITCH = DB > 2 ? 256 : 128, KS = 2 * DB;
-  constexpr int kTile = kAtKeys * PITCH;       // bytes of one K or V tile
-  constexpr int kLoads = kTile / 1024 / kAtWaves;    // 1 KiB loads of a wave a tile
+  constexpr int kTile = kAtKeys * PITCH;           // bytes of one K or V tile
+  constexpr int kLoads = kTile / 1024 / kAtWaves;  // 1 KiB loads of a wave a tile
   constexpr int kRowsPerLoad = 1024 / PITCH, kChunks = PITCH / 16;
   extern __shared__ __attribute__((aligned(1024))) unsigned char at_lds[];
   unsigned char HF_LDS* lds = (unsigned char HF_LDS*)at_lds;
@@ -116,9 +125,9 @@ __global__ __launch_bounds__(64 * kAtWaves, 2) void attention_kernel(AttentionAr
   }
 
   // A wave's loads of a tile: load i fills rows kRowsPerLoad (4 i + wave) ..; lane l row l / kChunks, chunk l % kChunks of
-  // LDS from chunk (l % kChunks) ^ f(row) of the key; f does not depend on i. Rows past the sequence and
-  // chunks past D read as zero: their offset lies past the descriptor, which starts at the tile, so that offsets stay
-  // small however long the sequence is.
+  // LDS from chunk (l % kChunks) ^ f(row) of the key; f does not depend on i. Rows past the sequence and chunks past D read
+  // as zero: their offset lies past the descriptor, which starts at the tile, so that offsets stay small however long the
+  // sequence is.
   const uint16_t* kbase = a.k + ((int64_t)it.k0 + it.key_lo) * a.k_token + it.head * a.k_head;
   const uint16_t* vbase = a.v + ((int64_t)it.k0 + it.key_lo) * a.v_token + it.head * a.v_head;
   const int kstride = (int)a.k_token, vstride = (int)a.v_token;
@@ -290,7 +299,9 @@ __global__ __launch_bounds__(64 * kAtWaves, 2) void attention_kernel(AttentionAr
   auto load_v = [&](int t) __attribute__((always_inline)) {
     if (t < tiles) load_tile(vbase, vstride, vpart, t, lds + (t & 1) * 2 * kTile + kTile);
   };
-  auto tile_at = [&](int t) __attribute__((always_inline)) -> const unsigned char HF_LDS* { return lds + (t & 1) * 2 * kTile; };
+  auto tile_at = [&](int t) __attribute__((always_inline)) -> const unsigned char HF_LDS* {
+    return lds + (t & 1) * 2 * kTile;
+  };
 
   auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -361,8 +372,8 @@ __global__ __launch_bounds__(64 * kAtWaves, 2) void attention_kernel(AttentionAr
       rescale(used);
       l += sum;
       used = m;
-      // Slot i holds product i, the reading of product i + kAhead's operand, and a share of the exponentials. The order is held slot by slot: two waves that run this share
-      // a SIMD, and each finds the matrix unit or the vector unit free.
+      // Slot i holds product i, the reading of product i + kAhead's operand, and a share of the exponentials. The order is
+      // held slot by slot: two waves that run this share a SIMD, and each finds the matrix unit or the vector unit free.
       constexpr int kScores = 4 * DB, kSlots = 8 * DB, kAhead = 4;
       const unsigned char HF_LDS* kt = tile_at(t + 1);
       const unsigned char HF_LDS* vt = tile_at(t - 1) + kTile;
@@ -408,7 +419,6 @@ __global__ __launch_bounds__(64 * kAtWaves, 2) void attention_kernel(AttentionAr
       finish(p1);
     }
   };
-  // Below kAtShort tiles the steps that the pipelined way adds at its ends cost more than it gains.
   if (tiles >= kAtShort) pipelined();
   else plainly(std::false_type{});
   // A key whose values are not finite poisons rows that do not see it (0 * inf); that shows as a NaN in the sums, and

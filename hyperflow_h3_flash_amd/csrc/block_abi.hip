@@ -443,7 +443,7 @@ int hf_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, 
   a.joins = (const hf::AttentionJoin*)(dev + (int64_t)h.items * (int64_t)sizeof(hf::AttentionItem));
   a.q_token = q_token, a.q_head = q_head, a.k_token = k_token, a.k_head = k_head;
   a.v_token = v_token, a.v_head = v_head, a.o_token = o_token, a.o_head = o_head;
-  a.group = h.heads / h.kv_heads, a.D = h.D, a.causal = h.causal, a.items_count = h.items;
+  a.group = h.heads / h.kv_heads, a.D = h.D, a.causal = h.causal;
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
   return dtype == HF_BF16 ? launch_attention_of<hf::Bf16>(a, h, (hipStream_t)stream)
                           : launch_attention_of<hf::Fp16>(a, h, (hipStream_t)stream);

@@ -2,16 +2,18 @@
 //
 //   n = x * rsqrt(mean(x^2) + eps) * w;   (a, b) -> (a c - b s, a s + b c) for each pair of channels
 //
-// HBM-bound: each element is read once and written once, ~10 operations each.
+// HBM-bound: each element is read once and written once, ~10 operations each. 37710 tokens x (56 + 56) heads of 128,
+// three axes: 400 us for 2.16 GB, 5.4 TB/s (a copy of 1 GiB: 5.2).
 //
 // A row is one head of one token. LPR lanes share it (D / 16 of them at work), each with two chunks of 8 channels that
 // lie half the rotary width apart, so that with either pair layout both channels of a pair are in one lane: halves pair
 // chunk with chunk, interleaved pairs lie inside a chunk. Channels after the rotary width are taken two neighbouring
 // chunks a lane. The sum of squares goes over LPR lanes by lane exchanges.
 //
-// A workgroup takes all query heads or all key heads (or a share of them, when there are few tokens) of a few tokens: their
-// sines and cosines are computed once into LDS and serve every head. The angle is reduced in fp64 to less than half a turn before the
-// sine, so positions of any size keep the sine's own accuracy: one fp64 product a token and pair, for 64 to 112 heads.
+// A workgroup takes all query heads or all key heads (or a share of them, when there are few tokens) of a few tokens:
+// their sines and cosines are computed once into LDS and serve every head. The angle is reduced in fp64 to less than
+// half a turn before the sine, so positions of any size keep the sine's own accuracy: one fp64 product a token, side and
+// pair.
 #pragma once
 
 #include "block_types.h"

@@ -55,8 +55,8 @@ int hf_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, int32_t head
  * does not see never reach it, whatever k and v hold there.
  *
  * hf_attention_plan (host) lays out the work of a batch once for all layers and steps of these lengths: with
- * plan == NULL it returns the plan's bytes (`cus`: the device's compute units, 0 for the current one's), otherwise it fills `plan` (host memory of that many bytes; `bytes` is
- * checked) and returns the bytes, or a negative HF_ERR_*. hf_attention_ws_bytes gives the workspace that a filled plan
+ * plan == NULL it returns the plan's bytes (`cus`: the device's compute units, 0 for the current one's), otherwise it
+ * fills `plan` (host memory of that many bytes; `bytes` is checked) and returns the bytes, or a negative HF_ERR_*. hf_attention_ws_bytes gives the workspace that a filled plan
  * needs (0: none), or HF_ERR_ARGUMENT for bytes that hold no plan. The caller copies the plan to the device and passes
  * both copies to hf_attention: `plan` (host) for the launch, `plan_dev` for the kernels.
  * Requires: D a multiple of 16 up to 128; heads a multiple of kv_heads; scale > 0 and finite; q, k, v, out 16-byte
