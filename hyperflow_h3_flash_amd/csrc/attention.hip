@@ -17,11 +17,15 @@
 // computed. Rows are 256 (D > 64) or 128 bytes; chunk c of row r lies at c ^ f(r) so that both the 16-row fragment reads
 // of K and the 4-row transposing reads of V touch every bank once.
 //
-// Bound: the card's power with long sequences, the keys' bytes with single tokens. 37710 tokens x 7 heads of 128: 4.62 ms,
-// 1103 TFLOP/s (71 % of what a large library product of the same type reaches, 1555); the matrix unit is busy 64 % of
-// the cycles, at 1.6 GHz; the same launch on zeros takes 3.3 ms (1530 TFLOP/s) at full clock. So energy counts, not slots:
-// leaving out the search for the maximum saved 1 %, adding the weights up two at a time with dot products nothing.
-// 16 single tokens of 32 / 8 heads against 77411 keys: 59 us and 4 for the join, 5.0 TB/s (a copy: 5.2).
+// Bound: the card's power with long sequences, the keys' bytes with single tokens. 37710 tokens x 7 heads of 128: 4.51 ms,
+// 1130 TFLOP/s (a large library product of the same type: 1555), the matrix unit busy 65 % at 1.62 GHz. The same launch on
+// zeros takes 3.26 ms at the full clock: so energy counts, not issue slots. Leaving out the search for the maximum saved
+// 1 %; adding the weights up two at a time with dot products nothing; running the products of neighbouring tiles under the
+// weights' arithmetic in one wave, with two tiles of scores in registers, raised the matrix unit's share of the cycles and
+// lowered the clock as much (4.63 ms): the two waves of a SIMD overlap well enough by themselves, once the products'
+// operands are read four products ahead (at_order). Three workgroups a compute unit for heads of at most 64, with
+// registers held to 168: 2.76 ms against 2.58 with two (37710 x 7 of 64).
+// 16 single tokens of 32 / 8 heads against 77411 keys: 57 us and 4 for the join, 5.3 TB/s (a copy: 5.2).
 #pragma once
 
 #include <type_traits>
@@ -35,10 +39,6 @@ constexpr int kAtWaves = 4, kAtRows = 32 * kAtWaves;  // of a workgroup
 // What a lane's weights of one tile may sum to before their maximum is taken anew: fp16 holds them, and the sums have as
 // much room for large values as that many keys of equal weight take.
 constexpr float kAtMost = 512.0f;
-// Tiles from which on a workgroup's keys are taken the pipelined way. Its two ends cost it a tile more: 8 tiles a row
-// (cross attention with 511 keys) 126 us plainly, 130 pipelined; prompts of 1 to 65 tiles 204 and 205; 590 tiles 4769 and
-// 4668.
-constexpr int kAtShort = 16;
 
 // A work item: rows row0 .. of sequence (q0, nq, k0, nk) and key head `head`, over keys [key_lo, key_hi). slot < 0: the
 // result goes to out; else the unnormalised sums go to workspace tile `slot`.
@@ -79,8 +79,20 @@ __device__ __forceinline__ void at_barrier() {
   asm volatile("s_barrier" ::: "memory");
   __builtin_amdgcn_sched_barrier(0);
 }
-// Keeps what is computed from v inside the loop (registers are scarcer there than vector operations).
-__device__ __forceinline__ void at_opaque(uint32_t& v) { asm volatile("" : "+v"(v)); }
+// The order of N products with READS reads of LDS each: operands are on their way four products ahead. Left to itself, the
+// compiler reads two and waits for them.
+template <int N, int READS>
+__device__ __forceinline__ void at_order() {
+  constexpr int kAhead = 4;
+  __builtin_amdgcn_sched_group_barrier(0x100, kAhead * READS, 0);  // LDS reads
+#pragma unroll
+  for (int i = 0; i < N - kAhead; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a product
+    __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+  __builtin_amdgcn_sched_barrier(0);
+}
 
 // Lane l exchanges with lane l ^ 32: max of both.
 __device__ __forceinline__ float half_max(float v) {
@@ -137,11 +149,11 @@ __global__ __launch_bounds__(64 * kAtWaves, 2) void attention_kernel(AttentionAr
     kpart = c * 8 < a.D ? (uint32_t)(lane / kChunks * kstride * 2 + c * 16) : 0x80000000u;
     vpart = c * 8 < a.D ? (uint32_t)(lane / kChunks * vstride * 2 + c * 16) : 0x80000000u;
   }
-  auto load_tile = [&](const uint16_t* base, int stride, uint32_t part, int t, unsigned char HF_LDS* dst,
-                       bool zeros = false) __attribute__((always_inline)) {
+  auto load_tile = [&](const uint16_t* base, int stride, uint32_t part, int t,
+                       unsigned char HF_LDS* dst) __attribute__((always_inline)) {
     const int rows = min(kAtKeys, it.nk - it.key_lo - t * kAtKeys);
     const __amdgpu_buffer_rsrc_t rsrc =
-        make_rsrc(base + (int64_t)t * kAtKeys * stride, zeros ? 0u : (uint32_t)((rows - 1) * stride * 2 + a.D * 2));
+        make_rsrc(base + (int64_t)t * kAtKeys * stride, (uint32_t)((rows - 1) * stride * 2 + a.D * 2));
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int blk = kAtWaves * i + wave;
@@ -153,8 +165,8 @@ __global__ __launch_bounds__(64 * kAtWaves, 2) void attention_kernel(AttentionAr
   // Fragment addresses within a tile. K: lane (key sub, half) reads chunk 2s + half of step s; V: 4 channels of key
   // 4 half + (lane % 16) / 4 (+ 8 for the second part p), channels 32 d + 16 ((lane / 16) % 2) + 4 (lane % 4). Steps,
   // parts and channel blocks change bits of the chunk that the swizzle changes too, so they are exclusive ors of one
-  // address each (taken anew in every tile: sixteen registers less).
-  uint32_t kaddr = (uint32_t)(sub * PITCH + ((half ^ at_swizzle<PITCH>(sub)) * 16));
+  // address each.
+  const uint32_t kaddr = (uint32_t)(sub * PITCH + ((half ^ at_swizzle<PITCH>(sub)) * 16));
   uint32_t vaddr;
   {
     const int r = 4 * half + ((lane & 15) >> 2), ch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
@@ -212,7 +224,6 @@ __global__ __launch_bounds__(64 * kAtWaves, 2) void attention_kernel(AttentionAr
     const float p1 = __builtin_amdgcn_exp2f(fmaf(s[b][v + 1], c, -mc));
     part[0] += p0;
     part[1] += p1;
-    asm volatile("" : "+v"(part[0]), "+v"(part[1]));  // here, not after the last slot
     pf[p >> 2][p & 3] = T::pack(p0, p1);
   };
   auto centre = [&]() __attribute__((always_inline)) { return m == -__builtin_inff() ? 0.0f : m * c; };
@@ -309,8 +320,7 @@ __global__ __launch_bounds__(64 * kAtWaves, 2) void attention_kernel(AttentionAr
     m = last >= it.key_lo ? -__builtin_inff() : 0.0f;  // rows that see none of the keys need no maximum
     l = 0.0f;
   };
-  // One tile after the other: few rows, where memory is what it waits for, and the safe way.
-  auto plainly = [&](auto safe_t) __attribute__((always_inline)) {
+  auto run = [&](auto safe_t) __attribute__((always_inline)) {
     clear();
     if (tiles <= 0) return;
     load_k(0);
@@ -327,6 +337,7 @@ __global__ __launch_bounds__(64 * kAtWaves, 2) void attention_kernel(AttentionAr
       v4u pf[4];
       float part[2] = {0.0f, 0.0f};
       scores(tile_at(t), s);
+      at_order<4 * DB, 1>();
       mask(key0, s);
       const float used = m, mc = centre();
 #pragma unroll
@@ -334,93 +345,16 @@ __global__ __launch_bounds__(64 * kAtWaves, 2) void attention_kernel(AttentionAr
       const float sum = settle(s, pf, part);
       rescale(used);
       l += sum;
-      if constexpr (decltype(safe_t)::value) safe_values(key0, tile_at(t) + kTile, pf);
-      else values(tile_at(t) + kTile, pf);
-    }
-  };
-
-  // Many rows, where the matrix and the vector unit are both near their bound: while the scores of tile t become weights,
-  // the matrix unit multiplies the scores of tile t + 1 and the weights and values of tile t - 1, all in one stretch of
-  // independent instructions. Keys t + 2 and values t are loaded meanwhile, into the buffers that keys t and values t - 2
-  // have left. The first tile multiplies zeros, the last one scores that nobody reads: steps of their own for them cost
-  // the loop the registers that it needs (the compiler then spills the queries, and the loop takes a third longer).
-  auto pipelined = [&]() __attribute__((always_inline)) {
-    clear();
-    if (tiles <= 0) return;
-    v16f s0[2], s1[2];
-    v4u p0[4], p1[4];
-    float used = m, sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) p1[i] = (v4u){0, 0, 0, 0};
-    load_k(0);
-    load_k(1);
-    load_tile(vbase, 0, vpart, 0, lds + 3 * kTile, true);
-    at_landed();
-    at_barrier();
-    scores(tile_at(0), s0);
-    auto step = [&](int t, v16f (&s)[2], v16f (&next)[2], v4u (&pf)[4], const v4u (&before)[4])
-                    __attribute__((always_inline)) {
-      at_barrier();
-      at_opaque(kpart);
-      at_opaque(vpart);
-      at_opaque(kaddr);
-      at_opaque(vaddr);
-      load_k(t + 2);
-      load_v(t);
-      mask(it.key_lo + t * kAtKeys, s);
-      // What the weights of tile t - 1 left to do before they are multiplied.
-      rescale(used);
-      l += sum;
-      used = m;
-      // Slot i holds product i, the reading of product i + kAhead's operand, and a share of the exponentials. The order is
-      // held slot by slot: two waves that run this share a SIMD, and each finds the matrix unit or the vector unit free.
-      constexpr int kScores = 4 * DB, kSlots = 8 * DB, kAhead = 4;
-      const unsigned char HF_LDS* kt = tile_at(t + 1);
-      const unsigned char HF_LDS* vt = tile_at(t - 1) + kTile;
-      auto operand = [&](int i) __attribute__((always_inline)) {
-        return i < kScores ? kfrag(kt, i >> 1, i & 1) : vfrag(vt, (i - kScores) / DB, (i - kScores) % DB);
-      };
-      v4u ring[kAhead];
-#pragma unroll
-      for (int i = 0; i < kAhead; ++i) ring[i] = operand(i);
-      float part[2] = {0.0f, 0.0f};
-      const float mc = centre();
-      next[0] = next[1] = (v16f){0};
-      __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int i = 0; i < kSlots; ++i) {
-        if (i < kScores) next[i & 1] = T::mfma(ring[i % kAhead], qf[i >> 1], next[i & 1]);
-        else o[(i - kScores) % DB] = T::mfma(ring[i % kAhead], before[(i - kScores) / DB], o[(i - kScores) % DB]);
-        if (i + kAhead < kSlots) ring[i % kAhead] = operand(i + kAhead);
-#pragma unroll
-        for (int p = (16 * i + kSlots - 1) / kSlots; p * kSlots < 16 * (i + 1); ++p) exponentials(s, pf, p, mc, part);
+      if constexpr (decltype(safe_t)::value) {
+        safe_values(key0, tile_at(t) + kTile, pf);
+      } else {
         __builtin_amdgcn_sched_barrier(0);
+        values(tile_at(t) + kTile, pf);
+        at_order<4 * DB, 2>();
       }
-      // The weights are wanted in this stretch, not after a branch.
-      asm volatile("" : "+v"(pf[0]), "+v"(pf[1]), "+v"(pf[2]), "+v"(pf[3]));
-      sum = settle(s, pf, part);
-    };
-    auto finish = [&](const v4u (&pf)[4]) __attribute__((always_inline)) {
-      rescale(used);
-      l += sum;
-      at_barrier();
-      values(tile_at(tiles - 1) + kTile, pf);
-    };
-    int t = 0;
-#pragma unroll 1
-    for (; t + 1 < tiles; t += 2) {
-      step(t, s0, s1, p0, p1);
-      step(t + 1, s1, s0, p1, p0);
-    }
-    if (t < tiles) {
-      step(t, s0, s1, p0, p1);
-      finish(p0);
-    } else {
-      finish(p1);
     }
   };
-  if (tiles >= kAtShort) pipelined();
-  else plainly(std::false_type{});
+  run(std::false_type{});
   // A key whose values are not finite poisons rows that do not see it (0 * inf); that shows as a NaN in the sums, and
   // then the item runs again the safe way.
   {
@@ -430,15 +364,14 @@ __global__ __launch_bounds__(64 * kAtWaves, 2) void attention_kernel(AttentionAr
 #pragma unroll
       for (int v = 0; v < 16; ++v) all += o[d][v];
     bool again = __any(live && all != all);
-    // The workgroup decides together. After the pipelined way nobody reads the keys' buffers any more; after the plain one
-    // the last tile's, which its number tells, may still be read.
+    // The workgroup decides together, through the buffer that the last tile, which may still be read, does not use.
     int HF_LDS* votes = (int HF_LDS*)(lds + (tiles & 1) * 2 * kTile);
     if (lane == 0) votes[wave] = again;
     at_barrier();
 #pragma unroll
     for (int w = 0; w < kAtWaves; ++w) again |= votes[w] != 0;
     if (again) at_barrier();
-    if (again) plainly(std::true_type{});
+    if (again) run(std::true_type{});
   }
   l = half_sum(l);
   if (last < it.key_lo) m = -__builtin_inff();
