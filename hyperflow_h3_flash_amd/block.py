@@ -349,8 +349,9 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, *, sc
     ``q`` [sum q_lengths, heads, head_dim], ``k`` and ``v`` [sum kv_lengths, kv_heads, head_dim], bfloat16 or float16,
     any token and head strides (slices of a fused projection or a cache); the result is like q. ``scale`` (default
     ``head_dim ** -0.5``) is positive. A query that sees no key gets zeros; what k and v hold at keys that a query does
-    not see never reaches it. Scores, weights' sums and outputs are summed in float32; the weights enter the second
-    product in the inputs' type."""
+    not see never reaches it. Scores, weights' sums and outputs are summed in float32, and divided by the weights' sum at the
+    end (values of v times the number of keys have to stay in its range); the weights enter the second product in the
+    inputs' type."""
     if q.shape != plan._q_shape or k.shape != plan._kv_shape or v.shape != plan._kv_shape:
         raise ValueError(f"the plan is for q {plan._q_shape} and k, v {plan._kv_shape}; got {tuple(q.shape)}, "
                          f"{tuple(k.shape)}, {tuple(v.shape)}")

@@ -4,7 +4,6 @@
 
 #include <algorithm>
 #include <mutex>
-#include <new>
 #include <vector>
 
 #include "../../include/hf_block.h"
@@ -17,6 +16,9 @@ namespace {
 inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
 inline int launch_status() { return hipGetLastError() == hipSuccess ? HF_OK : HF_ERR_LAUNCH; }
 inline int64_t up_to(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+// What the planners take: their host memory goes with both.
+constexpr int32_t kMostUnits = 1 << 16, kMostAdapters = 1 << 24;
 
 // Compute units of the current device, asked once per device (256 without one).
 int compute_units() {
@@ -382,7 +384,7 @@ int hf_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, int32_t head
 int64_t hf_attention_plan(const int64_t* q_lens, const int64_t* kv_lens, int64_t count, int32_t heads, int32_t kv_heads,
                           int32_t D, int32_t causal, int32_t cus, void* plan, int64_t bytes) {
   if (count < 0 || (count > 0 && (!q_lens || !kv_lens)) || heads < 1 || kv_heads < 1 || heads % kv_heads || D < 1 ||
-      cus < 0)
+      cus < 0 || cus > kMostUnits)
     return HF_ERR_ARGUMENT;
   if (D % 16) return HF_ERR_ALIGNMENT;
   if (D > 128) return HF_ERR_SIZE;
@@ -402,7 +404,7 @@ int64_t hf_attention_plan(const int64_t* q_lens, const int64_t* kv_lens, int64_t
       if (!w.joins.empty()) memcpy(to, w.joins.data(), w.joins.size() * sizeof(w.joins[0]));
     }
     return w.head.bytes;
-  } catch (const std::bad_alloc&) {
+  } catch (...) {  // no memory for that many
     return HF_ERR_SIZE;
   }
 }
@@ -451,7 +453,8 @@ int hf_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, 
 
 int64_t hf_adapter_plan(const int32_t* ids, const int64_t* lens, int64_t count, int32_t adapters, int32_t cus,
                         void* plan, int64_t bytes) {
-  if (count < 0 || (count > 0 && !ids) || adapters < 0 || cus < 0) return HF_ERR_ARGUMENT;
+  if (count < 0 || (count > 0 && !ids) || adapters < 0 || cus < 0 || cus > kMostUnits) return HF_ERR_ARGUMENT;
+  if (adapters > kMostAdapters) return HF_ERR_SIZE;
   int64_t rows = 0;
   for (int64_t i = 0; i < count; ++i) {
     if (ids[i] < -1 || ids[i] >= adapters || (lens && lens[i] < 0)) return HF_ERR_ARGUMENT;
@@ -498,7 +501,7 @@ int64_t hf_adapter_plan(const int32_t* ids, const int64_t* lens, int64_t count, 
       }
     }
     return h.bytes;
-  } catch (const std::bad_alloc&) {
+  } catch (...) {  // no memory for that many
     return HF_ERR_SIZE;
   }
 }

@@ -55,10 +55,11 @@ int hf_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, int32_t head
  * does not see never reach it, whatever k and v hold there.
  *
  * hf_attention_plan (host) lays out the work of a batch once for all layers and steps of these lengths: with
- * plan == NULL it returns the plan's bytes (`cus`: the device's compute units, 0 for the current one's), otherwise it
- * fills `plan` (host memory of that many bytes; `bytes` is checked) and returns the bytes, or a negative HF_ERR_*. hf_attention_ws_bytes gives the workspace that a filled plan
- * needs (0: none), or HF_ERR_ARGUMENT for bytes that hold no plan. The caller copies the plan to the device and passes
- * both copies to hf_attention: `plan` (host) for the launch, `plan_dev` for the kernels.
+ * plan == NULL it returns the plan's bytes (`cus`: the device's compute units, 0 for the current one's, up to 65536),
+ * otherwise it fills `plan` (host memory of that many bytes; `bytes` is checked) and returns the bytes, or a negative
+ * HF_ERR_*. hf_attention_ws_bytes gives the workspace that a filled plan needs (0: none), or HF_ERR_ARGUMENT for bytes
+ * that hold no plan. The caller copies the plan to the device and passes both copies to hf_attention: `plan` (host) for
+ * the launch, `plan_dev` for the kernels.
  * Requires: D a multiple of 16 up to 128; heads a multiple of kv_heads; scale > 0 and finite; q, k, v, out 16-byte
  * aligned, token and head strides multiples of 8, of k and v below 2^23; `ws` of at least hf_attention_ws_bytes,
  * 16-byte aligned. Sums of lengths below 2^31.
@@ -81,7 +82,7 @@ int hf_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, 
  * hf_adapter_plan (host) groups the rows by adapter once for all projections of a batch: `ids` holds one adapter or -1
  * for each of `count` requests, `lens` its rows (NULL: one each). Used like hf_attention_plan.
  * Requires: K, r, ldx multiples of 8, r <= 512; x, down, up 16-byte aligned; y, out 2-byte aligned (16-byte aligned with
- * strides and N multiples of 8 for whole-vector access); ws 16-byte aligned; M, N, K < 2^31.
+ * strides and N multiples of 8 for whole-vector access); ws 16-byte aligned; M, N, K < 2^31; adapters <= 2^24.
  */
 int64_t hf_adapter_plan(const int32_t* ids, const int64_t* lens, int64_t count, int32_t adapters, int32_t cus,
                         void* plan, int64_t bytes);

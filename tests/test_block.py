@@ -347,11 +347,19 @@ def test_argument_checks_reject_before_launching(lib):
     assert adapt(r=520) == -5
 
 
+def test_planners_refuse_sizes_that_their_memory_would_go_with(lib):
+    one, ids = (ctypes.c_int64 * 1)(5), (ctypes.c_int32 * 1)(0)
+    assert lib.hf_attention_plan(one, one, 1, 2, 1, 64, 0, 65537, None, 0) == -1
+    assert lib.hf_attention_plan(one, one, 1, 2, 1, 64, 0, 65536, None, 0) > 0
+    assert lib.hf_adapter_plan(ids, None, 1, 1, 65537, None, 0) == -1
+    assert lib.hf_adapter_plan(ids, None, 1, (1 << 24) + 1, 256, None, 0) == -5
+
+
 # ----------------------------------------------------------------------------------------------------------- planners
 
 @pytest.mark.parametrize("q,kv,heads,kv_heads,causal", [
     ([37710], [37710], 7, 7, 0), ([5, 0, 300, 1], [5, 9, 300, 4000], 8, 2, 1), ([1] * 16, list(range(1, 16001, 1000)), 32, 8, 1),
-    ([130, 40], [0, 50000], 4, 1, 0), ([900, 3], [100, 700], 6, 3, 1), ([], [], 2, 1, 0), ([64] * 40, [64] * 40, 1, 1, 1),
+    ([130, 40], [0, 50000], 4, 1, 0), ([900, 3], [100, 700], 6, 3, 1), ([], [], 2, 1, 0), ([64] * 40, [64] * 40, 1, 1, 1), ([3, 200], [0, 0], 2, 1, 0),
     ([4099, 1537, 300, 61, 2048], [4099, 1537, 300, 61, 2048], 32, 8, 1),
 ])
 def test_attention_plan_covers_every_row_and_key_once(lib, q, kv, heads, kv_heads, causal):

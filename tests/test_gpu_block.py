@@ -134,6 +134,14 @@ def test_packed_ragged_with_empty_sequences():
     attend(2, [3, 0, 64, 17], [0, 0, 10, 40], 4, 4, 128, True, HF)  # queries without a key; more queries than keys
 
 
+@pytest.mark.parametrize("causal", [False, True])
+def test_no_keys_at_all_and_no_queries_at_all(causal):
+    out = attend(3, [3, 200], [0, 0], 4, 2, 128, causal, BF)[4]
+    assert not out.any()
+    assert attend(4, [0, 0], [5, 70], 4, 2, 64, causal, HF)[4].shape == (0, 4, 64)
+    assert attend(5, [], [], 4, 2, 64, causal, HF)[4].shape == (0, 4, 64)
+
+
 @pytest.mark.parametrize("hq,hk", [(8, 8), (32, 8), (16, 1), (12, 12)])
 def test_single_tokens_against_caches(hq, hk):
     kv = [1, 2, 63, 64, 65, 1000, 4097, 300]
