@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import subprocess
 from concurrent.futures import ThreadPoolExecutor
 from functools import lru_cache
@@ -90,7 +91,15 @@ BLOCK_SIGNATURES = {
     "hf_adapter_ws_bytes": ([_P, _I64, _I64, _I32, _I32], ctypes.c_int64),
     "hf_adapter_add": ([_P, _I64, _P, _I64, _P, _P, _I32, _P, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64, _I32, _P],
                        ctypes.c_int),
+    "hf_qk_norm_rope_call": ([ctypes.c_char_p], ctypes.c_int),
+    "hf_attention_call": ([ctypes.c_char_p], ctypes.c_int),
+    "hf_adapter_add_call": ([ctypes.c_char_p], ctypes.c_int),
 }
+
+#: The launches' parameters as the structs of hf_block.h lay them out.
+ROPE_ARGS = struct.Struct("@PqqiPqqiPqqPqqPiqiPPiiiPPifqiiP")
+ATTENTION_ARGS = struct.Struct("@PqqPqqPqqPqqfPPqPqiP")
+ADAPTER_ARGS = struct.Struct("@PqPqPPiPPqqqPPqPqiP")
 
 #: Queries of hf_route.
 ROUTE_UP_ROWS, ROUTE_ROTATE_LOWRANK, ROUTE_STREAM_WEIGHT = 0, 1, 2

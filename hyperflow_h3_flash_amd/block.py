@@ -33,6 +33,8 @@ from .int8 import _check, _on, _raw_stream, _same_device
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
 _HERE = contextlib.nullcontext()
+_rope_args, _attention_args, _adapter_args = (s.pack for s in (
+    _native.ROPE_ARGS, _native.ATTENTION_ARGS, _native.ADAPTER_ARGS))
 #: The current device's index.
 _device_index = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 
@@ -209,7 +211,7 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: 
 
     device = q.device
     lib = _lib(device)
-    qw = kw = None
+    qw = kw = 0  # addresses: 0 for none
     wide = False
     if norm:
         wide = ((q_weight is not None and q_weight.dtype is not dtype)
@@ -227,8 +229,8 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: 
         qo, qot, qoh = q.new_empty((T, hq, D)), hq * D, D
     else:
         qo, qot, qoh = _heads(out[0])
-    ko = k_ptr = ko_ptr = None
-    kt = kh = kot = koh = 0
+    ko = None
+    k_ptr = ko_ptr = kt = kh = kot = koh = 0
     if k is not None:
         k, kt, kh = _heads(k)
         if out is None:
@@ -237,8 +239,7 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: 
             ko, kot, koh = _heads(out[1])
         k_ptr, ko_ptr = k.data_ptr(), ko.data_ptr()
     stream = _raw_stream(index)
-    pos_ptr = turns = axis = None
-    pos_type = ld = 0
+    pos_ptr = turns = axis = pos_type = ld = 0
     if rotary is not None:
         if not positions.is_contiguous() and (positions.stride(0) < axes or (axes > 1 and positions.stride(1) != 1)):
             positions = positions.contiguous()
@@ -247,10 +248,10 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: 
         tables = rotary._tables.get(index) or rotary.tables(device)
         turns, axis = tables[0].on(stream), tables[1].on(stream)
     with _current(index, device):
-        status = lib.hf_qk_norm_rope(
+        status = lib.hf_qk_norm_rope_call(_rope_args(
             q.data_ptr(), qt, qh, hq, k_ptr, kt, kh, hk, qo.data_ptr(), qot, qoh, ko_ptr, kot, koh, pos_ptr, pos_type,
             ld, axes, turns, axis, pairs, rotary is not None and rotary.interleaved, norm, qw, kw, wide, eps, T, D,
-            code, stream)
+            code, stream))
     _check(status, "hf_qk_norm_rope")
     if out is None:
         return qo, ko
@@ -384,10 +385,11 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, *, sc
         o, ot, oh = _heads(out)
     stream = _raw_stream(index)
     nbytes = plan.ws_bytes
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device).data_ptr() if nbytes else None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device).data_ptr() if nbytes else 0
     with _current(index, device):
-        status = lib.hf_attention(q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, o.data_ptr(), ot,
-                                  oh, scale, plan._host, plan.data.on(stream), plan.bytes, ws, nbytes, code, stream)
+        status = lib.hf_attention_call(_attention_args(
+            q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, o.data_ptr(), ot, oh, scale, plan._host,
+            plan.data.on(stream), plan.bytes, ws, nbytes, code, stream))
     _check(status, "hf_attention")
     return o if out is None or o is out else out.copy_(o)
 
@@ -500,9 +502,10 @@ def adapter_add(y: Tensor, x: Tensor, down: Tensor, up: Tensor, plan: AdapterPla
         nbytes = plan._ws.get((K, r, code))
         if nbytes is None:
             nbytes = plan._ws_bytes(lib, K, r, code)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device).data_ptr() if nbytes else None
-        status = lib.hf_adapter_add(x.data_ptr(), _ld(x), y.data_ptr(), _ld(y), down.data_ptr(), up.data_ptr(), r,
-                                    None if scale is None else scale.data_ptr(), o.data_ptr(), _ld(o), N, K,
-                                    plan._host, plan.data.on(stream), plan.bytes, ws, nbytes, code, stream)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device).data_ptr() if nbytes else 0
+        status = lib.hf_adapter_add_call(_adapter_args(
+            x.data_ptr(), _ld(x), y.data_ptr(), _ld(y), down.data_ptr(), up.data_ptr(), r,
+            0 if scale is None else scale.data_ptr(), o.data_ptr(), _ld(o), N, K, plan._host, plan.data.on(stream),
+            plan.bytes, ws, nbytes, code, stream))
     _check(status, "hf_adapter_add")
     return o if out is None or o is out else out.copy_(o)

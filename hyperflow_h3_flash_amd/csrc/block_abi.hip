@@ -551,4 +551,25 @@ int hf_adapter_add(const void* x, int64_t ldx, const void* y, int64_t ldy, const
                           : launch_adapters<hf::Fp16>(a, h, cut, vec, (hipStream_t)stream);
 }
 
+int hf_qk_norm_rope_call(const hf_qk_norm_rope_args* a) {
+  if (!a) return HF_ERR_ARGUMENT;
+  return hf_qk_norm_rope(a->q, a->q_token, a->q_head, a->heads_q, a->k, a->k_token, a->k_head, a->heads_k, a->q_out,
+                         a->qo_token, a->qo_head, a->k_out, a->ko_token, a->ko_head, a->pos, a->pos_type, a->ld_pos,
+                         a->axes, a->turns, a->axis, a->pairs, a->interleaved, a->norm, a->qw, a->kw, a->weight_f32,
+                         a->eps, a->T, a->D, a->dtype, a->stream);
+}
+
+int hf_attention_call(const hf_attention_args* a) {
+  if (!a) return HF_ERR_ARGUMENT;
+  return hf_attention(a->q, a->q_token, a->q_head, a->k, a->k_token, a->k_head, a->v, a->v_token, a->v_head, a->out,
+                      a->o_token, a->o_head, a->scale, a->plan, a->plan_dev, a->plan_bytes, a->ws, a->ws_bytes,
+                      a->dtype, a->stream);
+}
+
+int hf_adapter_add_call(const hf_adapter_add_args* a) {
+  if (!a) return HF_ERR_ARGUMENT;
+  return hf_adapter_add(a->x, a->ldx, a->y, a->ldy, a->down, a->up, a->r, a->scale, a->out, a->ldo, a->N, a->K,
+                        a->plan, a->plan_dev, a->plan_bytes, a->ws, a->ws_bytes, a->dtype, a->stream);
+}
+
 }  // extern "C"

@@ -92,6 +92,32 @@ int hf_adapter_add(const void* x, int64_t ldx, const void* y, int64_t ldy, const
                    const void* plan_dev, int64_t plan_bytes, void* ws, int64_t ws_bytes, int32_t dtype,
                    hf_stream_t stream);
 
+/*
+ * The three launches again with their parameters in a struct, in the order of the lists above: for callers to whom a
+ * long list of arguments costs host time (a foreign-function call from Python converts one value instead of 31: 1.0 us
+ * against 3.0). `args` is host memory, read before the call returns; NULL is HF_ERR_ARGUMENT.
+ */
+typedef struct {
+  const void* q; int64_t q_token; int64_t q_head; int32_t heads_q; const void* k; int64_t k_token; int64_t k_head;
+  int32_t heads_k; void* q_out; int64_t qo_token; int64_t qo_head; void* k_out; int64_t ko_token; int64_t ko_head;
+  const void* pos; int32_t pos_type; int64_t ld_pos; int32_t axes; const double* turns; const int32_t* axis;
+  int32_t pairs; int32_t interleaved; int32_t norm; const void* qw; const void* kw; int32_t weight_f32; float eps;
+  int64_t T; int32_t D; int32_t dtype; hf_stream_t stream;
+} hf_qk_norm_rope_args;
+typedef struct {
+  const void* q; int64_t q_token; int64_t q_head; const void* k; int64_t k_token; int64_t k_head; const void* v;
+  int64_t v_token; int64_t v_head; void* out; int64_t o_token; int64_t o_head; float scale; const void* plan;
+  const void* plan_dev; int64_t plan_bytes; void* ws; int64_t ws_bytes; int32_t dtype; hf_stream_t stream;
+} hf_attention_args;
+typedef struct {
+  const void* x; int64_t ldx; const void* y; int64_t ldy; const void* down; const void* up; int32_t r;
+  const float* scale; void* out; int64_t ldo; int64_t N; int64_t K; const void* plan; const void* plan_dev;
+  int64_t plan_bytes; void* ws; int64_t ws_bytes; int32_t dtype; hf_stream_t stream;
+} hf_adapter_add_args;
+int hf_qk_norm_rope_call(const hf_qk_norm_rope_args* args);
+int hf_attention_call(const hf_attention_args* args);
+int hf_adapter_add_call(const hf_adapter_add_args* args);
+
 #ifdef __cplusplus
 }
 #endif

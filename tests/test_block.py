@@ -347,6 +347,44 @@ def test_argument_checks_reject_before_launching(lib):
     assert adapt(r=520) == -5
 
 
+@pytest.mark.parametrize("name,packer", [("hf_qk_norm_rope", _native.ROPE_ARGS), ("hf_attention", _native.ATTENTION_ARGS),
+                                         ("hf_adapter_add", _native.ADAPTER_ARGS)])
+def test_structs_hold_the_parameters_in_their_order(name, packer):
+    text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+    declared = [" ".join(p.split()) for p in re.search(r"int " + name + r"\((.*?)\)", text, flags=re.S).group(1).split(",")]
+    body = re.search(r"typedef struct \{([^}]*)\} " + name + "_args;", text).group(1)
+    assert [" ".join(p.split()) for p in body.split(";")[:-1]] == declared
+    kinds = {"int64_t": "q", "int32_t": "i", "float": "f"}
+    assert packer.format == "@" + "".join(kinds.get(p.rsplit(" ", 1)[0], "P") for p in declared)
+    assert packer.size % struct.calcsize("P") == 0
+
+
+def test_calls_by_struct_refuse_as_the_lists_do(lib):
+    rope = [1 << 20, 128, 64, 2, 0, 64, 64, 0, 1 << 20, 128, 64, 0, 64, 64, 1 << 20, 0, 1, 1, 1 << 20, 1 << 20, 32, 1, 1,
+            0, 0, 0, 1e-6, 0, 64, 0, 0]
+    assert lib.hf_qk_norm_rope_call(_native.ROPE_ARGS.pack(*rope)) == 0  # no tokens
+    for at, value, status in ((0, 0, -1), (8, 0, -1), (28, 72, -3), (29, 2, -1), (27, 1 << 31, -5), (1, 130, -3)):
+        assert lib.hf_qk_norm_rope_call(_native.ROPE_ARGS.pack(*(
+            value if i == at else 4 if i == 27 else x for i, x in enumerate(rope)))) == status, at
+    plan = attention_plan(lib, [0], [5])
+    attend = [0, 128, 64, 0, 128, 64, 0, 128, 64, 0, 128, 64, 0.1, ctypes.addressof(plan), 0, len(plan.raw), 0, 0, 0, 0]
+    assert lib.hf_attention_call(_native.ATTENTION_ARGS.pack(*attend)) == 0  # no queries
+    for at, value in ((12, 0.0), (15, len(plan.raw) + 4), (18, 7)):
+        assert lib.hf_attention_call(_native.ATTENTION_ARGS.pack(*(
+            value if i == at else x for i, x in enumerate(attend)))) == -1, at
+    ids = (ctypes.c_int32 * 1)(0)
+    size = lib.hf_adapter_plan(ids, None, 1, 1, 256, None, 0)
+    buf = ctypes.create_string_buffer(size)
+    assert lib.hf_adapter_plan(ids, None, 1, 1, 256, buf, size) == size
+    adapt = [1 << 20, 512, 1 << 20, 64, 1 << 20, 1 << 20, 24, 0, 1 << 20, 64, 0, 512, ctypes.addressof(buf), 1 << 20, size,
+             0, 0, 1, 0]
+    assert lib.hf_adapter_add_call(_native.ADAPTER_ARGS.pack(*adapt)) == 0  # no columns
+    for at, value, status in ((6, 0, -1), (6, 520, -5), (11, 508, -3), (14, size + 1, -1), (17, 2, -1)):
+        assert lib.hf_adapter_add_call(_native.ADAPTER_ARGS.pack(*(
+            value if i == at else x for i, x in enumerate(adapt)))) == status, at
+    assert (lib.hf_qk_norm_rope_call(None) == lib.hf_attention_call(None) == lib.hf_adapter_add_call(None) == -1)
+
+
 def test_planners_refuse_sizes_that_their_memory_would_go_with(lib):
     one, ids = (ctypes.c_int64 * 1)(5), (ctypes.c_int32 * 1)(0)
     assert lib.hf_attention_plan(one, one, 1, 2, 1, 64, 0, 65537, None, 0) == -1
