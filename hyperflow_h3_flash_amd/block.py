@@ -85,6 +85,11 @@ def _heads(t: Tensor) -> tuple[Tensor, int, int]:
     return t, token, head
 
 
+def _new_like(t: Tensor) -> Tensor:
+    """A contiguous tensor of t's size, type and device (of a contiguous t's format: the quicker call)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 def _vector(t: Tensor) -> Tensor:
     """``t`` [n] with its values side by side from a 16-byte boundary."""
     return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
@@ -178,9 +183,7 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: 
             raise ValueError(f"{2 * pairs} rotated channels exceed the head's {D}")
         if positions is None or positions.dtype not in _POSITIONS:
             raise ValueError("positions must be an int32, int64 or float32 tensor")
-        if axes == 1 and positions.dim() == 1:
-            positions = positions[:, None]
-        if positions.shape != (T, axes):
+        if positions.shape != (T, axes) and (axes != 1 or positions.shape != (T,)):
             raise ValueError(f"positions must be [{T}, {axes}], got {tuple(positions.shape)}")
     else:
         positions = None
@@ -201,6 +204,8 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: 
         _forward_only("qk_norm_rope", q, k, q_weight, k_weight)
     code = _dtype_code("qk_norm_rope", dtype)
     if not q.is_cuda:
+        if positions is not None:
+            positions = positions.reshape(T, axes)
         result = host_block.qk_norm_rope(q, k, positions, rotary, q_weight, k_weight, norm, eps)
         if out is None:
             return result
@@ -226,7 +231,7 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: 
             kw = k_weight.data_ptr()
     q, qt, qh = _heads(q)
     if out is None:
-        qo, qot, qoh = q.new_empty((T, hq, D)), hq * D, D
+        qo, qot, qoh = _new_like(q), hq * D, D
     else:
         qo, qot, qoh = _heads(out[0])
     ko = None
@@ -234,7 +239,7 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: 
     if k is not None:
         k, kt, kh = _heads(k)
         if out is None:
-            ko, kot, koh = k.new_empty((T, hk, D)), hk * D, D
+            ko, kot, koh = _new_like(k), hk * D, D
         else:
             ko, kot, koh = _heads(out[1])
         k_ptr, ko_ptr = k.data_ptr(), ko.data_ptr()
@@ -380,7 +385,7 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, *, sc
     k, kt, kh = _keys(k)
     v, vt, vh = _keys(v)
     if out is None:
-        o, ot, oh = q.new_empty(plan._q_shape), plan.heads * plan.head_dim, plan.head_dim
+        o, ot, oh = _new_like(q), plan.heads * plan.head_dim, plan.head_dim
     else:
         o, ot, oh = _heads(out)
     stream = _raw_stream(index)
@@ -496,7 +501,7 @@ def adapter_add(y: Tensor, x: Tensor, down: Tensor, up: Tensor, plan: AdapterPla
         up = up.clone(memory_format=torch.contiguous_format)
     if scale is not None and not scale.is_contiguous():
         scale = scale.contiguous()
-    o = y if in_place else y.new_empty((rows, N)) if out is None else _rows2(out)
+    o = y if in_place else _new_like(y) if out is None else _rows2(out)
     stream = _raw_stream(index)
     with _current(index, device):
         nbytes = plan._ws.get((K, r, code))
