@@ -17,10 +17,10 @@
 // computed. Rows are 256 (D > 64) or 128 bytes; chunk c of row r lies at c ^ f(r) so that both the 16-row fragment reads
 // of K and the 4-row transposing reads of V touch every bank once.
 //
-// Bound: the card's power with long sequences, the keys' bytes with single tokens. 37710 tokens x 7 heads of 128: 4.51 ms,
-// 1130 TFLOP/s (a large library product of the same type: 1555), the matrix unit busy 65 % at 1.62 GHz. The same launch on
-// zeros takes 3.26 ms at the full clock: so energy counts, not issue slots. Leaving out the search for the maximum saved
-// 1 %; adding the weights up two at a time with dot products nothing; running the products of neighbouring tiles under the
+// Bound: the card's power with long sequences, the keys' bytes with single tokens. 37710 tokens x 7 heads of 128:
+// 4.41-4.51 ms, 1154-1130 TFLOP/s (a large library product of the same type: 1555), the matrix unit busy 65 % at 1.62 GHz.
+// The same launch on zeros takes 3.26 ms at the full clock: so energy counts, not issue slots. Leaving out the search for
+// the maximum saved 1 %; adding the weights up two at a time with dot products nothing; running the products of neighbouring tiles under the
 // weights' arithmetic in one wave, with two tiles of scores in registers, raised the matrix unit's share of the cycles and
 // lowered the clock as much (4.63 ms): the two waves of a SIMD overlap well enough by themselves, once the products'
 // operands are read four products ahead (at_order). Three workgroups a compute unit for heads of at most 64, with
