@@ -132,15 +132,23 @@ bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t cou
     std::push_heap(load.begin(), load.end(), less);
     left -= tiles[whole].cost;
   }
-  // No more parts than places, so that none waits for another; parts of six tiles and more.
-  int64_t part = std::max((left + places - 1) / places, (int64_t)6);
+  // No more parts than places, so that none waits for another. A wave's n tiles in parts of p take it p steps and then n / p
+  // reads in the join, a step about eleven reads long: p no less than sqrt(n / 11), and two, or three where a tile's many
+  // rows make the join's reads many. Against six whatever n (us; heads / key heads of 128): one token, 131072 keys, 8 / 1
+  // 37.6 -> 28.5, 4096 keys, 32 / 8 13.4 -> 11.3, 700 keys 12.7 -> 8.9; 300 tokens, 2000 keys, 8 / 8, three 17.6, two 19.5,
+  // six 18.8.
+  int64_t longest_cost = 0, most_rows = 0;
+  for (size_t t = whole; t < tiles.size(); ++t) {
+    const hf::AttentionItem& it = tiles[t].item;
+    longest_cost = std::max(longest_cost, tiles[t].cost);
+    most_rows = std::max(most_rows, std::min((int64_t)it.nq * group - it.row0, (int64_t)hf::kAtRows));
+  }
+  int64_t part = std::max((left + places - 1) / places, (int64_t)(most_rows <= 32 ? 2 : 3));
+  part = std::max(part, (int64_t)ceil(sqrt((double)longest_cost / 11.0)));
   for (;; part += part / 32 + 1) {
-    int64_t parts = 0, longest = 0;
-    for (size_t t = whole; t < tiles.size(); ++t) {
-      parts += std::max((tiles[t].cost + part - 1) / part, (int64_t)1);
-      longest = std::max(longest, tiles[t].cost);
-    }
-    if (parts <= places || part >= longest) break;
+    int64_t parts = 0;
+    for (size_t t = whole; t < tiles.size(); ++t) parts += std::max((tiles[t].cost + part - 1) / part, (int64_t)1);
+    if (parts <= places || part >= longest_cost) break;
   }
   int64_t slots = 0;
   for (size_t t = 0; t < tiles.size(); ++t) {
