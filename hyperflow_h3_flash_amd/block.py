@@ -390,11 +390,12 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, *, sc
         o, ot, oh = _heads(out)
     stream = _raw_stream(index)
     nbytes = plan.ws_bytes
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device).data_ptr() if nbytes else 0
+    # Held until its kernels are launched: given back before, it could be handed to another thread's call in between.
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     with _current(index, device):
         status = lib.hf_attention_call(_attention_args(
             q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, o.data_ptr(), ot, oh, scale, plan._host,
-            plan.data.on(stream), plan.bytes, ws, nbytes, code, stream))
+            plan.data.on(stream), plan.bytes, 0 if ws is None else ws.data_ptr(), nbytes, code, stream))
     _check(status, "hf_attention")
     return o if out is None or o is out else out.copy_(o)
 
@@ -507,10 +508,10 @@ def adapter_add(y: Tensor, x: Tensor, down: Tensor, up: Tensor, plan: AdapterPla
         nbytes = plan._ws.get((K, r, code))
         if nbytes is None:
             nbytes = plan._ws_bytes(lib, K, r, code)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=device).data_ptr() if nbytes else 0
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None  # held, as attention's
         status = lib.hf_adapter_add_call(_adapter_args(
             x.data_ptr(), _ld(x), y.data_ptr(), _ld(y), down.data_ptr(), up.data_ptr(), r,
             0 if scale is None else scale.data_ptr(), o.data_ptr(), _ld(o), N, K, plan._host, plan.data.on(stream),
-            plan.bytes, ws, nbytes, code, stream))
+            plan.bytes, 0 if ws is None else ws.data_ptr(), nbytes, code, stream))
     _check(status, "hf_adapter_add")
     return o if out is None or o is out else out.copy_(o)
