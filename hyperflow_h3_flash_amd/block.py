@@ -28,7 +28,7 @@ import torch
 from torch import Tensor, nn
 
 from . import _native, host_block
-from .int8 import _check, _on, _raw_stream, _same_device
+from .int8 import _check, _forget_input, _on, _raw_stream, _same_device
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
@@ -99,6 +99,23 @@ def _check_out(out: Tensor, like: Tensor, what: str) -> None:
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{what}: out is {tuple(out.shape)} {out.dtype} on {out.device}, expected "
                          f"{tuple(like.shape)} {like.dtype} on {like.device}")
+
+
+def _written(t: Tensor) -> None:
+    """A kernel wrote to ``t``, which was there before: torch is told as by an operation of its own. Autograd's check of
+    saved tensors and the codes that `Int8RotLinear` layers share go by a tensor's version; inference tensors have none."""
+    if t.is_inference():
+        _forget_input(t)
+    else:
+        torch.autograd.graph.increment_version(t)
+
+
+def _deliver(result: Tensor, out: Tensor) -> Tensor:
+    """``out`` holding ``result``, which the kernels wrote to ``out`` itself or to memory of its own."""
+    if result is out:
+        _written(out)
+        return out
+    return out.copy_(result)
 
 
 class _Resident:
@@ -260,10 +277,9 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: 
     _check(status, "hf_qk_norm_rope")
     if out is None:
         return qo, ko
-    if qo is not out[0]:
-        out[0].copy_(qo)
-    if ko is not None and ko is not out[1]:
-        out[1].copy_(ko)
+    _deliver(qo, out[0])
+    if ko is not None:
+        _deliver(ko, out[1])
     return out
 
 
@@ -397,7 +413,7 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, *, sc
             q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, o.data_ptr(), ot, oh, scale, plan._host,
             plan.data.on(stream), plan.bytes, 0 if ws is None else ws.data_ptr(), nbytes, code, stream))
     _check(status, "hf_attention")
-    return o if out is None or o is out else out.copy_(o)
+    return o if out is None else _deliver(o, out)
 
 
 # ----------------------------------------------------------------------------------------------------------- adapters
@@ -514,4 +530,4 @@ def adapter_add(y: Tensor, x: Tensor, down: Tensor, up: Tensor, plan: AdapterPla
             0 if scale is None else scale.data_ptr(), o.data_ptr(), _ld(o), N, K, plan._host, plan.data.on(stream),
             plan.bytes, 0 if ws is None else ws.data_ptr(), nbytes, code, stream))
     _check(status, "hf_adapter_add")
-    return o if out is None or o is out else out.copy_(o)
+    return o if out is None else _deliver(o, out)

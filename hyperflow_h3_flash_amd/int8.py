@@ -359,6 +359,13 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+def _forget_input(t: Tensor) -> None:
+    """Drops the codes that a layer left behind of an input in ``t``'s memory: for writes that no version tells of."""
+    x = Int8RotLinear._last_input.get("x")
+    if x is not None and x.untyped_storage().data_ptr() == t.untyped_storage().data_ptr():
+        Int8RotLinear._last_input.clear()
+
+
 def _workspace(device: torch.device, nbytes: int) -> tuple[Tensor | None, int]:
     """A device workspace of ``nbytes`` (None for 0) from torch's caching allocator; the kernels never allocate."""
     if nbytes <= 0:

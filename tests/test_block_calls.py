@@ -11,7 +11,8 @@ import weakref
 import pytest
 import torch
 
-from hyperflow_h3_flash_amd import AdapterPlan, AttentionPlan, RotaryAxes, adapter_add, packed_attention, qk_norm_rope
+from hyperflow_h3_flash_amd import (AdapterPlan, AttentionPlan, Int8RotLinear, RotaryAxes, adapter_add,
+                                    packed_attention, qk_norm_rope)
 from hyperflow_h3_flash_amd import _native, block
 
 BF = torch.bfloat16
@@ -123,3 +124,57 @@ def test_the_workspace_lives_until_its_kernels_are_launched(launches, monkeypatc
         monkeypatch.setattr(torch, "empty", tracked)
         adapter_add(y, x, down, up, plan)
     assert len(launches.seen) == 1
+
+
+# ------------------------------------------------------------------------------------------------- results in place
+
+def in_place_calls():
+    """(what is written, call) of each operator writing into tensors that were there."""
+    qkv = on_device(rnd(1, 6, 4, 64).to(BF))
+    q, k, v = qkv[:, :2], qkv[:, 2:3], qkv[:, 3:]
+    plan = attention_plan([6], [6], 2, 1, 64)
+    adapters = adapter_plan([0, -1], [4, 2], 1)
+    x, y, wide = (on_device(rnd(i, 6, n).to(BF)) for i, n in ((2, 64), (3, 48), (4, 56)))
+    down, up = on_device(rnd(5, 1, 8, 64).to(BF)), on_device(rnd(6, 1, 48, 8).to(BF))
+    return {
+        "rotation": ((q, k), lambda: qk_norm_rope(q, k, None, None, out=(q, k))),
+        "rotation of queries alone": ((q,), lambda: qk_norm_rope(q, None, None, None, out=(q, None))),
+        "attention": ((q,), lambda: packed_attention(q, k, v, plan, out=q)),
+        "adapters": ((y,), lambda: adapter_add(y, x, down, up, adapters, out=y)),
+        "adapters into a slice": ((wide,), lambda: adapter_add(y, x, down, up, adapters, out=wide[:, :48])),
+    }
+
+
+@pytest.mark.parametrize("name", ["rotation", "rotation of queries alone", "attention", "adapters",
+                                  "adapters into a slice"])
+def test_results_in_place_move_the_version(launches, name):
+    """Autograd's check of saved tensors and the codes that INT8 layers share go by a tensor's version."""
+    written, call = in_place_calls()[name]
+    before = [t._version for t in written]
+    call()
+    assert launches.seen and all(t._version > n for t, n in zip(written, before))
+
+
+@pytest.mark.parametrize("name", ["rotation", "attention", "adapters", "adapters into a slice"])
+def test_results_in_place_drop_codes_of_inference_tensors(launches, name):
+    """Inference tensors have no version, so codes that a layer left of one go when it is written; others stay."""
+    cache = Int8RotLinear._last_input
+    try:
+        with torch.inference_mode():
+            written, call = in_place_calls()[name]
+            assert written[0].is_inference()
+            for x, stays in ((written[0], False), (rnd(9, 4, 4), True)):
+                cache.clear()
+                cache.update(x=x, version=None, value=None)
+                call()
+                assert bool(cache) is stays
+    finally:
+        cache.clear()
+
+
+def test_new_results_leave_the_inputs_versions(launches):
+    q, k = on_device(rnd(1, 6, 2, 64).to(BF)), on_device(rnd(2, 6, 1, 64).to(BF))
+    before = q._version, k._version
+    qk_norm_rope(q, k, None, None)
+    packed_attention(q, k, k, attention_plan([6], [6], 2, 1, 64))
+    assert launches.seen and (q._version, k._version) == before

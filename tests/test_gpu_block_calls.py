@@ -9,7 +9,8 @@ import pytest
 import torch
 
 import block_utils as U
-from hyperflow_h3_flash_amd import AdapterPlan, AttentionPlan, RotaryAxes, adapter_add, packed_attention, qk_norm_rope
+from hyperflow_h3_flash_amd import (AdapterPlan, AttentionPlan, Int8RotLinear, RotaryAxes, adapter_add,
+                                    packed_attention, qk_norm_rope)
 
 pytestmark = pytest.mark.gpu
 BF, HF = torch.bfloat16, torch.float16
@@ -51,3 +52,47 @@ def test_two_threads_on_one_stream():
     for t in threads:
         t.join()
     assert not wrong
+
+
+# ------------------------------------------------------------------------------------------------- results in place
+
+def int8_layer(k, n, seed):
+    layer = Int8RotLinear(k, n, 256)
+    gen = torch.Generator().manual_seed(seed)
+    layer.qweight.copy_(torch.randint(-127, 128, layer.qweight.shape, generator=gen, dtype=torch.int8))
+    layer.wscale.fill_(k ** -0.5 / 73)
+    return layer.cuda()
+
+
+@pytest.mark.parametrize("mode", [torch.no_grad, torch.inference_mode])
+@pytest.mark.parametrize("op", ["rotation", "attention", "adapters"])
+def test_a_layer_after_an_update_in_place_takes_the_new_values(op, mode):
+    """The first of two layers that share one input leaves its codes; the input is updated in place between them."""
+    first, second = int8_layer(256, 128, 1), int8_layer(256, 96, 2)
+    first.keep_input = True
+    try:
+        with mode():
+            x = rnd(3, 20, 256).to(BF)
+            heads = x.view(20, 4, 64)
+            first(x)
+            assert torch.equal(second(x), second(x.clone()))  # shared, and right while x stays
+            first(x)
+            if op == "rotation":
+                qk_norm_rope(heads, None, torch.arange(20).cuda(), RotaryAxes((64,)), out=(heads, None))
+            elif op == "attention":
+                packed_attention(heads, heads.clone(), heads.clone(), AttentionPlan([20], heads=4, head_dim=64), out=heads)
+            else:
+                adapter_add(x, x.clone(), rnd(4, 1, 8, 256).to(BF), rnd(5, 1, 256, 8).to(BF),
+                            AdapterPlan([0], [20], adapters=1), out=x)
+            assert torch.equal(second(x), second(x.clone()))
+    finally:
+        Int8RotLinear._last_input.clear()
+
+
+def test_a_saved_tensor_that_is_overwritten_shows_in_backward():
+    y, x = rnd(1, 20, 64).to(BF), rnd(2, 20, 64).to(BF)
+    w = torch.ones(64, device="cuda", dtype=BF, requires_grad=True)
+    product = y * w  # y is kept for the gradient of w
+    adapter_add(y, x, rnd(3, 1, 8, 64).to(BF), rnd(4, 1, 64, 8).to(BF), AdapterPlan([0], [20], adapters=1), out=y)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.sum().backward()
