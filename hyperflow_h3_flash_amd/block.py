@@ -22,6 +22,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import math
+import threading
 from collections.abc import Sequence
 
 import torch
@@ -119,19 +120,42 @@ def _deliver(result: Tensor, out: Tensor) -> Tensor:
 
 
 class _Resident:
-    """A host buffer and its copy on a device, uploaded once. The copy is complete before the constructor returns, so any
-    stream may read it; `on` keeps its memory from being given out again while another stream than its own reads it."""
+    """A host buffer and its copy on a device, uploaded once and not changed after. The copy is complete when the upload
+    returns, so any stream may read it; `on` keeps its memory from being given out again while another stream than its own
+    reads it. Copies of the objects that hold one share it. Pickled, it is the host buffer: what was loaded uploads at its
+    first use, on a machine that has the device."""
+
+    _uploading = threading.Lock()
 
     def __init__(self, host: Tensor, device: torch.device) -> None:
-        self.host = host
-        self.device_copy = host.to(device)
-        self._ptr = self.device_copy.data_ptr()
-        self._stream = _raw_stream(self.device_copy.get_device())
+        self.__setstate__({"host": host, "device": device})
+        self._upload()
+
+    def _upload(self) -> None:
+        with self._uploading:  # one of several threads: another's copy would take this one's memory back
+            if self.device_copy is None:
+                there = self.host.to(self.device)
+                self._ptr, self._stream = there.data_ptr(), _raw_stream(there.get_device())
+                self.device_copy = there
 
     def on(self, stream: int) -> int:
+        if self.device_copy is None:
+            self._upload()
         if stream != self._stream:
             self.device_copy.record_stream(torch.cuda.current_stream(self.device_copy.device))
         return self._ptr
+
+    def __copy__(self) -> "_Resident":
+        return self
+
+    def __deepcopy__(self, memo: dict) -> "_Resident":
+        return self
+
+    def __getstate__(self) -> dict:
+        return {"host": self.host, "device": self.device}
+
+    def __setstate__(self, state: dict) -> None:
+        self.host, self.device, self.device_copy = state["host"], state["device"], None
 
 
 # ------------------------------------------------------------------------------------------------- norms and rotation
@@ -298,7 +322,10 @@ class _Plan:
         with _on(device):
             self.data = _Resident(host, device)
         self.bytes = size
-        self._host = host.data_ptr()
+
+    @property
+    def _host(self) -> int:
+        return self.data.host.data_ptr()
 
 
 def _plan_device(device: torch.device | str) -> torch.device:

@@ -4,8 +4,11 @@ device, and a library that looks at a launch's parameters instead of launching."
 from __future__ import annotations
 
 import contextlib
+import copy
 import ctypes
+import io
 import os
+import pickle
 import weakref
 
 import pytest
@@ -178,3 +181,57 @@ def test_new_results_leave_the_inputs_versions(launches):
     qk_norm_rope(q, k, None, None)
     packed_attention(q, k, k, attention_plan([6], [6], 2, 1, 64))
     assert launches.seen and (q._version, k._version) == before
+
+
+# -------------------------------------------------------------------------------------------------- copies of plans
+
+def by_pickle(x):
+    return pickle.loads(pickle.dumps(x))
+
+
+def by_torch_save(x):
+    held = io.BytesIO()
+    torch.save(x, held)
+    held.seek(0)
+    return torch.load(held, weights_only=False)
+
+
+@pytest.mark.parametrize("copied", [copy.copy, copy.deepcopy, by_pickle, by_torch_save])
+def test_copies_of_plans_and_tables_point_at_memory_of_their_own(launches, copied):
+    """Every address that a call with a copy passes on lies in a tensor that the copy itself keeps."""
+    rotary = RotaryAxes((32, 32))
+    rotary.tables(torch.device("cpu"))
+    attention, adapters = attention_plan([3], [700], 2, 1, 64), adapter_plan([0], [3], 1)
+    rotary2, attention2, adapters2 = (copied(x) for x in (rotary, attention, adapters))
+    keep = [r.device_copy.clone() for r in rotary.tables(torch.device("cpu"))]
+    q, k = on_device(rnd(1, 3, 2, 64).to(BF)), on_device(rnd(2, 700, 1, 64).to(BF))
+    rotary2._tables[0] = rotary2.tables(torch.device("cpu"))
+    qk_norm_rope(q, None, torch.zeros(3, 2, dtype=torch.int32).as_subclass(OnDevice), rotary2)
+    packed_attention(q, k, k, attention2)
+    x, y = on_device(rnd(3, 3, 64).to(BF)), on_device(rnd(4, 3, 48).to(BF))
+    adapter_add(y, x, on_device(rnd(5, 1, 8, 64).to(BF)), on_device(rnd(6, 1, 48, 8).to(BF)), adapters2)
+    (_, rope), (_, attend), (_, adapt) = launches.seen
+    tables = rotary2.tables(torch.device("cpu"))
+    assert list(rope[18:20]) == [t.device_copy.data_ptr() for t in tables]
+    assert all(torch.equal(t.device_copy, want) for t, want in zip(tables, keep))
+    for seen, at, plan, first in ((attend, 13, attention2, attention), (adapt, 12, adapters2, adapters)):
+        assert list(seen[at:at + 2]) == [plan.data.host.data_ptr(), plan.data.device_copy.data_ptr()]
+        assert torch.equal(plan.data.host, first.data.host)
+
+
+def test_a_copied_module_keeps_its_rotation(launches):
+    module = torch.nn.Linear(2, 2)
+    module.rotary = RotaryAxes((64,))
+    module.rotary.tables(torch.device("cpu"))
+    other = copy.deepcopy(module)
+    want = [t.device_copy.clone() for t in module.rotary.tables(torch.device("cpu"))]
+    del module
+    for t, w in zip(other.rotary.tables(torch.device("cpu")), want):
+        assert t.on(0) == t.device_copy.data_ptr() and torch.equal(t.device_copy, w)
+
+
+def test_a_plan_made_elsewhere_is_uploaded_at_its_first_use(launches):
+    """A pickled plan may be loaded where its device is not: it waits for a call."""
+    plan = by_pickle(attention_plan([3], [700], 2, 1, 64))
+    assert plan.data.device_copy is None
+    assert plan.data.on(0) == plan.data.device_copy.data_ptr()

@@ -3,6 +3,8 @@ layers, beyond 2^31 elements."""
 
 from __future__ import annotations
 
+import copy
+import pickle
 import threading
 
 import pytest
@@ -96,3 +98,36 @@ def test_a_saved_tensor_that_is_overwritten_shows_in_backward():
     adapter_add(y, x, rnd(3, 1, 8, 64).to(BF), rnd(4, 1, 64, 8).to(BF), AdapterPlan([0], [20], adapters=1), out=y)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         product.sum().backward()
+
+
+# -------------------------------------------------------------------------------------------------- copies of plans
+
+@pytest.mark.parametrize("copied", [copy.copy, copy.deepcopy, lambda x: pickle.loads(pickle.dumps(x))],
+                         ids=["copy", "deepcopy", "pickle"])
+def test_copies_outlive_the_plans_and_tables_they_were_made_of(copied):
+    kv = [3000, 40]
+    held = {"rotary": RotaryAxes((32, 32), device="cuda"),
+            "plan": AttentionPlan([2, 3], kv, heads=4, kv_heads=2, head_dim=64, causal=True),
+            "adapters": AdapterPlan([1, -1], [2, 3], adapters=2)}
+    q, k, v = rnd(1, 5, 4, 64).to(BF), rnd(2, sum(kv), 2, 64).to(BF), rnd(3, sum(kv), 2, 64).to(BF)
+    x, down, up = rnd(4, 5, 256).to(BF), rnd(5, 2, 16, 256).to(BF), rnd(6, 2, 256, 16).to(BF)
+    positions = torch.arange(10).view(5, 2).cuda()
+
+    def step():
+        turned, _ = qk_norm_rope(q, None, positions, held["rotary"])
+        o = packed_attention(turned, k, v, held["plan"])
+        return adapter_add(o.view(5, 256), x, down, up, held["adapters"])
+
+    want = step()
+    for name in list(held):
+        held[name] = copied(held[name])
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    taken = [torch.full((1 << 16,), 255, dtype=torch.uint8, device="cuda") for _ in range(20)]  # what was given back
+    assert torch.equal(step(), want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    side.synchronize()
+    assert torch.equal(got, want) and len(taken) == 20
