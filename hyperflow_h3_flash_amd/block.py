@@ -102,13 +102,58 @@ def _check_out(out: Tensor, like: Tensor, what: str) -> None:
                          f"{tuple(like.shape)} {like.dtype} on {like.device}")
 
 
+# A place: (address, rows, heads, row stride, head stride, width) of a tensor [rows, heads, width] of 16-bit elements.
+
+def _apart(a: tuple, b: tuple) -> bool:
+    """Whether no element of place ``a`` lies in place ``b``: separate memory, or slices of one buffer that take different
+    parts of a common period (False where that cannot be told)."""
+    p, rows_a, heads_a, row_a, head_a, width_a = a
+    o, rows_b, heads_b, row_b, head_b, width_b = b
+    heads_take_a, heads_take_b = (heads_a - 1) * head_a + width_a, (heads_b - 1) * head_b + width_b
+    if (p + 2 * ((rows_a - 1) * row_a + heads_take_a) <= o or o + 2 * ((rows_b - 1) * row_b + heads_take_b) <= p
+            or rows_a * heads_a * rows_b * heads_b == 0):
+        return True
+    ahead = (o - p) // 2
+    # What they take of each period: all heads of a row, all rows of a head, or the channels alone.
+    if row_a == row_b and row_a and heads_take_a <= ahead % row_a <= row_a - heads_take_b:
+        return True
+    if head_a == head_b and head_a and (
+            (rows_a - 1) * row_a + width_a <= ahead % head_a <= head_a - (rows_b - 1) * row_b - width_b):
+        return True
+    period = math.gcd(row_a, head_a, row_b, head_b)
+    return period > 0 and width_a <= ahead % period <= period - width_b
+
+
+def _spread(place: tuple) -> bool:
+    """Whether no two elements of a place lie in one."""
+    _, rows, heads, row, head, width = place
+    return (head >= width and row >= (heads - 1) * head + width) or (row >= width and head >= (rows - 1) * row + width)
+
+
+def _result(out: Tensor, own: tuple, *others: tuple) -> tuple[Tensor, int, int]:
+    """Where the kernels write a result that is to be in ``out`` [rows, heads, width], with its strides: out itself, or new
+    memory where out's layout is not theirs or some of it lies in ``others``, which other workgroups may still read, or in
+    ``own`` other than element by element (there each element is read by the workgroup that writes it)."""
+    o, row, head = _heads(out)
+    if o is out:
+        rows, heads, width = out.shape
+        place = (out.data_ptr(), rows, heads, row, head, width)
+        if not _spread(place) or not (place == own or _apart(place, own)) or not all(_apart(place, x) for x in others):
+            o, row, head = out.new_empty(out.shape), heads * width, width
+    return o, row, head
+
+
+#: Moves the versions of some tensors, as an operation of torch's own on them would.
+_increment_versions = getattr(torch._C, "_increment_version", None) or torch.autograd.graph.increment_version
+
+
 def _written(t: Tensor) -> None:
     """A kernel wrote to ``t``, which was there before: torch is told as by an operation of its own. Autograd's check of
     saved tensors and the codes that `Int8RotLinear` layers share go by a tensor's version; inference tensors have none."""
     if t.is_inference():
         _forget_input(t)
     else:
-        torch.autograd.graph.increment_version(t)
+        _increment_versions((t,))
 
 
 def _deliver(result: Tensor, out: Tensor) -> Tensor:
@@ -207,7 +252,8 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: 
     one; weights [D] in the inputs' type or float32), then the rotation of ``rotary`` (None: none) at ``positions``
     [T, axes] (or [T] for one axis; int32, int64 or float32). Computed in float32, rounded once to the inputs' type
     (bfloat16 or float16). q and k may be views with any token and head strides, such as slices of a fused projection.
-    ``out`` may name the results' tensors, the inputs themselves among them. D is a multiple of 16, up to 256."""
+    ``out`` may name the results' tensors, the inputs themselves among them (written directly where each is its own
+    input's, through new memory where they overlap otherwise). D is a multiple of 16, up to 256."""
     dtype, shape = q.dtype, q.shape
     if len(shape) != 3 or (k is not None and (k.dim() != 3 or k.shape[0] != shape[0] or k.shape[2] != shape[2])):
         raise ValueError("qk_norm_rope expects q [T, Hq, D] and k [T, Hk, D]")
@@ -271,19 +317,29 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: 
             k_weight = _vector(k_weight)
             kw = k_weight.data_ptr()
     q, qt, qh = _heads(q)
-    if out is None:
-        qo, qot, qoh = _new_like(q), hq * D, D
-    else:
-        qo, qot, qoh = _heads(out[0])
     ko = None
     k_ptr = ko_ptr = kt = kh = kot = koh = 0
     if k is not None:
         k, kt, kh = _heads(k)
-        if out is None:
+        k_ptr = k.data_ptr()
+    if out is None:
+        qo, qot, qoh = _new_like(q), hq * D, D
+        if k is not None:
             ko, kot, koh = _new_like(k), hk * D, D
+    else:
+        places = [(q.data_ptr(), T, hq, qt, qh, D)]
+        if k is not None:
+            places.append((k_ptr, T, hk, kt, kh, D))
+        if out[0] is q and (k is None or out[1] is k) and all(map(_spread, places)):
+            qo, qot, qoh = q, qt, qh  # in place: each element is read by the workgroup that writes it
+            if k is not None:
+                ko, kot, koh = k, kt, kh
         else:
-            ko, kot, koh = _heads(out[1])
-        k_ptr, ko_ptr = k.data_ptr(), ko.data_ptr()
+            qo, qot, qoh = _result(out[0], *places)
+            if k is not None:
+                ko, kot, koh = _result(out[1], *reversed(places))
+    if ko is not None:
+        ko_ptr = ko.data_ptr()
     stream = _raw_stream(index)
     pos_ptr = turns = axis = pos_type = ld = 0
     if rotary is not None:
@@ -400,7 +456,7 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, *, sc
     ``head_dim ** -0.5``) is positive. A query that sees no key gets zeros; what k and v hold at keys that a query does
     not see never reaches it. Scores, weights' sums and outputs are summed in float32, and divided by the weights' sum at the
     end (values of v times the number of keys have to stay in its range); the weights enter the second product in the
-    inputs' type."""
+    inputs' type. ``out`` may be any tensor like q, the inputs among them (new memory is used where it lies in k or v)."""
     if q.shape != plan._q_shape or k.shape != plan._kv_shape or v.shape != plan._kv_shape:
         raise ValueError(f"the plan is for q {plan._q_shape} and k, v {plan._kv_shape}; got {tuple(q.shape)}, "
                          f"{tuple(k.shape)}, {tuple(v.shape)}")
@@ -430,7 +486,9 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, *, sc
     if out is None:
         o, ot, oh = _new_like(q), plan.heads * plan.head_dim, plan.head_dim
     else:
-        o, ot, oh = _heads(out)
+        rows, heads, d = plan._kv_shape
+        o, ot, oh = _result(out, (q.data_ptr(), *plan._q_shape[:2], qt, qh, d), (k.data_ptr(), rows, heads, kt, kh, d),
+                            (v.data_ptr(), rows, heads, vt, vh, d))
     stream = _raw_stream(index)
     nbytes = plan.ws_bytes
     # Held until its kernels are launched: given back before, it could be handed to another thread's call in between.
@@ -546,6 +604,10 @@ def adapter_add(y: Tensor, x: Tensor, down: Tensor, up: Tensor, plan: AdapterPla
     if scale is not None and not scale.is_contiguous():
         scale = scale.contiguous()
     o = y if in_place else _new_like(y) if out is None else _rows2(out)
+    if o is out and not in_place:
+        here, there = (o.data_ptr(), rows, 1, _ld(o), N, N), (y.data_ptr(), rows, 1, _ld(y), N, N)
+        if here != there and not _apart(here, there):
+            o = out.new_empty(out.shape)  # rows of y that other workgroups may still read
     stream = _raw_stream(index)
     with _current(index, device):
         nbytes = plan._ws.get((K, r, code))

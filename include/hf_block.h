@@ -30,7 +30,8 @@ extern "C" {
  *   (a, b) -> (a cos - b sin, a sin + b cos), angle = 2 pi * pos[t, axis[p]] * turns[p], for the pairs p < pairs:
  *     interleaved != 0: channels (2p, 2p + 1);  interleaved == 0: channels (p, p + pairs)
  *   channels at and after 2 * pairs keep n. All in fp32 (the angle's whole turns are taken off in fp64), rounded once.
- * x: [T, heads, D] with strides (token, head), channels contiguous; out the same (may be x itself, with x's strides).
+ * x: [T, heads, D] with strides (token, head), channels contiguous; out the same (may be x itself, with x's strides, and
+ * otherwise overlaps neither side's x).
  * heads_k == 0 leaves k out (its pointers are not read). pos: [T, axes] of int32 (HF_POS_I32), int64 (HF_POS_I64) or
  * fp32 (HF_POS_F32), rows `ld_pos` apart; turns: fp64 [pairs], revolutions per position step (theta^(-2i/dim) / 2 pi);
  * axis: int32 [pairs], each in [0, axes). qw, kw: [D] of x's type, or fp32 with weight_f32 != 0, or NULL.
@@ -50,7 +51,8 @@ int hf_qk_norm_rope(const void* q, int64_t q_token, int64_t q_head, int32_t head
 /*
  * Attention over packed sequences. Sequence b has q_lens[b] queries and kv_lens[b] keys, one sequence behind the other
  * in q, out [sum q_lens, heads, D] and k, v [sum kv_lens, kv_heads, D]; query head h reads key head h / (heads /
- * kv_heads). out_i = sum_j w_ij v_j, w_i = softmax_j(scale * q_i . k_j) over the sequence's keys; causal: over the keys
+ * kv_heads). out may be q itself, with q's strides, and otherwise overlaps none of them.
+ * out_i = sum_j w_ij v_j, w_i = softmax_j(scale * q_i . k_j) over the sequence's keys; causal: over the keys
  * j <= i + kv_lens[b] - q_lens[b] (the last query sees every key). A query with no key gets zeros; keys that a query
  * does not see never reach it, whatever k and v hold there.
  *
@@ -76,8 +78,8 @@ int hf_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, 
  * Low-rank adapters of many requests beside a shared projection: for row m with adapter a = ids[m],
  *   out[m] = y[m] + scale[a] * (x[m] @ down[a]^T) @ up[a]^T,   out[m] = y[m] for a = -1,
  * summed in fp32 with the rank-wide intermediate kept to 16 bits of mantissa or more, rounded once.
- * x: [M, K]; y, out: [M, N] (out may be y itself, with y's stride); down: [adapters, r, K]; up: [adapters, N, r];
- * scale: fp32 [adapters] or NULL (ones).
+ * x: [M, K]; y, out: [M, N] (out may be y itself, with y's stride, and otherwise does not overlap it);
+ * down: [adapters, r, K]; up: [adapters, N, r]; scale: fp32 [adapters] or NULL (ones).
  *
  * hf_adapter_plan (host) groups the rows by adapter once for all projections of a batch: `ids` holds one adapter or -1
  * for each of `count` requests, `lens` its rows (NULL: one each). Used like hf_attention_plan.

@@ -235,3 +235,61 @@ def test_a_plan_made_elsewhere_is_uploaded_at_its_first_use(launches):
     plan = by_pickle(attention_plan([3], [700], 2, 1, 64))
     assert plan.data.device_copy is None
     assert plan.data.on(0) == plan.data.device_copy.data_ptr()
+
+
+# --------------------------------------------------------------------------------------------- results over the inputs
+
+def test_attention_never_writes_where_it_still_reads(launches):
+    """Workgroups read keys and values long after others have written rows of the result."""
+    qkv = on_device(rnd(1, 6, 4, 64).to(BF))
+    q, k, v = qkv[:, :2], qkv[:, 2:3], qkv[:, 3:]
+    plan, alike = attention_plan([6], [6], 2, 1, 64), attention_plan([6], [6], 2, 2, 64)
+    whole = on_device(rnd(2, 6, 2, 64).to(BF))
+    halves = on_device(rnd(3, 6, 2, 3, 64).to(BF))  # q, k and v of a head side by side
+    heads_first = on_device(rnd(4, 4, 6, 64).to(BF)).transpose(0, 1)
+    shifted = on_device(rnd(5, 8, 2, 64).to(BF))
+    for args, out, direct in (
+        ((q, k, v, plan), q, True), ((q, k, v, plan), on_device(rnd(6, 6, 2, 64).to(BF)), True),
+        ((*halves.unbind(2), alike), halves[:, :, 0], True),
+        ((heads_first[:, :2], heads_first[:, 2:3], heads_first[:, 3:], plan), heads_first[:, :2], True),
+        ((whole, whole, whole, alike), whole, False), ((q, whole, qkv[:, 2:], alike), whole, False),
+        ((q, qkv[:, 2:], whole, alike), whole, False), ((q, k, v, plan), qkv[:, 1:3], False),
+        ((shifted[:6], whole, whole, alike), shifted[2:], False),  # the queries of another row
+        ((*halves.unbind(2), alike), halves[:, :, 1], False),
+    ):
+        packed_attention(*args, out=out)
+        assert (launches.seen[-1][1][9] == out.data_ptr()) is direct
+
+
+def test_rotation_and_adapters_never_write_where_they_still_read(launches):
+    q, k, other = (on_device(rnd(i, 6, 2, 64).to(BF)) for i in range(3))
+    long = on_device(rnd(3, 9, 2, 64).to(BF))
+    for args, out, direct in (
+        ((q, k), (q, k), (True, True)), ((q, k), (q, other), (True, True)), ((q, k), (q.view(6, 2, 64), k), (True, True)),
+        ((q, k), (k, q), (False, False)), ((q, k), (k, other), (False, True)), ((q, k), (other, q), (True, False)),
+        ((long[:6], None), (long[1:7], None), (False, True)),
+    ):
+        qk_norm_rope(*args, None, None, out=out)
+        seen = launches.seen[-1][1]
+        assert (seen[8] == out[0].data_ptr()) is direct[0]
+        assert out[1] is None or (seen[11] == out[1].data_ptr()) is direct[1]
+    plan = adapter_plan([0, -1], [4, 2], 1)
+    x, wide, rows = on_device(rnd(4, 6, 64).to(BF)), on_device(rnd(5, 6, 128).to(BF)), on_device(rnd(6, 9, 64).to(BF))
+    down, up = on_device(rnd(7, 1, 8, 64).to(BF)), on_device(rnd(8, 1, 64, 8).to(BF))
+    y = wide[:, :64]
+    for y, out, direct in ((y, y, True), (y, wide[:, :64], True), (y, wide[:, 64:], True), (y, wide[:, 8:72], False),
+                           (rows[:6], rows[3:], False), (y, x, True)):  # x is read before anything is written
+        adapter_add(y, x, down, up, plan, out=out)
+        assert (launches.seen[-1][1][8] == out.data_ptr()) is direct
+
+
+def test_results_that_overlap_themselves_are_refused(launches):
+    """As torch's own operations refuse to write several values to one place."""
+    q = on_device(rnd(1, 6, 2, 64).to(BF))
+    out = on_device(torch.zeros(1, 2, 64, dtype=BF)).expand(6, 2, 64)
+    for bad in (lambda: qk_norm_rope(q, None, None, None, out=(out, None)),
+                lambda: packed_attention(q, q, q, attention_plan([6], [6], 2, 2, 64), out=out),
+                lambda: adapter_add(q[:, 0], q[:, 1], on_device(rnd(3, 1, 8, 64).to(BF)), on_device(rnd(4, 1, 64, 8).to(BF)),
+                                    adapter_plan([0], [6], 1), out=out[:, 0])):
+        with pytest.raises(RuntimeError, match="single memory location|overlap"):
+            bad()

@@ -131,3 +131,31 @@ def test_copies_outlive_the_plans_and_tables_they_were_made_of(copied):
         got = step()
     side.synchronize()
     assert torch.equal(got, want) and len(taken) == 20
+
+
+def test_results_over_the_inputs_are_those_of_a_separate_result():
+    """A result may name memory that the call reads: keys, values, the other side's heads, rows of y further on."""
+    lens, H, D = [500, 40], 4, 64
+    n = sum(lens)
+    plan, positions, rotary = AttentionPlan(lens, heads=H, head_dim=D), torch.arange(n).cuda(), RotaryAxes((D,))
+
+    def fresh():
+        return [rnd(i, n, H, D).to(BF) for i in range(3)]
+
+    q, k, v = fresh()
+    want, (q_want, k_want) = packed_attention(q, k, v, plan), qk_norm_rope(q, k, positions, rotary)
+    for name in range(3):
+        t = fresh()
+        assert torch.equal(packed_attention(*t, plan, out=t[name]), want)
+        x = fresh()[0]
+        assert torch.equal(packed_attention(x, x, x, plan, out=x), packed_attention(*[fresh()[0]] * 3, plan))
+    for out in ((1, 0), (1, 2), (2, 0), (0, 1)):
+        t = fresh()
+        qk_norm_rope(t[0], t[1], positions, rotary, out=(t[out[0]], t[out[1]]))
+        assert torch.equal(t[out[0]], q_want) and torch.equal(t[out[1]], k_want)
+    adapters, down, up = AdapterPlan([0, -1], lens, adapters=1), rnd(5, 1, 8, 64).to(BF), rnd(6, 1, 64, 8).to(BF)
+    x, rows = rnd(7, n, 64).to(BF), rnd(8, n + 3, 64).to(BF)
+    want = adapter_add(rows[:n].clone(), x, down, up, adapters)
+    assert torch.equal(adapter_add(rows[:n], x, down, up, adapters, out=rows[3:]), want)
+    y = rnd(8, n + 3, 64).to(BF)[:n]
+    assert torch.equal(adapter_add(y, x, down, up, adapters, out=x), want)
