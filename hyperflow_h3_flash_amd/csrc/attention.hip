@@ -36,9 +36,17 @@ namespace hf {
 
 constexpr int kAtKeys = 64;
 constexpr int kAtWaves = 4, kAtRows = 32 * kAtWaves;  // of a workgroup
-// What a lane's weights of one tile may sum to before their maximum is taken anew: fp16 holds them, and the sums have as
-// much room for large values as that many keys of equal weight take.
-constexpr float kAtMost = 512.0f;
+// The largest weight is 2^at_lift when its maximum is taken, not 1: the factor is in the weights' sum too and leaves with
+// the quotient. fp16 loses bits under 2^-14 and everything under 2^-25, so with a largest of 1, small weights beside a
+// dominant one would be lost to the product and kept in the sum (40000 keys of weight 2^-25.06 beside one of 1: 1.1e-3 of
+// the result). Six powers up they keep all bits down to 2^-20 and some down to 2^-31. bfloat16 has float32's exponents.
+template <class T>
+constexpr int at_lift() { return T::kNarrow ? 6 : 0; }
+// What a lane's weights of one tile may sum to before their maximum is taken anew: 512 times the largest when that was
+// taken. fp16 holds them (at most 2^15), and bfloat16's sums have as much room for large values as that many keys of equal
+// weight take.
+template <class T>
+constexpr float at_most() { return (float)(512 << at_lift<T>()); }
 
 // A work item: rows row0 .. of sequence (q0, nq, k0, nk) and key head `head`, over keys [key_lo, key_hi). slot < 0: the
 // result goes to out; else the unnormalised sums go to workspace tile `slot`.
@@ -59,6 +67,7 @@ struct AttentionArgs {
   int64_t q_token, q_head, k_token, k_head, v_token, v_head, o_token, o_head;
   int group, D, causal;
   float scale_log2;
+  float lift;  // at_lift in units of the scores
 };
 
 template <int PITCH>
@@ -214,7 +223,7 @@ __global__ __launch_bounds__(64 * kAtWaves, 2) void attention_kernel(AttentionAr
 
   // Scores to weights, in the operand order of the second product: p = 2^(c (s - m)). m need not be the running maximum,
   // only near enough that the weights keep their precision and their sums stay in range: it is taken in the first tile
-  // that a row sees, and anew when a tile's weights sum to more than kAtMost (or to NaN). Looking for the maximum in every
+  // that a row sees, and anew when a tile's weights sum to more than at_most (or to NaN). Looking for the maximum in every
   // tile would be a seventh of the vector unit's work. Each row goes by its own scores alone, so that its bits do not
   // depend on the rows that share its wave. The sums over the keys are rescaled when m moves (`rescale`).
   auto exponentials = [&](const v16f (&s)[2], v4u (&pf)[4], int p, float mc, float (&part)[2])
@@ -230,12 +239,13 @@ __global__ __launch_bounds__(64 * kAtWaves, 2) void attention_kernel(AttentionAr
   // After all 16: their sum, or, where m has to move, new weights first.
   auto settle = [&](const v16f (&s)[2], v4u (&pf)[4], float (&part)[2]) __attribute__((always_inline)) {
     float sum = part[0] + part[1];
-    if (__any(!(sum <= kAtMost) || m == -__builtin_inff())) {
+    if (__any(!(sum <= at_most<T>()) || m == -__builtin_inff())) {
       float top = m;
 #pragma unroll
       for (int v = 0; v < 16; ++v) top = fmaxf(fmaxf(top, s[0][v]), s[1][v]);
       top = half_max(top);
-      const bool move = half_max(sum <= kAtMost ? 0.0f : 1.0f) > 0.0f || m == -__builtin_inff();
+      const bool move = half_max(sum <= at_most<T>() ? 0.0f : 1.0f) > 0.0f || m == -__builtin_inff();
+      if constexpr (at_lift<T>() > 0) top -= a.lift;
       m = move ? top : m;
       const float mc = centre();
       part[0] = part[1] = 0.0f;

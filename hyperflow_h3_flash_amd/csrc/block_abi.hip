@@ -455,6 +455,8 @@ int hf_attention(const void* q, int64_t q_token, int64_t q_head, const void* k, 
   a.v_token = v_token, a.v_head = v_head, a.o_token = o_token, a.o_head = o_head;
   a.group = h.heads / h.kv_heads, a.D = h.D, a.causal = h.causal;
   a.scale_log2 = (float)((double)scale * 1.4426950408889634);
+  // Finite however small the scale: there every weight is one, whatever is taken off.
+  a.lift = (float)std::min((dtype == HF_FP16 ? hf::at_lift<hf::Fp16>() : 0) / (double)a.scale_log2, 0x1p127);
   return dtype == HF_BF16 ? launch_attention_of<hf::Bf16>(a, h, (hipStream_t)stream)
                           : launch_attention_of<hf::Fp16>(a, h, (hipStream_t)stream);
 }

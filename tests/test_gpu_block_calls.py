@@ -4,6 +4,7 @@ layers, beyond 2^31 elements."""
 from __future__ import annotations
 
 import copy
+import math
 import pickle
 import threading
 
@@ -159,3 +160,43 @@ def test_results_over_the_inputs_are_those_of_a_separate_result():
     assert torch.equal(adapter_add(rows[:n], x, down, up, adapters, out=rows[3:]), want)
     y = rnd(8, n + 3, 64).to(BF)[:n]
     assert torch.equal(adapter_add(y, x, down, up, adapters, out=x), want)
+
+
+# ------------------------------------------------------------------------------------------------ attention's weights
+
+@pytest.mark.parametrize("exponent", [14.0, 20.0, 25.0625, 29.0])
+@pytest.mark.parametrize("dtype", [HF, BF])
+def test_small_weights_beside_a_dominant_one(dtype, exponent):
+    """One key that takes nearly all of the weight and 40000 of equal small weights, in tiles of rows that are not cut (a
+    share without the dominant key has a maximum of its own). Rounding errs by at most u of a weight where fp16 is normal,
+    and by 2^-31 of the largest weight below that: fp16's least step of 2^-24, halved, with weights taken up to 2^6."""
+    n, D, M = 40001, 64, 65536
+    q = torch.zeros(M, 1, D, device="cuda", dtype=dtype)
+    q[..., 0] = 1
+    k = torch.zeros(n, 1, D, device="cuda", dtype=dtype)
+    k[5, 0, 0] = exponent
+    for v in (torch.ones(n, 1, D, device="cuda"), 0.5 + rnd(1, n, 1, D)):
+        v = v.to(dtype)
+        v[5] = 0
+        plan = AttentionPlan([M], [n], heads=1, head_dim=D)
+        assert plan.ws_bytes == 0
+        scale = math.log(2.0)
+        got = packed_attention(q, k, v, plan, scale=scale)
+        assert (got == got[0]).all()
+        w = torch.exp2(k[:, 0, 0].double() * (scale * math.log2(math.e)))
+        w /= w.sum()
+        want, size = w @ v[:, 0].double(), w @ v[:, 0].double().abs()
+        u = U.UNIT[dtype]
+        # A score errs by a few float32 roundings of its size, which moves a weight in proportion; sums run over n keys.
+        off = (exponent * (D + 8) + n) * 2.0 ** -24
+        lost = 2.0 ** -31 * v[:, 0].double().abs().sum(0) if dtype is HF else 0.0
+        U.check(got[0, 0], want, u * want.abs() + (u + off) * size + lost + U.TINY[dtype], str(exponent))
+
+
+def test_scores_of_no_weight_in_fp16():
+    """The smallest scales make every weight one; one of them is a share's, joined."""
+    for rows, n in ((300, 70), (3, 5000)):
+        q, k, v = rnd(1, rows, 1, 64).to(HF), rnd(2, n, 1, 64).to(HF), rnd(3, n, 1, 64).to(HF)
+        plan = AttentionPlan([rows], [n], heads=1, head_dim=64)
+        for scale in (1e-6, 1e-30, 1e-37):
+            U.check(packed_attention(q, k, v, plan, scale=scale), *U.attention(q, k, v, [rows], [n], False, scale))
