@@ -10,7 +10,8 @@ from __future__ import annotations
 import torch
 from torch import Tensor, nn
 
-from .block import AdapterPlan, AttentionPlan, RotaryAxes, adapter_add, packed_attention, qk_norm_rope
+from .block import (AdapterPlan, AttentionPlan, RotaryAxes, _differentiable, _forward_only, adapter_add, packed_attention,
+                    qk_norm_rope)
 from .int8 import Int8RotLinear
 from .lowrank import fuse_qkv
 
@@ -101,11 +102,13 @@ class AttentionBlock(nn.Module):
                         p, device=device))
         return block
 
-    @torch.no_grad()
     def forward(self, x: Tensor, plan: AttentionPlan, *, positions: Tensor | None = None,
                 rotary: RotaryAxes | None = None, adapters: AdapterPlan | None = None) -> Tensor:
         """``x`` [tokens, dim] (bfloat16), the tokens of ``plan``'s sequences one behind the other; ``positions``
-        [tokens, axes] with ``rotary``; ``adapters`` names the adapter of each request's tokens."""
+        [tokens, axes] with ``rotary``; ``adapters`` names the adapter of each request's tokens. Forward only, as its
+        operators are: x that requires a gradient is refused unless gradients are off."""
+        if _differentiable():
+            _forward_only("AttentionBlock", x)
         if adapters is not None and self.qkv_adapters is None:
             raise ValueError("the block was built without adapters")
         heads, kv_heads = self.heads, self.kv_heads

@@ -27,6 +27,7 @@ from collections.abc import Sequence
 
 import torch
 from torch import Tensor, nn
+from torch.autograd import forward_ad
 
 from . import _native, host_block
 from .int8 import _check, _forget_input, _on, _raw_stream, _same_device
@@ -43,11 +44,19 @@ _device_index = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current
 # With few rows the host time of a call is as long as its kernels (a kernel of 5 us in a call of 10): the functions below
 # read each property once, and leave their straight path only where something is unusual.
 
+def _differentiable() -> bool:
+    """Whether gradients or forward-mode tangents may be recorded; ``torch.no_grad`` leaves the latter on."""
+    return torch.is_grad_enabled() or forward_ad._current_level >= 0
+
+
 def _forward_only(what: str, *tensors: Tensor | None) -> None:
+    """Refuses tensors that the call would have to be differentiated for (where `_differentiable`)."""
+    grads, tangents = torch.is_grad_enabled(), forward_ad._current_level >= 0
     for t in tensors:
-        if t is not None and t.requires_grad:
+        if t is not None and ((grads and t.requires_grad)
+                              or (tangents and forward_ad.unpack_dual(t).tangent is not None)):
             raise RuntimeError(f"{what} is forward only: call it under torch.no_grad(), or on tensors that do not "
-                               "require a gradient")
+                               "require a gradient and have no tangent")
 
 
 def _lib(device: torch.device) -> ctypes.CDLL:
@@ -287,8 +296,8 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: 
     for t in (k, positions, q_weight, k_weight):
         if t is not None and t.get_device() != index:
             _same_device(q.device, t)
-    if torch.is_grad_enabled():
-        _forward_only("qk_norm_rope", q, k, q_weight, k_weight)
+    if _differentiable():
+        _forward_only("qk_norm_rope", q, k, positions, q_weight, k_weight, *(out or ()))
     code = _dtype_code("qk_norm_rope", dtype)
     if not q.is_cuda:
         if positions is not None:
@@ -473,8 +482,8 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, *, sc
     if k.get_device() != index or v.get_device() != index or index != plan._index:
         _same_device(q.device, k, v)
         raise ValueError(f"tensors on {q.device}, the plan is for {plan.device}")
-    if torch.is_grad_enabled():
-        _forward_only("packed_attention", q, k, v)
+    if _differentiable():
+        _forward_only("packed_attention", q, k, v, out)
     if not q.is_cuda:
         result = host_block.packed_attention(q, k, v, plan, scale)
         return result if out is None else out.copy_(result)
@@ -586,8 +595,8 @@ def adapter_add(y: Tensor, x: Tensor, down: Tensor, up: Tensor, plan: AdapterPla
             or (scale is not None and scale.get_device() != index)):
         _same_device(y.device, x, down, up, scale)
         raise ValueError(f"tensors on {y.device}, the plan is for {plan.device}")
-    if torch.is_grad_enabled():
-        _forward_only("adapter_add", y, x, down, up, scale)
+    if _differentiable():
+        _forward_only("adapter_add", y, x, down, up, scale, out)
     if plan.live_rows == 0:  # no row has an adapter: y itself
         return y.clone() if out is None else out if out is y else out.copy_(y)
     if not y.is_cuda:

@@ -13,6 +13,7 @@ import weakref
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from hyperflow_h3_flash_amd import (AdapterPlan, AttentionPlan, Int8RotLinear, RotaryAxes, adapter_add,
                                     packed_attention, qk_norm_rope)
@@ -293,3 +294,65 @@ def test_results_that_overlap_themselves_are_refused(launches):
                                     adapter_plan([0], [6], 1), out=out[:, 0])):
         with pytest.raises(RuntimeError, match="single memory location|overlap"):
             bad()
+
+
+# ----------------------------------------------------------------------------------------------------- forward only
+
+def operators(device):
+    """Each operator as (name, its tensors by name, call)."""
+    move = on_device if device else (lambda t: t)
+    t = {n: move(rnd(i, *shape).to(BF)) for i, (n, shape) in enumerate(
+        (("q", (6, 2, 64)), ("k", (6, 1, 64)), ("v", (6, 1, 64)), ("w", (64,)), ("x", (6, 32)), ("y", (6, 48)),
+         ("down", (1, 8, 32)), ("up", (1, 48, 8)), ("out", (6, 2, 64)), ("out2", (6, 48))))}
+    t["positions"], t["scale"] = move(torch.arange(6.0)), move(torch.ones(1))
+    plan, adapters = attention_plan([6], [6], 2, 1, 64), adapter_plan([0], [6], 1)
+    if not device:
+        plan._index = adapters._index = -1
+    rotary = RotaryAxes((64,))
+    rotary._tables[0] = rotary.tables(torch.device("cpu"))
+    return (
+        (("q", "k", "positions", "w", "out"), t, lambda t: qk_norm_rope(
+            t["q"], t["k"], t["positions"], rotary, q_weight=t["w"], out=(t["out"], t["k"]))),
+        (("q", "k", "v", "out"), t, lambda t: packed_attention(t["q"], t["k"], t["v"], plan, out=t["out"])),
+        (("x", "y", "down", "up", "scale", "out2"), t, lambda t: adapter_add(
+            t["y"], t["x"], t["down"], t["up"], adapters, scale=t["scale"], out=t["out2"])),
+    )
+
+
+@pytest.mark.parametrize("device", [False, True], ids=["host", "device"])
+def test_what_would_have_to_be_differentiated_is_refused(launches, device):
+    """Gradients and forward-mode tangents of every tensor that a call takes, its result's among them."""
+    for names, tensors, call in operators(device):
+        call(tensors)
+        for name in names:
+            leaf = tensors[name].clone().requires_grad_()
+            with pytest.raises(RuntimeError, match="forward only"):
+                call({**tensors, name: leaf})
+            with torch.no_grad():
+                call({**tensors, name: leaf})
+            with forward_ad.dual_level():
+                dual = forward_ad.make_dual(tensors[name].clone(), torch.ones_like(tensors[name]))
+                with pytest.raises(RuntimeError, match="forward only"):
+                    call({**tensors, name: dual})
+                with pytest.raises(RuntimeError, match="forward only"), torch.no_grad():  # which keeps tangents
+                    call({**tensors, name: dual})
+                call(tensors)
+
+
+def test_the_block_refuses_what_would_have_to_be_differentiated():
+    from test_block import make_block
+
+    block = make_block()
+    plan = AttentionPlan([4], heads=4, kv_heads=2, head_dim=16, device="cpu")
+    x = rnd(1, 4, 64).to(BF)
+    want = block(x, plan)
+    assert not want.requires_grad
+    with torch.no_grad():
+        assert torch.equal(block(x.clone().requires_grad_(), plan), want)
+    with pytest.raises(RuntimeError, match="forward only"):
+        block(x.clone().requires_grad_(), plan)
+    with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward only"):
+        block(forward_ad.make_dual(x, torch.ones_like(x)), plan)
+    block.norm_q.requires_grad_()
+    with pytest.raises(RuntimeError, match="forward only"):
+        block(x, plan)
