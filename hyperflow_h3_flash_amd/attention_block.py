@@ -54,7 +54,10 @@ class AdapterBank(nn.Module):
         self.scale[index] = scale
 
     def forward(self, y: Tensor, x: Tensor, plan: AdapterPlan, out: Tensor | None = None) -> Tensor:
-        return adapter_add(y, x, self.down, self.up, plan, scale=self.scale, out=out)
+        down, up, scale = self.down, self.up, self.scale
+        if down.dtype is not y.dtype or scale.dtype is not torch.float32:  # after `Module.to`, as `Int8RotLinear`'s wscale
+            down, up, scale = down.to(y.dtype), up.to(y.dtype), scale.to(torch.float32)
+        return adapter_add(y, x, down, up, plan, scale=scale, out=out)
 
 
 class AttentionBlock(nn.Module):

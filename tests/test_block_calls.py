@@ -356,3 +356,27 @@ def test_the_block_refuses_what_would_have_to_be_differentiated():
     block.norm_q.requires_grad_()
     with pytest.raises(RuntimeError, match="forward only"):
         block(x, plan)
+
+
+# ----------------------------------------------------------------------------------------------------------- the block
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32, torch.float64])
+def test_adapters_of_a_converted_module(dtype):
+    """`nn.Module.to` converts every floating point parameter; the INT8 layers of the block take theirs back too."""
+    from test_block import make_block
+
+    block = make_block()
+    lengths = [3, 4]
+    x = rnd(1, 7, 64).to(BF)
+    plan = AttentionPlan(lengths, heads=4, kv_heads=2, head_dim=16, device="cpu")
+    adapters = AdapterPlan([1, 0], lengths, adapters=2, device="cpu")
+    for bank in (block.qkv_adapters, block.out_adapters):
+        bank.scale.copy_(torch.tensor([0.25, 0.75]))  # values that every type holds, as those of the wscale that follows
+    for layer in (block.qkv, block.out):
+        layer.wscale.fill_(2.0 ** -9)
+    block.norm_q.copy_(1 + torch.arange(16) / 32)
+    for p in (block.qkv_adapters.down, block.qkv_adapters.up, block.out_adapters.down, block.out_adapters.up):
+        p.copy_(p.clamp(-1, 1).mul(64).round().div(64))
+    want = block(x, plan, adapters=adapters)
+    got = block.to(dtype)(x, plan, adapters=adapters)
+    assert got.dtype is BF and torch.equal(got, want)
