@@ -7,6 +7,8 @@ one projection. The reference's blocks do the same between ``to_q``/``to_k``/``t
 
 from __future__ import annotations
 
+import warnings
+
 import torch
 from torch import Tensor, nn
 
@@ -86,8 +88,24 @@ class AttentionBlock(nn.Module):
 
     @classmethod
     def from_projections(cls, to_q: Int8RotLinear, to_k: Int8RotLinear, to_v: Int8RotLinear, to_out: Int8RotLinear,
-                         head_dim: int, **more) -> "AttentionBlock":
-        """The block of a model's own projections: q, k and v fused into one layer (bitwise the same outputs)."""
+                         head_dim: int, *, norm_q: Tensor | None = None, norm_k: Tensor | None = None,
+                         qk_norm: bool | None = None, **more) -> "AttentionBlock":
+        """The block of a model's own projections: q, k and v fused into one layer (bitwise the same outputs).
+
+        ``norm_q`` and ``norm_k`` are the weights [head_dim] of the model's RMS norms of query and key heads, kept in their
+        type (their eps is ``eps``). Without them ``qk_norm`` says whether there are norms: False for a model that has
+        none, True for norms whose weights are one, which is also taken, with a warning, when nothing is said."""
+        if (norm_q is None) != (norm_k is None):
+            raise ValueError("norm_q and norm_k come together")
+        if norm_q is not None:
+            if qk_norm is False:
+                raise ValueError("qk_norm=False contradicts norm_q and norm_k")
+            if norm_q.shape != (head_dim,) or norm_k.shape != (head_dim,):
+                raise ValueError(f"norm_q and norm_k must be [{head_dim}], one weight a channel of a head, got "
+                                 f"{tuple(norm_q.shape)} and {tuple(norm_k.shape)}")
+        elif qk_norm is None:
+            warnings.warn("from_projections without norm_q and norm_k: queries and keys get RMS norms whose weights are "
+                          "one; give the model's weights, or qk_norm=False for none", UserWarning, stacklevel=2)
         if to_q.out_features % head_dim or to_k.out_features % head_dim or to_k.out_features != to_v.out_features:
             raise ValueError(f"projections of {to_q.out_features}, {to_k.out_features} and {to_v.out_features} columns "
                              f"are not heads of {head_dim}")
@@ -95,7 +113,7 @@ class AttentionBlock(nn.Module):
             raise ValueError(f"to_out takes {to_out.in_features} columns, the heads give {to_q.out_features}")
         with torch.device("meta"):
             block = cls(to_q.in_features, to_q.out_features // head_dim, head_dim, to_q.group,
-                        kv_heads=to_k.out_features // head_dim, **more)
+                        kv_heads=to_k.out_features // head_dim, qk_norm=qk_norm is not False, **more)
         device = to_q.qweight.device
         block.qkv, block.out = fuse_qkv(to_q, to_k, to_v), to_out
         for module in (block, block.qkv_adapters, block.out_adapters):
@@ -103,6 +121,8 @@ class AttentionBlock(nn.Module):
                 if p is not None:
                     module._parameters[name] = _frozen((torch.zeros_like if name in ("down", "up") else torch.ones_like)(
                         p, device=device))
+        if norm_q is not None:
+            block.norm_q, block.norm_k = (_frozen(w.detach().to(device)) for w in (norm_q, norm_k))
         return block
 
     def forward(self, x: Tensor, plan: AttentionPlan, *, positions: Tensor | None = None,

@@ -15,7 +15,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from hyperflow_h3_flash_amd import (AdapterPlan, AttentionPlan, Int8RotLinear, RotaryAxes, adapter_add,
+from hyperflow_h3_flash_amd import (AdapterPlan, AttentionBlock, AttentionPlan, Int8RotLinear, RotaryAxes, adapter_add,
                                     packed_attention, qk_norm_rope)
 from hyperflow_h3_flash_amd import _native, block
 
@@ -380,3 +380,46 @@ def test_adapters_of_a_converted_module(dtype):
     want = block(x, plan, adapters=adapters)
     got = block.to(dtype)(x, plan, adapters=adapters)
     assert got.dtype is BF and torch.equal(got, want)
+
+
+def block_and_its_projections():
+    from test_block import make_block
+
+    block = make_block(adapters=0)
+    layers = [Int8RotLinear(64, n, 16) for n in (64, 32, 32)]
+    for layer, rows in zip(layers, (slice(0, 64), slice(64, 96), slice(96, 128))):
+        layer.qweight.copy_(block.qkv.qweight[rows])
+        layer.wscale.copy_(block.qkv.wscale[rows])
+    return block, (*layers, block.out, 16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_a_block_of_a_models_projections_has_its_norms(recwarn, dtype):
+    block, projections = block_and_its_projections()
+    assert not (block.norm_q == 1).all() and not (block.norm_k == 1).all()
+    plan, x = AttentionPlan([5], heads=4, kv_heads=2, head_dim=16, device="cpu"), rnd(1, 5, 64).to(BF)
+    weights = {"norm_q": torch.nn.Parameter(block.norm_q.to(dtype)), "norm_k": torch.nn.Parameter(block.norm_k.to(dtype))}
+    again = AttentionBlock.from_projections(*projections, **weights)
+    assert torch.equal(again(x, plan), block(x, plan))
+    assert not any(p.requires_grad or p.is_meta for p in again.parameters()) and weights["norm_q"].requires_grad
+    none = AttentionBlock.from_projections(*projections, qk_norm=False)
+    assert none.norm_q is None and none.norm_k is None
+    ones = AttentionBlock.from_projections(*projections, qk_norm=True)
+    assert (ones.norm_q == 1).all() and (ones.norm_k == 1).all()
+    assert not [w for w in recwarn.list if w.category is UserWarning]
+
+
+def test_a_block_of_projections_alone_says_what_it_takes_for_the_norms():
+    _, projections = block_and_its_projections()
+    with pytest.warns(UserWarning, match="norm_q"):
+        block = AttentionBlock.from_projections(*projections)
+    assert (block.norm_q == 1).all() and (block.norm_k == 1).all()
+
+
+def test_refusals_of_norms_that_do_not_fit():
+    block, projections = block_and_its_projections()
+    w = torch.ones(16)
+    for bad in ({"norm_q": w}, {"norm_k": w}, {"norm_q": w, "norm_k": w, "qk_norm": False},
+                {"norm_q": torch.ones(64), "norm_k": torch.ones(32)}, {"norm_q": w, "norm_k": torch.ones(1, 16)}):
+        with pytest.raises(ValueError):
+            AttentionBlock.from_projections(*projections, **bad)
