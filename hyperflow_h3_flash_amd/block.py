@@ -34,6 +34,7 @@ from .int8 import _check, _forget_input, _on, _raw_stream, _same_device
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}
 _POSITIONS = {torch.int32: 0, torch.int64: 1, torch.float32: 2}
+_FLOAT_MAX = torch.finfo(torch.float32).max
 _HERE = contextlib.nullcontext()
 _rope_args, _attention_args, _adapter_args = (s.pack for s in (
     _native.ROPE_ARGS, _native.ATTENTION_ARGS, _native.ADAPTER_ARGS))
@@ -286,8 +287,8 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: 
     for w in (q_weight, k_weight):
         if w is not None and (not norm or w.shape != (D,)):
             raise ValueError(f"a weight must be [{D}] and needs norm=True")
-    if not eps >= 0:
-        raise ValueError(f"eps must not be negative, got {eps}")
+    if not eps >= 0 or _FLOAT_MAX < eps < math.inf:
+        raise ValueError(f"eps must not be negative nor outside of float32, got {eps}")
     if out is not None:
         _check_out(out[0], q, "qk_norm_rope")
         if k is not None:
@@ -474,8 +475,8 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, *, sc
         raise ValueError(f"q, k and v differ in type: {dtype}, {k.dtype}, {v.dtype}")
     code = _dtype_code("packed_attention", dtype)
     scale = plan.head_dim ** -0.5 if scale is None else float(scale)
-    if not 0 < scale < math.inf:
-        raise ValueError(f"scale must be positive and finite, got {scale}")
+    if not 0 < scale <= _FLOAT_MAX:
+        raise ValueError(f"scale must be positive and finite in float32, got {scale}")
     if out is not None:
         _check_out(out, q, "packed_attention")
     index = q.get_device()

@@ -423,3 +423,20 @@ def test_refusals_of_norms_that_do_not_fit():
                 {"norm_q": torch.ones(64), "norm_k": torch.ones(32)}, {"norm_q": w, "norm_k": torch.ones(1, 16)}):
         with pytest.raises(ValueError):
             AttentionBlock.from_projections(*projections, **bad)
+
+
+@pytest.mark.parametrize("device", [False, True], ids=["host", "device"])
+def test_numbers_outside_of_float32_are_refused_as_arguments(launches, device):
+    """scale and eps reach the kernels in float32."""
+    move = on_device if device else (lambda t: t)
+    q = move(rnd(1, 6, 2, 64).to(BF))
+    plan = attention_plan([6], [6], 2, 2, 64)
+    if not device:
+        plan._index = -1
+    for value in (1e39, float("inf")):
+        with pytest.raises(ValueError, match="scale"):
+            packed_attention(q, q, q, plan, scale=value)
+    with pytest.raises(ValueError, match="eps"):
+        qk_norm_rope(q, None, None, None, eps=1e39)
+    packed_attention(q, q, q, plan, scale=1e38)
+    qk_norm_rope(q, None, None, None, eps=1e38)
