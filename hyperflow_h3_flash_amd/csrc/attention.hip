@@ -23,8 +23,11 @@
 // the maximum saved 1 %; adding the weights up two at a time with dot products nothing; running the products of neighbouring tiles under the
 // weights' arithmetic in one wave, with two tiles of scores in registers, raised the matrix unit's share of the cycles and
 // lowered the clock as much (4.63 ms): the two waves of a SIMD overlap well enough by themselves, once the products'
-// operands are read four products ahead (at_order). Three workgroups a compute unit for heads of at most 64, with
-// registers held to 168: 2.76 ms against 2.58 with two (37710 x 7 of 64).
+// operands are read four products ahead (at_order).
+// Heads of at most 64 need 167 (bfloat16) and 168 (float16) vector registers, a third of them, and 32 KB of LDS, so three
+// workgroups share a compute unit; two, by more LDS, are slower (37710 tokens x 7 heads of 64 2524 us against 2451, prompts
+// 111 against 105, cross attention with 511 and 77 keys 70 against 60). A test holds the built kernels to 168: launch bounds
+// of three make the compiler spill 2 and 4 registers, 0.3 % slower. Wider heads take two workgroups.
 // 16 single tokens of 32 / 8 heads against 77411 keys: 57 us and 4 for the join, 5.3 TB/s (a copy: 5.2).
 #pragma once
 

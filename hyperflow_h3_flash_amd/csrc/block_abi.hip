@@ -116,7 +116,9 @@ bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t cou
     k0 += nk;
   }
   std::stable_sort(tiles.begin(), tiles.end(), [](const Piece& x, const Piece& y) { return x.cost > y.cost; });
-  // The device takes `places` workgroups at a time, the longest tiles first. Tiles that would end well after an equal share
+  // The device takes `places` workgroups at a time, the longest tiles first (half as many again of heads of at most 64, but
+  // shares laid out for all of those are shorter than they are worth: 37710 tokens x 7 heads of 64 2888 us against 2692, 16
+  // single tokens against 77411 keys, 32 / 8 heads of 64, 33.2 against 31.1). Tiles that would end well after an equal share
   // of all work (few rows over many keys, or the last round of equal tiles) are cut along the keys into parts that fill
   // what the whole ones leave; a part costs about two tiles of keys more (its start, its sums' way through memory).
   const int64_t places = 2 * (int64_t)cus, share = (total + places - 1) / places;

@@ -9,6 +9,7 @@ import ctypes
 import io
 import os
 import pickle
+import re
 import weakref
 
 import pytest
@@ -440,3 +441,30 @@ def test_numbers_outside_of_float32_are_refused_as_arguments(launches, device):
         qk_norm_rope(q, None, None, None, eps=1e39)
     packed_attention(q, q, q, plan, scale=1e38)
     qk_norm_rope(q, None, None, None, eps=1e38)
+
+
+# --------------------------------------------------------------------------------------------------- built kernels
+
+def kernel_metadata(path):
+    """{kernel's symbol: {field: number}} of the code object's notes: MessagePack maps with sorted keys, in which a kernel's
+    register counts follow its symbol."""
+    data = open(path, "rb").read()
+    found = {}
+    for m in re.finditer(rb"\.symbol(?:[\xa0-\xbf]|\xd9.)([\x21-\x7e]+?)\.kd", data, flags=re.S):
+        fields = {}
+        for name in (b".vgpr_count", b".vgpr_spill_count"):
+            at = data.index(name, m.end()) + len(name)
+            size = {0xcc: 1, 0xcd: 2, 0xce: 4}.get(data[at], 0)
+            fields[name.decode()[1:]] = int.from_bytes(data[at + 1:at + 1 + size], "big") if size else data[at]
+        found[m.group(1).decode()] = fields
+    return found
+
+
+def test_three_workgroups_of_narrow_heads_share_a_compute_unit():
+    """A SIMD's 512 vector registers hold three waves of up to 168: attention on heads of at most 64 depends on it."""
+    kernels = {n: f for n, f in kernel_metadata(_native.BLOCK_LIB_PATH).items() if "attention_kernel" in n}
+    assert len(kernels) == 6
+    for name, fields in kernels.items():
+        assert fields["vgpr_spill_count"] == 0 and 0 < fields["vgpr_count"] <= 256, (name, fields)
+        if "ELi2E" in name:
+            assert fields["vgpr_count"] <= 168, (name, fields)
