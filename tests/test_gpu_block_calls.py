@@ -200,3 +200,72 @@ def test_scores_of_no_weight_in_fp16():
         plan = AttentionPlan([rows], [n], heads=1, head_dim=64)
         for scale in (1e-6, 1e-30, 1e-37):
             U.check(packed_attention(q, k, v, plan, scale=scale), *U.attention(q, k, v, [rows], [n], False, scale))
+
+
+@pytest.mark.parametrize("top", [60.0, 3000.0])
+@pytest.mark.parametrize("rows,n,heads", [(700, 700, 200), (700, 700, 1), (3, 6000, 1), (40, 3000, 1)])
+@pytest.mark.parametrize("dtype", [HF, BF])
+def test_rising_and_falling_scores(dtype, rows, n, heads, top):
+    """The maximum moves in every tile, or stays that of the first, in whole tiles of rows and in shares of cut ones."""
+    D = 64
+    plan = AttentionPlan([rows], [n], heads=heads, head_dim=D, causal=True)
+    assert (plan.ws_bytes > 0) == (heads == 1)
+    ramp = torch.linspace(0, top, n).cuda()
+    q = torch.zeros(rows, 1, D, device="cuda", dtype=dtype)
+    q[..., 0] = 8.0  # scores are the ramp at the scale of 1 / 8
+    for order in (ramp, ramp.flip(0), -ramp, ramp[torch.arange(n).cuda() * 7919 % n]):
+        k, v = rnd(3, n, 1, D).to(dtype), rnd(4, n, 1, D).to(dtype)
+        k[:, 0, 0] = order.to(dtype)
+        got = packed_attention(*(t.expand(-1, heads, D) for t in (q, k, v)), plan)
+        assert (got == got[:, :1]).all()
+        U.check(got[:, :1], *U.attention(q, k, v, [rows], [n], True, D ** -0.5))
+
+
+@pytest.mark.parametrize("rows,n", [(90, 90), (3, 6000)])
+def test_infinities_and_nan_in_fp16(rows, n):
+    """Values that are seen show, in whole and in cut rows; those that are not leave no trace."""
+    D = 64
+    q, k, v = rnd(1, rows, 1, D).to(HF), rnd(2, n, 1, D).to(HF), rnd(3, n, 1, D).to(HF)
+    plan = AttentionPlan([rows], [n], heads=1, head_dim=D, causal=True)
+    clean = packed_attention(q, k, v, plan)
+    last = rows - 2  # the last query but one sees all keys but the last
+    v[n - 1, 0, 3], v[n - 2, 0, 4], v[0, 0, 5] = float("inf"), float("-inf"), float("nan")
+    got = packed_attention(q, k, v, plan)
+    assert got[rows - 1, 0, 3] == float("inf") and torch.equal(got[:last + 1, 0, 3], clean[:last + 1, 0, 3])
+    assert (got[last:, 0, 4] == float("-inf")).all() and torch.equal(got[:last, 0, 4], clean[:last, 0, 4])
+    assert got[:, 0, 5].isnan().all() and torch.equal(got[:, 0, 6:], clean[:, 0, 6:])
+
+
+# ------------------------------------------------------------------------------------------------- past 2^31 elements
+
+def test_adapters_past_32_bits():
+    M, K, N, r = 150016, 14400, 15368, 16
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x, y = (torch.randn(M, n, generator=gen, device="cuda", dtype=BF) for n in (K, N))
+    assert x.numel() > 2 ** 31 and y.numel() > 2 ** 31
+    down, up = (rnd(2, 2, r, K) / K ** 0.5).to(BF), (rnd(3, 2, N, r) / r ** 0.5).to(BF)
+    lens, ids = [70000, 16, M - 70016], [0, -1, 1]
+    plan = AdapterPlan(ids, lens, adapters=2)
+    picked = torch.cat([torch.arange(a, a + 40) for a in (0, 69980, 2 ** 31 // N - 20, 2 ** 31 // K - 20, M - 40)]).cuda()
+    which = torch.repeat_interleave(torch.tensor(ids), torch.tensor(lens))[picked.cpu()].tolist()
+    want = U.adapters(y[picked], x[picked], down, up, which, [1] * len(which), None)
+    U.check(adapter_add(y, x, down, up, plan, out=y)[picked], *want)
+
+
+def test_rotation_past_32_bits():
+    T, H, D = 140003, 120, 128
+    q = torch.randn(T, H, D, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda", dtype=BF)
+    assert q.numel() > 2 ** 31
+    positions = torch.arange(T).cuda()
+    picked = torch.cat([torch.arange(a, a + 8) for a in (0, 2 ** 31 // (H * D) - 4, T - 8)]).cuda()
+    want = U.rotate(q[picked], None, positions[picked, None], (D,), 1e4, True, True)
+    U.check(qk_norm_rope(q, None, positions, RotaryAxes((D,)), out=(q, None))[0][picked], *want)
+
+
+@pytest.mark.parametrize("theta", [1e4, 5.0])
+def test_positions_to_the_ends_of_int32(theta):
+    positions = torch.tensor([[2 ** 31 - 1], [-2 ** 31], [2 ** 31 - 3], [123456789]]).cuda()
+    q = rnd(2, 4, 3, 128).to(HF)
+    for p in (positions, positions.int()):
+        got, _ = qk_norm_rope(q, None, p, RotaryAxes((128,), theta=theta), norm=False)
+        U.check(got, *U.rotate(q, None, positions, (128,), theta, True, False))
