@@ -4,8 +4,9 @@
   token's position on one or several axes (time, height, width), in one pass;
 * `packed_attention` with `AttentionPlan`: attention over the sequences of several requests packed one behind the
   other, full or causal, with grouped heads, from single tokens against a cache to whole clips;
-* `adapter_add` with `AdapterPlan` and `AdapterBank`: low-rank adapters of many requests beside a shared projection;
-* `AttentionBlock`: all of them between an `Int8RotLinear` q/k/v projection and an output projection.
+* `adapter_add` with `AdapterPlan`: low-rank adapters of many requests beside a shared projection.
+
+`attention_block.py` has the modules that run them between an `Int8RotLinear` q/k/v projection and an output projection.
 
 The reference holds these layers in its model library (the blocks its transformer keeps,
 src/hyperflow_h3_flash/transformer.py:339-380, call them between ``to_q``/``to_k``/``to_v`` and ``to_out``); they have
@@ -26,7 +27,7 @@ import threading
 from collections.abc import Sequence
 
 import torch
-from torch import Tensor, nn
+from torch import Tensor
 from torch.autograd import forward_ad
 
 from . import _native, host_block
@@ -211,6 +212,7 @@ class _Resident:
 
     def __setstate__(self, state: dict) -> None:
         self.host, self.device, self.device_copy = state["host"], state["device"], None
+        self.host_address = self.host.data_ptr()
 
 
 # ------------------------------------------------------------------------------------------------- norms and rotation
@@ -260,7 +262,8 @@ def qk_norm_rope(q: Tensor, k: Tensor | None, positions: Tensor | None, rotary: 
 
     ``x / sqrt(mean(x ** 2) + eps) * weight`` over the head's channels (``norm=False``: as it is; a weight of None is
     one; weights [D] in the inputs' type or float32), then the rotation of ``rotary`` (None: none) at ``positions``
-    [T, axes] (or [T] for one axis; int32, int64 or float32). Computed in float32, rounded once to the inputs' type
+    [T, axes] (or [T] for one axis; int32, int64 or float32; up to 2^31 either way the angle keeps float32's accuracy,
+    beyond it loses a bit with every doubling). Computed in float32, rounded once to the inputs' type
     (bfloat16 or float16). q and k may be views with any token and head strides, such as slices of a fused projection.
     ``out`` may name the results' tensors, the inputs themselves among them (written directly where each is its own
     input's, through new memory where they overlap otherwise). D is a multiple of 16, up to 256."""
@@ -389,10 +392,6 @@ class _Plan:
             self.data = _Resident(host, device)
         self.bytes = size
 
-    @property
-    def _host(self) -> int:
-        return self.data.host.data_ptr()
-
 
 def _plan_device(device: torch.device | str) -> torch.device:
     device = torch.device(device)
@@ -445,7 +444,7 @@ class AttentionPlan(_Plan):
         cus = torch.cuda.get_device_properties(self.device).multi_processor_count
         self._fill("hf_attention_plan", lib, self.device, ctypes.addressof(q), ctypes.addressof(kv),
                    len(self.q_lengths), self.heads, self.kv_heads, self.head_dim, self.causal, cus)
-        self.ws_bytes = lib.hf_attention_ws_bytes(self._host, self.bytes)
+        self.ws_bytes = lib.hf_attention_ws_bytes(self.data.host_address, self.bytes)
 
 
 def _keys(t: Tensor) -> tuple[Tensor, int, int]:
@@ -505,8 +504,9 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, *, sc
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     with _current(index, device):
         status = lib.hf_attention_call(_attention_args(
-            q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, o.data_ptr(), ot, oh, scale, plan._host,
-            plan.data.on(stream), plan.bytes, 0 if ws is None else ws.data_ptr(), nbytes, code, stream))
+            q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, o.data_ptr(), ot, oh, scale,
+            plan.data.host_address, plan.data.on(stream), plan.bytes, 0 if ws is None else ws.data_ptr(), nbytes, code,
+            stream))
     _check(status, "hf_attention")
     return o if out is None else _deliver(o, out)
 
@@ -540,7 +540,7 @@ class AdapterPlan(_Plan):
                    ctypes.addressof(lens_c), len(self.ids), self.adapters, cus)
 
     def _ws_bytes(self, lib: ctypes.CDLL, K: int, r: int, code: int) -> int:
-        found = lib.hf_adapter_ws_bytes(self._host, self.bytes, K, r, code)
+        found = lib.hf_adapter_ws_bytes(self.data.host_address, self.bytes, K, r, code)
         _check(min(found, 0), "hf_adapter_ws_bytes")
         self._ws[K, r, code] = found
         return found
@@ -626,7 +626,7 @@ def adapter_add(y: Tensor, x: Tensor, down: Tensor, up: Tensor, plan: AdapterPla
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None  # held, as attention's
         status = lib.hf_adapter_add_call(_adapter_args(
             x.data_ptr(), _ld(x), y.data_ptr(), _ld(y), down.data_ptr(), up.data_ptr(), r,
-            0 if scale is None else scale.data_ptr(), o.data_ptr(), _ld(o), N, K, plan._host, plan.data.on(stream),
-            plan.bytes, 0 if ws is None else ws.data_ptr(), nbytes, code, stream))
+            0 if scale is None else scale.data_ptr(), o.data_ptr(), _ld(o), N, K, plan.data.host_address,
+            plan.data.on(stream), plan.bytes, 0 if ws is None else ws.data_ptr(), nbytes, code, stream))
     _check(status, "hf_adapter_add")
     return o if out is None else _deliver(o, out)

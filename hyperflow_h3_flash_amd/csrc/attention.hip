@@ -231,6 +231,8 @@ __global__ __launch_bounds__(64 * kAtWaves, 2) void attention_kernel(AttentionAr
   // depend on the rows that share its wave. The sums over the keys are rescaled when m moves (`rescale`).
   auto exponentials = [&](const v16f (&s)[2], v4u (&pf)[4], int p, float mc, float (&part)[2])
                           __attribute__((always_inline)) {  // two of them, p of 16
+    // Rounded to the inputs' type for the second product, whose matrix instructions take 16-bit operands (weights in two
+    // parts would double its work); their sum is of the unrounded ones.
     const int b = p >> 3, v = 2 * (p & 7);
     const float p0 = __builtin_amdgcn_exp2f(fmaf(s[b][v], c, -mc));
     const float p1 = __builtin_amdgcn_exp2f(fmaf(s[b][v + 1], c, -mc));

@@ -480,7 +480,8 @@ int64_t hf_adapter_plan(const int32_t* ids, const int64_t* lens, int64_t count, 
     std::vector<int64_t> at(keys + 1, 0);
     for (int64_t i = 0; i < count; ++i) at[(ids[i] < 0 ? adapters : ids[i]) + 1] += lens ? lens[i] : 1;
     for (size_t i = 0; i < keys; ++i) at[i + 1] += at[i];
-    // Tiles of 64 rows read the weights half as often, tiles of 32 are twice as many: 64 once those fill the device
+    // Tiles of 64 rows read the first product's weights half as often (the second takes 32 rows a workgroup either way),
+    // tiles of 32 are twice as many: 64 once those fill the device
     // (rows, rank, tiles of 32 -> 64: 8192, 64: 75 -> 77 us; 16384, 32: 114 -> 108; 32768, 64: 330 -> 306; 32768, 128:
     // 475 -> 428; 300, 64: 20 -> 23).
     int64_t wide = 0;

@@ -16,10 +16,6 @@ struct Bf16 {
   static __device__ __forceinline__ float lo(uint32_t pair) { return bf16_lo(pair); }
   static __device__ __forceinline__ float hi(uint32_t pair) { return bf16_hi(pair); }
   static __device__ __forceinline__ uint32_t pack(float a, float b) { return pack_bf16x2(a, b); }
-  static __device__ __forceinline__ float sum(uint32_t pair, float c) {  // both values plus c
-    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, pair), __builtin_bit_cast(b2, 0x3f803f80u), c, false);
-  }
   static __device__ __forceinline__ v16f mfma(v4u a, v4u b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
   }
@@ -37,10 +33,6 @@ struct Fp16 {
   static __device__ __forceinline__ uint32_t pack(float a, float b) {  // round to nearest even
     typedef _Float16 h2 __attribute__((ext_vector_type(2)));
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f){a, b}, h2));
-  }
-  static __device__ __forceinline__ float sum(uint32_t pair, float c) {  // both values plus c
-    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, pair), __builtin_bit_cast(h2, 0x3c003c00u), c, false);
   }
   static __device__ __forceinline__ v16f mfma(v4u a, v4u b, v16f c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);

@@ -12,8 +12,9 @@
 //
 // A workgroup takes all query heads or all key heads (or a share of them, when there are few tokens) of a few tokens:
 // their sines and cosines are computed once into LDS and serve every head. The angle is reduced in fp64 to less than
-// half a turn before the sine, so positions of any size keep the sine's own accuracy: one fp64 product a token, side and
-// pair.
+// half a turn before the sine: one fp64 product a token, side and pair. The rounding of that product and of the rate grows
+// with the position: at 2^31 the angle of a pair that turns by 1 errs by 1e-7 (an ulp or two of the fp32 sine), at 2^40 by
+// 7e-5, and int64 positions past 2^53 are rounded.
 #pragma once
 
 #include "block_types.h"
@@ -21,7 +22,6 @@
 namespace hf {
 
 constexpr int kRopeThreads = 256;
-constexpr int kRopeMaxPairs = 128;
 
 struct RopeSide {
   const uint16_t* x;

@@ -81,7 +81,7 @@ def attention_plan(q_lens, kv_lens, heads, kv_heads, head_dim, causal=False):
     q, kv = block._array(ctypes.c_int64, plan.q_lengths), block._array(ctypes.c_int64, plan.kv_lengths)
     plan._fill("hf_attention_plan", lib, plan.device, ctypes.addressof(q), ctypes.addressof(kv), len(q_lens), heads,
                kv_heads, head_dim, causal, 256)
-    plan.ws_bytes = lib.hf_attention_ws_bytes(plan._host, plan.bytes)
+    plan.ws_bytes = lib.hf_attention_ws_bytes(plan.data.host_address, plan.bytes)
     plan._index = 0
     return plan
 
