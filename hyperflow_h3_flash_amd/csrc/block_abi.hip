@@ -134,7 +134,7 @@ bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t cou
     std::push_heap(load.begin(), load.end(), less);
     left -= tiles[whole].cost;
   }
-  // No more parts than places, so that none waits for another. A wave's n tiles in parts of p take it p steps and then n / p
+  // No more parts than places where they are about equal, so that none waits for another. A wave's n tiles in parts of p take it p steps and then n / p
   // reads in the join, a step about eleven reads long: p no less than sqrt(n / 11), and two, or three where a tile's many
   // rows make the join's reads many. Against six whatever n (us; heads / key heads of 128): one token, 131072 keys, 8 / 1
   // 37.6 -> 28.5, 4096 keys, 32 / 8 13.4 -> 11.3, 700 keys 12.7 -> 8.9; 300 tokens, 2000 keys, 8 / 8, three 17.6, two 19.5,
@@ -145,12 +145,19 @@ bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t cou
     longest_cost = std::max(longest_cost, tiles[t].cost);
     most_rows = std::max(most_rows, std::min((int64_t)it.nq * group - it.row0, (int64_t)hf::kAtRows));
   }
-  int64_t part = std::max((left + places - 1) / places, (int64_t)(most_rows <= 32 ? 2 : 3));
-  part = std::max(part, (int64_t)ceil(sqrt((double)longest_cost / 11.0)));
+  int64_t least = std::max((left + places - 1) / places, (int64_t)(most_rows <= 32 ? 2 : 3));
+  least = std::max(least, (int64_t)ceil(sqrt((double)longest_cost / 11.0)));
+  int64_t part = least;
   for (;; part += part / 32 + 1) {
     int64_t parts = 0;
     for (size_t t = whole; t < tiles.size(); ++t) parts += std::max((tiles[t].cost + part - 1) / part, (int64_t)1);
     if (parts <= places || part >= longest_cost) break;
+    // With many short tiles beside long ones the number says nothing: parts longer than twice an equal share would be what
+    // all others wait for, while short tiles fill places one behind the other.
+    if (part > 2 * least) {
+      part = least;
+      break;
+    }
   }
   int64_t slots = 0;
   for (size_t t = 0; t < tiles.size(); ++t) {

@@ -6,12 +6,15 @@ from __future__ import annotations
 import contextlib
 import copy
 import ctypes
+import heapq
 import io
 import os
 import pickle
 import re
+import struct
 import weakref
 
+import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -468,3 +471,39 @@ def test_three_workgroups_of_narrow_heads_share_a_compute_unit():
         assert fields["vgpr_spill_count"] == 0 and 0 < fields["vgpr_count"] <= 256, (name, fields)
         if "ELi2E" in name:
             assert fields["vgpr_count"] <= 168, (name, fields)
+
+
+# ----------------------------------------------------------------------------------------------------- uneven batches
+
+@pytest.mark.parametrize("q,kv,heads,kv_heads", [
+    ([1] * 65, [131072] + [1000] * 64, 8, 8), ([1] * 60, [65536] * 4 + [2000] * 56, 32, 8),
+    ([1] * 1001, [131072] + [1000] * 1000, 8, 8),
+])
+def test_a_long_cache_among_many_others_is_cut(q, kv, heads, kv_heads):
+    """No single share of a tile's keys takes more than twice an equal share of all the work, and places that take the items
+    as they come end within one and a half (a part costs its start and its sums, two tiles of keys)."""
+    plan = attention_plan_bytes(q, kv, heads, kv_heads)
+    items, joins = struct.unpack_from("2i", plan, 20)
+    item = np.frombuffer(plan, np.int32, items * 12, 128).reshape(items, 12)
+    tiles = ((item[:, 6] - item[:, 5] + 63) // 64).tolist()
+    places = [0] * 512
+    for n in tiles:
+        heapq.heapreplace(places, places[0] + n + 2)
+    share = -(-sum(tiles) // 512)
+    assert joins > 0 and max(tiles) <= 2 * share and max(places) <= 1.5 * share
+    # every key of every tile of rows once
+    rows = {}
+    for i in item.tolist():
+        rows.setdefault((i[0], i[4], i[7]), []).append((i[5], i[6]))
+    for parts in rows.values():
+        parts.sort()
+        assert parts[0][0] == 0 and all(a[1] == b[0] for a, b in zip(parts, parts[1:]))
+
+
+def attention_plan_bytes(q, kv, heads, kv_heads):
+    lib = _native.block_library()
+    qa, ka = (ctypes.c_int64 * len(q))(*q), (ctypes.c_int64 * len(kv))(*kv)
+    args = qa, ka, len(q), heads, kv_heads, 128, 1, 256
+    held = ctypes.create_string_buffer(lib.hf_attention_plan(*args, None, 0))
+    assert lib.hf_attention_plan(*args, held, len(held)) == len(held)
+    return held.raw
