@@ -461,7 +461,8 @@ def packed_attention(q: Tensor, k: Tensor, v: Tensor, plan: AttentionPlan, *, sc
     """Attention of packed sequences: ``softmax(scale q k^T) v`` within each sequence of ``plan``.
 
     ``q`` [sum q_lengths, heads, head_dim], ``k`` and ``v`` [sum kv_lengths, kv_heads, head_dim], bfloat16 or float16,
-    any token and head strides (slices of a fused projection or a cache); the result is like q. ``scale`` (default
+    any token and head strides (slices of a fused projection or a cache, whose sequences lie one behind the other without
+    gaps); the result is like q. ``scale`` (default
     ``head_dim ** -0.5``) is positive. A query that sees no key gets zeros; what k and v hold at keys that a query does
     not see never reaches it. Scores, weights' sums and outputs are summed in float32, and divided by the weights' sum at the
     end (values of v times the number of keys have to stay in its range); the weights enter the second product in the

@@ -2,7 +2,7 @@
 // adapter of row m, or out[m] = y[m] where it has none.
 //
 // HBM-bound with many rows (x once, y once, out once; the adapters' weights stay in the L2s), latency-bound with few.
-// 32768 rows x 5120 -> 15360, rank 32: 80 us (4.2 TB/s) and 380 (5.3 TB/s; a copy: 5.2); 64 single rows of 16 adapters,
+// 32768 rows x 5120 -> 15360, rank 32: 82 us (4.1 TB/s) and 384 (5.2 TB/s; a copy: 5.2); 64 single rows of 16 adapters,
 // 5120 -> 5120, rank 16: 8 us and 5.
 //
 // The plan holds the rows sorted by adapter and cut into tiles of 32 or 64 rows of one adapter, so requests in any order

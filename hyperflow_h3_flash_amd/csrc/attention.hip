@@ -17,18 +17,19 @@
 // computed. Rows are 256 (D > 64) or 128 bytes; chunk c of row r lies at c ^ f(r) so that both the 16-row fragment reads
 // of K and the 4-row transposing reads of V touch every bank once.
 //
-// Bound: the card's power with long sequences, the keys' bytes with single tokens. 37710 tokens x 7 heads of 128:
-// 4.41-4.51 ms, 1154-1130 TFLOP/s (a large library product of the same type: 1555), the matrix unit busy 65 % at 1.62 GHz.
-// The same launch on zeros takes 3.26 ms at the full clock: so energy counts, not issue slots. Leaving out the search for
-// the maximum saved 1 %; adding the weights up two at a time with dot products nothing; running the products of neighbouring tiles under the
-// weights' arithmetic in one wave, with two tiles of scores in registers, raised the matrix unit's share of the cycles and
-// lowered the clock as much (4.63 ms): the two waves of a SIMD overlap well enough by themselves, once the products'
-// operands are read four products ahead (at_order).
+// Bound: the card's power with long sequences, the keys' bytes with single tokens. 37710 tokens x 7 heads of 128: 4.44 ms
+// among other calls, 1148 TFLOP/s (a large library product of the same type: 1555); in a profiled run of 4.68 ms the matrix
+// unit is busy 65 % at 1.64 GHz. On zeros the same launch takes 3.18 ms against 4.35 on random values, both in turn: so
+// energy counts, not issue slots. Leaving out the search for the maximum saved 1 %; adding the weights up two at a time with
+// dot products nothing; running the products of neighbouring tiles under the weights' arithmetic in one wave, with two tiles
+// of scores in registers, raised the matrix unit's share of the cycles and lowered the clock as much (4.63 ms against 4.55):
+// the two waves of a SIMD overlap well enough by themselves, once the products' operands are read four products ahead
+// (at_order).
 // Heads of at most 64 need 167 (bfloat16) and 168 (float16) vector registers, a third of them, and 32 KB of LDS, so three
 // workgroups share a compute unit; two, by more LDS, are slower (37710 tokens x 7 heads of 64 2524 us against 2451, prompts
 // 111 against 105, cross attention with 511 and 77 keys 70 against 60). A test holds the built kernels to 168: launch bounds
 // of three make the compiler spill 2 and 4 registers, 0.3 % slower. Wider heads take two workgroups.
-// 16 single tokens of 32 / 8 heads against 77411 keys: 57 us and 4 for the join, 5.3 TB/s (a copy: 5.2).
+// 16 single tokens of 32 / 8 heads against 77411 keys: 56 us and 4 for the join, 5.6 TB/s (a copy: 5.2).
 #pragma once
 
 #include <type_traits>
