@@ -10,6 +10,7 @@ import heapq
 import io
 import os
 import pickle
+import random
 import re
 import struct
 import weakref
@@ -286,6 +287,32 @@ def test_rotation_and_adapters_never_write_where_they_still_read(launches):
                            (rows[:6], rows[3:], False), (y, x, True)):  # x is read before anything is written
         adapter_add(y, x, down, up, plan, out=out)
         assert (launches.seen[-1][1][8] == out.data_ptr()) is direct
+
+
+def test_places_that_are_called_apart_share_no_element():
+    rng = random.Random(3)
+
+    def elements(place):
+        address, rows, heads, row, head, width = place
+        return [address // 2 + i * row + j * head + k for i in range(rows) for j in range(heads) for k in range(width)]
+
+    def place():
+        head, heads = rng.choice([0, 8, 16, 24, 32, 48]), rng.randint(0, 3)
+        row = rng.choice([0, 8, 16, 48, 64, 96, head * max(heads, 1), head * 3])
+        return 16 * rng.randint(0, 30), rng.randint(0, 4), heads, row, head, rng.choice([8, 16])
+
+    told = 0
+    for _ in range(20000):
+        a, b = place(), place()
+        if rng.random() < 0.6:
+            b = (*b[:3], *a[3:])
+        mine, others = elements(a), elements(b)
+        if block._apart(a, b):
+            told += 1
+            assert not set(mine) & set(others), (a, b)
+        if block._spread(a):
+            assert len(set(mine)) == len(mine), a
+    assert told > 10000
 
 
 def test_results_that_overlap_themselves_are_refused(launches):
