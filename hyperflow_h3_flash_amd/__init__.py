@@ -20,7 +20,9 @@ from .int8 import (
     set_arithmetic_options,
     set_kernel_options,
 )
+from .kv_cache import CachePlan, KVCache, cache_append, cache_read, cached_attention, copy_pages
 from .lowrank import RANK_MULTIPLE, LowRankLinear, fuse_qkv, set_lowrank_rank_multiple
+from .residual_norm import RowPlan, residual_norm
 
 __version__ = "0.1.0"
 
@@ -31,20 +33,28 @@ __all__ = [
     "AdapterPlan",
     "AttentionBlock",
     "AttentionPlan",
+    "CachePlan",
     "INT8_GEMMS",
     "KERNEL_OPTIONS",
     "ROTATE_ARITHMETICS",
     "ROTATE_QUANTS",
     "Int8RotLinear",
+    "KVCache",
     "LowRankLinear",
     "RANK_MULTIPLE",
     "RotaryAxes",
+    "RowPlan",
     "adapter_add",
+    "cache_append",
+    "cache_read",
+    "cached_attention",
+    "copy_pages",
     "fuse_qkv",
     "hadamard_factors",
     "packed_attention",
     "qk_norm_rope",
     "regular_hadamard",
+    "residual_norm",
     "resolve_int8_gemm",
     "set_arithmetic_options",
     "set_kernel_options",

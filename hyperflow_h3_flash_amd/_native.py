@@ -1,5 +1,5 @@
-"""ctypes binding of ``libhf_convrot.so`` and ``libhf_block.so`` (the C ABIs of include/hf_convrot.h and
-include/hf_block.h) and the build recipe that makes them.
+"""ctypes binding of ``libhf_convrot.so`` and ``libhf_block.so`` (the C ABIs of include/hf_convrot.h, and of
+include/hf_block.h and include/hf_cache.h) and the build recipe that makes them.
 
 Each library is built in-tree by ``build_library()`` (hipcc, gfx950) and loaded from next to this file. There is no
 fallback: when one is missing or does not load, ``library()`` or ``block_library()`` raises.
@@ -18,7 +18,7 @@ PACKAGE_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PACKAGE_DIR)
 LIB_PATH = os.path.join(PACKAGE_DIR, "libhf_convrot.so")
 SOURCE = os.path.join(PACKAGE_DIR, "csrc", "convrot_abi.hip")
-#: The operators around the INT8 linears of an attention block (include/hf_block.h), a library of their own.
+#: The operators around the INT8 linears of a block (include/hf_block.h, include/hf_cache.h), a library of their own.
 BLOCK_LIB_PATH = os.path.join(PACKAGE_DIR, "libhf_block.so")
 BLOCK_SOURCE = os.path.join(PACKAGE_DIR, "csrc", "block_abi.hip")
 #: The benchmark's calibration kernels (matrix-core ceiling), a library of their own outside the C ABI.
@@ -96,10 +96,27 @@ BLOCK_SIGNATURES = {
     "hf_adapter_add_call": ([ctypes.c_char_p], ctypes.c_int),
 }
 
-#: The launches' parameters as the structs of hf_block.h lay them out.
+#: Every function include/hf_cache.h declares (of the same library as hf_block.h's).
+CACHE_SIGNATURES = {
+    "hf_cache_page_bytes": ([_I32, _I32, _I32], ctypes.c_int64),
+    "hf_cache_plan": ([_P, _P, _P, _I64, _P, _I64, _I32, _I32, _I32, _I32, _I32, _I32, _P, _I64], ctypes.c_int64),
+    "hf_cache_ws_bytes": ([_P, _I64], ctypes.c_int64),
+    "hf_cache_append": ([ctypes.c_char_p], ctypes.c_int),
+    "hf_cache_read": ([ctypes.c_char_p], ctypes.c_int),
+    "hf_cached_attention": ([ctypes.c_char_p], ctypes.c_int),
+    "hf_copy_pages": ([ctypes.c_char_p], ctypes.c_int),
+    "hf_residual_norm": ([ctypes.c_char_p], ctypes.c_int),
+}
+
+#: The launches' parameters as the structs of hf_block.h and hf_cache.h lay them out.
 ROPE_ARGS = struct.Struct("@PqqiPqqiPqqPqqPiqiPPiiiPPifqiiP")
 ATTENTION_ARGS = struct.Struct("@PqqPqqPqqPqqfPPqPqiP")
 ADAPTER_ARGS = struct.Struct("@PqPqPPiPPqqqPPqPqiP")
+CACHE_APPEND_ARGS = struct.Struct("@PqqPqqPPPqiP")
+CACHE_READ_ARGS = struct.Struct("@PPPPPqiP")
+CACHED_ATTENTION_ARGS = struct.Struct("@PqqPPqqfPPqPqiP")
+COPY_PAGES_ARGS = struct.Struct("@PqqqqPPqP")
+RESIDUAL_NORM_ARGS = struct.Struct("@PqPqPqPqPqPqPqPPPqqiiiiiiiffP")
 
 #: Queries of hf_route.
 ROUTE_UP_ROWS, ROUTE_ROTATE_LOWRANK, ROUTE_STREAM_WEIGHT = 0, 1, 2
@@ -161,7 +178,7 @@ def library() -> ctypes.CDLL:
 @lru_cache(maxsize=None)
 def block_library() -> ctypes.CDLL:
     """The attention block's operators, as `library`."""
-    return _load(BLOCK_LIB_PATH, BLOCK_SIGNATURES)
+    return _load(BLOCK_LIB_PATH, {**BLOCK_SIGNATURES, **CACHE_SIGNATURES})
 
 
 @lru_cache(maxsize=None)

@@ -79,9 +79,10 @@ struct AttentionWork {
   std::vector<hf::AttentionJoin> joins;
 };
 
-// Lays out the work; false when a size does not fit the kernels' indexes.
+// Lays out the work; false when a size does not fit the kernels' indexes. q_starts: where each sequence's queries begin (NULL:
+// one sequence behind the other).
 bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t count, int heads, int kv_heads, int D,
-                      int causal, int cus, AttentionWork* w) {
+                      int causal, int cus, AttentionWork* w, const int64_t* q_starts = nullptr) {
   const int64_t group = heads / kv_heads, limit = 0x7fffffff;
   int64_t q_rows = 0, kv_rows = 0;
   for (int64_t b = 0; b < count; ++b) {
@@ -99,6 +100,7 @@ bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t cou
   int64_t q0 = 0, k0 = 0;
   for (int64_t b = 0; b < count; ++b) {
     const int64_t nq = q_lens[b], nk = kv_lens[b];
+    if (q_starts) q0 = q_starts[b];
     for (int h = 0; h < kv_heads; ++h)
       for (int64_t r = 0; r < nq * group; r += hf::kAtRows) {
         const int64_t last = std::min(r + hf::kAtRows, nq * group) - 1;
@@ -186,6 +188,15 @@ bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t cou
   w->head.bytes = (int64_t)sizeof(w->head) + (int64_t)(w->items.size() * sizeof(hf::AttentionItem)) +
                   (int64_t)(w->joins.size() * sizeof(hf::AttentionJoin));
   return true;
+}
+
+// The plan as its bytes.
+void attention_write(const AttentionWork& w, unsigned char* to) {
+  memcpy(to, &w.head, sizeof(w.head));
+  to += sizeof(w.head);
+  if (!w.items.empty()) memcpy(to, w.items.data(), w.items.size() * sizeof(w.items[0]));
+  to += w.items.size() * sizeof(hf::AttentionItem);
+  if (!w.joins.empty()) memcpy(to, w.joins.data(), w.joins.size() * sizeof(w.joins[0]));
 }
 
 int64_t attention_slot_bytes(const AttentionHeader& h) {
@@ -413,12 +424,7 @@ int64_t hf_attention_plan(const int64_t* q_lens, const int64_t* kv_lens, int64_t
       return HF_ERR_SIZE;
     if (plan) {
       if (bytes < w.head.bytes) return HF_ERR_SIZE;
-      unsigned char* to = (unsigned char*)plan;
-      memcpy(to, &w.head, sizeof(w.head));
-      to += sizeof(w.head);
-      if (!w.items.empty()) memcpy(to, w.items.data(), w.items.size() * sizeof(w.items[0]));
-      to += w.items.size() * sizeof(hf::AttentionItem);
-      if (!w.joins.empty()) memcpy(to, w.joins.data(), w.joins.size() * sizeof(w.joins[0]));
+      attention_write(w, (unsigned char*)plan);
     }
     return w.head.bytes;
   } catch (...) {  // no memory for that many
@@ -593,3 +599,5 @@ int hf_adapter_add_call(const hf_adapter_add_args* a) {
 }
 
 }  // extern "C"
+
+#include "cache_abi.hip"

@@ -1,0 +1,159 @@
+// Keys and values in pages of 4-bit codes: written, read back, and pages copied. The layout is hf_cache.h's.
+#pragma once
+
+#include "block_types.h"
+
+namespace hf {
+
+// Rows of one page: tokens first .. first + rows - 1 of the page are rows row0 .. of the packed tensors.
+struct CacheSegment {
+  int32_t page, first, rows, row0;
+};
+
+__host__ __device__ constexpr int kv_scale_bytes(int groups) { return groups == 3 ? 4 : groups; }
+// Bytes of a page's tokens of one head.
+__host__ __device__ constexpr int64_t kv_slab(int groups, int page) {
+  return (int64_t)page * 2 * (16 * groups + kv_scale_bytes(groups));
+}
+
+struct CacheTypeBf16 {
+  typedef Bf16 Type;
+  static constexpr int kLeast = -125, kMost = 125;
+};
+struct CacheTypeFp16 {
+  typedef Fp16 Type;
+  static constexpr int kLeast = -23, kMost = 13;
+};
+
+// Two codes of byte `I` of a dword as a pair of the type, times 2^(exponent of scale): exact (all bytes and the exponents
+// that are written were compared).
+template <class T, int I>
+__device__ __forceinline__ uint32_t kv_pair(uint32_t codes, float scale) {
+  if constexpr (T::kNarrow) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, I));
+  else return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, I));
+}
+template <class T>
+__device__ __forceinline__ v4u kv_values(uint32_t codes, float scale) {
+  return (v4u){kv_pair<T, 0>(codes, scale), kv_pair<T, 1>(codes, scale), kv_pair<T, 2>(codes, scale),
+               kv_pair<T, 3>(codes, scale)};
+}
+
+struct CacheWriteArgs {
+  const uint16_t* x[2];  // k, v
+  int64_t token[2], head[2], page_bytes;
+  unsigned char* cache;
+  const CacheSegment* segments;
+  int D, page;
+};
+
+constexpr int kCacheThreads = 256;
+
+// A workgroup takes one segment and head. Four lanes share a group of a token (16 bytes of input and 4 of codes each);
+// neighbouring fours take neighbouring tokens, so that codes and scales go out side by side.
+template <class CT, int G>
+__global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(CacheWriteArgs a) {
+  typedef typename CT::Type T;
+  constexpr int S = kv_scale_bytes(G);
+  const CacheSegment seg = a.segments[blockIdx.x];
+  const int head = blockIdx.y, part = threadIdx.x & 3;
+  unsigned char* slab = a.cache + (int64_t)seg.page * a.page_bytes + head * kv_slab(G, a.page);
+  const int quads = 2 * G * seg.rows;
+  for (int i = threadIdx.x >> 2; i < quads; i += kCacheThreads / 4) {
+    const int which = i / (G * seg.rows), j = i - which * G * seg.rows;
+    const int g = j / seg.rows, row = j - g * seg.rows, c = 32 * g + 8 * part, at = seg.first + row;
+    const uint16_t* x = a.x[which] + (seg.row0 + (int64_t)row) * a.token[which] + head * a.head[which];
+    const v4u in = c < a.D ? *(const v4u*)(x + c) : (v4u){0, 0, 0, 0};
+    float h[8], top = 0.0f;
+    bool finite = true;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      h[2 * e] = T::lo(in[e]);
+      h[2 * e + 1] = T::hi(in[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      top = fmaxf(top, __builtin_fabsf(h[e]));
+      finite &= __builtin_fabsf(h[e]) < __builtin_inff();
+    }
+    top = finite ? top : __builtin_inff();
+#pragma unroll
+    for (int off = 1; off <= 2; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+    finite = top < __builtin_inff();
+    // top = m 2^x with m in [0.5, 1): top <= 7 2^e from e = x - 3 on for m <= 7 / 8, else from x - 2.
+    int x2;
+    const float m = frexpf(finite ? top : 1.0f, &x2);
+    const int e2 = min(max(x2 - (m <= 0.875f ? 3 : 2), CT::kLeast), CT::kMost);
+    const float scale = __uint_as_float((uint32_t)(e2 + 127) << 23);
+    // Nearest, ties to even, saturating: compared for every 16-bit float.
+    uint32_t codes = 0;
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, h[0], h[1], scale, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, h[2], h[3], scale, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, h[4], h[5], scale, 2);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, h[6], h[7], scale, 3);
+    unsigned char* to = slab + which * (int64_t)G * a.page * 16;
+    *(uint32_t*)(to + ((int64_t)g * a.page + at) * 16 + 4 * part) = finite ? codes : 0u;
+    if (part == 0) {
+      unsigned char* scales = slab + (int64_t)2 * G * a.page * 16 + which * (int64_t)a.page * S;
+      scales[at * S + g] = finite ? (unsigned char)(e2 + 127) : 255;
+    }
+  }
+}
+
+struct CacheReadArgs {
+  const unsigned char* cache;
+  uint16_t* out[2];  // k, v: [rows, heads, D]
+  const CacheSegment* segments;
+  int64_t page_bytes;
+  int D, page, heads;
+};
+
+// A workgroup takes one segment and head; lanes side by side take 8 channels each of one token after the other.
+template <class CT, int G>
+__global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(CacheReadArgs a) {
+  typedef typename CT::Type T;
+  constexpr int S = kv_scale_bytes(G);
+  const CacheSegment seg = a.segments[blockIdx.x];
+  const int head = blockIdx.y, chunks = a.D / 8;
+  const unsigned char* slab = a.cache + (int64_t)seg.page * a.page_bytes + head * kv_slab(G, a.page);
+  const int n = 2 * seg.rows * chunks;
+  for (int i = threadIdx.x; i < n; i += kCacheThreads) {
+    const int which = i / (seg.rows * chunks), j = i - which * seg.rows * chunks;
+    const int row = j / chunks, c = j - row * chunks, g = c >> 2, at = seg.first + row;
+    const unsigned char* from = slab + which * (int64_t)G * a.page * 16;
+    const uint32_t codes = *(const uint32_t*)(from + ((int64_t)g * a.page + at) * 16 + 4 * (c & 3));
+    const uint32_t e = slab[(int64_t)2 * G * a.page * 16 + which * (int64_t)a.page * S + at * S + g];
+    v4u out = kv_values<T>(codes, __uint_as_float((e == 255 ? 0u : e) << 23));
+    if (e == 255) out = (v4u){0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};  // NaN in either type
+    *(v4u*)(a.out[which] + ((seg.row0 + (int64_t)row) * a.heads + head) * a.D + 8 * c) = out;
+  }
+}
+
+// Pages of a launch, with their numbers among its parameters: nothing to upload, and nothing that a captured graph would
+// have to keep.
+constexpr int kCopyPairs = 256;
+struct CopyArgs {
+  unsigned char* pool;
+  int64_t layer_bytes, page_bytes;
+  int32_t src[kCopyPairs], dst[kCopyPairs];
+};
+constexpr int kCopyBytes = kCacheThreads * 16 * 4;  // of a workgroup
+
+__global__ __launch_bounds__(kCacheThreads) void copy_pages_kernel(CopyArgs a) {
+  const int64_t at = (int64_t)blockIdx.x * kCopyBytes;
+  unsigned char* layer = a.pool + (int64_t)blockIdx.z * a.layer_bytes;
+  const unsigned char* from = layer + (int64_t)a.src[blockIdx.y] * a.page_bytes;
+  unsigned char* to = layer + (int64_t)a.dst[blockIdx.y] * a.page_bytes;
+  v4u v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t o = at + (i * kCacheThreads + threadIdx.x) * 16;
+    if (o < a.page_bytes) v[i] = *(const v4u*)(from + o);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t o = at + (i * kCacheThreads + threadIdx.x) * 16;
+    if (o < a.page_bytes) *(v4u*)(to + o) = v[i];
+  }
+}
+
+}  // namespace hf
