@@ -12,11 +12,11 @@ constexpr int32_t kCacheMagic = 0x48464b56;
 struct CacheHeader {
   int32_t magic, heads, kv_heads, D, causal, page, items, joins;
   int64_t bytes, slots, q_rows, kv_rows, new_rows, wide_rows;
-  int32_t reads, writes, wides, join_rows;
+  int32_t reads, writes, wides, join_rows;  // join_rows: of the fullest tile that is joined
   // Where each part starts: items, joins, tables, segments read, written and expanded, the plan of the expanded ones.
   int64_t at_items, at_joins, at_tables, at_reads, at_writes, at_wides, at_attention, attention_bytes;
   int64_t pool_pages;
-  int32_t pad[22];
+  int32_t row_blocks, pad[21];
 };
 static_assert(sizeof(CacheHeader) == 256, "parts start on 128-byte lines behind it");
 
@@ -82,6 +82,12 @@ int cache_layout(const int64_t* q_lens, const int64_t* kv_lens, const int64_t* n
     hf::CachedItem item;
     int64_t cost, rows;
   };
+  // Rows of a tile: 16 hold the tokens and heads of most batches; two blocks where a sequence has more, so that its keys are
+  // read and made values of once.
+  int64_t most = 0;
+  for (int64_t b = 0; b < count; ++b)
+    if (q_lens[b] * group <= kCachedRows) most = std::max(most, q_lens[b] * group);
+  const int row_blocks = most > hf::kCaRows ? 2 : 1, tile_rows = hf::kCaRows * row_blocks;
   std::vector<Tile> tiles;
   std::vector<int64_t> wide_q, wide_kv, wide_q0;
   int64_t total = 0, q0 = 0, k0 = 0, n0 = 0, wide_rows = 0;
@@ -97,8 +103,8 @@ int cache_layout(const int64_t* q_lens, const int64_t* kv_lens, const int64_t* n
       wide_rows += nk;
     } else {
       for (int h = 0; h < kv_heads; ++h)
-        for (int64_t r = 0; r < nq * group; r += hf::kCaRows) {
-          const int64_t last = std::min(r + hf::kCaRows, nq * group) - 1;
+        for (int64_t r = 0; r < nq * group; r += tile_rows) {
+          const int64_t last = std::min(r + tile_rows, nq * group) - 1;
           const int64_t hi = causal ? std::min(std::max(last / group + nk - nq + 1, (int64_t)0), nk) : nk;
           Tile t;
           memset(&t, 0, sizeof(t));
@@ -149,6 +155,7 @@ int cache_layout(const int64_t* q_lens, const int64_t* kv_lens, const int64_t* n
   }
   h.heads = heads, h.kv_heads = kv_heads, h.D = D, h.causal = causal != 0, h.page = page;
   h.items = (int32_t)w->items.size(), h.joins = (int32_t)w->joins.size(), h.slots = slots, h.join_rows = join_rows;
+  h.row_blocks = row_blocks;
   h.q_rows = q_rows, h.kv_rows = kv_rows, h.new_rows = new_rows, h.wide_rows = wide_rows, h.pool_pages = pool_pages;
   h.reads = (int32_t)w->reads.size(), h.writes = (int32_t)w->writes.size(), h.wides = (int32_t)w->wides.size();
   int64_t at = sizeof(h);
@@ -174,7 +181,7 @@ struct CacheSpace {
 };
 CacheSpace cache_space(const CacheHeader& h, int64_t attention_ws) {
   CacheSpace s;
-  s.k = up_to(h.slots * hf::ca_slot_floats(cache_groups(h.D)) * 4, 256);
+  s.k = up_to(h.slots * hf::ca_slot_floats(cache_groups(h.D), h.row_blocks) * 4, 256);
   s.v = s.k + up_to(h.wide_rows * h.kv_heads * h.D * 2, 256);
   s.attention = s.v + up_to(h.wide_rows * h.kv_heads * h.D * 2, 256);
   s.bytes = s.attention + attention_ws;
@@ -219,24 +226,29 @@ int cache_read(const CacheHeader& h, const void* cache, void* k, void* v, const 
   return launch_status();
 }
 
-template <class T, int G>
+template <class T, int G, int R>
 int launch_cached_rows(const hf::CachedArgs& a, const CacheHeader& h, hipStream_t stream) {
-  hipLaunchKernelGGL((hf::cached_rows_kernel<T, G>), dim3(h.items), dim3(64 * hf::kCaWaves), 0, stream, a);
+  hipLaunchKernelGGL((hf::cached_rows_kernel<T, G, R>), dim3(h.items), dim3(64 * hf::kCaWaves), 0, stream, a);
   if (int st = launch_status()) return st;
   if (h.joins == 0) return HF_OK;
-  hipLaunchKernelGGL((hf::cached_join_kernel<T, G>), dim3(h.joins, (h.join_rows + hf::kJoinRows - 1) / hf::kJoinRows),
+  hipLaunchKernelGGL((hf::cached_join_kernel<T, G, R>), dim3(h.joins, (h.join_rows + hf::kJoinRows - 1) / hf::kJoinRows),
                      dim3(64 * hf::kJoinRows), 0, stream, a);
   return launch_status();
 }
 
-template <class T>
+template <class T, int R>
 int launch_cached(const hf::CachedArgs& a, const CacheHeader& h, hipStream_t stream) {
   switch (cache_groups(h.D)) {
-    case 1: return launch_cached_rows<T, 1>(a, h, stream);
-    case 2: return launch_cached_rows<T, 2>(a, h, stream);
-    case 3: return launch_cached_rows<T, 3>(a, h, stream);
-    default: return launch_cached_rows<T, 4>(a, h, stream);
+    case 1: return launch_cached_rows<T, 1, R>(a, h, stream);
+    case 2: return launch_cached_rows<T, 2, R>(a, h, stream);
+    case 3: return launch_cached_rows<T, 3, R>(a, h, stream);
+    default: return launch_cached_rows<T, 4, R>(a, h, stream);
   }
+}
+
+template <class T>
+int launch_cached_blocks(const hf::CachedArgs& a, const CacheHeader& h, hipStream_t stream) {
+  return h.row_blocks > 1 ? launch_cached<T, 2>(a, h, stream) : launch_cached<T, 1>(a, h, stream);
 }
 
 template <class T, bool WIDE>
@@ -369,8 +381,8 @@ int hf_cached_attention(const hf_cached_attention_args* p) {
     a.page_bytes = cache_page_bytes(h), a.group = h.heads / h.kv_heads, a.D = h.D, a.causal = h.causal, a.page = h.page;
     a.scale_log2 = (float)((double)p->scale * 1.4426950408889634);
     a.lift = (float)std::min((p->dtype == HF_FP16 ? hf::at_lift<hf::Fp16>() : 0) / (double)a.scale_log2, 0x1p127);
-    const int st = p->dtype == HF_BF16 ? launch_cached<hf::Bf16>(a, h, (hipStream_t)p->stream)
-                                       : launch_cached<hf::Fp16>(a, h, (hipStream_t)p->stream);
+    const int st = p->dtype == HF_BF16 ? launch_cached_blocks<hf::Bf16>(a, h, (hipStream_t)p->stream)
+                                       : launch_cached_blocks<hf::Fp16>(a, h, (hipStream_t)p->stream);
     if (st) return st;
   }
   if (h.attention_bytes == 0) return HF_OK;

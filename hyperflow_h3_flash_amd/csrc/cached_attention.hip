@@ -1,13 +1,16 @@
 // Attention of few rows over keys and values in pages of 4-bit codes (kv_cache.hip).
 //
-// Rows, items and the running maximum and sum are those of attention.hip: a row is a (token, head of the group) pair, here
-// up to 32 of them a workgroup, and scores are computed transposed. The four waves of a workgroup take the item's blocks of
-// 32 keys in turn, each with sums of its own, and join them at the end through LDS.
+// Rows, items and the running maximum and sum are those of attention.hip: a row is a (token, head of the group) pair, here 16
+// or 32 of them a workgroup (R blocks of 16), and scores are computed transposed. The four waves of a workgroup take the
+// item's blocks of 32 keys in turn, each with sums of its own and no barrier, and join them at the end through LDS.
 //
-// Operands. Codes go from memory to registers, 16 bytes (a group of 32 channels of a key) a lane: for the scores that is
-// already the order of the first product's operand, four steps of 8 channels a lane, when the queries' channels are taken in
-// the same order; codes become values of the type two at a time with the group's scale (exact). Values are turned
-// into the second product's operand through LDS, by wave: written by key, read transposed, as in attention.hip.
+// Operands (matrix instructions of 16 x 16 x 32). Codes go from memory to registers: lane l takes the channels of quarter
+// l / 16 (a group of 32 channels, or a quarter of a narrower head) of keys l % 16 and 16 + l % 16. For the scores that is
+// already the order of the first product's operand, 8 channels a step, when the queries' channels are taken in the same
+// order; codes become values of the type two at a time with the group's scale (exact). A lane's scores are of row l % 16 and
+// keys 16 b + 4 (l / 16) + i: the second product's operand when its keys are numbered so. Values are turned through LDS, by
+// wave: written by key, read transposed four keys at a time, as in attention.hip.
+//
 #pragma once
 
 #include "attention.hip"
@@ -15,7 +18,7 @@
 
 namespace hf {
 
-constexpr int kCaRows = 32, kCaWaves = 4, kCaKeys = 32;
+constexpr int kCaRows = 16, kCaWaves = 4, kCaKeys = 32;  // of a block of rows, of a workgroup, of a step
 
 struct CachedItem {
   int32_t q0, nq, nk, row0, key_lo, key_hi, head, slot, table0, pad[3];
@@ -37,292 +40,319 @@ struct CachedArgs {
   float scale_log2, lift;
 };
 
-// Floats of a workspace tile: O [kCaRows][32 G], then m and l per row.
-__host__ __device__ constexpr int ca_slot_floats(int groups) { return kCaRows * (32 * groups + 2); }
+// Floats of a workspace tile: O [16 R][32 G], then m and l per row.
+__host__ __device__ constexpr int ca_slot_floats(int groups, int blocks) { return kCaRows * blocks * (32 * groups + 2); }
 __host__ __device__ constexpr int ca_pitch(int groups) { return groups > 2 ? 256 : 128; }
-// LDS: a wave's values of a block; two waves' sums at the end; each row's maximum and sum by wave.
-__host__ __device__ constexpr int ca_lds(int groups) {
-  return kCaWaves * kCaKeys * ca_pitch(groups) > 2 * 4096 * groups ? kCaWaves * kCaKeys * ca_pitch(groups)
-                                                                   : 2 * 4096 * groups;
+
+__device__ __forceinline__ v4f ca_mfma(v4u a, v4u b, v4f c, Bf16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ v4f ca_mfma(v4u a, v4u b, v4f c, Fp16) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-template <class T, int G>
-__global__ __launch_bounds__(64 * kCaWaves) void cached_rows_kernel(CachedArgs a) {
-  constexpr int G2 = (G + 1) / 2, S = kv_scale_bytes(G), PITCH = ca_pitch(G);
-  __shared__ __attribute__((aligned(1024))) unsigned char ca_mem[ca_lds(G)];
-  __shared__ v2f ca_stat[kCaWaves][kCaRows];
+// Over the four lanes of a row.
+__device__ __forceinline__ float quad_max(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+template <class T, int G, int R>
+__global__ __launch_bounds__(64 * kCaWaves, R > 1 ? 2 : G > 2 ? 3 : 4) void cached_rows_kernel(CachedArgs a) {
+  constexpr int PITCH = ca_pitch(G);
+  constexpr int W = G > 2 ? 4 : G;      // dwords of codes a lane takes of a key, steps of the first product
+  constexpr int DB = 2 * G;             // blocks of 16 channels
+  constexpr int kTile = kCaKeys * PITCH;
+  constexpr int kSums = kCaWaves * DB * 1024;  // bytes of the waves' sums of a block of rows
+  __shared__ __attribute__((aligned(1024))) unsigned char ca_mem[kCaWaves * kTile > kSums ? kCaWaves * kTile : kSums];
+  __shared__ v2f ca_stat[kCaWaves][kCaRows * R];
   const CachedItem it = a.items[blockIdx.x];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int sub = lane & 31, half = lane >> 5;
+  const int sub = lane & 15, quarter = lane >> 4;
+  // The group of the lane's channels, and the dword of its codes where they begin.
+  const int g = G > 2 ? min(quarter, G - 1) : G == 2 ? quarter >> 1 : 0;
+  const int dword = G > 2 ? 0 : G == 2 ? 2 * (quarter & 1) : quarter;
 
-  const int64_t row = (int64_t)it.row0 + sub;
-  const bool live = row < (int64_t)it.nq * a.group;
-  const int token = live ? (int)((uint32_t)row / (uint32_t)a.group) : 0;
-  const int head = it.head * a.group + (live ? (int)(row - (int64_t)token * a.group) : 0);
-  const int last = live ? (a.causal ? min(token + it.nk - it.nq, it.nk - 1) : it.nk - 1) : -1;
-  const int first_last = __builtin_amdgcn_readfirstlane(last);  // the first row sees the fewest keys
-
-  // Queries in the order of the codes: step (i, w) takes channels 32 (2 i + half) + 8 w ..
-  v4u qf[G2][4];
-  {
-    const uint16_t* q = a.q + (it.q0 + (int64_t)token) * a.q_token + head * a.q_head;
+  bool live[R];
+  int token[R], head[R], last[R];
+  v4u qf[R][W];
 #pragma unroll
-    for (int i = 0; i < G2; ++i)
+  for (int r = 0; r < R; ++r) {
+    const int64_t row = (int64_t)it.row0 + kCaRows * r + sub;
+    live[r] = row < (int64_t)it.nq * a.group;
+    token[r] = live[r] ? (int)((uint32_t)row / (uint32_t)a.group) : 0;
+    head[r] = it.head * a.group + (live[r] ? (int)(row - (int64_t)token[r] * a.group) : 0);
+    last[r] = live[r] ? (a.causal ? min(token[r] + it.nk - it.nq, it.nk - 1) : it.nk - 1) : -1;
+    // Queries in the order of the codes.
+    const uint16_t* q = a.q + (it.q0 + (int64_t)token[r]) * a.q_token + head[r] * a.q_head;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const int c = 32 * (2 * i + half) + 8 * w;
-        qf[i][w] = live && c < a.D ? *(const v4u*)(q + c) : (v4u){0, 0, 0, 0};
-      }
+    for (int w = 0; w < W; ++w) {
+      const int c = 8 * (W * quarter + w);
+      qf[r][w] = live[r] && c < a.D ? *(const v4u*)(q + c) : (v4u){0, 0, 0, 0};
+    }
   }
+  const int first_last = __builtin_amdgcn_readfirstlane(last[0]);  // the first row sees the fewest keys
 
+  typedef uint32_t Codes[W];
   struct Block {
-    v4u k[G2], v[G2];
-    uint32_t ks, vs;
+    Codes k[2], v[2];
+    uint32_t ks[2], vs[2];  // scale bytes of the key
   };
   const int page_shift = 31 - __builtin_clz(a.page);
   const int64_t slab_bytes = kv_slab(G, a.page);
-  auto load = [&](int key0, Block& b) __attribute__((always_inline)) {
-    const int page = a.tables[it.table0 + (key0 >> page_shift)];
+  const int blocks = (it.key_hi - it.key_lo + kCaKeys - 1) / kCaKeys;
+  // Past the item's last block its last one again: loads without a condition, so that waiting for one block's loads is not
+  // waiting for the next one's.
+  auto key_of = [&](int i) __attribute__((always_inline)) { return it.key_lo + kCaKeys * min(i, blocks - 1); };
+  auto page_of = [&](int i) __attribute__((always_inline)) { return a.tables[it.table0 + (key_of(i) >> page_shift)]; };
+  auto load = [&](int key0, int page, Block& b) __attribute__((always_inline)) {
     const unsigned char* slab = a.cache + (int64_t)page * a.page_bytes + it.head * slab_bytes;
     const int at = (key0 & (a.page - 1)) + sub;
 #pragma unroll
-    for (int i = 0; i < G2; ++i) {
-      const int g = min(2 * i + half, G - 1);
-      b.k[i] = *(const v4u*)(slab + ((int64_t)g * a.page + at) * 16);
-      b.v[i] = *(const v4u*)(slab + ((int64_t)(G + g) * a.page + at) * 16);
-    }
-    const unsigned char* scales = slab + (int64_t)2 * G * a.page * 16 + at * S;
-    if constexpr (S == 4) {
-      b.ks = *(const uint32_t*)scales;
-      b.vs = *(const uint32_t*)(scales + (int64_t)a.page * S);
-    } else if constexpr (S == 2) {
-      b.ks = *(const uint16_t*)scales;
-      b.vs = *(const uint16_t*)(scales + (int64_t)a.page * S);
-    } else {
-      b.ks = *scales;
-      b.vs = *(scales + (int64_t)a.page * S);
+    for (int h = 0; h < 2; ++h) {
+      const unsigned char* k = slab + (g * a.page + at + 16 * h) * 16 + 4 * dword;
+      const unsigned char* v = k + G * a.page * 16;
+      const unsigned char* s = slab + 2 * G * a.page * 16 + (at + 16 * h) * 2 * kv_scale_bytes(G);
+      if constexpr (W == 4) {
+        const v4u x = *(const v4u*)k, y = *(const v4u*)v;
+        const uint2 z = *(const uint2*)s;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) b.k[h][w] = x[w], b.v[h][w] = y[w];
+        b.ks[h] = z.x, b.vs[h] = z.y;
+      } else if constexpr (W == 2) {
+        const uint2 x = *(const uint2*)k, y = *(const uint2*)v;
+        const uint32_t z = *(const uint32_t*)s;
+        b.k[h][0] = x.x, b.k[h][1] = x.y, b.v[h][0] = y.x, b.v[h][1] = y.y;
+        b.ks[h] = z & 0xffffu, b.vs[h] = z >> 16;
+      } else {
+        const uint16_t z = *(const uint16_t*)s;
+        b.k[h][0] = *(const uint32_t*)k, b.v[h][0] = *(const uint32_t*)v;
+        b.ks[h] = z & 255u, b.vs[h] = z >> 8;
+      }
     }
   };
-  auto scale_of = [&](uint32_t scales, int i) __attribute__((always_inline)) {
-    const int g = min(2 * i + half, G - 1);
+  auto scale_of = [&](uint32_t scales) __attribute__((always_inline)) {
     return __uint_as_float(((scales >> (8 * g)) & 255u) << 23);
   };
-  auto any_nan = [&](uint32_t scales) __attribute__((always_inline)) {
-    bool bad = false;
-#pragma unroll
-    for (int g = 0; g < G; ++g) bad |= ((scales >> (8 * g)) & 255u) == 255u;
-    return bad;
-  };
 
-  unsigned char HF_LDS* tile = (unsigned char HF_LDS*)ca_mem + wave * kCaKeys * PITCH;
-  uint32_t vaddr;
+  unsigned char HF_LDS* tile = (unsigned char HF_LDS*)ca_mem + wave * kTile;
+  const uint32_t vwrite = (uint32_t)(sub * PITCH + (((W * quarter) ^ at_swizzle<PITCH>(sub)) * 16));
+  uint32_t vread;
   {
-    const int r = 4 * half + ((lane & 15) >> 2), ch = 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    vaddr = (uint32_t)(r * PITCH + ((ch ^ at_swizzle<PITCH>(r)) * 16) + (lane & 1) * 8);
+    const int r = 4 * quarter + (sub >> 2), ch = (lane & 3) >> 1;
+    vread = (uint32_t)(r * PITCH + ((ch ^ at_swizzle<PITCH>(r)) * 16) + (lane & 1) * 8);
   }
-  auto vfrag = [&](int ks, int d) __attribute__((always_inline)) {
+  auto vfrag = [&](int d) __attribute__((always_inline)) {  // channels 16 d + sub of keys 4 quarter + i, 16 + 4 quarter + i
     typedef short v8s __attribute__((ext_vector_type(8)));
-    const unsigned char HF_LDS* at = tile + ks * 16 * PITCH;
-    const v4s f0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s HF_LDS*)(at + (vaddr ^ (uint32_t)(64 * d))));
-    const v4s f1 =
-        __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s HF_LDS*)(at + 8 * PITCH + (vaddr ^ (uint32_t)(64 * d + 32))));
+    const unsigned char HF_LDS* at = tile + (vread ^ (uint32_t)(32 * d));
+    const v4s f0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s HF_LDS*)at);
+    const v4s f1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((v4s HF_LDS*)(at + 16 * PITCH));
     return __builtin_bit_cast(v4u, (v8s)__builtin_shufflevector(f0, f1, 0, 1, 2, 3, 4, 5, 6, 7));
   };
 
   const float c = a.scale_log2;
-  v16f o[G];
-#pragma unroll
-  for (int d = 0; d < G; ++d) o[d] = (v16f){0};
-  float m = -__builtin_inff(), l = 0.0f;
+  v4f o[R][DB];
+  float m[R], l[R];
 
-  auto step = [&](int key0, Block& b) __attribute__((always_inline)) {
+  // SAFE: groups of values that are NaN are taken out and their first keys kept (keys come in rising order).
+  int nan_from[G];
+  auto step = [&](auto safe_t, int key0, Block& b) __attribute__((always_inline)) {
     // What lies past the sequence in its last page counts nothing, whatever it is.
-    if (key0 + sub >= it.nk) b.ks = b.vs = 0;
-    uint32_t knan = 0, vnan[G];
-    const bool odd = __any(any_nan(b.ks) || any_nan(b.vs));
-    if (odd) {
-      knan = (uint32_t)__ballot(any_nan(b.ks));
+    if (key0 + kCaKeys > it.nk) {
 #pragma unroll
-      for (int g = 0; g < G; ++g) vnan[g] = (uint32_t)__ballot(((b.vs >> (8 * g)) & 255u) == 255u);
-      if (any_nan(b.ks)) b.ks = 0;
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-        if (((b.vs >> (8 * g)) & 255u) == 255u) b.vs &= ~(255u << (8 * g));
+      for (int h = 0; h < 2; ++h)
+        if (key0 + 16 * h + sub >= it.nk) b.ks[h] = b.vs[h] = 0;
     }
-    v16f s = (v16f){0};
+    if constexpr (decltype(safe_t)::value) {
 #pragma unroll
-    for (int i = 0; i < G2; ++i) {
-      const float scale = scale_of(b.ks, i);
+      for (int x = 0; x < G; ++x)
 #pragma unroll
-      for (int w = 0; w < 4; ++w) s = T::mfma(kv_values<T>(b.k[i][w], scale), qf[i][w], s);
-    }
-    // Value v is key 8 (v / 4) + 4 half + v % 4 of the block.
-    if (odd && knan) {
-#pragma unroll
-      for (int v = 0; v < 16; ++v)
-        if ((knan >> (8 * (v >> 2) + 4 * half + (v & 3))) & 1u) s[v] = __builtin_nanf("");
-    }
-    if (key0 + kCaKeys - 1 > first_last) {
-      const int left = last - key0 - 4 * half;
-#pragma unroll
-      for (int v = 0; v < 16; ++v)
-        if (8 * (v >> 2) + (v & 3) > left) s[v] = -__builtin_inff();
-    }
-    // A lane's values of its key to LDS.
-#pragma unroll
-    for (int i = 0; i < G2; ++i) {
-      const float scale = scale_of(b.vs, i);
-      const int g = 2 * i + half;
-      if (g < G) {
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          *(v4u HF_LDS*)(tile + sub * PITCH + (((4 * g + w) ^ at_swizzle<PITCH>(sub)) * 16)) =
-              kv_values<T>(b.v[i][w], scale);
-      }
-    }
-    float top = s[0];
-#pragma unroll
-    for (int v = 1; v < 16; ++v) top = fmaxf(top, s[v]);
-    top = half_max(top);
-    // The maximum is taken anew where a weight would pass 2^8 (see attention.hip on at_lift); each row goes by its own
-    // scores, so that its bits do not depend on the rows that share its wave.
-    const bool move = (top - m) * c > 8.0f + at_lift<T>();
-    if (__any(move)) {
-      const float next = move ? top - a.lift : m;
-      const float alpha = move ? __builtin_amdgcn_exp2f((m - next) * c) : 1.0f;
-      m = next;
-      l *= alpha;
-#pragma unroll
-      for (int d = 0; d < G; ++d)
-#pragma unroll
-        for (int v = 0; v < 16; ++v) o[d][v] *= alpha;
-    }
-    const float mc = m == -__builtin_inff() ? 0.0f : m * c;
-    v4u pf[2];
-#pragma unroll
-    for (int p = 0; p < 8; ++p) {
-      // Rounded to the type for the second product (attention.hip); the sum is of the unrounded ones.
-      const float p0 = __builtin_amdgcn_exp2f(fmaf(s[2 * p], c, -mc)), p1 = __builtin_amdgcn_exp2f(fmaf(s[2 * p + 1], c, -mc));
-      l += p0 + p1;
-      pf[p >> 2][p & 3] = T::pack(p0, p1);
-    }
-    wave_lds_sync();
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-#pragma unroll
-      for (int d = 0; d < G; ++d) o[d] = T::mfma(vfrag(ks, d), pf[ks], o[d]);
-    if (odd) {
-#pragma unroll
-      for (int g = 0; g < G; ++g)
-        if (vnan[g] && key0 + __builtin_ctz(vnan[g]) <= last)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) o[g][v] = __builtin_nanf("");
-    }
-    wave_lds_sync();
-  };
-
-  constexpr int kStride = kCaWaves * kCaKeys;
-  int key0 = it.key_lo + wave * kCaKeys;
-  if (key0 < it.key_hi) {
-    Block b;
-    load(key0, b);
-#pragma unroll 1
-    for (;;) {
-      const int next = key0 + kStride;
-      Block ahead;
-      if (next < it.key_hi) load(next, ahead);
-      step(key0, b);
-      if (next >= it.key_hi) break;
-      b = ahead;
-      key0 = next;
-    }
-  }
-  l = half_sum(l);
-  if (l != l && m == -__builtin_inff()) m = 0.0f;  // only scores that are NaN: seen, so not to be left out below
-
-  // The waves' sums joined: each row's maximum over the waves, every wave's sums to that, then added two by two.
-  if (half == 0) ca_stat[wave][sub] = (v2f){m, l};
-  __syncthreads();
-  float top = -__builtin_inff(), total = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kCaWaves; ++w) top = fmaxf(top, ca_stat[w][sub][0]);
-#pragma unroll
-  for (int w = 0; w < kCaWaves; ++w) {
-    const v2f ml = ca_stat[w][sub];
-    total += ml[0] == -__builtin_inff() ? 0.0f : ml[1] * __builtin_amdgcn_exp2f((ml[0] - top) * c);
-  }
-  const float f = m == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m - top) * c);
-  auto hand = [&](int place) __attribute__((always_inline)) {
-#pragma unroll
-    for (int d = 0; d < G; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *(v4f*)(ca_mem + place * 4096 * G + ((4 * d + g) * 64 + lane) * 16) =
-            (v4f){o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
-  };
-  auto take = [&](int place) __attribute__((always_inline)) {
-#pragma unroll
-    for (int d = 0; d < G; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        const v4f x = *(const v4f*)(ca_mem + place * 4096 * G + ((4 * d + g) * 64 + lane) * 16);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[d][4 * g + e] += x[e];
-      }
-  };
-#pragma unroll
-  for (int d = 0; d < G; ++d)
-#pragma unroll
-    for (int v = 0; v < 16; ++v) o[d][v] = m == -__builtin_inff() ? 0.0f : o[d][v] * f;
-  if (wave >= 2) hand(wave - 2);
-  __syncthreads();
-  if (wave < 2) take(wave);
-  __syncthreads();
-  if (wave == 1) hand(0);
-  __syncthreads();
-  if (wave > 0) return;
-  take(0);
-
-  if (it.slot >= 0) {
-    float* part = a.ws + (int64_t)it.slot * ca_slot_floats(G);
-    if (!live) return;
-#pragma unroll
-    for (int d = 0; d < G; ++d)
-#pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *(v4f*)(part + sub * 32 * G + 32 * d + 8 * g + 4 * half) =
-            (v4f){o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]};
-    if (half == 0) *(v2f*)(part + kCaRows * 32 * G + 2 * sub) = (v2f){top, total};
-    return;
-  }
-  const float inv = 1.0f / total;
-  uint16_t* out = a.out + (it.q0 + (int64_t)token) * a.o_token + head * a.o_head;
-#pragma unroll
-  for (int d = 0; d < G; ++d)
-#pragma unroll
-    for (int g = 0; g < 4; g += 2) {
-      uint32_t w[2][2];
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int v = 4 * (g + x) + 2 * e;
-          w[x][e] = last < 0 ? 0u : T::pack(o[d][v] * inv, o[d][v + 1] * inv);
+        for (int h = 0; h < 2; ++h) {
+          const bool bad = ((b.vs[h] >> (8 * x)) & 255u) == 255u;
+          const uint32_t keys = (uint32_t)__ballot(bad) & 0xffffu;
+          if (keys) nan_from[x] = min(nan_from[x], key0 + 16 * h + __builtin_ctz(keys));
+          if (bad) b.vs[h] &= ~(255u << (8 * x));
         }
-      v4u line;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const auto r = __builtin_amdgcn_permlane32_swap(w[0][e], w[1][e], false, false);
-        line[e] = r[0];
-        line[2 + e] = r[1];
-      }
-      const int channel = 32 * d + 8 * (g + half);
-      if (live && channel < a.D) *(v4u*)(out + channel) = line;
     }
+    v4f s[R][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float scale = scale_of(b.ks[h]);
+#pragma unroll
+      for (int r = 0; r < R; ++r) s[r][h] = (v4f){0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const v4u k = kv_values<T>(b.k[h][w], scale);
+#pragma unroll
+        for (int r = 0; r < R; ++r) s[r][h] = ca_mfma(k, qf[r][w], s[r][h], T());
+      }
+    }
+    // A lane's values of its keys to LDS.
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float scale = scale_of(b.vs[h]);
+      if (G != 3 || quarter < 3) {
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+          *(v4u HF_LDS*)(tile + (vwrite ^ (uint32_t)(16 * w)) + 16 * h * PITCH) = kv_values<T>(b.v[h][w], scale);
+      }
+    }
+    v4u pf[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (key0 + kCaKeys - 1 > first_last) {  // value i of half h is key 16 h + 4 quarter + i of the block
+        const int left = last[r] - key0 - 4 * quarter;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (16 * h + i > left) s[r][h][i] = -__builtin_inff();
+      }
+      float top = s[r][0][0];
+#pragma unroll
+      for (int v = 1; v < 8; ++v) top = fmaxf(top, s[r][v >> 2][v & 3]);
+      top = quad_max(top);
+      // The maximum is taken anew where a weight would pass 2^8 (attention.hip on at_lift); each row goes by its own scores,
+      // so that its bits do not depend on the rows that share its wave.
+      const bool move = (top - m[r]) * c > 8.0f + at_lift<T>();
+      if (__any(move)) {
+        const float next = move ? top - a.lift : m[r];
+        const float alpha = move ? __builtin_amdgcn_exp2f((m[r] - next) * c) : 1.0f;
+        m[r] = next;
+        l[r] *= alpha;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) o[r][d][v] *= alpha;
+      }
+      const float mc = m[r] == -__builtin_inff() ? 0.0f : m[r] * c;
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        // Rounded to the type for the second product (attention.hip); the sum is of the unrounded ones.
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(s[r][p >> 1][2 * (p & 1)], c, -mc));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(s[r][p >> 1][2 * (p & 1) + 1], c, -mc));
+        l[r] += p0 + p1;
+        pf[r][p] = T::pack(p0, p1);
+      }
+    }
+    wave_lds_sync();
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      const v4u v = vfrag(d);
+#pragma unroll
+      for (int r = 0; r < R; ++r) o[r][d] = ca_mfma(v, pf[r], o[r][d], T());
+    }
+    wave_lds_sync();
+  };
+  auto run = [&](auto safe_t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d) o[r][d] = (v4f){0, 0, 0, 0};
+      m[r] = -__builtin_inff(), l[r] = 0.0f;
+    }
+#pragma unroll
+    for (int x = 0; x < G; ++x) nan_from[x] = 0x7fffffff;
+    if (wave >= blocks) return;
+    Block b[2];
+    load(key_of(wave), page_of(wave), b[0]);
+    int page = page_of(wave + kCaWaves);
+#pragma unroll 1
+    for (int i = wave;;) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        load(key_of(i + kCaWaves), page, b[1 - x]);
+        page = page_of(i + 2 * kCaWaves);
+        step(safe_t, key_of(i), b[x]);
+        i += kCaWaves;
+        if (i >= blocks) return;
+      }
+    }
+  };
+  run(std::false_type{});
+  // A value that is NaN poisons rows that do not see it (0 * NaN); then the wave's keys are taken again the safe way. Keys
+  // that are NaN need none of it: scores that a row does not see are replaced.
+  {
+    bool again = false;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      float all = 0.0f;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) all += o[r][d][v];
+      again |= live[r] && all != all;
+    }
+    if (__any(again)) {
+      run(std::true_type{});
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+          if (nan_from[d >> 1] <= last[r]) o[r][d] = (v4f){1, 1, 1, 1} * __builtin_nanf("");
+    }
+  }
+
+  // The waves' sums joined: each row's maximum over the waves, every wave's sums to that, then a block of 16 channels a wave
+  // summed over the waves.
+  float top[R], total[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    l[r] = quad_sum(l[r]);
+    if (l[r] != l[r] && m[r] == -__builtin_inff()) m[r] = 0.0f;  // only scores that are NaN: seen, so not to be left out
+    if (quarter == 0) ca_stat[wave][kCaRows * r + sub] = (v2f){m[r], l[r]};
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    top[r] = -__builtin_inff(), total[r] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kCaWaves; ++w) top[r] = fmaxf(top[r], ca_stat[w][kCaRows * r + sub][0]);
+#pragma unroll
+    for (int w = 0; w < kCaWaves; ++w) {
+      const v2f ml = ca_stat[w][kCaRows * r + sub];
+      total[r] += ml[0] == -__builtin_inff() ? 0.0f : ml[1] * __builtin_amdgcn_exp2f((ml[0] - top[r]) * c);
+    }
+    const float f = m[r] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((m[r] - top[r]) * c);
+    if (r > 0) __syncthreads();
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      v4f x = o[r][d];
+#pragma unroll
+      for (int v = 0; v < 4; ++v) x[v] = m[r] == -__builtin_inff() ? 0.0f : x[v] * f;
+      *(v4f*)(ca_mem + ((wave * DB + d) * 64 + lane) * 16) = x;
+    }
+    __syncthreads();
+    const float inv = 1.0f / total[r];
+#pragma unroll
+    for (int d0 = 0; d0 < DB; d0 += kCaWaves) {
+      const int d = d0 + wave;
+      if (d >= DB) break;
+      v4f x = *(const v4f*)(ca_mem + (d * 64 + lane) * 16);
+#pragma unroll
+      for (int w = 1; w < kCaWaves; ++w) x += *(const v4f*)(ca_mem + ((w * DB + d) * 64 + lane) * 16);
+      const int channel = 16 * d + 4 * quarter;
+      if (!live[r]) continue;
+      if (it.slot >= 0) {
+        float* part = a.ws + (int64_t)it.slot * ca_slot_floats(G, R) + (kCaRows * r + sub) * 32 * G;
+        *(v4f*)(part + channel) = x;
+      } else if (channel < a.D) {
+        uint16_t* out = a.out + (it.q0 + (int64_t)token[r]) * a.o_token + head[r] * a.o_head + channel;
+        *(uint2*)out = last[r] < 0 ? make_uint2(0, 0) : make_uint2(T::pack(x[0] * inv, x[1] * inv), T::pack(x[2] * inv, x[3] * inv));
+      }
+    }
+    if (it.slot >= 0 && wave == 0 && quarter == 0 && live[r])
+      *(v2f*)(a.ws + (int64_t)it.slot * ca_slot_floats(G, R) + kCaRows * R * 32 * G + 2 * (kCaRows * r + sub)) =
+          (v2f){top[r], total[r]};
+  }
 }
 
 // The shares of a tile joined, as attention_join_kernel does. blockIdx.y takes kJoinRows rows of the tile.
-template <class T, int G>
+template <class T, int G, int R>
 __global__ __launch_bounds__(64 * kJoinRows) void cached_join_kernel(CachedArgs a) {
   const CachedJoin j = a.joins[blockIdx.x];
   const int lane = threadIdx.x & 63, group = lane >> 4;
@@ -331,9 +361,9 @@ __global__ __launch_bounds__(64 * kJoinRows) void cached_join_kernel(CachedArgs 
   const int64_t row = (int64_t)j.row0 + r;
   const int token = (int)((uint32_t)row / (uint32_t)a.group);
   const int head = j.head * a.group + (int)(row - (int64_t)token * a.group);
-  const int64_t step = ca_slot_floats(G);
+  const int64_t step = ca_slot_floats(G, R);
   const float* part = a.ws + (int64_t)j.slot0 * step;
-  const float* stat = part + kCaRows * 32 * G + 2 * r;
+  const float* stat = part + kCaRows * R * 32 * G + 2 * r;
   float top = -__builtin_inff();
   for (int s = lane; s < j.slots; s += 64) top = fmaxf(top, stat[s * step]);
 #pragma unroll

@@ -93,8 +93,8 @@ __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(CacheWriteAr
     unsigned char* to = slab + which * (int64_t)G * a.page * 16;
     *(uint32_t*)(to + ((int64_t)g * a.page + at) * 16 + 4 * part) = finite ? codes : 0u;
     if (part == 0) {
-      unsigned char* scales = slab + (int64_t)2 * G * a.page * 16 + which * (int64_t)a.page * S;
-      scales[at * S + g] = finite ? (unsigned char)(e2 + 127) : 255;
+      unsigned char* scales = slab + 2 * G * a.page * 16 + which * S;
+      scales[at * 2 * S + g] = finite ? (unsigned char)(e2 + 127) : 255;
     }
   }
 }
@@ -121,7 +121,7 @@ __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(CacheReadArgs
     const int row = j / chunks, c = j - row * chunks, g = c >> 2, at = seg.first + row;
     const unsigned char* from = slab + which * (int64_t)G * a.page * 16;
     const uint32_t codes = *(const uint32_t*)(from + ((int64_t)g * a.page + at) * 16 + 4 * (c & 3));
-    const uint32_t e = slab[(int64_t)2 * G * a.page * 16 + which * (int64_t)a.page * S + at * S + g];
+    const uint32_t e = slab[2 * G * a.page * 16 + (2 * at + which) * S + g];
     v4u out = kv_values<T>(codes, __uint_as_float((e == 255 ? 0u : e) << 23));
     if (e == 255) out = (v4u){0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};  // NaN in either type
     *(v4u*)(a.out[which] + ((seg.row0 + (int64_t)row) * a.heads + head) * a.D + 8 * c) = out;

@@ -54,11 +54,11 @@ def dequantize(codes: Tensor, scales: Tensor, dim: int, dtype: torch.dtype) -> T
 
 
 def _views(cache, layer: int) -> tuple[Tensor, Tensor]:
-    """A layer's pages as codes [pages, heads, k or v, groups, page_size, 16] and scales [pages, heads, k or v, page_size,
+    """A layer's pages as codes [pages, heads, k or v, groups, page_size, 16] and scales [pages, heads, page_size, k or v,
     bytes]."""
     G, P, S = cache.groups, cache.page_size, scale_bytes(cache.groups)
     slabs = cache.data[layer].view(cache.pages, cache.kv_heads, -1)
-    return (slabs[..., :2 * G * P * 16].unflatten(-1, (2, G, P, 16)), slabs[..., 2 * G * P * 16:].unflatten(-1, (2, P, S)))
+    return (slabs[..., :2 * G * P * 16].unflatten(-1, (2, G, P, 16)), slabs[..., 2 * G * P * 16:].unflatten(-1, (P, 2, S)))
 
 
 def _slots(cache, table: list[int], first: int, last: int) -> tuple[Tensor, Tensor]:
@@ -75,7 +75,7 @@ def append(cache, layer: int, k: Tensor, v: Tensor, plan) -> None:
         for which, x in enumerate((k, v)):
             c, s = quantize(x[row:row + new])
             codes[page, :, which, :, at] = c
-            scales[page, :, which, at, :G] = s
+            scales[page, :, at, which, :G] = s
         row += new
 
 
@@ -85,7 +85,7 @@ def read(cache, layer: int, plan, k: Tensor, v: Tensor) -> None:
     for table, total in zip(plan.tables, plan.kv_lengths):
         page, at = _slots(cache, table, 0, total)
         for which, x in enumerate((k, v)):
-            x[row:row + total] = dequantize(codes[page, :, which, :, at], scales[page, :, which, at, :G], cache.head_dim,
+            x[row:row + total] = dequantize(codes[page, :, which, :, at], scales[page, :, at, which, :G], cache.head_dim,
                                             cache.dtype)
         row += total
 

@@ -10,7 +10,7 @@
  * THE PAGES. A cache is [layers][pages][kv_heads][slab]: a page holds page_size tokens (32, 64, 128 or 256) of one layer,
  * and a slab a page's tokens of one head. With G = ceil(D / 32) groups of 32 channels (the last one filled with zeros) and
  * S = G, but 4 for G = 3, a slab is
- *   keys' codes [G][page_size][16 bytes], values' codes the same, keys' scales [page_size][S bytes], values' scales the same.
+ *   keys' codes [G][page_size][16 bytes], values' codes the same, scales [page_size][S bytes of keys, S bytes of values].
  * A group's 16 bytes are its 32 codes, the even channel in the low half of a byte. A code is a sign bit above three bits for
  * 0, 0.5, 1, 1.5, 2, 3, 4, 6; a scale byte E is the power of two 2^(E - 127), and 255 a group of which every value is NaN.
  * WRITING: scale = the least 2^e that is at least a seventh of the group's largest magnitude (so that the largest is rounded

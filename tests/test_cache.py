@@ -360,7 +360,8 @@ def parts(raw):
     reads, writes, wides, join_rows = struct.unpack_from("4i", raw, 80)
     at = dict(zip("items joins tables reads writes wides attention attention_bytes".split(), struct.unpack_from("8q", raw, 96)))
     grid = lambda name, n, width: np.frombuffer(raw, np.int32, n * width, at[name]).reshape(n, width)
-    return {"slots": slots, "join_rows": join_rows, "items": grid("items", items, 12), "joins": grid("joins", joins, 8),
+    rows, = struct.unpack_from("i", raw, 168)
+    return {"rows": 16 * rows, "slots": slots, "join_rows": join_rows, "items": grid("items", items, 12), "joins": grid("joins", joins, 8),
             "reads": grid("reads", reads, 4), "writes": grid("writes", writes, 4), "wides": grid("wides", wides, 4),
             "tables": np.frombuffer(raw, np.int32, (at["reads"] - at["tables"]) // 4, at["tables"]),
             "attention": raw[at["attention"]:at["attention"] + at["attention_bytes"]]}
@@ -406,9 +407,9 @@ def test_plan_covers_every_row_key_and_token_once(lib, q, kv, new, heads, kv_hea
         if b in wide:
             continue
         for head in range(kv_heads):
-            for row0 in range(0, q[b] * group, 32):
+            for row0 in range(0, q[b] * group, p["rows"]):
                 spans = sorted(seen.pop((b, head, row0)))
-                last = min(row0 + 32, q[b] * group) - 1
+                last = min(row0 + p["rows"], q[b] * group) - 1
                 hi = min(max(last // group + kv[b] - q[b] + 1, 0), kv[b]) if causal else kv[b]
                 assert spans[0][0] == 0 and spans[-1][1] == hi and all(x[1] == y[0] for x, y in zip(spans, spans[1:]))
                 assert (spans[0][2] < 0) == (len(spans) == 1)
