@@ -107,16 +107,6 @@ __device__ __forceinline__ void at_order() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// Lane l exchanges with lane l ^ 32: max of both.
-__device__ __forceinline__ float half_max(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-__device__ __forceinline__ float half_sum(float v) {
-  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
-}
-
 // D up to 32 * DB channels.
 template <class T, int DB>
 __global__ __launch_bounds__(64 * kAtWaves, 2) void attention_kernel(AttentionArgs a) {

@@ -80,9 +80,10 @@ struct AttentionWork {
 };
 
 // Lays out the work; false when a size does not fit the kernels' indexes. q_starts: where each sequence's queries begin (NULL:
-// one sequence behind the other).
+// one sequence behind the other). fill: tiles that are cut give each place what it lacks of an equal share, instead of parts
+// of one length: 266 tiles of 590 on 512 places, cut in two, would fill one round and a twentieth of the next.
 bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t count, int heads, int kv_heads, int D,
-                      int causal, int cus, AttentionWork* w, const int64_t* q_starts = nullptr) {
+                      int causal, int cus, AttentionWork* w, const int64_t* q_starts = nullptr, bool fill = false) {
   const int64_t group = heads / kv_heads, limit = 0x7fffffff;
   int64_t q_rows = 0, kv_rows = 0;
   for (int64_t b = 0; b < count; ++b) {
@@ -161,11 +162,27 @@ bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t cou
       break;
     }
   }
+  const int64_t shortest = std::max((int64_t)3, (int64_t)ceil(sqrt((double)longest_cost / 11.0)));
   int64_t slots = 0;
+  std::vector<int64_t> ends;  // of a tile's parts, in key tiles
   for (size_t t = 0; t < tiles.size(); ++t) {
     const Piece& p = tiles[t];
-    const int64_t parts = t < whole ? 1 : std::max((p.cost + part - 1) / part, (int64_t)1);
-    if (parts == 1) {
+    ends.clear();
+    if (fill && t >= whole) {
+      for (int64_t at = 0; at < p.cost;) {
+        int64_t n = std::max(share - load.front(), shortest);
+        if (p.cost - at - n < shortest) n = p.cost - at;
+        std::pop_heap(load.begin(), load.end(), less);
+        load.back() += n;
+        std::push_heap(load.begin(), load.end(), less);
+        ends.push_back(at += n);
+      }
+    } else {
+      const int64_t n = t < whole ? 1 : std::max((p.cost + part - 1) / part, (int64_t)1);
+      for (int64_t i = 1; i <= n; ++i) ends.push_back(p.cost * i / n);
+    }
+    const int64_t parts = (int64_t)ends.size();
+    if (parts <= 1) {
       w->items.push_back(p.item);
       continue;
     }
@@ -174,12 +191,16 @@ bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t cou
     w->joins.push_back(j);
     for (int64_t i = 0; i < parts; ++i) {
       hf::AttentionItem it = p.item;
-      it.key_lo = (int32_t)(p.cost * i / parts * hf::kAtKeys);
-      it.key_hi = (int32_t)std::min(p.cost * (i + 1) / parts * hf::kAtKeys, (int64_t)p.item.key_hi);
+      it.key_lo = (int32_t)((i > 0 ? ends[i - 1] : 0) * hf::kAtKeys);
+      it.key_hi = (int32_t)std::min(ends[i] * hf::kAtKeys, (int64_t)p.item.key_hi);
       it.slot = (int32_t)slots++;
       w->items.push_back(it);
     }
   }
+  if (fill)  // the longest first, as places take them
+    std::stable_sort(w->items.begin(), w->items.end(), [](const hf::AttentionItem& x, const hf::AttentionItem& y) {
+      return x.key_hi - x.key_lo > y.key_hi - y.key_lo;
+    });
   memset(&w->head, 0, sizeof(w->head));
   w->head.magic = kAttentionMagic;
   w->head.heads = heads, w->head.kv_heads = kv_heads, w->head.D = D, w->head.causal = causal != 0;

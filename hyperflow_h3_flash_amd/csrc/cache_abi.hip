@@ -149,7 +149,7 @@ int cache_layout(const int64_t* q_lens, const int64_t* kv_lens, const int64_t* n
   h.magic = kCacheMagic;
   if (!wide_q.empty()) {
     if (!attention_layout(wide_q.data(), wide_kv.data(), (int64_t)wide_q.size(), heads, kv_heads, D, causal, cus,
-                          &w->attention, wide_q0.data()))
+                          &w->attention, wide_q0.data(), true))
       return HF_ERR_SIZE;
     h.attention_bytes = w->attention.head.bytes;
   }
@@ -251,22 +251,31 @@ int launch_cached_blocks(const hf::CachedArgs& a, const CacheHeader& h, hipStrea
   return h.row_blocks > 1 ? launch_cached<T, 2>(a, h, stream) : launch_cached<T, 1>(a, h, stream);
 }
 
-template <class T, bool WIDE>
-void launch_norm(const hf::NormArgs& a, hipStream_t stream) {
-  // Waves of a row by its width, so that a lane holds up to four chunks of 8 channels.
+template <class T, bool WIDE, bool VF32, bool Y, int W, int NV>
+void launch_norm_rows(const hf::NormArgs& a, hipStream_t stream) {
+  constexpr int kWaves = hf::norm_waves(W), kRows = kWaves / W;
+  const dim3 grid((unsigned)((a.T + kRows - 1) / kRows));
+  hipLaunchKernelGGL((hf::residual_norm_kernel<T, WIDE, VF32, Y, W, NV>), grid, dim3(64 * kWaves), 0, stream, a);
+}
+
+template <class T, bool WIDE, bool VF32, bool Y>
+void launch_norm_width(const hf::NormArgs& a, hipStream_t stream) {
+  // Waves of a row by its width, two or three chunks of 8 channels a lane.
   const int chunks = a.C / 8;
-#define HF_NORM(W, NV)                                                                                          \
-  hipLaunchKernelGGL((hf::residual_norm_kernel<T, WIDE, W, NV>), dim3((unsigned)((a.T + (W > 1 ? 1 : 4) - 1) / (W > 1 ? 1 : 4))), \
-                     dim3(W > 4 ? 64 * W : 256), 0, stream, a)
-  if (chunks <= 64) HF_NORM(1, 1);
-  else if (chunks <= 128) HF_NORM(1, 2);
-  else if (chunks <= 256) HF_NORM(4, 1);
-  else if (chunks <= 512) HF_NORM(4, 2);
-  else if (chunks <= 768) HF_NORM(4, 3);
-  else if (chunks <= 1024) HF_NORM(4, 4);
-  else if (chunks <= 1536) HF_NORM(8, 3);
-  else HF_NORM(8, 4);
-#undef HF_NORM
+  if (chunks <= 64) launch_norm_rows<T, WIDE, VF32, Y, 1, 1>(a, stream);
+  else if (chunks <= 128) launch_norm_rows<T, WIDE, VF32, Y, 1, 2>(a, stream);
+  else if (chunks <= 256) launch_norm_rows<T, WIDE, VF32, Y, 2, 2>(a, stream);
+  else if (chunks <= 512) launch_norm_rows<T, WIDE, VF32, Y, 4, 2>(a, stream);
+  else if (chunks <= 768) launch_norm_rows<T, WIDE, VF32, Y, 4, 3>(a, stream);
+  else if (chunks <= 1024) launch_norm_rows<T, WIDE, VF32, Y, 8, 2>(a, stream);
+  else if (chunks <= 1536) launch_norm_rows<T, WIDE, VF32, Y, 8, 3>(a, stream);
+  else launch_norm_rows<T, WIDE, VF32, Y, 16, 2>(a, stream);
+}
+
+template <class T, bool VF32>
+void launch_norm(const hf::NormArgs& a, bool wide, hipStream_t stream) {
+  if (wide) a.y ? launch_norm_width<T, true, VF32, true>(a, stream) : launch_norm_width<T, true, VF32, false>(a, stream);
+  else a.y ? launch_norm_width<T, false, VF32, true>(a, stream) : launch_norm_width<T, false, VF32, false>(a, stream);
 }
 
 }  // namespace
@@ -458,11 +467,17 @@ int hf_residual_norm(const hf_residual_norm_args* p) {
   a.gate = p->gate, a.scale = p->scale, a.shift = p->shift, a.post_weight = p->post_weight, a.weight = p->weight;
   a.group = p->group, a.ldx = p->ldx, a.ldy = p->ldy, a.ldr = p->ldr, a.ldn = p->ldn;
   a.ld_gate = p->ld_gate, a.ld_scale = p->ld_scale, a.ld_shift = p->ld_shift;
-  a.T = p->T, a.C = p->C, a.post = p->post, a.norm = p->norm, a.per_row = p->per_row, a.vectors_f32 = p->vectors_f32;
+  a.T = p->T, a.C = p->C, a.post = p->post, a.norm = p->norm, a.per_row = p->per_row;
   a.residual = p->residual, a.eps = p->eps;
+  // Results that the Infinity Cache (256 MiB) does not hold go past it (r and n of 37710 rows, us: of 5376 channels 284 ->
+  // 278, of 2048 110 -> 107, of 1024, which it holds, 58.5 -> 61.7).
+  a.stream = ((p->y ? (p->wide ? 4 : 2) : 0) + (p->n ? 2 : 0)) * p->T * p->C > (int64_t)256 << 20;
   hipStream_t stream = (hipStream_t)p->stream;
-  if (p->dtype == HF_BF16) p->wide ? launch_norm<hf::Bf16, true>(a, stream) : launch_norm<hf::Bf16, false>(a, stream);
-  else p->wide ? launch_norm<hf::Fp16, true>(a, stream) : launch_norm<hf::Fp16, false>(a, stream);
+  const bool wide = p->wide != 0;
+  if (p->dtype == HF_BF16)
+    p->vectors_f32 ? launch_norm<hf::Bf16, true>(a, wide, stream) : launch_norm<hf::Bf16, false>(a, wide, stream);
+  else
+    p->vectors_f32 ? launch_norm<hf::Fp16, true>(a, wide, stream) : launch_norm<hf::Fp16, false>(a, wide, stream);
   return launch_status();
 }
 

@@ -51,16 +51,6 @@ __device__ __forceinline__ v4f ca_mfma(v4u a, v4u b, v4f c, Fp16) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), c, 0, 0, 0);
 }
 
-// Over the four lanes of a row.
-__device__ __forceinline__ float quad_max(float v) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return half_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
-}
-__device__ __forceinline__ float quad_sum(float v) {
-  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return half_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
-}
-
 template <class T, int G, int R>
 __global__ __launch_bounds__(64 * kCaWaves, R > 1 ? 2 : G > 2 ? 3 : 4) void cached_rows_kernel(CachedArgs a) {
   constexpr int PITCH = ca_pitch(G);
