@@ -37,9 +37,17 @@ int cache_sizes(int32_t kv_heads, int32_t D, int32_t page) {
 
 int64_t cache_page_bytes(const CacheHeader& h) { return h.kv_heads * hf::kv_slab(cache_groups(h.D), h.page); }
 
-// Rows of a sequence's key head up to which it is computed on the pages; more rows are worth the keys and values expanded
-// to a workspace for attention_kernel.
-constexpr int64_t kCachedRows = 64;
+// Which sequences have their keys and values expanded to a workspace for attention_kernel, which multiplies about twice as
+// fast as the kernel on the pages (that makes codes values anew for every 32 rows): those of many rows a key head, if their
+// products together are worth the expansion and its launches. us, on the pages and expanded, 32 / 8 heads of 128: 600 rows x
+// 16000 keys 74 and 71, 800 105 and 87, 1200 141 and 110; 8 x 800 x 4000 158 and 166, 8 x 1200 218 and 189; but 2000 x 1000
+// 17 and 30, 2000 x 4000 50 and 53. 16 heads of 64: 200 x 16000 44 and 46, 400 77 and 64; 800 x 1000 11 and 24.
+constexpr int64_t cache_wide_rows(int D) { return D > 64 ? 640 : 320; }
+constexpr double kWidePairs = 64 << 20;  // of rows and keys, over the key heads
+// Values of the keys of the other sequences up to which they are expanded too where some are: the kernel on the pages and its
+// join would be two launches more, one behind the other (4096, 8191 keys expanded beside 733 and 2500, 8 heads of 128: 124 us
+// with those on the pages, 108 with all expanded).
+constexpr int64_t kWideRest = 6 << 20;
 
 struct CacheWork {
   CacheHeader head;
@@ -77,6 +85,13 @@ int cache_layout(const int64_t* q_lens, const int64_t* kv_lens, const int64_t* n
     table += n;
   }
   w->tables.assign(pages, pages + table);
+  double pairs = 0;
+  int64_t rest = 0;
+  for (int64_t b = 0; b < count; ++b)
+    if (q_lens[b] * group >= cache_wide_rows(D)) pairs += (double)(q_lens[b] * group) * kv_lens[b] * kv_heads;
+    else rest += kv_lens[b];
+  const bool all = rest <= kWideRest / ((int64_t)kv_heads * D);
+  const int64_t direct_rows = pairs < kWidePairs ? limit : all ? 0 : cache_wide_rows(D) - 1;  // of a sequence on its pages
 
   struct Tile {
     hf::CachedItem item;
@@ -86,7 +101,7 @@ int cache_layout(const int64_t* q_lens, const int64_t* kv_lens, const int64_t* n
   // read and made values of once.
   int64_t most = 0;
   for (int64_t b = 0; b < count; ++b)
-    if (q_lens[b] * group <= kCachedRows) most = std::max(most, q_lens[b] * group);
+    if (q_lens[b] * group <= direct_rows) most = std::max(most, q_lens[b] * group);
   const int row_blocks = most > hf::kCaRows ? 2 : 1, tile_rows = hf::kCaRows * row_blocks;
   std::vector<Tile> tiles;
   std::vector<int64_t> wide_q, wide_kv, wide_q0;
@@ -97,7 +112,7 @@ int cache_layout(const int64_t* q_lens, const int64_t* kv_lens, const int64_t* n
     const int32_t* mine = w->tables.data() + table;
     cache_segments(&w->reads, mine, page, 0, nk, k0);
     cache_segments(&w->writes, mine, page, nk - new_lens[b], nk, n0);
-    if (nq * group > kCachedRows) {
+    if (nq * group > direct_rows) {
       cache_segments(&w->wides, mine, page, 0, nk, wide_rows);
       wide_q.push_back(nq), wide_kv.push_back(nk), wide_q0.push_back(q0);
       wide_rows += nk;
@@ -121,13 +136,38 @@ int cache_layout(const int64_t* q_lens, const int64_t* kv_lens, const int64_t* n
     table += (nk + page - 1) / page;
   }
   std::stable_sort(tiles.begin(), tiles.end(), [](const Tile& x, const Tile& y) { return x.cost > y.cost; });
-  // Parts of equal length: as many as the device takes at a time, and four blocks (one a wave) or more each.
-  const int64_t places = 2 * (int64_t)cus;
-  const int64_t part = std::max((total + places - 1) / places, (int64_t)hf::kCaWaves);
+  // A tile of n blocks is cut into parts of about `part` blocks: no shorter than sqrt(n), where a wave's steps and the join's
+  // reads take about as long (30000 keys, 32 / 8 heads: parts of 15 17.2 us, 30 15.0, 64 20.8). Up to kWhole blocks it is not
+  // cut, for the join's launch costs as much (700 keys 8.6 us against 12.6). Of the lengths that make one to three parts a
+  // compute unit, that with the soonest end: if each unit takes the longest part left (a start costs about kStart blocks),
+  // and a join its tile's shares (four cost about a block). 131072 keys, 64 / 8 heads: one part a unit 32.9 us, one and a
+  // quarter 38.8, two 34.7; 16 caches of 1 to 16384 keys, 32 / 8 heads: one 23.5, one and three quarters 21.9, two 25.2.
+  constexpr int64_t kWhole = 32, kStart = 8;
+  const int64_t longest = tiles.empty() ? 0 : tiles[0].cost;
+  const auto less = [](int64_t x, int64_t y) { return x > y; };
+  const auto parts_of = [&](int64_t cost, int64_t part) { return cost <= kWhole ? 1 : (cost + part - 1) / part; };
+  int64_t part = std::max(longest, (int64_t)1), best = -1;
+  for (int quarters = 4; quarters <= 12 && longest > kWhole; ++quarters) {
+    const int64_t n = std::max({(4 * total + quarters * (int64_t)cus - 1) / (quarters * (int64_t)cus),
+                                (int64_t)ceil(sqrt((double)longest)), (int64_t)2 * hf::kCaWaves});
+    std::vector<int64_t> costs, units((size_t)cus, 0);
+    for (const Tile& t : tiles) {
+      const int64_t parts = parts_of(t.cost, n);
+      costs.insert(costs.end(), (size_t)parts, (t.cost + parts - 1) / parts + kStart);
+    }
+    std::sort(costs.begin(), costs.end(), less);
+    for (int64_t c : costs) {
+      std::pop_heap(units.begin(), units.end(), less);
+      units.back() += c;
+      std::push_heap(units.begin(), units.end(), less);
+    }
+    const int64_t end = *std::max_element(units.begin(), units.end()) + parts_of(longest, n) / 4;
+    if (best < 0 || end < best) best = end, part = n;
+  }
   int64_t slots = 0;
   int32_t join_rows = 0;
   for (const Tile& t : tiles) {
-    const int64_t parts = std::max((t.cost + part - 1) / part, (int64_t)1);
+    const int64_t parts = parts_of(t.cost, part);
     if (parts == 1) {
       w->items.push_back(t.item);
       continue;
@@ -144,6 +184,9 @@ int cache_layout(const int64_t* q_lens, const int64_t* kv_lens, const int64_t* n
       w->items.push_back(it);
     }
   }
+  std::stable_sort(w->items.begin(), w->items.end(), [](const hf::CachedItem& x, const hf::CachedItem& y) {
+    return x.key_hi - x.key_lo > y.key_hi - y.key_lo;
+  });
   CacheHeader& h = w->head;
   memset(&h, 0, sizeof(h));
   h.magic = kCacheMagic;

@@ -48,53 +48,71 @@ struct CacheWriteArgs {
 
 constexpr int kCacheThreads = 256;
 
-// A workgroup takes one segment and head. Four lanes share a group of a token (16 bytes of input and 4 of codes each);
+// Groups that a workgroup takes side by side, and the tokens of one round of it (fours of lanes over both).
+constexpr int kv_side(int groups) { return groups == 3 ? 4 : groups; }
+constexpr int kv_round(int groups) { return kCacheThreads / 4 / kv_side(groups); }
+
+// HBM-bound, and short: a workgroup takes up to kCacheRounds rounds of a segment's tokens of one head, and every load of them
+// is on its way before the first is used. Four lanes share a group of a token (16 bytes of input and 4 of codes each);
 // neighbouring fours take neighbouring tokens, so that codes and scales go out side by side.
+constexpr int kCacheRounds = 4;
 template <class CT, int G>
 __global__ __launch_bounds__(kCacheThreads) void cache_write_kernel(CacheWriteArgs a) {
   typedef typename CT::Type T;
-  constexpr int S = kv_scale_bytes(G);
+  constexpr int S = kv_scale_bytes(G), kTokens = kv_round(G);
   const CacheSegment seg = a.segments[blockIdx.x];
-  const int head = blockIdx.y, part = threadIdx.x & 3;
+  const int head = blockIdx.y, part = threadIdx.x & 3, four = threadIdx.x >> 2;
+  const int g = four / kTokens, c = 32 * g + 8 * part;
   unsigned char* slab = a.cache + (int64_t)seg.page * a.page_bytes + head * kv_slab(G, a.page);
-  const int quads = 2 * G * seg.rows;
-  for (int i = threadIdx.x >> 2; i < quads; i += kCacheThreads / 4) {
-    const int which = i / (G * seg.rows), j = i - which * G * seg.rows;
-    const int g = j / seg.rows, row = j - g * seg.rows, c = 32 * g + 8 * part, at = seg.first + row;
-    const uint16_t* x = a.x[which] + (seg.row0 + (int64_t)row) * a.token[which] + head * a.head[which];
-    const v4u in = c < a.D ? *(const v4u*)(x + c) : (v4u){0, 0, 0, 0};
-    float h[8], top = 0.0f;
-    bool finite = true;
+  for (int row0 = 0; row0 < seg.rows; row0 += kTokens * kCacheRounds) {
+    v4u in[kCacheRounds][2];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      h[2 * e] = T::lo(in[e]);
-      h[2 * e + 1] = T::hi(in[e]);
+    for (int i = 0; i < kCacheRounds; ++i) {
+      const int row = row0 + i * kTokens + four % kTokens;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        in[i][which] = (v4u){0, 0, 0, 0};
+        if (row < seg.rows && c < a.D)
+          in[i][which] = *(const v4u*)(a.x[which] + (seg.row0 + (int64_t)row) * a.token[which] + head * a.head[which] + c);
+      }
     }
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      top = fmaxf(top, __builtin_fabsf(h[e]));
-      finite &= __builtin_fabsf(h[e]) < __builtin_inff();
-    }
-    top = finite ? top : __builtin_inff();
+    for (int i = 0; i < kCacheRounds; ++i) {
+      const int row = row0 + i * kTokens + four % kTokens, at = seg.first + row;
 #pragma unroll
-    for (int off = 1; off <= 2; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-    finite = top < __builtin_inff();
-    // top = m 2^x with m in [0.5, 1): top <= 7 2^e from e = x - 3 on for m <= 7 / 8, else from x - 2.
-    int x2;
-    const float m = frexpf(finite ? top : 1.0f, &x2);
-    const int e2 = min(max(x2 - (m <= 0.875f ? 3 : 2), CT::kLeast), CT::kMost);
-    const float scale = __uint_as_float((uint32_t)(e2 + 127) << 23);
-    // Nearest, ties to even, saturating: compared for every 16-bit float.
-    uint32_t codes = 0;
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, h[0], h[1], scale, 0);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, h[2], h[3], scale, 1);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, h[4], h[5], scale, 2);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, h[6], h[7], scale, 3);
-    unsigned char* to = slab + which * (int64_t)G * a.page * 16;
-    *(uint32_t*)(to + ((int64_t)g * a.page + at) * 16 + 4 * part) = finite ? codes : 0u;
-    if (part == 0) {
-      unsigned char* scales = slab + 2 * G * a.page * 16 + which * S;
-      scales[at * 2 * S + g] = finite ? (unsigned char)(e2 + 127) : 255;
+      for (int which = 0; which < 2; ++which) {
+        float h[8], top = 0.0f;
+        bool finite = true;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          h[2 * e] = T::lo(in[i][which][e]);
+          h[2 * e + 1] = T::hi(in[i][which][e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          top = fmaxf(top, __builtin_fabsf(h[e]));
+          finite &= __builtin_fabsf(h[e]) < __builtin_inff();
+        }
+        top = finite ? top : __builtin_inff();
+#pragma unroll
+        for (int off = 1; off <= 2; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+        finite = top < __builtin_inff();
+        // top = m 2^x with m in [0.5, 1): top <= 7 2^e from e = x - 3 on for m <= 7 / 8, else from x - 2.
+        int x2;
+        const float m = frexpf(finite ? top : 1.0f, &x2);
+        const int e2 = min(max(x2 - (m <= 0.875f ? 3 : 2), CT::kLeast), CT::kMost);
+        const float scale = __uint_as_float((uint32_t)(e2 + 127) << 23);
+        // Nearest, ties to even, saturating: compared for every 16-bit float.
+        uint32_t codes = 0;
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, h[0], h[1], scale, 0);
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, h[2], h[3], scale, 1);
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, h[4], h[5], scale, 2);
+        codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, h[6], h[7], scale, 3);
+        if (row >= seg.rows || g >= G) continue;
+        *(uint32_t*)(slab + ((which * G + g) * a.page + at) * 16 + 4 * part) = finite ? codes : 0u;
+        if (part == 0)
+          slab[2 * G * a.page * 16 + (2 * at + which) * S + g] = finite ? (unsigned char)(e2 + 127) : 255;
+      }
     }
   }
 }
@@ -107,24 +125,36 @@ struct CacheReadArgs {
   int D, page, heads;
 };
 
-// A workgroup takes one segment and head; lanes side by side take 8 channels each of one token after the other.
+// As the writing, with lanes side by side over the channels of a token.
 template <class CT, int G>
 __global__ __launch_bounds__(kCacheThreads) void cache_read_kernel(CacheReadArgs a) {
   typedef typename CT::Type T;
-  constexpr int S = kv_scale_bytes(G);
+  constexpr int S = kv_scale_bytes(G), kTokens = kv_round(G), kLanes = 4 * kv_side(G);
   const CacheSegment seg = a.segments[blockIdx.x];
-  const int head = blockIdx.y, chunks = a.D / 8;
+  const int head = blockIdx.y, lane = threadIdx.x % kLanes, token = threadIdx.x / kLanes;
+  const int g = lane >> 2, c = 8 * lane;
+  if (c >= a.D) return;
   const unsigned char* slab = a.cache + (int64_t)seg.page * a.page_bytes + head * kv_slab(G, a.page);
-  const int n = 2 * seg.rows * chunks;
-  for (int i = threadIdx.x; i < n; i += kCacheThreads) {
-    const int which = i / (seg.rows * chunks), j = i - which * seg.rows * chunks;
-    const int row = j / chunks, c = j - row * chunks, g = c >> 2, at = seg.first + row;
-    const unsigned char* from = slab + which * (int64_t)G * a.page * 16;
-    const uint32_t codes = *(const uint32_t*)(from + ((int64_t)g * a.page + at) * 16 + 4 * (c & 3));
-    const uint32_t e = slab[2 * G * a.page * 16 + (2 * at + which) * S + g];
-    v4u out = kv_values<T>(codes, __uint_as_float((e == 255 ? 0u : e) << 23));
-    if (e == 255) out = (v4u){0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu};  // NaN in either type
-    *(v4u*)(a.out[which] + ((seg.row0 + (int64_t)row) * a.heads + head) * a.D + 8 * c) = out;
+  for (int row0 = 0; row0 < seg.rows; row0 += kTokens * kCacheRounds) {
+    uint32_t codes[kCacheRounds][2], e[kCacheRounds][2];
+#pragma unroll
+    for (int i = 0; i < kCacheRounds; ++i) {
+      const int row = row0 + i * kTokens + token, at = seg.first + min(row, seg.rows - 1);
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        codes[i][which] = *(const uint32_t*)(slab + ((which * G + g) * a.page + at) * 16 + 4 * (lane & 3));
+        e[i][which] = slab[2 * G * a.page * 16 + (2 * at + which) * S + g];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kCacheRounds; ++i) {
+      const int row = row0 + i * kTokens + token;
+      if (row >= seg.rows) return;
+#pragma unroll
+      for (int which = 0; which < 2; ++which)  // a scale byte of 255 gives NaN
+        *(v4u*)(a.out[which] + ((seg.row0 + (int64_t)row) * a.heads + head) * a.D + c) =
+            kv_values<T>(codes[i][which], __uint_as_float(e[i][which] << 23));
+    }
   }
 }
 

@@ -371,7 +371,8 @@ def parts(raw):
 @pytest.mark.parametrize("q,kv,new,heads,kv_heads,causal,page", [
     ([1] * 16, [8191, 4096, 733, 1, 16384, 2500, 6001, 127, 9999, 3000, 512, 7777, 64, 12001, 1025, 5000], [1] * 16, 32, 8, 1, 64),
     ([5, 0, 300, 1, 7], [5, 9, 300, 40000, 0], [5, 0, 20, 1, 0], 8, 2, 1, 32), ([1], [131072], [0], 64, 8, 0, 256),
-    ([], [], [], 2, 1, 0, 64), ([3, 65], [0, 0], [0, 0], 2, 2, 1, 64), ([40], [3], [3], 1, 1, 1, 128), ([900], [1000], [900], 1, 1, 0, 64)])
+    ([], [], [], 2, 1, 0, 64), ([1, 800, 0, 90, 700], [50000, 60000, 5, 300, 9000], [1, 3, 0, 0, 700], 4, 2, 1, 128),
+    ([1, 800, 0, 90], [70, 60000, 5, 300], [1, 3, 0, 0], 4, 2, 1, 128), ([3, 65], [0, 0], [0, 0], 2, 2, 1, 64), ([40], [3], [3], 1, 1, 1, 128), ([900], [1000], [900], 1, 1, 0, 64)])
 def test_plan_covers_every_row_key_and_token_once(lib, q, kv, new, heads, kv_heads, causal, page, cus):
     counts = [-(-n // page) for n in kv]
     order = list(range(sum(counts)))
@@ -392,7 +393,8 @@ def test_plan_covers_every_row_key_and_token_once(lib, q, kv, new, heads, kv_hea
 
     assert rows(p["reads"]) == want([(b, (0, n)) for b, n in enumerate(kv)])
     assert rows(p["writes"]) == want([(b, (n - m, n)) for b, (n, m) in enumerate(zip(kv, new))])
-    wide = [b for b in range(len(q)) if p["attention"] and q[b] * group > 64]
+    assert bool(p["attention"]) == (60000 in kv)
+    wide = [b for b in range(len(q)) if p["attention"] and q[b] * group >= (320 if 50000 in kv else 1)]
     assert rows(p["wides"]) == want([(b, (0, kv[b])) for b in wide])
     # items: every row of the sequences that are not expanded, over every key that its last row sees, once
     seen = {}

@@ -173,6 +173,15 @@ def test_few_and_many_rows_in_one_batch():
     run_attention([300, 1, 200], [100, 9, 0], 4, 4, 64, causal=False)
 
 
+@pytest.mark.parametrize("dtype,D,causal", [(BF, 128, True), (HF, 64, False), (HF, 96, True)])
+def test_expanded_sequences_beside_others(dtype, D, causal):
+    """Many rows over many keys go through a workspace of 16-bit keys and values, few rows of the same batch do not."""
+    for one in (300, 50000):
+        cache, plan, *_ = run_attention([2, 360, 0, 40], [one, 100001, 5, 900], 4, 2, D, dtype, causal)
+        rows = 100001 + (0 if one > 300 else 300 + 5 + 900)
+        assert 0 <= plan.ws_bytes - 2 * rows * 2 * D * 2 < 60 << 20  # shares come to less
+
+
 @pytest.mark.parametrize("causal", [False, True])
 def test_queries_without_keys_and_caches_without_queries(causal):
     for q, kv in (([5, 90], [0, 0]), ([9, 200], [3, 5]), ([0, 0], [70, 5]), ([0], [0]), ([], [])):
@@ -201,10 +210,10 @@ def test_rising_maxima_and_a_dominant_key(dtype):
     U.check(cached_attention(q, cache, 0, plan, scale=1.0), ref, bound)
 
 
-@pytest.mark.parametrize("rows", [3, 130])
-def test_unseen_nan_stays_out_and_seen_nan_shows(rows):
+@pytest.mark.parametrize("rows,kv", [(3, 200), (130, 200), (400, 90000)])
+def test_unseen_nan_stays_out_and_seen_nan_shows(rows, kv):
     """A key or value group that is not finite reaches the rows that see it and no other; on pages and expanded."""
-    kv, hq, D = 200, 2, 128
+    hq, D = 2, 128
     k, v = keys(1, kv, 1, D, BF), keys(2, kv, 1, D, BF)
     k[kv - 2, 0, 3] = float("inf")  # seen by the last two queries
     v[kv - 1, 0, 70] = float("nan")  # by the last
