@@ -1,5 +1,6 @@
 """MI355X-native INT8 "convrot" linear for HyperFlow H3 Flash: a drop-in for ``hyperflow_h3_flash.int8``, and the
-operators of an attention block around it (norms and rotation, packed attention, adapters of many requests).
+operators of a transformer block around it (norms and rotation, packed attention, adapters of many requests, keys and values
+held in 4 bits, norms with gates and residuals).
 
 Importing the package does not touch the GPU or load the HIP library; the first device forward does.
 """
@@ -23,6 +24,7 @@ from .int8 import (
 from .kv_cache import CachePlan, KVCache, cache_append, cache_read, cached_attention, copy_pages
 from .lowrank import RANK_MULTIPLE, LowRankLinear, fuse_qkv, set_lowrank_rank_multiple
 from .residual_norm import RowPlan, residual_norm
+from .transformer_block import TransformerBlock, TransformerStack
 
 __version__ = "0.1.0"
 
@@ -44,6 +46,8 @@ __all__ = [
     "RANK_MULTIPLE",
     "RotaryAxes",
     "RowPlan",
+    "TransformerBlock",
+    "TransformerStack",
     "adapter_add",
     "cache_append",
     "cache_read",

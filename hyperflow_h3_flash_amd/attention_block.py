@@ -15,6 +15,7 @@ from torch import Tensor, nn
 from .block import (AdapterPlan, AttentionPlan, RotaryAxes, _differentiable, _forward_only, adapter_add, packed_attention,
                     qk_norm_rope)
 from .int8 import Int8RotLinear
+from .kv_cache import CachePlan, cache_append, cached_attention
 from .lowrank import fuse_qkv
 
 
@@ -125,15 +126,20 @@ class AttentionBlock(nn.Module):
             block.norm_q, block.norm_k = (_frozen(w.detach().to(device)) for w in (norm_q, norm_k))
         return block
 
-    def forward(self, x: Tensor, plan: AttentionPlan, *, positions: Tensor | None = None,
-                rotary: RotaryAxes | None = None, adapters: AdapterPlan | None = None) -> Tensor:
+    def forward(self, x: Tensor, plan: AttentionPlan | CachePlan, *, positions: Tensor | None = None,
+                rotary: RotaryAxes | None = None, adapters: AdapterPlan | None = None, layer: int = 0) -> Tensor:
         """``x`` [tokens, dim] (bfloat16), the tokens of ``plan``'s sequences one behind the other; ``positions``
-        [tokens, axes] with ``rotary``; ``adapters`` names the adapter of each request's tokens. Forward only, as its
-        operators are: x that requires a gradient is refused unless gradients are off."""
+        [tokens, axes] with ``rotary``; ``adapters`` names the adapter of each request's tokens. With a `CachePlan` the
+        tokens are the new ones of its requests: their keys and values are written to layer ``layer`` of its cache, and they
+        attend to all that is held there. Forward only, as its operators are: x that requires a gradient is refused unless
+        gradients are off."""
         if _differentiable():
             _forward_only("AttentionBlock", x)
         if adapters is not None and self.qkv_adapters is None:
             raise ValueError("the block was built without adapters")
+        cached = isinstance(plan, CachePlan)
+        if cached and plan.new_lengths != plan.q_lengths:
+            raise ValueError("the block's tokens are both a step's queries and its new tokens")
         heads, kv_heads = self.heads, self.kv_heads
         qkv = self.qkv(x)
         if adapters is not None:
@@ -143,7 +149,12 @@ class AttentionBlock(nn.Module):
         if self.norm_q is not None or rotary is not None:
             qk_norm_rope(q, k, positions, rotary, q_weight=self.norm_q, k_weight=self.norm_k,
                          norm=self.norm_q is not None, eps=self.eps, out=(q, k))
-        o = packed_attention(q, k, v, plan).view(-1, heads * self.head_dim)
+        if cached:
+            cache_append(plan.cache, layer, k, v, plan)
+            o = cached_attention(q, plan.cache, layer, plan)
+        else:
+            o = packed_attention(q, k, v, plan)
+        o = o.view(-1, heads * self.head_dim)
         y = self.out(o)
         if adapters is not None:
             self.out_adapters(y, o, adapters, out=y)

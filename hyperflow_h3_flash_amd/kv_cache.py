@@ -125,7 +125,7 @@ class KVCache:
             raise ValueError(f"page_size must be one of {PAGE_SIZES}, got {page_size}")
         if pages * page_size > 0x7fffffff or kv_heads > 65535 or layers > 65535:
             raise ValueError(f"{pages} pages of {page_size} tokens, {kv_heads} heads, {layers} layers exceed the indexes")
-        _dtype_code("KVCache", dtype)
+        self._code = _dtype_code("KVCache", dtype)
         self.layers, self.kv_heads, self.head_dim, self.pages = int(layers), int(kv_heads), int(head_dim), int(pages)
         self.page_size, self.dtype = int(page_size), dtype
         self.device = _plan_device(device)
@@ -134,6 +134,7 @@ class KVCache:
         self.groups = -(-self.head_dim // host_cache.GROUP)
         self.page_bytes = self.kv_heads * host_cache.slab_bytes(self.groups, self.page_size)
         self.data = torch.zeros(self.layers, self.pages, self.page_bytes, dtype=torch.uint8, device=self.device)
+        self._sample = torch.empty(0, dtype=dtype, device=self.device)  # new tensors are made like it
         self._uses = [0] * self.pages
         self._unused = list(range(self.pages))  # a heap: the lowest page first
         self._requests: dict[int, _Request] = {}
@@ -327,7 +328,7 @@ def cache_append(cache: KVCache, layer: int, k: Tensor, v: Tensor, plan: CachePl
     with _current(cache._index, device):
         status = lib.hf_cache_append(_append_args(
             k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, address, plan.data.host_address, plan.data.on(stream), plan.bytes,
-            _dtype_code("cache_append", dtype), stream))
+            cache._code, stream))
     _check(status, "hf_cache_append")
     _written(cache.data)
 
@@ -337,10 +338,11 @@ def cache_read(cache: KVCache, layer: int, plan: CachePlan) -> tuple[Tensor, Ten
     request behind the other: what `packed_attention` takes, and what `cached_attention` computes with."""
     plan._check_good(cache, False)
     address = _layer(cache, layer)
-    k, v = (torch.empty(plan._kv_shape, dtype=cache.dtype, device=cache.device) for _ in range(2))
+    shape = plan._kv_shape
+    k, v = cache._sample.new_empty(shape), cache._sample.new_empty(shape)
     if plan.kv_rows == 0:
         return k, v
-    if not cache.data.is_cuda:
+    if cache._index < 0:
         host_cache.read(cache, layer, plan, k, v)
         return k, v
     device = cache.device
@@ -349,7 +351,7 @@ def cache_read(cache: KVCache, layer: int, plan: CachePlan) -> tuple[Tensor, Ten
     with _current(cache._index, device):
         status = lib.hf_cache_read(_read_args(
             address, k.data_ptr(), v.data_ptr(), plan.data.host_address, plan.data.on(stream), plan.bytes,
-            _dtype_code("cache_read", cache.dtype), stream))
+            cache._code, stream))
     _check(status, "hf_cache_read")
     return k, v
 
@@ -396,7 +398,7 @@ def cached_attention(q: Tensor, cache: KVCache, layer: int, plan: CachePlan, *, 
     with _current(index, device):
         status = lib.hf_cached_attention(_attend_args(
             q.data_ptr(), qt, qh, address, o.data_ptr(), ot, oh, scale, plan.data.host_address, plan.data.on(stream),
-            plan.bytes, 0 if ws is None else ws.data_ptr(), nbytes, _dtype_code("cached_attention", dtype), stream))
+            plan.bytes, 0 if ws is None else ws.data_ptr(), nbytes, cache._code, stream))
     _check(status, "hf_cached_attention")
     return o if out is None else _deliver(o, out)
 

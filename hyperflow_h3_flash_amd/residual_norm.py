@@ -52,12 +52,9 @@ def _rows(t: Tensor) -> Tensor:
     return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
 
 
-def _new_rows(t: Tensor) -> Tensor:
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
-
-
-def _ld(t: Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _new_rows(t: Tensor, dtype: torch.dtype) -> Tensor:
+    """Contiguous rows like t's, of a type (the quicker call where t is that)."""
+    return torch.empty_like(t) if t.dtype is dtype and t.is_contiguous() else t.new_empty(t.shape, dtype=dtype)
 
 
 def _place(t: Tensor) -> tuple:
@@ -78,12 +75,10 @@ def _writable(out: Tensor, inputs: list[Tensor], others: list[Tensor]) -> bool:
             and all(_apart(place, p) for p in map(_place, others)))
 
 
-def _modulation(t: Tensor | None, groups: int) -> tuple[Tensor | None, int, int]:
+def _modulation(t: Tensor) -> tuple[Tensor, int, int]:
     """A vector for all rows or one a group, as the kernel reads it: the tensor, its address and its row stride (0: one)."""
-    if t is None:
-        return None, 0, 0
     if t.dim() == 1 or t.shape[0] == 1:
-        t = _vector(t.view(-1) if t.is_contiguous() else t.reshape(-1))
+        t = _vector(t.reshape(-1))
         return t, t.data_ptr(), 0
     t = _rows(t)
     return t, t.data_ptr(), t.stride(0)
@@ -133,24 +128,25 @@ def residual_norm(x: Tensor, y: Tensor | None = None, *, rows: RowPlan | None = 
         raise ValueError(f"the plan has {rows.rows} rows, x has {T}")
     groups = T if rows is None else rows.requests
     wide = x.dtype is not kind
-    f32 = False
-    for t in (post_weight, weight):
-        if t is not None:
-            if t.shape != (C,):
-                raise ValueError(f"a weight must be [{C}], got {tuple(t.shape)}")
-            f32 |= t.dtype is not kind
-    for t in (gate, scale, shift):
-        if t is not None:
-            if t.shape != (C,) and t.shape != (1, C) and t.shape != (groups, C):
-                raise ValueError(f"gate, scale and shift must be [{C}] or [{groups}, {C}], got {tuple(t.shape)}")
-            f32 |= t.dtype is not kind
     index = x.get_device()
-    for t in (y, gate, scale, shift, post_weight, weight):
-        if t is not None:
-            if t.dtype is not kind and t.dtype is not torch.float32:
+    if y is not None and y.get_device() != index:
+        _same_device(x.device, y)
+    f32 = False
+    for t in (gate, scale, shift, post_weight, weight):
+        if t is None:
+            continue
+        if t.dtype is not kind:
+            f32 = True
+            if t.dtype is not torch.float32:
                 raise ValueError(f"vectors must be {kind} or float32, got {t.dtype}")
-            if t.get_device() != index:
-                _same_device(x.device, t)
+        shape = t.shape
+        if t is weight or t is post_weight:
+            if shape != (C,):
+                raise ValueError(f"a weight must be [{C}], got {tuple(shape)}")
+        elif shape != (groups, C) and shape != (C,) and shape != (1, C):
+            raise ValueError(f"gate, scale and shift must be [{C}] or [{groups}, {C}], got {tuple(shape)}")
+        if t.get_device() != index:
+            _same_device(x.device, t)
     if rows is not None and rows._index != index:
         raise ValueError(f"tensors on {x.device}, the plan is for {rows.device}")
     r_out = n_out = None
@@ -162,7 +158,7 @@ def residual_norm(x: Tensor, y: Tensor | None = None, *, rows: RowPlan | None = 
             _check_out(r_out, x, "residual_norm")
         if n_out is not None and (n_out.shape != x.shape or n_out.dtype is not kind or n_out.device != x.device):
             raise ValueError(f"residual_norm: out[1] must be {tuple(x.shape)} {kind} on {x.device}")
-        if r_out is not None and n_out is not None and T and r_out.data_ptr() == n_out.data_ptr():
+        if r_out is not None and n_out is not None and T and not _apart(_place(r_out), _place(n_out)):
             raise ValueError("the two results need places of their own")
     if _differentiable():
         _forward_only("residual_norm", x, y, gate, scale, shift, post_weight, weight, r_out, n_out)
@@ -180,34 +176,46 @@ def residual_norm(x: Tensor, y: Tensor | None = None, *, rows: RowPlan | None = 
     if f32:  # float32 is read as it is, and serves any mixture
         gate, scale, shift, post_weight, weight = (
             None if t is None else t.to(torch.float32) for t in (gate, scale, shift, post_weight, weight))
-    (gate, gate_at, gate_ld), (scale, scale_at, scale_ld), (shift, shift_at, shift_ld) = (
-        _modulation(t, groups) for t in (gate, scale, shift))
-    post_weight, weight = (None if t is None else _vector(t) for t in (post_weight, weight))
+    gate_at = gate_ld = scale_at = scale_ld = shift_at = shift_ld = post_at = weight_at = 0
+    y_at = y_ld = r_at = r_ld = n_at = n_ld = 0
+    if gate is not None:
+        gate, gate_at, gate_ld = _modulation(gate)
+    if scale is not None:
+        scale, scale_at, scale_ld = _modulation(scale)
+    if shift is not None:
+        shift, shift_at, shift_ld = _modulation(shift)
+    if post_weight is not None:
+        post_weight = _vector(post_weight)
+        post_at = post_weight.data_ptr()
+    if weight is not None:
+        weight = _vector(weight)
+        weight_at = weight.data_ptr()
     stream_in = x
     x = _rows(x)
     r = n = None
     if y is not None:
         y = _rows(y)
-        r = _new_rows(x) if r_out is None else _rows(r_out)
+        y_at, y_ld = y.data_ptr(), y.stride(0) if T > 1 else C
+        r = _new_rows(x, x.dtype) if r_out is None else _rows(r_out)
     if want:
-        n = torch.empty((T, C), dtype=kind, device=device) if n_out is None else _rows(n_out)
+        n = _new_rows(x if y is None else y, kind) if n_out is None else _rows(n_out)
     if out is not None:
         inputs = [x] if y is None else [x, y]
         vectors = [t for t in (gate, scale, shift, post_weight, weight) if t is not None]
         if r_out is not None and (r is not r_out or not _writable(r, inputs, vectors if n is None else [n, *vectors])):
-            r = _new_rows(x)
+            r = _new_rows(x, x.dtype)
         if n_out is not None and (n is not n_out or not _writable(n, inputs, vectors if r is None else [r, *vectors])):
-            n = torch.empty((T, C), dtype=kind, device=device)
+            n = _new_rows(x, kind)
+    if r is not None:
+        r_at, r_ld = r.data_ptr(), r.stride(0) if T > 1 else C
+    if n is not None:
+        n_at, n_ld = n.data_ptr(), n.stride(0) if T > 1 else C
     stream = _raw_stream(index)
-
     with _current(index, device):
         status = lib.hf_residual_norm(_args(
-            x.data_ptr(), _ld(x), 0 if y is None else y.data_ptr(), 0 if y is None else _ld(y),
-            0 if r is None else r.data_ptr(), 0 if r is None else _ld(r), 0 if n is None else n.data_ptr(),
-            0 if n is None else _ld(n), gate_at, gate_ld, scale_at, scale_ld, shift_at, shift_ld,
-            0 if post_weight is None else post_weight.data_ptr(), 0 if weight is None else weight.data_ptr(),
-            0 if rows is None else rows.data.on(stream), groups, T, C, NORMS[post_norm], NORMS[norm], rows is None, wide,
-            f32, code, residual, eps, stream))
+            x.data_ptr(), x.stride(0) if T > 1 else C, y_at, y_ld, r_at, r_ld, n_at, n_ld, gate_at, gate_ld, scale_at,
+            scale_ld, shift_at, shift_ld, post_at, weight_at, 0 if rows is None else rows.data.on(stream), groups, T, C, NORMS[post_norm],
+            NORMS[norm], rows is None, wide, f32, code, residual, eps, stream))
     _check(status, "hf_residual_norm")
     if r_out is not None:
         r = _deliver(r, r_out)

@@ -149,9 +149,15 @@ def test_outputs_in_place_and_strides():
     xs = x[:1].expand(70, 640)
     r, _ = residual_norm(xs, y)
     assert torch.equal(r, residual_norm(xs.contiguous(), y)[0])
+    single = residual_norm(odd[:1, 1:], y[:1], norm="layer", residual=0.5)  # one row, at any stride and start
+    assert torch.equal(single[0], want[0][:1]) and torch.equal(single[1], want[1][:1])
+    single = residual_norm(odd[:1].new_zeros(1, 649)[:, :640], y[:1, :640])
+    assert torch.equal(single[0], y[:1])
     one = torch.empty_like(x)
     with pytest.raises(ValueError, match="places of their own"):
         residual_norm(x, y, norm="layer", residual=0.5, out=(one, one.view(70, 640)))
+    with pytest.raises(ValueError, match="places of their own"):
+        residual_norm(x[:69], y[:69], norm="layer", out=(one[:69], one[1:]))
 
 
 def test_a_tensor_past_2_31_elements():
