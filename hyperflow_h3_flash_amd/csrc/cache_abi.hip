@@ -187,6 +187,9 @@ int cache_layout(const int64_t* q_lens, const int64_t* kv_lens, const int64_t* n
   std::stable_sort(w->items.begin(), w->items.end(), [](const hf::CachedItem& x, const hf::CachedItem& y) {
     return x.key_hi - x.key_lo > y.key_hi - y.key_lo;
   });
+  for (hf::CachedItem& it : w->items)
+    for (int i = 0; i < hf::kCaWaves; ++i)
+      if (it.key_lo + i * hf::kCaKeys < it.key_hi) it.first[i] = w->tables[it.table0 + (it.key_lo + i * hf::kCaKeys) / page];
   CacheHeader& h = w->head;
   memset(&h, 0, sizeof(h));
   h.magic = kCacheMagic;

@@ -20,8 +20,10 @@ namespace hf {
 
 constexpr int kCaRows = 16, kCaWaves = 4, kCaKeys = 32;  // of a block of rows, of a workgroup, of a step
 
+// As AttentionItem; table0: where the sequence's pages begin among all; first: the page of each wave's first block (one load
+// less one behind the other at a workgroup's start).
 struct CachedItem {
-  int32_t q0, nq, nk, row0, key_lo, key_hi, head, slot, table0, pad[3];
+  int32_t q0, nq, nk, row0, key_lo, key_hi, head, slot, table0, first[kCaWaves], pad[3];
 };
 struct CachedJoin {
   int32_t q0, nq, nk, row0, head, slot0, slots, rows;
@@ -63,6 +65,7 @@ __global__ __launch_bounds__(64 * kCaWaves, R > 1 ? 2 : G > 2 ? 3 : 4) void cach
   const CachedItem it = a.items[blockIdx.x];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int sub = lane & 15, quarter = lane >> 4;
+  const int first_page = a.items[blockIdx.x].first[wave];  // (as it.first[wave] the whole item would go through memory)
   // The group of the lane's channels, and the dword of its codes where they begin.
   const int g = G > 2 ? min(quarter, G - 1) : G == 2 ? quarter >> 1 : 0;
   const int dword = G > 2 ? 0 : G == 2 ? 2 * (quarter & 1) : quarter;
@@ -249,7 +252,7 @@ __global__ __launch_bounds__(64 * kCaWaves, R > 1 ? 2 : G > 2 ? 3 : 4) void cach
     for (int x = 0; x < G; ++x) nan_from[x] = 0x7fffffff;
     if (wave >= blocks) return;
     Block b[2];
-    load(key_of(wave), page_of(wave), b[0]);
+    load(key_of(wave), first_page, b[0]);
     int page = page_of(wave + kCaWaves);
 #pragma unroll 1
     for (int i = wave;;) {
@@ -354,32 +357,53 @@ __global__ __launch_bounds__(64 * kJoinRows) void cached_join_kernel(CachedArgs 
   const int64_t step = ca_slot_floats(G, R);
   const float* part = a.ws + (int64_t)j.slot0 * step;
   const float* stat = part + kCaRows * R * 32 * G + 2 * r;
-  float top = -__builtin_inff();
-  for (int s = lane; s < j.slots; s += 64) top = fmaxf(top, stat[s * step]);
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-  float l = 0.0f, o[8];
+  // One pass: each group of lanes sums its shares to a maximum of its own, then the four are joined.
+  float top = -__builtin_inff(), l = 0.0f, o[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] = 0.0f;
   const bool inside = d < 32 * G;
-#pragma unroll 4
-  for (int s = group; s < j.slots; s += 4) {
-    const v2f ml = *(const v2f*)(stat + s * step);
-    const float* p = part + s * step + r * 32 * G + (inside ? d : 0);
-    const v4f x = *(const v4f*)p, y = *(const v4f*)(p + 4);
-    const float f = ml[0] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((ml[0] - top) * a.scale_log2);
-    l = fmaf(ml[1], f, l);
+  constexpr int kAtOnce = 4;
+  for (int s0 = group; s0 < j.slots; s0 += 4 * kAtOnce) {
+    v2f ml[kAtOnce];
+    v4f x[kAtOnce], y[kAtOnce];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      o[e] = fmaf(x[e], f, o[e]);
-      o[4 + e] = fmaf(y[e], f, o[4 + e]);
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int64_t s = min(s0 + 4 * i, j.slots - 1);
+      const float* p = part + s * step + r * 32 * G + (inside ? d : 0);
+      ml[i] = *(const v2f*)(stat + s * step);
+      x[i] = *(const v4f*)p;
+      y[i] = *(const v4f*)(p + 4);
+    }
+    float next = top;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (s0 + 4 * i >= j.slots) ml[i] = (v2f){-__builtin_inff(), 0.0f};
+      next = fmaxf(next, ml[i][0]);
+    }
+    // A share whose keys the row does not see has m = -inf and adds nothing.
+    const float f0 = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((top - next) * a.scale_log2);
+    top = next;
+    l *= f0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e] *= f0;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (ml[i][0] == -__builtin_inff()) continue;
+      const float f = __builtin_amdgcn_exp2f((ml[i][0] - top) * a.scale_log2);
+      l = fmaf(ml[i][1], f, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o[e] = fmaf(x[i][e], f, o[e]);
+        o[4 + e] = fmaf(y[i][e], f, o[4 + e]);
+      }
     }
   }
+  {
+    const float all = quad_max(top);
+    const float f = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((top - all) * a.scale_log2);
+    l = quad_sum(top == -__builtin_inff() ? 0.0f : l * f);
 #pragma unroll
-  for (int off = 16; off <= 32; off <<= 1) {
-    l += __shfl_xor(l, off, 64);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] += __shfl_xor(o[e], off, 64);
+    for (int e = 0; e < 8; ++e) o[e] = quad_sum(top == -__builtin_inff() ? 0.0f : o[e] * f);
   }
   if (group != 0 || d >= a.D) return;
   const int last = a.causal ? min(token + j.nk - j.nq, j.nk - 1) : j.nk - 1;

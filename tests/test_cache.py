@@ -361,7 +361,7 @@ def parts(raw):
     at = dict(zip("items joins tables reads writes wides attention attention_bytes".split(), struct.unpack_from("8q", raw, 96)))
     grid = lambda name, n, width: np.frombuffer(raw, np.int32, n * width, at[name]).reshape(n, width)
     rows, = struct.unpack_from("i", raw, 168)
-    return {"rows": 16 * rows, "slots": slots, "join_rows": join_rows, "items": grid("items", items, 12), "joins": grid("joins", joins, 8),
+    return {"rows": 16 * rows, "slots": slots, "join_rows": join_rows, "items": grid("items", items, 16), "joins": grid("joins", joins, 8),
             "reads": grid("reads", reads, 4), "writes": grid("writes", writes, 4), "wides": grid("wides", wides, 4),
             "tables": np.frombuffer(raw, np.int32, (at["reads"] - at["tables"]) // 4, at["tables"]),
             "attention": raw[at["attention"]:at["attention"] + at["attention_bytes"]]}
@@ -404,6 +404,7 @@ def test_plan_covers_every_row_key_and_token_once(lib, q, kv, new, heads, kv_hea
         b = next(b for b in range(len(q)) if q0[b] == a and q[b] == nq and sum(counts[:b]) == table0 and kv[b] == nk and q[b])
         assert b not in wide and lo % 32 == 0 and 0 <= lo <= hi <= nk and (hi % 32 == 0 or hi <= nk)
         seen.setdefault((b, head, row0), []).append((lo, hi, slot))
+        assert all(item[9 + i] == tables[b][key // page] for i, key in enumerate(range(lo, min(hi, lo + 128), 32)))
     slots = []
     for b in range(len(q)):
         if b in wide:
