@@ -147,7 +147,8 @@ int cache_layout(const int64_t* q_lens, const int64_t* kv_lens, const int64_t* n
   const auto less = [](int64_t x, int64_t y) { return x > y; };
   const auto parts_of = [&](int64_t cost, int64_t part) { return cost <= kWhole ? 1 : (cost + part - 1) / part; };
   int64_t part = std::max(longest, (int64_t)1), best = -1;
-  for (int quarters = 4; quarters <= 12 && longest > kWhole; ++quarters) {
+  // With many tiles a unit their order evens them out, and only long ones are cut.
+  for (int quarters = tiles.size() > (size_t)8 * cus ? 12 : 4; quarters <= 12 && longest > kWhole; ++quarters) {
     const int64_t n = std::max({(4 * total + quarters * (int64_t)cus - 1) / (quarters * (int64_t)cus),
                                 (int64_t)ceil(sqrt((double)longest)), (int64_t)2 * hf::kCaWaves});
     std::vector<int64_t> costs, units((size_t)cus, 0);

@@ -3,6 +3,7 @@ definitions in float64, rounded once, and the same bytes in the pages."""
 
 from __future__ import annotations
 
+from collections.abc import Sequence
 from types import SimpleNamespace
 
 import torch
@@ -61,10 +62,10 @@ def _views(cache, layer: int) -> tuple[Tensor, Tensor]:
     return (slabs[..., :2 * G * P * 16].unflatten(-1, (2, G, P, 16)), slabs[..., 2 * G * P * 16:].unflatten(-1, (P, 2, S)))
 
 
-def _slots(cache, table: list[int], first: int, last: int) -> tuple[Tensor, Tensor]:
+def _slots(cache, table: Sequence[int], first: int, last: int) -> tuple[Tensor, Tensor]:
     """(page, place in it) of a request's tokens first .. last - 1."""
     at = torch.arange(first, last)
-    return torch.tensor(table, dtype=torch.int64)[at // cache.page_size], at % cache.page_size
+    return torch.tensor(list(table), dtype=torch.int64)[at // cache.page_size], at % cache.page_size
 
 
 def append(cache, layer: int, k: Tensor, v: Tensor, plan) -> None:

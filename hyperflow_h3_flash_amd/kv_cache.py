@@ -20,6 +20,7 @@ from __future__ import annotations
 import ctypes
 import heapq
 import math
+from array import array
 from collections.abc import Sequence
 
 import torch
@@ -27,8 +28,8 @@ from torch import Tensor
 
 from . import _native, host_cache
 from .block import (_array, _check_out, _current, _deliver, _differentiable, _dtype_code, _FLOAT_MAX, _forward_only, _heads,
-                    _lengths, _lib, _new_like, _Plan, _plan_device, _result, _written)
-from .int8 import _check, _raw_stream, _same_device
+                    _lengths, _lib, _new_like, _plan_device, _Resident, _result, _written)
+from .int8 import _check, _on, _raw_stream, _same_device
 
 PAGE_SIZES = (32, 64, 128, 256)
 _append_args, _read_args, _attend_args, _copy_args = (s.pack for s in (
@@ -42,17 +43,19 @@ class _Request:
     __slots__ = ("length", "table", "moved", "shared")
 
     def __init__(self, length: int = 0, table: Sequence[int] = ()) -> None:
-        self.length, self.table, self.moved, self.shared = length, list(table), 0, 0
+        self.length, self.table, self.moved, self.shared = length, array("i", table), 0, 0
 
 
-class CachePlan(_Plan):
+class CachePlan:
     """One step of a batch over a `KVCache`, for its operators in every layer (`KVCache.plan` builds it): ``q_lengths``
     queries, ``kv_lengths`` tokens in the cache and ``new_lengths`` of them written in this step, by request.
 
     A plan stays good while its requests keep their pages and tokens: longer requests do no harm, `KVCache.truncate`, `free`
     and a `compact` that moves their pages end it, and after a `fork` it writes no more. What was ended is refused."""
 
-    def __init__(self, cache: "KVCache", requests: Sequence[_Request], tables: list[list[int]], q_lengths: list[int],
+    _ROOM = 1 << 18
+
+    def __init__(self, cache: "KVCache", requests: Sequence[_Request], tables: list[array], q_lengths: list[int],
                  kv_lengths: list[int], new_lengths: list[int], heads: int, causal: bool) -> None:
         self.cache, self.device, self._index = cache, cache.device, cache._index
         self.q_lengths, self.kv_lengths, self.new_lengths, self.tables = q_lengths, kv_lengths, new_lengths, tables
@@ -70,10 +73,22 @@ class CachePlan(_Plan):
     def _lay_out(self, lib: ctypes.CDLL, cus: int) -> None:
         cache = self.cache
         q, kv, new = (_array(ctypes.c_int64, n) for n in (self.q_lengths, self.kv_lengths, self.new_lengths))
-        pages = _array(ctypes.c_int32, [p for table in self.tables for p in table])
-        self._fill("hf_cache_plan", lib, self.device, ctypes.addressof(q), ctypes.addressof(kv), ctypes.addressof(new),
-                   len(self.q_lengths), ctypes.addressof(pages), cache.pages, cache.page_size, self.heads, self.kv_heads,
-                   self.head_dim, self.causal, cus)
+        pages = array("i", b"".join(map(bytes, self.tables)) or bytes(4))
+        args = (ctypes.addressof(q), ctypes.addressof(kv), ctypes.addressof(new), len(self.q_lengths),
+                pages.buffer_info()[0], cache.pages, cache.page_size, self.heads, self.kv_heads, self.head_dim, self.causal,
+                cus)
+        # A plan a step: laid out once into room that holds most, not first for its size.
+        host = torch.empty(self._ROOM, dtype=torch.uint8)
+        size = lib.hf_cache_plan(*args, host.data_ptr(), self._ROOM)
+        if size < 0:
+            size = lib.hf_cache_plan(*args, None, 0)
+            _check(min(size, 0), "hf_cache_plan")
+            host = torch.empty(size, dtype=torch.uint8)
+            size = lib.hf_cache_plan(*args, host.data_ptr(), size)
+            _check(min(size, 0), "hf_cache_plan")
+        with _on(self.device):
+            self.data = _Resident(host[:size].clone(), self.device)
+        self.bytes = size
         self.ws_bytes = lib.hf_cache_ws_bytes(self.data.host_address, self.bytes)
 
     def _start(self) -> None:
@@ -216,7 +231,7 @@ class KVCache:
             to = dict(zip(src, dst))
             for request in self._requests.values():
                 if any(p in to for p in request.table):
-                    request.table = [to.get(p, p) for p in request.table]
+                    request.table = array("i", [to.get(p, p) for p in request.table])
                     request.moved += 1
             for a, b in to.items():
                 self._uses[b], self._uses[a] = self._uses[a], 0
@@ -246,7 +261,7 @@ class KVCache:
         given: dict[int, int] = {}  # uses that the step takes from shared pages
         tables, copies, need = [], [], 0
         for r, n in zip(found, new):
-            table = list(r.table)
+            table = r.table[:]
             if n and r.length % P:
                 page = table[-1]
                 if self._uses[page] - given.get(page, 0) > 1:
@@ -267,7 +282,7 @@ class KVCache:
             tables[i][0][j] = fresh[at]
             at += 1
         for table, grow in tables:
-            table += fresh[at:at + grow]
+            table.extend(fresh[at:at + grow])
             at += grow
         plan = CachePlan(self, found, [table for table, _ in tables], q, [r.length + n for r, n in zip(found, new)], new,
                          heads, bool(causal))
@@ -285,7 +300,7 @@ class KVCache:
             self._changes += 1
         for r, n, (table, _) in zip(found, new, tables):
             if n:
-                r.table, r.length = list(table), r.length + n
+                r.table, r.length = table[:], r.length + n
         plan._start()
         return plan
 
@@ -431,6 +446,8 @@ def copy_pages(pool: Tensor, src: Sequence[int], dst: Sequence[int]) -> Tensor:
             pool[:, list(dst)] = pool[:, list(src)]
         return pool
     n = len(src)
+    if n and not (0 <= min(src) and max(src) < pages and 0 <= min(dst) and max(dst) < pages):
+        raise ValueError(f"pages must be 0 .. {pages - 1}")
     try:
         a, b = (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst)
     except TypeError as exc:
