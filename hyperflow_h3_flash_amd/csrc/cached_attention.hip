@@ -46,6 +46,15 @@ struct CachedArgs {
 __host__ __device__ constexpr int ca_slot_floats(int groups, int blocks) { return kCaRows * blocks * (32 * groups + 2); }
 __host__ __device__ constexpr int ca_pitch(int groups) { return groups > 2 ? 256 : 128; }
 
+// Chunk c (16 bytes) of row r lies at c ^ f(r): 16 rows' same chunk, as it is written, and two chunks of rows 4 q .. 4 q + 3
+// for the two quarters q that the transposing read takes at a time touch every bank once (with at_swizzle, whose halves read
+// other chunks, each such read takes two turns).
+template <int PITCH>
+__device__ __forceinline__ int ca_swizzle(int r) {
+  const int q = ((r >> 1) & 2) | ((r >> 3) & 1);
+  return PITCH == 256 ? ((r & 3) << 2) | q : (((r >> 1) & 1) << 2) | q;
+}
+
 __device__ __forceinline__ v4f ca_mfma(v4u a, v4u b, v4f c, Bf16) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
 }
@@ -133,11 +142,11 @@ __global__ __launch_bounds__(64 * kCaWaves, R > 1 ? 2 : G > 2 ? 3 : 4) void cach
   };
 
   unsigned char HF_LDS* tile = (unsigned char HF_LDS*)ca_mem + wave * kTile;
-  const uint32_t vwrite = (uint32_t)(sub * PITCH + (((W * quarter) ^ at_swizzle<PITCH>(sub)) * 16));
+  const uint32_t vwrite = (uint32_t)(sub * PITCH + (((W * quarter) ^ ca_swizzle<PITCH>(sub)) * 16));
   uint32_t vread;
   {
     const int r = 4 * quarter + (sub >> 2), ch = (lane & 3) >> 1;
-    vread = (uint32_t)(r * PITCH + ((ch ^ at_swizzle<PITCH>(r)) * 16) + (lane & 1) * 8);
+    vread = (uint32_t)(r * PITCH + ((ch ^ ca_swizzle<PITCH>(r)) * 16) + (lane & 1) * 8);
   }
   auto vfrag = [&](int d) __attribute__((always_inline)) {  // channels 16 d + sub of keys 4 quarter + i, 16 + 4 quarter + i
     typedef short v8s __attribute__((ext_vector_type(8)));

@@ -53,8 +53,6 @@ class CachePlan:
     A plan stays good while its requests keep their pages and tokens: longer requests do no harm, `KVCache.truncate`, `free`
     and a `compact` that moves their pages end it, and after a `fork` it writes no more. What was ended is refused."""
 
-    _ROOM = 1 << 18
-
     def __init__(self, cache: "KVCache", requests: Sequence[_Request], tables: list[array], q_lengths: list[int],
                  kv_lengths: list[int], new_lengths: list[int], heads: int, causal: bool) -> None:
         self.cache, self.device, self._index = cache, cache.device, cache._index
@@ -77,9 +75,12 @@ class CachePlan:
         args = (ctypes.addressof(q), ctypes.addressof(kv), ctypes.addressof(new), len(self.q_lengths),
                 pages.buffer_info()[0], cache.pages, cache.page_size, self.heads, self.kv_heads, self.head_dim, self.causal,
                 cus)
-        # A plan a step: laid out once into room that holds most, not first for its size.
-        host = torch.empty(self._ROOM, dtype=torch.uint8)
-        size = lib.hf_cache_plan(*args, host.data_ptr(), self._ROOM)
+        # A plan a step: laid out once into room that is enough (tiles of rows, their parts, pages in two lists of segments
+        # and a table), not first for its size.
+        tiles = sum(-(-n * self.heads // self.kv_heads // 16) for n in self.q_lengths) * self.kv_heads
+        room = 4096 + 96 * (tiles + 4 * cus) + 64 * len(pages)
+        host = torch.empty(room, dtype=torch.uint8)
+        size = lib.hf_cache_plan(*args, host.data_ptr(), room)
         if size < 0:
             size = lib.hf_cache_plan(*args, None, 0)
             _check(min(size, 0), "hf_cache_plan")
