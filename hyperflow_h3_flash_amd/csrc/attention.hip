@@ -476,4 +476,66 @@ __global__ __launch_bounds__(64 * kJoinRows) void attention_join_kernel(Attentio
   *(v4u*)(a.out + (j.q0 + (int64_t)token) * a.o_token + head * a.o_head + d) = out;
 }
 
+// The same for tiles of many rows and not too many shares: 16 lanes a row, eight shares' loads on their way at once. 208 tiles
+// of 128 rows in about 600 shares 9.0 us against 13.3 a wave a row, 266 in 778 13.1 against 17.3.
+constexpr int kJoinFew = 32, kJoinFewRows = 16, kJoinAtOnce = 8;  // shares of a tile at most; rows of a workgroup
+template <class T, int DB>
+__global__ __launch_bounds__(256) void attention_join_few_kernel(AttentionArgs a) {
+  const AttentionJoin j = a.joins[blockIdx.x];
+  const int r = blockIdx.y * kJoinFewRows + (threadIdx.x >> 4), d = 8 * (threadIdx.x & 15);
+  const int64_t row = (int64_t)j.row0 + r;
+  if (row >= (int64_t)j.nq * a.group || d >= a.D) return;
+  const int64_t step = at_slot_floats(DB);
+  const float* part = a.ws + (int64_t)j.slot0 * step;
+  const float* stat = part + kAtRows * 32 * DB + 2 * r;
+  float top = -__builtin_inff(), l = 0.0f, o[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = 0.0f;
+#pragma unroll 1
+  for (int s0 = 0; s0 < j.slots; s0 += kJoinAtOnce) {
+    v2f ml[kJoinAtOnce];
+    v4f x[kJoinAtOnce], y[kJoinAtOnce];
+#pragma unroll
+    for (int i = 0; i < kJoinAtOnce; ++i) {
+      ml[i] = (v2f){-__builtin_inff(), 0.0f};
+      x[i] = y[i] = (v4f){0, 0, 0, 0};
+      if (s0 + i < j.slots) {
+        const float* p = part + (s0 + i) * step + r * 32 * DB + d;
+        ml[i] = *(const v2f*)(stat + (s0 + i) * step);
+        x[i] = *(const v4f*)p;
+        y[i] = *(const v4f*)(p + 4);
+      }
+    }
+    float next = top;
+#pragma unroll
+    for (int i = 0; i < kJoinAtOnce; ++i) next = fmaxf(next, ml[i][0]);
+    if (s0 > 0) {
+      const float f = top == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((top - next) * a.scale_log2);
+      l *= f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] *= f;
+    }
+    top = next;
+#pragma unroll
+    for (int i = 0; i < kJoinAtOnce; ++i) {
+      // A share whose keys the row does not see has m = -inf and adds nothing.
+      const float f = ml[i][0] == -__builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f((ml[i][0] - top) * a.scale_log2);
+      l = fmaf(ml[i][1], f, l);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        o[e] = fmaf(x[i][e], f, o[e]);
+        o[4 + e] = fmaf(y[i][e], f, o[4 + e]);
+      }
+    }
+  }
+  const int token = (int)((uint32_t)row / (uint32_t)a.group);
+  const int head = j.head * a.group + (int)(row - (int64_t)token * a.group);
+  const int last = a.causal ? min(token + j.nk - j.nq, j.nk - 1) : j.nk - 1;
+  const float inv = 1.0f / l;
+  v4u out;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] = last < 0 ? 0u : T::pack(o[2 * e] * inv, o[2 * e + 1] * inv);
+  *(v4u*)(a.out + (j.q0 + (int64_t)token) * a.o_token + head * a.o_head + d) = out;
+}
+
 }  // namespace hf

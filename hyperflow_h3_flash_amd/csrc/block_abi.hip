@@ -59,7 +59,7 @@ void launch_rope_lanes(const hf::RopeArgs& a, int lanes, bool interleaved, bool 
 
 constexpr int32_t kAttentionMagic = 0x48464154;
 struct AttentionHeader {
-  int32_t magic, heads, kv_heads, D, causal, items, joins, pad0;
+  int32_t magic, heads, kv_heads, D, causal, items, joins, few;  // few: tiles have few shares each (attention_join_few_kernel)
   int64_t bytes, slots, q_rows, kv_rows;
   int32_t pad[16];
 };
@@ -229,6 +229,11 @@ bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t cou
   w->head.magic = kAttentionMagic;
   w->head.heads = heads, w->head.kv_heads = kv_heads, w->head.D = D, w->head.causal = causal != 0;
   w->head.items = (int32_t)w->items.size(), w->head.joins = (int32_t)w->joins.size();
+  if (fill) {  // (plans of packed sequences keep their order of sums)
+    int32_t most = 0;
+    for (const hf::AttentionJoin& j : w->joins) most = std::max(most, j.slots);
+    w->head.few = most <= hf::kJoinFew;
+  }
   w->head.slots = slots, w->head.q_rows = q_rows, w->head.kv_rows = kv_rows;
   w->head.bytes = (int64_t)sizeof(w->head) + (int64_t)(w->items.size() * sizeof(hf::AttentionItem)) +
                   (int64_t)(w->joins.size() * sizeof(hf::AttentionJoin));
@@ -256,6 +261,11 @@ int launch_attention(const hf::AttentionArgs& a, const AttentionHeader& h, hipSt
   static_assert(lds <= 64 * 1024, "dynamic LDS that needs no attribute");
   hipLaunchKernelGGL((hf::attention_kernel<T, DB>), dim3(h.items), dim3(64 * hf::kAtWaves), lds, stream, a);
   if (int st = launch_status()) return st;
+  if (h.joins > 0 && h.few) {
+    hipLaunchKernelGGL((hf::attention_join_few_kernel<T, DB>), dim3(h.joins, hf::kAtRows / hf::kJoinFewRows), dim3(256), 0,
+                       stream, a);
+    return launch_status();
+  }
   if (h.joins > 0) {
     hipLaunchKernelGGL((hf::attention_join_kernel<T, DB>), dim3(h.joins, hf::kAtRows / hf::kJoinRows),
                        dim3(64 * hf::kJoinRows), 0, stream,
