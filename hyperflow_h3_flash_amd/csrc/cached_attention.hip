@@ -11,6 +11,13 @@
 // keys 16 b + 4 (l / 16) + i: the second product's operand when its keys are numbered so. Values are turned through LDS, by
 // wave: written by key, read transposed four keys at a time, as in attention.hip.
 //
+// Bound: the keys' bytes with long caches, a wave's own chain of about 0.7 us a step (codes, product, maximum, exponentials,
+// LDS, product) with short ones. One token of 64 / 8 heads against 131072 keys: 29 us and 4 for the join, 4.9 TB/s (a copy:
+// 5.0); 16 tokens of 32 / 8 heads against 77411 keys 16.6 and 3.0; 100 tokens of 32 / 8 heads against 16000 keys 57 us, 0.46
+// PFLOP/s (codes become values for every 32 rows anew). Loads of the next block have no condition, and its page number is known
+// a step earlier: with loads under a condition each wait was one for all of them (54 us for the 16 tokens). Blocks two or
+// three steps ahead (25.5 -> 26.7, 27.7) and 64 keys a step (28.0 -> 30.0 for 64 caches of 2000) were slower: more registers,
+// fewer waves.
 #pragma once
 
 #include "attention.hip"
