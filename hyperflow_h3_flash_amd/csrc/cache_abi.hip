@@ -191,6 +191,9 @@ int cache_layout(const int64_t* q_lens, const int64_t* kv_lens, const int64_t* n
   for (hf::CachedItem& it : w->items)
     for (int i = 0; i < hf::kCaWaves; ++i)
       if (it.key_lo + i * hf::kCaKeys < it.key_hi) it.first[i] = w->tables[it.table0 + (it.key_lo + i * hf::kCaKeys) / page];
+  // A launch has fewer than 2^32 threads.
+  constexpr size_t kMostGroups = (1 << 24) - 1;
+  if (w->items.size() > kMostGroups || w->reads.size() > kMostGroups) return HF_ERR_SIZE;
   CacheHeader& h = w->head;
   memset(&h, 0, sizeof(h));
   h.magic = kCacheMagic;
@@ -301,8 +304,13 @@ int launch_cached_blocks(const hf::CachedArgs& a, const CacheHeader& h, hipStrea
 template <class T, bool WIDE, bool VF32, bool Y, int W, int NV>
 void launch_norm_rows(const hf::NormArgs& a, hipStream_t stream) {
   constexpr int kWaves = hf::norm_waves(W), kRows = kWaves / W;
-  const dim3 grid((unsigned)((a.T + kRows - 1) / kRows));
-  hipLaunchKernelGGL((hf::residual_norm_kernel<T, WIDE, VF32, Y, W, NV>), grid, dim3(64 * kWaves), 0, stream, a);
+  constexpr int64_t kMost = ((int64_t)1 << 31) / (64 * kWaves) * kRows;  // rows of a launch, of fewer than 2^32 threads
+  for (int64_t t0 = 0; t0 < a.T; t0 += kMost) {
+    hf::NormArgs part = a;
+    part.t0 = t0, part.T = std::min(a.T, t0 + kMost);
+    const dim3 grid((unsigned)((part.T - t0 + kRows - 1) / kRows));
+    hipLaunchKernelGGL((hf::residual_norm_kernel<T, WIDE, VF32, Y, W, NV>), grid, dim3(64 * kWaves), 0, stream, part);
+  }
 }
 
 template <class T, bool WIDE, bool VF32, bool Y>

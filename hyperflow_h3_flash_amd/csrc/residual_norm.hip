@@ -28,7 +28,7 @@ struct NormArgs {
   const void *gate, *scale, *shift, *post_weight, *weight;
   const int32_t* group;
   int64_t ldx, ldy, ldr, ldn, ld_gate, ld_scale, ld_shift;
-  int64_t T;
+  int64_t t0, T;  // rows of this launch: t0 .. T - 1
   int C, post, norm, per_row, stream;
   float residual, eps;
 };
@@ -100,7 +100,7 @@ __global__ __launch_bounds__(64 * norm_waves(W)) void residual_norm_kernel(NormA
   constexpr int kRows = norm_waves(W) / W;
   __shared__ float partial[2][W];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int64_t t = (int64_t)blockIdx.x * kRows + wave / W;
+  const int64_t t = a.t0 + (int64_t)blockIdx.x * kRows + wave / W;
   if (t >= a.T) return;  // a whole workgroup where rows have several waves
   const uint32_t first = (wave % W) * 64 + lane;
   auto channel = [&](int i) __attribute__((always_inline)) { return 8 * (first + 64 * W * i); };

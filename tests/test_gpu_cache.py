@@ -415,6 +415,26 @@ def test_another_stream_and_a_graph():
         assert torch.equal(cache.data[0, -1], cache.data[0, cache.table(requests[0])[-1]])
 
 
+def test_caches_of_inference_mode_and_others():
+    for outer, inner in ((torch.inference_mode, torch.no_grad), (torch.no_grad, torch.inference_mode)):
+        with outer():
+            cache = KVCache(1, 2, 32, 6)
+            request = cache.new()
+        with inner():
+            k, v = keys(1, 100, 2, 32, BF), keys(2, 100, 2, 32, BF)
+            plan = cache.plan([request], [100], causal=True)
+            cache_append(cache, 0, k, v, plan)
+            cache.fork(request)
+            cache.plan([request], [1])
+            got = cache_read(cache, 0, cache.plan([request], [0]))
+            assert torch.equal(got[0][:100].double(), C.held(k))
+            ref, bound = C.attention(k, k, v, [100], [100], True, 32 ** -0.5)
+            other = KVCache(1, 2, 32, 2)
+            step = other.plan([other.new()], [100], causal=True)
+            cache_append(other, 0, k, v, step)
+            U.check(cached_attention(k, other, 0, step), ref, bound)
+
+
 def test_two_threads_on_one_stream():
     cache, requests, k, v = filled([9000, 3000], 2, 128)
     plan = cache.plan(requests, [1, 100], new_lengths=[0, 0], heads=8, causal=True)

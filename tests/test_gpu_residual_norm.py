@@ -171,6 +171,17 @@ def test_a_tensor_past_2_31_elements():
         assert torch.equal(r[i], a[0]) and torch.equal(n[i], b[0])
 
 
+def test_more_rows_than_one_launch_takes():
+    T = (1 << 25) + 70001
+    x = torch.zeros(T, 8, device="cuda", dtype=BF)
+    x[-1], x[1 << 25], x[(1 << 25) - 1] = 3.0, 5.0, 7.0
+    gate = torch.ones(T, 8, device="cuda", dtype=BF)
+    gate[-1] = 2.0
+    r, n = residual_norm(x, x, gate=gate)
+    assert r[-1].eq(9).all() and r[1 << 25].eq(10).all() and r[(1 << 25) - 1].eq(14).all() and n[-1].eq(1).all()
+    assert r.count_nonzero() == 24 and n.count_nonzero() == 24
+
+
 def test_no_rows():
     e = torch.empty(0, 64, device="cuda", dtype=BF)
     r, n = residual_norm(e, e.clone(), rows=RowPlan([0, 0]), gate=torch.zeros(2, 64, device="cuda", dtype=BF))
