@@ -379,8 +379,8 @@ def cached_attention(q: Tensor, cache: KVCache, layer: int, plan: CachePlan, *, 
 
     ``q`` [sum q_lengths, heads, head_dim] of the cache's type, any token and head strides; the result is like q. ``scale``
     (default ``head_dim ** -0.5``) is positive. As in `packed_attention` a query that sees no key gets zeros, keys that a
-    query does not see never reach it, and scores, sums and outputs are float32 with weights in the inputs' type. ``out`` may
-    be any tensor like q, q among them."""
+    query does not see never reach it, and scores, sums and outputs are float32 with weights in the inputs' type (values of v
+    times 256 times the number of keys have to stay in float32's range). ``out`` may be any tensor like q, q among them."""
     if q.shape != plan._q_shape:
         raise ValueError(f"the plan is for q {plan._q_shape}, got {tuple(q.shape)}")
     dtype = cache.dtype
