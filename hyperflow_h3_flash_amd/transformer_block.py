@@ -3,7 +3,7 @@ and residuals around an `AttentionBlock` and a feed-forward.
 
 The reference's blocks do the same steps (src/hyperflow_h3_flash/transformer.py:339-380) one by one and for one request. Here
 `residual_norm` takes what stands between two linears in one pass, across the end of a block too: a block's last residual and
-the next block's first norm are one call (`TransformerStack`)."""
+the next block's first norm are one call (`TransformerStack`), unless the former's own norm has another eps than the latter."""
 
 from __future__ import annotations
 
@@ -91,6 +91,12 @@ def _run(blocks: list[TransformerBlock], x: Tensor, plan, modulation: Sequence[T
         f = block.down(block.up(n))
         after = blocks[i + 1] if i + 1 < len(blocks) else None
         shift, scale = of[i + 1][:2] if after is not None else (None, None)
+        if after is not None and block.post_norm is not None and block.eps != after.eps:  # an eps each: two calls
+            x, _ = residual_norm(x, f, rows=rows, gate=ff_gate, post_norm=block.post_norm, post_weight=block.post_ff, norm=None,
+                                 eps=block.eps)
+            _, n = residual_norm(x, rows=rows, norm=after.norm, weight=after.norm_attention, scale=scale, shift=shift,
+                                 eps=after.eps)
+            continue
         x, n = residual_norm(x, f, rows=rows, gate=ff_gate, post_norm=block.post_norm, post_weight=block.post_ff,
                              norm=None if after is None else after.norm,
                              weight=None if after is None else after.norm_attention, scale=scale, shift=shift,

@@ -77,6 +77,25 @@ def test_a_stack_is_its_parts(device, norm, post, stream):
 
 
 @pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("stream", [BF, torch.float32])
+@pytest.mark.parametrize("eps", [(1e-6, 1.0), (1.0, 1e-6)])
+def test_each_block_of_a_stack_keeps_its_eps(device, stream, eps):
+    """The norm behind a block's feed-forward has that block's eps, the one before the next block's attention the next
+    block's. The blocks one by one round the stream in the same place, so the results are the same bits."""
+    size = SIZES[device]
+    blocks = [make(10 * i, device, norm="rms", post_norm="rms", eps=e, **size) for i, e in enumerate(eps)]
+    x = (0.5 * rnd(1, 15, blocks[0].dim)).to(stream).to(device)
+    plan = AttentionPlan([5, 9, 1], heads=size.get("heads", 4), kv_heads=size.get("kv_heads", 2),
+                         head_dim=size.get("head_dim", 16), device=device)
+    m = [(0.3 * rnd(2 + i, 3, 6, blocks[0].dim)).to(BF).to(device) for i in range(2)]
+    rows = RowPlan([5, 9, 1], device=device)
+    want = x
+    for block, mod in zip(blocks, m):
+        want = block(want, plan, modulation=mod, rows=rows)
+    assert torch.equal(TransformerStack(blocks)(x, plan, modulation=m, rows=rows), want)
+
+
+@pytest.mark.parametrize("device", DEVICES)
 def test_steps_over_the_cache_agree_with_each_other(device):
     """A prompt in one step, in two, and its last token alone give the same last rows; a fork does not change its source."""
     size = SIZES[device]
