@@ -274,7 +274,7 @@ class KVCache:
             tables.append((table, grow))
         if need > len(self._unused):
             raise RuntimeError(f"the step needs {need} pages, {len(self._unused)} of {self.pages} are free")
-        fresh = heapq.nsmallest(need, self._unused)
+        fresh = [heapq.heappop(self._unused) for _ in range(need)]
         at = 0
         src, dst = [], []
         for i, j in copies:
@@ -285,12 +285,15 @@ class KVCache:
         for table, grow in tables:
             table.extend(fresh[at:at + grow])
             at += grow
-        plan = CachePlan(self, found, [table for table, _ in tables], q, [r.length + n for r, n in zip(found, new)], new,
-                         heads, bool(causal))
-        if src:
-            copy_pages(self.data, src, dst)
-        for _ in range(need):
-            heapq.heappop(self._unused)
+        try:
+            plan = CachePlan(self, found, [table for table, _ in tables], q, [r.length + n for r, n in zip(found, new)], new,
+                             heads, bool(causal))
+            if src:
+                copy_pages(self.data, src, dst)
+        except BaseException:
+            for page in fresh:
+                heapq.heappush(self._unused, page)
+            raise
         for page in fresh:
             self._uses[page] = 1
         for page, n in given.items():

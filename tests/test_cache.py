@@ -198,6 +198,45 @@ def test_a_step_that_does_not_fit_changes_nothing():
     assert cache.free_pages == 0 and cache.table(a)[1] != cache.table(b)[1]
 
 
+def test_a_step_costs_its_own_pages_not_the_pools():
+    """A step that takes 16 pages compares page numbers on the way of 16 of a heap, not once for each free page."""
+    compared = 0
+
+    class Page(int):
+        def __lt__(self, other):
+            nonlocal compared
+            compared += 1
+            return int(self) < int(other)
+
+    cache = KVCache(1, 1, 16, 1 << 16, page_size=32, device="cpu")
+    requests = [cache.new() for _ in range(16)]
+    cache._unused = [Page(p) for p in cache._unused]
+    cache.plan(requests, [1] * 16)
+    assert [cache.table(r) for r in requests] == [[i] for i in range(16)]
+    assert compared <= 16 * 2 * 17  # two a level, 2^16 pages
+
+
+@pytest.mark.parametrize("broken", ["CachePlan", "copy_pages"])
+def test_a_step_that_fails_while_it_is_built_changes_nothing(monkeypatch, broken):
+    from hyperflow_h3_flash_amd import kv_cache
+
+    def fail(*args, **kwargs):
+        raise MemoryError("no")
+
+    cache = KVCache(1, 1, 16, 9, page_size=32, device="cpu")
+    a = cache.new()
+    cache.plan([a], [40])
+    b = cache.fork(a)
+    tables = cache.table(a), cache.table(b)
+    with monkeypatch.context() as m:
+        m.setattr(kv_cache, broken, fail)
+        with pytest.raises(MemoryError):
+            cache.plan([a, b], [40, 1])
+    assert (cache.table(a), cache.table(b)) == tables and cache.free_pages == 7 and cache.length(a) == cache.length(b) == 40
+    cache.plan([a, b], [40, 1])
+    assert cache.table(a) == [0, 2, 3] and cache.table(b) == [0, 1]
+
+
 def test_refusals():
     for bad in (dict(layers=0), dict(kv_heads=0), dict(head_dim=24), dict(head_dim=144), dict(page_size=48), dict(pages=-1),
                 dict(dtype=torch.float32), dict(pages=1 << 26)):
