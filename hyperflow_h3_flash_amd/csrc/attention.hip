@@ -476,9 +476,14 @@ __global__ __launch_bounds__(64 * kJoinRows) void attention_join_kernel(Attentio
   *(v4u*)(a.out + (j.q0 + (int64_t)token) * a.o_token + head * a.o_head + d) = out;
 }
 
-// The same for tiles of many rows and not too many shares: 16 lanes a row, eight shares' loads on their way at once. 208 tiles
-// of 128 rows in about 600 shares 9.0 us against 13.3 a wave a row, 266 in 778 13.1 against 17.3.
-constexpr int kJoinFew = 32, kJoinFewRows = 16, kJoinAtOnce = 8;  // shares of a tile at most; rows of a workgroup
+// The same for many tiles in few shares each: 16 lanes a row, eight shares' loads on their way at once. Its time is about 5 us
+// and an eighth for each share of the tile that has most, whose reads go one behind the other, the other's about 6 us and a
+// twenty-fifth for each tile, whose rows take a wave each: this one is taken where a tile has a quarter as many shares as there
+// are tiles, or fewer (at_few_shares). us, this one and the other, by tiles joined and most shares of one: 266, 32 13.2 and
+// 16.9; 266, 34 13.0 and 16.3; 259, 73 18.2 and 17.9; 232, 6 8.7 and 13.2; 256, 2 8.0 and 14.4; 182, 55 13.4 and 12.1; 96, 5
+// 6.4 and 9.1; 56, 9 6.7 and 7.1; 48, 10 7.2 and 7.5; 12, 41 9.3 and 6.8; 8, 64 11.8 and 7.4; 5, 98 16.9 and 8.1.
+constexpr int kJoinFewRows = 16, kJoinAtOnce = 8;  // rows of a workgroup
+constexpr bool at_few_shares(int64_t most, int64_t joins) { return 4 * most <= joins; }
 template <class T, int DB>
 __global__ __launch_bounds__(256) void attention_join_few_kernel(AttentionArgs a) {
   const AttentionJoin j = a.joins[blockIdx.x];

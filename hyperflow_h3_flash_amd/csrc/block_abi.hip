@@ -59,7 +59,7 @@ void launch_rope_lanes(const hf::RopeArgs& a, int lanes, bool interleaved, bool 
 
 constexpr int32_t kAttentionMagic = 0x48464154;
 struct AttentionHeader {
-  int32_t magic, heads, kv_heads, D, causal, items, joins, few;  // few: tiles have few shares each (attention_join_few_kernel)
+  int32_t magic, heads, kv_heads, D, causal, items, joins, few;  // few: attention_join_few_kernel joins
   int64_t bytes, slots, q_rows, kv_rows;
   int32_t pad[16];
 };
@@ -239,7 +239,7 @@ bool attention_layout(const int64_t* q_lens, const int64_t* kv_lens, int64_t cou
   if (fill) {  // (plans of packed sequences keep their order of sums)
     int32_t most = 0;
     for (const hf::AttentionJoin& j : w->joins) most = std::max(most, j.slots);
-    w->head.few = most <= hf::kJoinFew;
+    w->head.few = hf::at_few_shares(most, w->head.joins);
   }
   w->head.slots = slots, w->head.q_rows = q_rows, w->head.kv_rows = kv_rows;
   w->head.bytes = (int64_t)sizeof(w->head) + (int64_t)(w->items.size() * sizeof(hf::AttentionItem)) +

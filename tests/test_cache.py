@@ -468,6 +468,62 @@ def test_plan_covers_every_row_key_and_token_once(lib, q, kv, new, heads, kv_hea
         assert {tuple(i[:4]) for i in items} == starts
 
 
+def expanded(raw):
+    """The items and joins of a plan's attention over expanded keys, and whether the join for few shares takes them."""
+    raw = parts(raw)["attention"]
+    items, joins, few = struct.unpack_from("3i", raw, 20)
+    slots, = struct.unpack_from("q", raw, 40)
+    assert len(raw) == 128 + 48 * items + 32 * joins
+    return (np.frombuffer(raw, np.int32, items * 12, 128).reshape(-1, 12).tolist(),
+            np.frombuffer(raw, np.int32, joins * 8, 128 + 48 * items).reshape(-1, 8).tolist(), slots, bool(few))
+
+
+@pytest.mark.parametrize("q,kv,heads,kv_heads,D,causal,few,unequal", [
+    ([4860], [37710], 7, 7, 128, 0, True, True), ([4860], [40000], 7, 7, 128, 0, True, True),
+    ([4700], [37710], 7, 7, 128, 0, False, True), ([512, 300, 61, 1], [4096, 8191, 733, 2500], 32, 8, 128, 1, True, True),
+    ([2000], [4000], 16, 16, 128, 0, True, False), ([400], [90000], 2, 1, 128, 1, False, False),
+    ([2300], [5000], 16, 16, 80, 1, True, True), ([700, 650, 900], [3000, 5000, 9000], 16, 8, 96, 1, True, True),
+    ([1500, 0, 320], [6001, 70, 0], 24, 24, 64, 0, True, True), ([800, 5], [16000, 9], 8, 8, 128, 1, True, False)])
+def test_expanded_parts_cover_each_tile_of_rows_once(lib, q, kv, heads, kv_heads, D, causal, few, unequal):
+    """Parts of a tile of 128 rows take all keys that its last row sees once, from one key tile's start to another's, each with
+    a share of its own that one join reads; the cuts and the join are the ones that the case stands for."""
+    counts = [-(-n // 64) for n in kv]
+    group = heads // kv_heads
+    for cus in (256, 7):
+        raw = cache_plan(lib, q, kv, [0] * len(q), list(range(sum(counts))), heads, kv_heads, D, causal, 64, sum(counts), cus).raw
+        items, joins, slots, quick = expanded(raw)
+        wide = [b for b in range(len(q)) if any(i[0] == sum(q[:b]) and i[1] == q[b] for i in items) and q[b]]
+        assert wide
+        want = {}  # (first query, queries, first key, keys, first row, head): keys of the tile
+        for i, b in enumerate(wide):
+            for head in range(kv_heads):
+                for row0 in range(0, q[b] * group, 128):
+                    last = min(row0 + 128, q[b] * group) - 1
+                    hi = min(max(last // group + kv[b] - q[b] + 1, 0), kv[b]) if causal else kv[b]
+                    want[sum(q[:b]), q[b], sum(kv[w] for w in wide[:i]), kv[b], row0, head] = hi
+        spans = {}
+        for q0, nq, k0, nk, row0, lo, hi, head, slot, *_ in items:
+            spans.setdefault((q0, nq, k0, nk, row0, head), []).append((lo, hi, slot))
+        assert spans.keys() == want.keys()
+        joined = {(q0, nq, k0, nk, row0, head): list(range(slot, slot + n)) for q0, nq, k0, nk, row0, head, slot, n in joins}
+        assert len(joined) == len(joins)
+        uneven, seen = 0, []
+        for tile, cut in spans.items():
+            cut.sort()
+            assert cut[0][0] == 0 and cut[-1][1] == want[tile] and all(a[1] == b[0] for a, b in zip(cut, cut[1:]))
+            assert all(lo % 64 == 0 and (lo < hi or hi == 0) for lo, hi, _ in cut)
+            shares = [slot for *_, slot in cut]
+            assert sorted(shares) == joined.pop(tile, [-1]) and (len(cut) > 1) == (shares[0] >= 0)
+            seen += [s for s in shares if s >= 0]
+            sizes = [hi - lo for lo, hi, _ in cut]
+            uneven += max(sizes) - min(sizes) > 128  # equal cuts differ by a key tile and the end of the last
+        assert not joined and sorted(seen) == list(range(slots))
+        most = max([n for *_, n in joins], default=0)
+        assert quick == (4 * most <= len(joins))
+        if cus == 256:
+            assert joins and quick == few and (uneven > 0) == unequal
+
+
 # ------------------------------------------------------------------------------------------------------- residual norms
 
 @pytest.mark.parametrize("norm,post", [("rms", None), ("layer", "rms"), (None, "layer")])

@@ -11,6 +11,7 @@ import torch
 import block_utils as U
 import cache_utils as C
 from hyperflow_h3_flash_amd import KVCache, cache_append, cache_read, cached_attention, copy_pages
+from test_cache import expanded
 
 pytestmark = pytest.mark.gpu
 BF, HF = torch.bfloat16, torch.float16
@@ -180,6 +181,46 @@ def test_expanded_sequences_beside_others(dtype, D, causal):
         cache, plan, *_ = run_attention([2, 360, 0, 40], [one, 100001, 5, 900], 4, 2, D, dtype, causal)
         rows = 100001 + (0 if one > 300 else 300 + 5 + 900)
         assert 0 <= plan.ws_bytes - 2 * rows * 2 * D * 2 < 60 << 20  # shares come to less
+
+
+CUTS = [  # (..., the join for few shares, cuts of unequal length): test_cache.py holds the plans to them
+    ([2300], [5000], 16, 16, 80, True, True, True), ([1500, 0, 320], [6001, 70, 0], 24, 24, 64, False, True, True),
+    ([2000], [4000], 16, 16, 128, False, True, False), ([700, 650, 900], [3000, 5000, 9000], 16, 8, 96, True, True, True),
+    ([4700], [37710], 7, 7, 128, False, False, True), ([400], [90000], 2, 1, 128, True, False, False)]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("q,kv,hq,hk,D,causal,few,unequal", CUTS)
+def test_expanded_cuts_and_both_joins(q, kv, hq, hk, D, causal, few, unequal, dtype):
+    _, plan, *_ = run_attention(q, kv, hq, hk, D, dtype, causal)
+    items, joins, _, quick = expanded(plan.data.host.numpy().tobytes())
+    spans = {}
+    for q0, _, _, _, row0, lo, hi, head, *_ in items:
+        spans.setdefault((q0, row0, head), []).append(hi - lo)
+    assert joins and quick == few and any(max(n) - min(n) > 128 for n in spans.values()) == unequal
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_nan_that_some_rows_see_through_unequal_cuts(dtype):
+    q_len, kv, heads, D = 2300, 5000, 16, 80
+    k, v = keys(1, kv, heads, D, dtype), keys(2, kv, heads, D, dtype)
+    fine = v.clone()
+    v[kv - 51, 3, 70] = float("nan")  # seen by the last 51 queries
+    v[100, 5, 10] = float("inf")  # by all
+    k[kv - 2, 7, 3] = float("nan")  # by the last two
+    nan = torch.zeros(q_len, heads, D, dtype=torch.bool, device="cuda")
+    nan[-51:, 3, 64:80] = nan[:, 5, :32] = nan[-2:, 7] = True
+    fine[kv - 51, 3, 64:80] = fine[100, 5, :32] = 0
+    kk = k.clone()
+    kk[kv - 2, 7, :32] = 0
+    cache, requests, _, _ = filled([kv], heads, D, dtype, k=k, v=v)
+    q = rnd(3, q_len, heads, D).to(dtype)
+    plan = cache.plan(requests, [q_len], new_lengths=[0], heads=heads, causal=True)
+    assert expanded(plan.data.host.numpy().tobytes())[3]
+    got = cached_attention(q, cache, 0, plan)
+    assert torch.equal(got.isnan(), nan)
+    ref, bound = C.attention(q, kk, fine, [q_len], [kv], True, D ** -0.5)
+    U.check(torch.where(nan, 0.0, got.double()), torch.where(nan, 0.0, ref), bound)
 
 
 @pytest.mark.parametrize("causal", [False, True])
