@@ -11,14 +11,22 @@ namespace {
 constexpr int32_t kCacheMagic = 0x48464b56;
 struct CacheHeader {
   int32_t magic, heads, kv_heads, D, causal, page, items, joins;
-  int64_t bytes, slots, q_rows, kv_rows, new_rows, wide_rows;
+  int64_t bytes, slots, q_rows, kv_rows, new_rows, wide_rows;  // wide_rows: of the pass that expands most
   int32_t reads, writes, wides, join_rows;  // join_rows: of the fullest tile that is joined
-  // Where each part starts: items, joins, tables, segments read, written and expanded, the plan of the expanded ones.
+  // Where each part starts: items, joins, tables, segments read, written and expanded, the passes' plans (and their bytes).
   int64_t at_items, at_joins, at_tables, at_reads, at_writes, at_wides, at_attention, attention_bytes;
   int64_t pool_pages;
-  int32_t row_blocks, pad[21];
+  int32_t row_blocks, passes;
+  int64_t at_passes;
+  int32_t pad[18];
 };
 static_assert(sizeof(CacheHeader) == 256, "parts start on 128-byte lines behind it");
+
+// Sequences that are expanded and attended to at a time: their segments, rows of keys, and plan.
+struct CachePass {
+  int32_t first, count;
+  int64_t rows, at_attention, attention_bytes;
+};
 
 bool cache_header(const void* plan, int64_t bytes, CacheHeader* h) {
   if (!plan || bytes < (int64_t)sizeof(*h)) return false;
@@ -49,13 +57,21 @@ constexpr double kWidePairs = 64 << 20;  // of rows and keys, over the key heads
 // with those on the pages, 108 with all expanded).
 constexpr int64_t kWideRest = 6 << 20;
 
+// Bytes of expanded keys and values up to which sequences share a pass. What is more is expanded pass by pass into the same
+// workspace, so that it does not grow with the batch (a sequence is not divided). ms, in one pass and in passes of this size,
+// and the workspaces, 8 key heads of 128: 24 x 200 tokens over 100000, 32 heads 13.8 and 11.0, 9.2 and 3.8 GiB; 100 x 160 over
+// 30000 13.7 and 12.5, 11.4 and 3.9; 8 x 1000 over 300000, 8 heads 14.7 and 13.2, 9.2 and 3.5. Passes of a quarter of this end
+// their attention more often than they gain: 3 x 1000 over 300000 4.7 in one, 5.4 in three.
+constexpr int64_t kMostExpanded = (int64_t)1 << 32;
+
 struct CacheWork {
   CacheHeader head;
   std::vector<hf::CachedItem> items;
   std::vector<hf::CachedJoin> joins;
   std::vector<int32_t> tables;
   std::vector<hf::CacheSegment> reads, writes, wides;
-  AttentionWork attention;
+  std::vector<CachePass> passes;
+  std::vector<AttentionWork> attentions;  // of each pass
 };
 
 // Segments of tokens lo .. hi - 1 of a sequence.
@@ -104,8 +120,12 @@ int cache_layout(const int64_t* q_lens, const int64_t* kv_lens, const int64_t* n
     if (q_lens[b] * group <= direct_rows) most = std::max(most, q_lens[b] * group);
   const int row_blocks = most > hf::kCaRows ? 2 : 1, tile_rows = hf::kCaRows * row_blocks;
   std::vector<Tile> tiles;
-  std::vector<int64_t> wide_q, wide_kv, wide_q0;
-  int64_t total = 0, q0 = 0, k0 = 0, n0 = 0, wide_rows = 0;
+  struct Wide {
+    std::vector<int64_t> q, kv, q0;
+  };
+  std::vector<Wide> wides;  // of each pass
+  const int64_t pass_rows = kMostExpanded / (4 * (int64_t)kv_heads * D);
+  int64_t total = 0, q0 = 0, k0 = 0, n0 = 0;
   table = 0;
   for (int64_t b = 0; b < count; ++b) {
     const int64_t nq = q_lens[b], nk = kv_lens[b];
@@ -113,9 +133,15 @@ int cache_layout(const int64_t* q_lens, const int64_t* kv_lens, const int64_t* n
     cache_segments(&w->reads, mine, page, 0, nk, k0);
     cache_segments(&w->writes, mine, page, nk - new_lens[b], nk, n0);
     if (nq * group > direct_rows) {
-      cache_segments(&w->wides, mine, page, 0, nk, wide_rows);
-      wide_q.push_back(nq), wide_kv.push_back(nk), wide_q0.push_back(q0);
-      wide_rows += nk;
+      if (wides.empty() || (w->passes.back().rows > 0 && w->passes.back().rows + nk > pass_rows)) {
+        wides.emplace_back();
+        w->passes.push_back({(int32_t)w->wides.size(), 0, 0, 0, 0});
+      }
+      CachePass& pass = w->passes.back();
+      cache_segments(&w->wides, mine, page, 0, nk, pass.rows);
+      pass.count = (int32_t)w->wides.size() - pass.first;
+      pass.rows += nk;
+      wides.back().q.push_back(nq), wides.back().kv.push_back(nk), wides.back().q0.push_back(q0);
     } else {
       for (int h = 0; h < kv_heads; ++h)
         for (int64_t r = 0; r < nq * group; r += tile_rows) {
@@ -197,16 +223,21 @@ int cache_layout(const int64_t* q_lens, const int64_t* kv_lens, const int64_t* n
   CacheHeader& h = w->head;
   memset(&h, 0, sizeof(h));
   h.magic = kCacheMagic;
-  if (!wide_q.empty()) {
-    if (!attention_layout(wide_q.data(), wide_kv.data(), (int64_t)wide_q.size(), heads, kv_heads, D, causal, cus,
-                          &w->attention, wide_q0.data(), true))
+  w->attentions.resize(wides.size());
+  for (size_t i = 0; i < wides.size(); ++i) {
+    if (!attention_layout(wides[i].q.data(), wides[i].kv.data(), (int64_t)wides[i].q.size(), heads, kv_heads, D, causal, cus,
+                          &w->attentions[i], wides[i].q0.data(), true))
       return HF_ERR_SIZE;
-    h.attention_bytes = w->attention.head.bytes;
+    w->passes[i].attention_bytes = w->attentions[i].head.bytes;
+    w->passes[i].at_attention = h.attention_bytes;
+    h.attention_bytes = (i + 1 < wides.size() ? up_to(h.attention_bytes + w->passes[i].attention_bytes, 128)
+                                              : h.attention_bytes + w->passes[i].attention_bytes);
+    h.wide_rows = std::max(h.wide_rows, w->passes[i].rows);
   }
   h.heads = heads, h.kv_heads = kv_heads, h.D = D, h.causal = causal != 0, h.page = page;
   h.items = (int32_t)w->items.size(), h.joins = (int32_t)w->joins.size(), h.slots = slots, h.join_rows = join_rows;
   h.row_blocks = row_blocks;
-  h.q_rows = q_rows, h.kv_rows = kv_rows, h.new_rows = new_rows, h.wide_rows = wide_rows, h.pool_pages = pool_pages;
+  h.q_rows = q_rows, h.kv_rows = kv_rows, h.new_rows = new_rows, h.pool_pages = pool_pages;
   h.reads = (int32_t)w->reads.size(), h.writes = (int32_t)w->writes.size(), h.wides = (int32_t)w->wides.size();
   int64_t at = sizeof(h);
   const auto place = [&](int64_t* where, int64_t bytes) {
@@ -220,12 +251,21 @@ int cache_layout(const int64_t* q_lens, const int64_t* kv_lens, const int64_t* n
   place(&h.at_writes, h.writes * (int64_t)sizeof(hf::CacheSegment));
   place(&h.at_wides, h.wides * (int64_t)sizeof(hf::CacheSegment));
   place(&h.at_attention, h.attention_bytes);
+  h.passes = (int32_t)w->passes.size();
+  place(&h.at_passes, h.passes * (int64_t)sizeof(CachePass));
+  for (CachePass& pass : w->passes) pass.at_attention += h.at_attention;
   h.bytes = at;
   return HF_OK;
 }
 
-// The workspace of an attention call: shares of the rows computed on the pages, expanded keys and values, and the workspace
-// of the attention over those.
+CachePass cache_pass(const CacheHeader& h, const void* plan, int i) {
+  CachePass pass;
+  memcpy(&pass, (const unsigned char*)plan + h.at_passes + i * (int64_t)sizeof(pass), sizeof(pass));
+  return pass;
+}
+
+// The workspace of an attention call: shares of the rows computed on the pages, expanded keys and values of a pass, and the
+// workspace of the attention over those.
 struct CacheSpace {
   int64_t k, v, attention, bytes;
 };
@@ -239,7 +279,12 @@ CacheSpace cache_space(const CacheHeader& h, int64_t attention_ws) {
 }
 
 int64_t cache_attention_ws(const CacheHeader& h, const void* plan) {
-  return h.attention_bytes ? hf_attention_ws_bytes((const unsigned char*)plan + h.at_attention, h.attention_bytes) : 0;
+  int64_t most = 0;
+  for (int i = 0; i < h.passes; ++i) {
+    const CachePass pass = cache_pass(h, plan, i);
+    most = std::max(most, hf_attention_ws_bytes((const unsigned char*)plan + pass.at_attention, pass.attention_bytes));
+  }
+  return most;
 }
 
 #define HF_CACHE_GROUPS(G, CALL)  \
@@ -370,7 +415,8 @@ int64_t hf_cache_plan(const int64_t* q_lens, const int64_t* kv_lens, const int64
       put(h.at_reads, w.reads);
       put(h.at_writes, w.writes);
       put(h.at_wides, w.wides);
-      if (h.attention_bytes) attention_write(w.attention, to + h.at_attention);
+      put(h.at_passes, w.passes);
+      for (size_t i = 0; i < w.passes.size(); ++i) attention_write(w.attentions[i], to + w.passes[i].at_attention);
     }
     return h.bytes;
   } catch (...) {  // no memory for that many
@@ -449,15 +495,21 @@ int hf_cached_attention(const hf_cached_attention_args* p) {
                                        : launch_cached_blocks<hf::Fp16>(a, h, (hipStream_t)p->stream);
     if (st) return st;
   }
-  if (h.attention_bytes == 0) return HF_OK;
-  if (h.wide_rows > 0)
-    if (int st = cache_read(h, p->cache, ws + space.k, ws + space.v, dev + h.at_wides, h.wides, p->dtype,
-                            (hipStream_t)p->stream))
-      return st;
   const int64_t token = (int64_t)h.kv_heads * h.D;
-  return hf_attention(p->q, p->q_token, p->q_head, ws + space.k, token, h.D, ws + space.v, token, h.D, p->out, p->o_token,
-                      p->o_head, p->scale, (const unsigned char*)p->plan + h.at_attention, dev + h.at_attention,
-                      h.attention_bytes, attention_ws ? ws + space.attention : nullptr, attention_ws, p->dtype, p->stream);
+  for (int i = 0; i < h.passes; ++i) {
+    const CachePass pass = cache_pass(h, p->plan, i);
+    if (pass.count > 0)
+      if (int st = cache_read(h, p->cache, ws + space.k, ws + space.v,
+                              dev + h.at_wides + pass.first * (int64_t)sizeof(hf::CacheSegment), pass.count, p->dtype,
+                              (hipStream_t)p->stream))
+        return st;
+    if (int st = hf_attention(p->q, p->q_token, p->q_head, ws + space.k, token, h.D, ws + space.v, token, h.D, p->out,
+                              p->o_token, p->o_head, p->scale, (const unsigned char*)p->plan + pass.at_attention,
+                              dev + pass.at_attention, pass.attention_bytes, attention_ws ? ws + space.attention : nullptr,
+                              attention_ws, p->dtype, p->stream))
+      return st;
+  }
+  return HF_OK;
 }
 
 int hf_copy_pages(const hf_copy_pages_args* p) {

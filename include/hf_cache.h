@@ -35,7 +35,9 @@ int64_t hf_cache_page_bytes(int32_t kv_heads, int32_t D, int32_t page_size);
  * last new_lens[b] are written by hf_cache_append. Its pages are ceil(kv_lens[b] / page_size) entries of `pages`, one
  * sequence behind the other, each in [0, pool_pages). Query heads share key heads and `causal` masks as in
  * hf_attention_plan. Used like that function: with plan == NULL it returns the plan's bytes, otherwise fills `plan`; the
- * caller copies it to the device. A plan serves all layers. hf_cache_ws_bytes gives hf_cached_attention's workspace.
+ * caller copies it to the device. A plan serves all layers. hf_cache_ws_bytes gives hf_cached_attention's workspace: shares of
+ * what is cut, and where many rows attend to many keys those keys and values in `dtype`, of one sequence or of several up to
+ * 2^32 bytes at a time.
  * Requires: D a multiple of 16 up to 128; sums of lengths below 2^31; pool_pages * page_size below 2^31.
  */
 int64_t hf_cache_plan(const int64_t* q_lens, const int64_t* kv_lens, const int64_t* new_lens, int64_t count,

@@ -524,6 +524,45 @@ def test_expanded_parts_cover_each_tile_of_rows_once(lib, q, kv, heads, kv_heads
             assert joins and quick == few and (uneven > 0) == unequal
 
 
+def passes(raw):
+    """The passes of a plan's expanded sequences: (first segment, segments, rows, where the plan of its attention lies, bytes)."""
+    n, = struct.unpack_from("i", raw, 172)
+    at, = struct.unpack_from("q", raw, 176)
+    return [struct.unpack_from("2i3q", raw, at + 32 * i) for i in range(n)]
+
+
+@pytest.mark.parametrize("q,kv,heads,kv_heads,D,sizes", [
+    ([200] * 24, [100000] * 24, 32, 8, 128, [1000000, 1000000, 400000]),
+    ([200, 0, 200, 700, 200], [1 << 20, 9000, 1, 1200000, (1 << 20) - 1], 32, 8, 128, [1 << 20, 1, 1200000, (1 << 20) - 1]),
+    ([4860], [37710], 7, 7, 128, [37710]), ([400, 400], [2500000, 2000000], 16, 4, 64, [2500000, 2000000])])
+def test_expanded_sequences_share_a_bounded_workspace(lib, q, kv, heads, kv_heads, D, sizes):
+    """Long batches are expanded pass by pass: up to 2^32 bytes of keys and values, or one sequence, at a time."""
+    counts = [-(-n // 64) for n in kv]
+    pages = list(range(sum(counts)))[::-1]
+    plan = cache_plan(lib, q, kv, [0] * len(q), pages, heads, kv_heads, D, 1, 64, sum(counts))
+    found = passes(plan.raw)
+    assert [rows for _, _, rows, _, _ in found] == sizes
+    assert lib.hf_cache_ws_bytes(plan, len(plan.raw)) <= max(1 << 32, 4 * max(sizes) * kv_heads * D) + (100 << 20)
+    segments = parts(plan.raw)["wides"].tolist()
+    b = segment = 0
+    for first, count, rows, at, size in found:
+        assert first == segment
+        segment += count
+        want, items, row = [], set(), 0  # segments of the pass's sequences, one behind the other, their queries and first keys
+        while row < rows:
+            if q[b]:  # those without queries are not expanded
+                items.add((sum(q[:b]), q[b], row, kv[b]))
+                table = pages[sum(counts[:b]):sum(counts[:b + 1])]
+                want += [[page, 0, min(64, kv[b] - 64 * i), row + 64 * i] for i, page in enumerate(table)]
+                row += kv[b]
+            b += 1
+        assert row == rows and segments[first:segment] == want
+        n, = struct.unpack_from("i", plan.raw, at + 20)
+        raw = plan.raw[at:at + size]
+        assert {tuple(i[:4]) for i in np.frombuffer(raw, np.int32, n * 12, 128).reshape(n, 12).tolist()} == items
+    assert b == len(q) and segment == len(segments)
+
+
 # ------------------------------------------------------------------------------------------------------- residual norms
 
 @pytest.mark.parametrize("norm,post", [("rms", None), ("layer", "rms"), (None, "layer")])

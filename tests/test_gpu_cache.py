@@ -11,7 +11,7 @@ import torch
 import block_utils as U
 import cache_utils as C
 from hyperflow_h3_flash_amd import KVCache, cache_append, cache_read, cached_attention, copy_pages
-from test_cache import expanded
+from test_cache import expanded, passes
 
 pytestmark = pytest.mark.gpu
 BF, HF = torch.bfloat16, torch.float16
@@ -198,6 +198,22 @@ def test_expanded_cuts_and_both_joins(q, kv, hq, hk, D, causal, few, unequal, dt
     for q0, _, _, _, row0, lo, hi, head, *_ in items:
         spans.setdefault((q0, row0, head), []).append(hi - lo)
     assert joins and quick == few and any(max(n) - min(n) > 128 for n in spans.values()) == unequal
+
+
+def test_sequences_expanded_pass_by_pass():
+    """More keys than a pass takes: the workspace is the longest pass's, results are those of the sequences alone."""
+    q_lens, kv_lens, hq, hk, D = [170, 200, 3, 180], [500003, 500000, 900, 120001], 32, 8, 128
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    k, v = (torch.randn(sum(kv_lens), hk, D, generator=gen, device="cuda").to(BF) for _ in range(2))
+    cache, requests, _, _ = filled(kv_lens, hk, D, k=k, v=v)
+    q = rnd(2, sum(q_lens), hq, D).to(BF)
+    plan = cache.plan(requests, q_lens, new_lengths=[0] * 4, heads=hq, causal=True)
+    assert len(passes(plan.data.host.numpy().tobytes())) == 2 and plan.ws_bytes < (1 << 32) + (100 << 20)
+    got = cached_attention(q, cache, 0, plan)
+    held_k, held_v = cache_read(cache, 0, plan)
+    ref, bound = U.attention(q, held_k, held_v, q_lens, kv_lens, True, D ** -0.5)
+    U.check(got, ref, bound)
+    assert torch.equal(cached_attention(q, cache, 0, plan, out=q), got)
 
 
 @pytest.mark.parametrize("dtype", [BF, HF])
