@@ -321,8 +321,10 @@ def cache_append(cache: KVCache, layer: int, k: Tensor, v: Tensor, plan: CachePl
     layer's pages. Any token and head strides (slices of a fused projection).
 
     Each 32 channels of a head become 4-bit values times a power of two, the least that is a seventh of their largest
-    magnitude or more; a value lies half a step of its codes away from what it is read as, at most. A group with a value that
-    is not finite is read as NaN. Pages are written where their request's tokens lie and nowhere else."""
+    magnitude or more; a value lies half a step of its codes away from what it is read as, at most, up to the largest
+    magnitudes that a type's scales reach (57344 in float16, 7 * 2^125 in bfloat16: what is above is read as six sevenths of
+    that). A group with a value that is not finite is read as NaN. Pages are written where their request's tokens lie and
+    nowhere else."""
     if k.shape != plan._new_shape or v.shape != plan._new_shape:
         raise ValueError(f"the plan is for k, v {plan._new_shape}; got {tuple(k.shape)}, {tuple(v.shape)}")
     dtype = cache.dtype

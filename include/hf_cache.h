@@ -15,8 +15,9 @@
  * 0, 0.5, 1, 1.5, 2, 3, 4, 6; a scale byte E is the power of two 2^(E - 127), and 255 a group of which every value is NaN.
  * WRITING: scale = the least 2^e that is at least a seventh of the group's largest magnitude (so that the largest is rounded
  * by half a step of the codes at most), e from -125 to 125 for bfloat16 and -23 to 13 for float16, which keeps every code's
- * value finite and exact in the type; code = the nearest to x / scale, ties to the even one, values past 6 to 6. A group with
- * a value that is not finite is written as NaN.
+ * value finite and exact in the type; 2^-3 for a group of zeros. code = the nearest to x / scale, ties to the even one, values
+ * past 6 to 6 (magnitudes above 7 2^125 or, in float16, 7 2^13 = 57344 among them: off by up to a step). A group with a value
+ * that is not finite is written as NaN.
  */
 #ifndef HF_CACHE_H
 #define HF_CACHE_H

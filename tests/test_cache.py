@@ -70,6 +70,35 @@ def test_ties_limits_and_groups_that_are_not_finite():
         assert k[0].eq(6.0 * 2.0 ** C.LIMITS[dtype][1]).all() and k[1].isnan().all()
 
 
+def scale_bytes(cache, page, head, token):
+    """The scale bytes of a token's keys and values as the header lays them out, on the host."""
+    G, P = -(-cache.head_dim // 32), cache.page_size
+    S = 4 if G == 3 else G
+    slab = cache.data[0, page].view(cache.kv_heads, -1)[head]
+    at = 2 * G * P * 16 + token * 2 * S
+    return slab[at:at + G].tolist(), slab[at + S:at + S + G].tolist()
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("dtype,least,most", [(BF, 2, 252), (HF, 104, 140)])
+@pytest.mark.parametrize("D", [16, 80, 128])
+def test_scales_are_the_headers(D, dtype, least, most, device):
+    """The least power of two that is a seventh of the largest, within the type's limits, and 2^-3 (byte 124) for zeros."""
+    text = " ".join(open(HEADER).read().replace("*", " ").split())
+    assert "2^-3 for a group of zeros" in text and "e from -125 to 125 for bfloat16 and -23 to 13 for float16" in text
+    tiny, top = torch.finfo(dtype).smallest_normal * 2.0 ** -7, torch.finfo(dtype).max
+    k = torch.zeros(5, 1, D)
+    v = torch.zeros(5, 1, D)
+    v[1, 0, 3], v[2, 0, 3], v[3, 0, 3], v[4, 0, 3] = tiny, top, 7.0, 7.0 * (1 + 2.0 ** -6)
+    k[4, 0] = -0.0
+    k, v = k.to(dtype).to(device), v.to(dtype).to(device)
+    cache = KVCache(1, 1, D, 1, page_size=32, dtype=dtype, device=device)
+    cache_append(cache, 0, k, v, cache.plan([cache.new()], [5]))
+    G = -(-D // 32)
+    for token, first in enumerate((124, least, most, 127, 128)):
+        assert scale_bytes(cache, 0, 0, token) == ([124] * G, [first] + [124] * (G - 1))
+
+
 @pytest.mark.parametrize("causal", [False, True])
 def test_host_attention(causal):
     q_lens, kv_lens = [1, 9, 0, 40], [70, 9, 33, 31]
