@@ -8,7 +8,8 @@
 * `copy_pages`: pages of all layers copied within a pool.
 
 A value is one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 with a sign (4 bits) times a power of two for each 32 channels of a head
-(include/hf_cache.h has the layout and the rounding): 17/64 of 16-bit keys and values.
+(include/hf_cache.h has the layout and the rounding): 17/64 of 16-bit keys and values for heads of 32, 64 and 128, 13/48 of 96;
+others are held as if they had the next multiple of 32 channels.
 
 Beside `packed_attention`, whose caches lie one behind the other without gaps, a pool has room for every request to grow. A
 `CachePlan` holds the lengths and pages of one step, is built on the host and serves all layers. As the other operators these
@@ -127,9 +128,9 @@ class KVCache:
     tokens (32, 64, 128 or 256); ``dtype`` (bfloat16 or float16) is the type of keys, values and queries. ``data`` is the
     pool, uint8 [layers, pages, bytes of a page].
 
-    Requests are numbers that `new` and `fork` give. `plan` counts a step's new tokens and finds pages for them; the accounts
-    are the host's, so they run ahead of the device, whose work on one stream follows in order. Not for use by several
-    threads at once."""
+    Requests are numbers that `new` and `fork` give. `plan` counts a step's new tokens and finds pages for them. The accounts
+    are the host's and the device's work on one stream follows them in order; a plan's upload waits for what the current stream
+    has been given before. Not for use by several threads at once."""
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, pages: int, *, page_size: int = 64,
                  dtype: torch.dtype = torch.bfloat16, device: torch.device | str = "cuda") -> None:
