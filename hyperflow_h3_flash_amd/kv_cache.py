@@ -244,18 +244,20 @@ class KVCache:
     def plan(self, requests: Sequence[int], q_lengths: Sequence[int], *, new_lengths: Sequence[int] | None = None,
              heads: int | None = None, causal: bool = False) -> CachePlan:
         """The next step of some requests: ``q_lengths[i]`` queries of request i, ``new_lengths[i]`` tokens (default: as many)
-        that `cache_append` writes behind those it has. ``heads`` query heads (default: kv_heads) share the key heads in
+        that `cache_append` writes behind those it has. A request without new tokens may be named several times. ``heads`` query heads (default: kv_heads) share the key heads in
         equal groups. ``causal``: the last query sees every key, each one before it one key less.
 
         The new tokens are counted at once and get their pages; a shared page that they begin in is copied, on the current
         stream. RuntimeError, and nothing changed, when too few pages are free."""
+        requests = list(requests)
         found = [self._request(r) for r in requests]
         q = _lengths(q_lengths, "q_lengths")
         new = list(q) if new_lengths is None else _lengths(new_lengths, "new_lengths")
         if not len(found) == len(q) == len(new):
             raise ValueError(f"{len(found)} requests, {len(q)} query lengths, {len(new)} new lengths")
-        if any(new) and len(set(requests)) != len(found):
-            raise ValueError("a request that gets tokens is named twice")
+        if len(set(requests)) != len(found):  # a request may be read several times, unless it gets tokens
+            if any(n and requests.count(r) > 1 for r, n in zip(requests, new)):
+                raise ValueError("a request that gets tokens is named twice")
         heads = self.kv_heads if heads is None else int(heads)
         if heads < 1 or heads % self.kv_heads:
             raise ValueError(f"{heads} heads cannot share {self.kv_heads} key heads equally")

@@ -245,6 +245,22 @@ def test_a_step_costs_its_own_pages_not_the_pools():
     assert compared <= 16 * 2 * 17  # two a level, 2^16 pages
 
 
+def test_a_request_read_twice_beside_one_that_gets_tokens():
+    cache = KVCache(1, 1, 16, 8, page_size=32, device="cpu")
+    a = cache.new()
+    k = rnd(1, 41, 1, 16).to(BF)
+    cache_append(cache, 0, k[:40], k[:40], cache.plan([a], [40]))
+    b = cache.fork(a)
+    plan = cache.plan(iter([a, b, a]), [1, 1, 1], new_lengths=[0, 1, 0])
+    cache_append(cache, 0, k[40:], k[40:], plan)
+    got, _ = cache_read(cache, 0, plan)
+    assert torch.equal(got.double(), C.held(torch.cat([k[:40], k, k[:40]])))
+    for requests, new in (([a, b, a], [0, 0, 1]), ([a, a], [1, 1]), (iter([a, a]), [1, 0])):
+        with pytest.raises(ValueError, match="named twice"):
+            cache.plan(requests, [1] * len(new), new_lengths=new)
+    assert cache.length(a) == 40 and cache.length(b) == 41 and cache.free_pages == 5
+
+
 @pytest.mark.parametrize("broken", ["CachePlan", "copy_pages"])
 def test_a_step_that_fails_while_it_is_built_changes_nothing(monkeypatch, broken):
     from hyperflow_h3_flash_amd import kv_cache
