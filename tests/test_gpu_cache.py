@@ -317,6 +317,38 @@ def test_ends_of_the_type(dtype):
         U.check(out, C.held(v)[:1], C.held(v)[:1] * 2 * 2.0 ** -11)
 
 
+@pytest.mark.parametrize("rows", [1, 40])
+def test_values_up_to_the_stated_range_of_bfloat16(rows):
+    """Values times 256 times the number of keys may reach float32's range; equal values past it overflow their sum."""
+    n = 70
+    inside = 6.0 * 2.0 ** 111  # times 256 * 70: 2.8e38
+    assert inside * 256 * n < torch.finfo(torch.float32).max < 2 * inside * 256 * n
+    k, q = keys(1, n, 1, 32, BF), rnd(2, rows, 1, 32).to(BF)
+    for value, finite in ((inside, True), (-inside, True), (torch.finfo(BF).max, False)):
+        v = torch.full((n, 1, 32), value, dtype=BF, device="cuda")
+        v[:, 0, 1] *= 0.25  # another level of the same scale
+        cache, requests, _, _ = filled([n], 1, 32, k=k, v=v)
+        got = cached_attention(q, cache, 0, cache.plan(requests, [rows], new_lengths=[0]))
+        ref, bound = C.attention(q, k, v, [rows], [n], False, 32 ** -0.5)
+        if finite:
+            U.check(got, ref, bound)
+        else:  # 70 weights of up to 2^8, of which one is 1 or more: a sum of at least the value, up to infinity, never NaN
+            assert not got.isnan().any() and (got.double() >= (ref - bound).clamp_max(torch.finfo(BF).max)).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_no_farther_from_packed_attention_than_both_may_be_off(dtype):
+    from hyperflow_h3_flash_amd import AttentionPlan, packed_attention
+    q_lens, kv_lens = [2, 130, 1, 40], [700, 300, 64, 0]
+    cache, plan, q, *_, got = run_attention(q_lens, kv_lens, 8, 4, 128, dtype, causal=True)
+    k, v = cache_read(cache, 0, plan)
+    other = packed_attention(q, k, v, AttentionPlan(q_lens, kv_lens, heads=8, kv_heads=4, head_dim=128, causal=True))
+    ref, bound = U.attention(q, k, v, q_lens, kv_lens, True, 128 ** -0.5)
+    U.check(got, ref, bound)
+    U.check(other, ref, bound)
+    assert ((got.double() - other.double()).abs() <= 2 * bound).all()
+
+
 def test_out_in_place_and_strided():
     cache, plan, q, k, v, want = run_attention([3, 200], [300, 200], 4, 2, 64, causal=True)
     for out in (torch.empty_like(q), torch.zeros(203, 9, 64, dtype=BF, device="cuda")[:, 2:6],

@@ -54,6 +54,18 @@ def test_widths(width, norm, post):
     run([3, 0, 2], width, norm, post, weights=True, seed=width)
 
 
+@pytest.mark.parametrize("width", [512, 1024, 2048, 4096, 6144, 8192, 12288, 16384])
+@pytest.mark.parametrize("norm,post", [("layer", "rms"), ("rms", "layer")])
+@pytest.mark.parametrize("stream,vectors", [(BF, BF), (F32, F32)])
+def test_sums_by_the_kernels_own_chains(width, norm, post, stream, vectors, monkeypatch):
+    """The widest row of each shape, held to the additions that its sums make one behind the other: 8 terms for each of a lane's
+    chunks (1 or 2; 3 with 4 or 8 waves), 6 exchanges, and the row's 1 to 16 waves: at most 16 + 6 + 16 or 24 + 6 + 8. With the
+    quotient by the width 39 roundings."""
+    monkeypatch.setattr(C, "SUM", 39 * 2.0 ** -24)
+    for mean in (0.0, 20.0):
+        run([3, 2], width, norm, post, BF, stream, weights=True, vectors=vectors, mean=mean, seed=width)
+
+
 @pytest.mark.parametrize("norm", ["rms", "layer", None])
 @pytest.mark.parametrize("post", ["rms", "layer", None])
 @pytest.mark.parametrize("dtype,stream", [(BF, BF), (HF, HF), (BF, F32), (HF, F32)])
