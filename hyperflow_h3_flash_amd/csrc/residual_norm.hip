@@ -4,9 +4,9 @@
 //
 // HBM-bound: each element of x and y is read once, of r and n written once. A row stays in the registers of its waves from
 // the first read to the last write, up to NV chunks of 8 channels a lane (rows above 12288 channels with fp32 vectors nearly:
-// their sixteen waves have 128 registers each, and 4 of a lane's, 12 with x in fp32, go through scratch memory); the sums of its norms go over the lanes by
-// exchanges between registers and over the waves through LDS. Variances are sums of squared differences from the mean, not
-// differences of sums: a row far from zero keeps its digits.
+// their sixteen waves have 128 registers each, and 4 of a lane's, 12 with x in fp32, go through scratch memory). The sums of its
+// norms go over the lanes by exchanges between registers and over the waves through LDS. Variances are sums of squared
+// differences from the mean, not differences of sums: a row far from zero keeps its digits.
 //
 // Every load of a row is on its way before the first sum, the vectors' among them (from the caches), through descriptors of
 // the row: past its end loads give zero and stores nothing, and what is absent has a descriptor of no bytes, so there is no
