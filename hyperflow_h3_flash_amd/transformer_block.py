@@ -79,27 +79,32 @@ def _run(blocks: list[TransformerBlock], x: Tensor, plan, modulation: Sequence[T
             raise ValueError(f"a modulation must be [requests, 6, {blocks[0].dim}], got {tuple(m.shape)}")
     if not blocks:
         return x
+    kind = torch.float16 if x.dtype is torch.float16 else torch.bfloat16
+
+    def weight(w: Tensor | None) -> Tensor | None:  # after `Module.to`, as `AdapterBank`'s
+        return w if w is None or w.dtype is kind or w.dtype is torch.float32 else w.to(torch.float32)
+
     of = [(None,) * 6 if modulation is None else modulation[i].unbind(1) for i in range(len(blocks))]
     shift, scale = of[0][:2]
-    _, n = residual_norm(x, rows=rows, norm=blocks[0].norm, weight=blocks[0].norm_attention, scale=scale, shift=shift,
+    _, n = residual_norm(x, rows=rows, norm=blocks[0].norm, weight=weight(blocks[0].norm_attention), scale=scale, shift=shift,
                          eps=blocks[0].eps)
     for i, block in enumerate(blocks):
         gate, ff_shift, ff_scale, ff_gate = of[i][2:]
         a = block.attention(n, plan, positions=positions, rotary=rotary, adapters=adapters, layer=layer + i)
-        x, n = residual_norm(x, a, rows=rows, gate=gate, post_norm=block.post_norm, post_weight=block.post_attention,
-                             norm=block.norm, weight=block.norm_ff, scale=ff_scale, shift=ff_shift, eps=block.eps)
+        x, n = residual_norm(x, a, rows=rows, gate=gate, post_norm=block.post_norm, post_weight=weight(block.post_attention),
+                             norm=block.norm, weight=weight(block.norm_ff), scale=ff_scale, shift=ff_shift, eps=block.eps)
         f = block.down(block.up(n))
         after = blocks[i + 1] if i + 1 < len(blocks) else None
         shift, scale = of[i + 1][:2] if after is not None else (None, None)
         if after is not None and block.post_norm is not None and block.eps != after.eps:  # an eps each: two calls
-            x, _ = residual_norm(x, f, rows=rows, gate=ff_gate, post_norm=block.post_norm, post_weight=block.post_ff, norm=None,
-                                 eps=block.eps)
-            _, n = residual_norm(x, rows=rows, norm=after.norm, weight=after.norm_attention, scale=scale, shift=shift,
+            x, _ = residual_norm(x, f, rows=rows, gate=ff_gate, post_norm=block.post_norm, post_weight=weight(block.post_ff),
+                                 norm=None, eps=block.eps)
+            _, n = residual_norm(x, rows=rows, norm=after.norm, weight=weight(after.norm_attention), scale=scale, shift=shift,
                                  eps=after.eps)
             continue
-        x, n = residual_norm(x, f, rows=rows, gate=ff_gate, post_norm=block.post_norm, post_weight=block.post_ff,
+        x, n = residual_norm(x, f, rows=rows, gate=ff_gate, post_norm=block.post_norm, post_weight=weight(block.post_ff),
                              norm=None if after is None else after.norm,
-                             weight=None if after is None else after.norm_attention, scale=scale, shift=shift,
+                             weight=None if after is None else weight(after.norm_attention), scale=scale, shift=shift,
                              eps=block.eps if after is None else after.eps)
     return x
 

@@ -124,6 +124,28 @@ def test_steps_over_the_cache_agree_with_each_other(device):
     assert cache.length(c) == n and cache.table(b)[1] != cache.table(c)[1]
 
 
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("to", [torch.float16, torch.float32])
+def test_a_converted_block_keeps_working(device, to):
+    """Weights that every type holds (one, quarters), after `Module.to`: the same bits."""
+    size = SIZES[device]
+    blocks = [make(10 * i, device, norm="rms", post_norm="rms", **size) for i in range(2)]
+    for block in blocks:
+        for name in ("norm_attention", "norm_ff", "post_attention", "post_ff"):
+            getattr(block, name).copy_(1 + torch.arange(block.dim) % 3 / 4)
+        for w in (block.attention.norm_q, block.attention.norm_k):
+            w.fill_(1.25)
+    plan = AttentionPlan([7], heads=size.get("heads", 4), kv_heads=size.get("kv_heads", 2), head_dim=size.get("head_dim", 16),
+                         device=device)
+    stack = TransformerStack(blocks)
+    for layer in stack.modules():  # scales of the INT8 layers that float16 holds too
+        if isinstance(layer, Int8RotLinear):
+            layer.wscale.fill_(2.0 ** -9)
+    x = rnd(1, 7, blocks[0].dim).to(BF).to(device)
+    want = stack(x, plan)
+    assert torch.equal(stack.to(to)(x, plan), want)
+
+
 def test_refusals_of_the_blocks():
     block = make(0, "cpu")
     x, plan = rnd(1, 3, 64).to(BF), AttentionPlan([3], heads=4, kv_heads=2, head_dim=16, device="cpu")
