@@ -244,8 +244,9 @@ class KVCache:
     def plan(self, requests: Sequence[int], q_lengths: Sequence[int], *, new_lengths: Sequence[int] | None = None,
              heads: int | None = None, causal: bool = False) -> CachePlan:
         """The next step of some requests: ``q_lengths[i]`` queries of request i, ``new_lengths[i]`` tokens (default: as many)
-        that `cache_append` writes behind those it has. A request without new tokens may be named several times. ``heads`` query heads (default: kv_heads) share the key heads in
-        equal groups. ``causal``: the last query sees every key, each one before it one key less.
+        that `cache_append` writes behind those it has. A request without new tokens may be named several times. ``heads``
+        query heads (default: kv_heads) share the key heads in equal groups. ``causal``: the last query sees every key, each one
+        before it one key less.
 
         The new tokens are counted at once and get their pages; a shared page that they begin in is copied, on the current
         stream. RuntimeError, and nothing changed, when too few pages are free."""
